@@ -162,10 +162,16 @@ int gq_ctx_create(int device, gq_ctx **out) {
       break;
     }
     if ((e = cudaMemset(ctx->dev_err, 0, sizeof(uint32_t))) != cudaSuccess) { rc = GQ_ERR_CUDA; break; }
+    if ((e = cudaMalloc(reinterpret_cast<void **>(&ctx->counters), kCtxCounters * sizeof(uint32_t))) != cudaSuccess ||
+        (e = cudaMemset(ctx->counters, 0, kCtxCounters * sizeof(uint32_t))) != cudaSuccess) {
+      rc = GQ_ERR_CUDA;
+      break;
+    }
     const char *pdl = getenv("GQ_PDL");
     ctx->pdl = !(pdl && pdl[0] == '0');
   } while (0);
   if (rc != GQ_OK) {
+    if (ctx->counters) cudaFree(ctx->counters);
     if (ctx->dev_err) cudaFree(ctx->dev_err);
     if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
     delete ctx;
@@ -182,6 +188,7 @@ int gq_ctx_destroy(gq_ctx *ctx) {
   for (int i = 0; i < 2; ++i)
     if (ctx->scratch[i]) cudaFree(ctx->scratch[i]);
   if (ctx->ws) cudaFree(ctx->ws);
+  if (ctx->counters) cudaFree(ctx->counters);
   if (ctx->dev_err) cudaFree(ctx->dev_err);
   if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
   delete ctx;
@@ -217,6 +224,7 @@ int gq_sync(gq_ctx *ctx) {
     if (flags & GQ_DEVERR_BAD_ID) msg += " embedding id out of range;";
     if (flags & GQ_DEVERR_WAIT_TIMEOUT) msg += " pipeline wait timed out;";
     if (flags & GQ_DEVERR_SAMPLE_CAP) msg += " top-p nucleus larger than the device sampler's 256 candidates;";
+    if (flags & GQ_DEVERR_PAGES) msg += " a page, slot or length outside the paged cache's pool;";
     return gq_fail(ctx, GQ_ERR_DEVICE, msg);
   }
   return GQ_OK;

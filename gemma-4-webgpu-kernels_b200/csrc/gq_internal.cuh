@@ -51,10 +51,15 @@ struct gq_ctx {
   // workspace of the tensor-core prefill path (f16 copy of the activations, row exponents)
   void *ws = nullptr;
   size_t ws_cap = 0;
+  // arrival counters of kernels whose last CTA finishes the work (the paged-cache ops):
+  // zero between launches, the last CTA to arrive at one puts it back to zero
+  uint32_t *counters = nullptr;
   // set by gq_linear_softcap_peers(_signal) for the duration of one call
   PeerDst peers = {};
   PeerDst peer_signal = {};
 };
+
+constexpr size_t kCtxCounters = 4096;
 
 struct gq_qweight {
   gq_ctx *ctx = nullptr;

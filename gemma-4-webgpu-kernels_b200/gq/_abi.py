@@ -21,6 +21,12 @@ GQ_ERR_DEVICE = 5
 GQ_DEVERR_BAD_ID = 0x1
 GQ_DEVERR_WAIT_TIMEOUT = 0x2
 GQ_DEVERR_SAMPLE_CAP = 0x4
+GQ_DEVERR_PAGES = 0x8
+
+GQ_KV_F32 = 0
+GQ_KV_F16 = 1
+GQ_KV_BF16 = 2
+GQ_KV_E4M3 = 3
 
 
 class SampleOpts(ctypes.Structure):
@@ -32,6 +38,13 @@ class ChainOp(ctypes.Structure):
     """gq_chain_op (include/gq.h): one one-row MATMUL_Q call of a decode chain."""
     _fields_ = [("mode", c_int32), ("w", c_void_p), ("w2", c_void_p), ("x", c_void_p), ("y", c_void_p),
                 ("b", c_void_p), ("b_offset", c_int64), ("cap", c_float)]
+
+
+class KvPagesStruct(ctypes.Structure):
+    """gq_kv_pages (include/gq.h): one layer's pages of a paged key-value cache."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("n_pages", c_int64), ("page_size", c_int64), ("heads", c_int64),
+                ("head_dim", c_int64), ("page_stride", c_int64), ("type", c_int32), ("k_scale", c_float),
+                ("v_scale", c_float)]
 
 
 class GqError(RuntimeError):
@@ -148,6 +161,16 @@ SIGNATURES = {
     "gq_scale": (c_int, [c_void_p, c_void_p, c_int64, c_float, c_void_p]),
     "gq_scale_by_tensor": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "gq_copy_rows": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64]),
+    "gq_paged_reserve": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                                 c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "gq_paged_release": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                                 c_void_p, c_void_p, c_void_p]),
+    "gq_paged_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p]),
+    "gq_paged_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                   c_float, c_uint32, c_float, c_void_p]),
+    "gq_process_logits": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
+                                  c_void_p, c_int64]),
 }
 
 GQ_ATTN_KPOS_ASCENDING = 0x1

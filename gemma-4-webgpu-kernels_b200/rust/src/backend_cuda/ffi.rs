@@ -52,6 +52,22 @@ pub struct GqSampleOpts {
     pub repetition_penalty: f32,
 }
 
+/// gq_kv_pages: one layer's pages of a paged key-value cache.
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct GqKvPages {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub n_pages: i64,
+    pub page_size: i64,
+    pub heads: i64,
+    pub head_dim: i64,
+    pub page_stride: i64,
+    pub kv_type: i32,
+    pub k_scale: f32,
+    pub v_scale: f32,
+}
+
 pub const GQ_OK: c_int = 0;
 pub const GQ_ERR_INVALID_ARGUMENT: c_int = 1;
 pub const GQ_ERR_UNSUPPORTED: c_int = 2;
@@ -61,6 +77,11 @@ pub const GQ_ERR_DEVICE: c_int = 5;
 pub const GQ_DEVERR_BAD_ID: u32 = 0x1;
 pub const GQ_DEVERR_WAIT_TIMEOUT: u32 = 0x2;
 pub const GQ_DEVERR_SAMPLE_CAP: u32 = 0x4;
+pub const GQ_DEVERR_PAGES: u32 = 0x8;
+pub const GQ_KV_F32: i32 = 0;
+pub const GQ_KV_F16: i32 = 1;
+pub const GQ_KV_BF16: i32 = 2;
+pub const GQ_KV_E4M3: i32 = 3;
 pub const GQ_ATTN_KPOS_ASCENDING: u32 = 0x1;
 pub const GQ_ATTN_KPOS_IDENTITY: u32 = 0x2;
 
@@ -189,4 +210,21 @@ extern "C" {
     pub fn gq_scale_by_tensor(ctx: *mut GqCtx, a: *const f32, n: i64, s: *const f32, y: *mut f32) -> c_int;
     pub fn gq_copy_rows(ctx: *mut GqCtx, src: *const f32, rows: i64, cols: i64, src_stride: i64,
         dst: *mut f32, dst_stride: i64) -> c_int;
+    // paged KV cache and logits of many requests
+    pub fn gq_paged_reserve(ctx: *mut GqCtx, batch: i64, page_size: i64, seq_lens: *const i32, new_lens: *const i32,
+        block_table: *mut i32, table_stride: i64, free_pages: *const i32, n_pages: i64, free_count: *const i32,
+        free_left: *mut i32, max_tokens: i64, slots: *mut i64, positions: *mut i32, owners: *mut i32,
+        totals: *mut i32) -> c_int;
+    pub fn gq_paged_release(ctx: *mut GqCtx, batch: i64, page_size: i64, seq_lens: *const i32, keep_lens: *const i32,
+        block_table: *const i32, table_stride: i64, free_pages: *mut i32, n_pages: i64, free_count: *const i32,
+        free_left: *mut i32, totals: *mut i32) -> c_int;
+    pub fn gq_paged_append(ctx: *mut GqCtx, pages: *const GqKvPages, k: *const f32, v: *const f32, t: i64,
+        k_tok_stride: i64, v_tok_stride: i64, slots: *const i64) -> c_int;
+    pub fn gq_paged_attention(ctx: *mut GqCtx, pages: *const GqKvPages, q: *const f32, batch: i64, hq: i64,
+        q_tok_stride: i64, block_table: *const i32, table_stride: i64, seq_lens: *const i32, scale: f32,
+        sliding_window: u32, attn_softcap: f32, out: *mut f32) -> c_int;
+    pub fn gq_process_logits(ctx: *mut GqCtx, logits: *const f32, m: i64, vocab: i64, ld: i64, tokens: *const i32,
+        tok_stride: i64, prompt_lens: *const i32, lens: *const i32, penalties: *const f32, bias_ids: *const i32,
+        bias_values: *const f32, bias_offsets: *const i32, masks: *const u32, n_masks: i64, mask_stride: i64,
+        mask_rows: *const i32, y: *mut f32, ldy: i64) -> c_int;
 }

@@ -49,6 +49,7 @@ typedef enum gq_status {
 #define GQ_DEVERR_BAD_ID 0x1u       /* embed id >= table rows (output row zeroed) */
 #define GQ_DEVERR_WAIT_TIMEOUT 0x2u /* a bounded pipeline wait gave up */
 #define GQ_DEVERR_SAMPLE_CAP 0x4u   /* a top-p nucleus exceeded the device sampler's candidates */
+#define GQ_DEVERR_PAGES 0x8u        /* a paged-cache call met a page, slot or pool outside its bounds */
 
 typedef struct gq_ctx gq_ctx;         /* device + stream + error word + workspace */
 typedef struct gq_qweight gq_qweight; /* packed weight resident on the device */
@@ -498,6 +499,119 @@ int gq_scale_by_tensor(gq_ctx *ctx, const float *a, int64_t n, const float *s, f
  * slice_cols, concat_rows and kv_append of rust/src/backend.rs:122-130. */
 int gq_copy_rows(gq_ctx *ctx, const float *src, int64_t rows, int64_t cols, int64_t src_stride, float *dst,
                  int64_t dst_stride);
+
+/* ---- paged KV cache and logits of many requests ---------------------------------
+ * A decode step that serves many requests of different lengths: each request's keys
+ * and values live in pages of a pool shared by all of them, found through a block
+ * table (row b, entry p: the page holding tokens p * page_size .. of request b).
+ * Lengths, tables and the free list stay on the device, so one recorded step
+ * (gq_graph_*) serves every following token. Calls that may
+ * overlap on two streams need a context each (they share its workspace and arrival
+ * counters). No counterpart in the reference (its caches are one contiguous tensor per
+ * layer of one sequence). */
+
+/* Storage of a page's values. An e4m3 code stands for code * k_scale (or v_scale). */
+#define GQ_KV_F32 0
+#define GQ_KV_F16 1
+#define GQ_KV_BF16 2
+#define GQ_KV_E4M3 3
+
+/* One layer's pages, in caller-owned device memory: value (page, head, row, c) of the
+ * keys is element page * page_stride + (head * page_size + row) * head_dim + c of k
+ * (page_stride = 0: heads * page_size * head_dim, packed; a larger stride lets keys
+ * and values, or several layers, interleave in one allocation). head_dim a multiple
+ * of 4 up to 512, page_size 1 .. 65536, heads up to 65535, k and v 16-byte aligned,
+ * page_stride a multiple of 4. k_scale and v_scale are positive and finite
+ * for GQ_KV_E4M3 and 1 for the other types. */
+typedef struct gq_kv_pages {
+  void *k, *v;
+  int64_t n_pages, page_size, heads, head_dim, page_stride;
+  int32_t type;
+  float k_scale, v_scale;
+} gq_kv_pages;
+
+/* Take pages for the tokens that a step adds. Request b holds seq_lens[b] tokens in
+ * the first ceil(seq_lens[b] / page_size) entries of its block_table row
+ * (table_stride entries) and gets new_lens[b] more (negative lengths count as 0).
+ * Its further entries are filled from the top of the free list: the i-th page taken
+ * by all requests, in request order, is free_pages[free_count[0] - 1 - i].
+ * The step's tokens are numbered in request order; token t's owners[t] is its request,
+ * positions[t] its position there and slots[t] = page * page_size + row where its key
+ * and value go (gq_paged_append). Places from the last token up to max_tokens get slot
+ * -1, position 0, owner -1. totals[b] = seq_lens[b] + new_lens[b], free_left[0] = what
+ * remains of free_count[0]; they may be seq_lens and free_count themselves.
+ * All or nothing: when the pool (n_pages entries of free_pages), a table row or
+ * max_tokens is too small, no page is taken, every slot is -1, totals = seq_lens,
+ * free_left = free_count and GQ_DEVERR_PAGES is raised at the next gq_sync. A page id
+ * outside [0, n_pages) in the table or the list gives slot -1 and the same error.
+ * All pointers are device pointers. batch <= 16384, max_tokens < 2^31. */
+int gq_paged_reserve(gq_ctx *ctx, int64_t batch, int64_t page_size, const int32_t *seq_lens, const int32_t *new_lens,
+                     int32_t *block_table, int64_t table_stride, const int32_t *free_pages, int64_t n_pages,
+                     const int32_t *free_count, int32_t *free_left, int64_t max_tokens, int64_t *slots,
+                     int32_t *positions, int32_t *owners, int32_t *totals);
+
+/* Give pages back: request b keeps its first min(keep_lens[b], seq_lens[b]) tokens (0
+ * ends the request; a rejected draft keeps what was accepted), and the pages past
+ * those go back to the free list, in the order that undoes gq_paged_reserve exactly:
+ * the i-th of R pages given back (request order, then table order) becomes
+ * free_pages[free_count[0] + R - 1 - i]. totals[b] is the kept length, free_left[0] =
+ * free_count[0] + R; they may be seq_lens and free_count. The block table is not
+ * changed (entries past a request's length mean nothing). All or nothing: when the
+ * list would outgrow its n_pages entries, or a length its row, nothing is given back,
+ * totals = seq_lens, free_left = free_count, and GQ_DEVERR_PAGES is raised.
+ * batch <= 16384. */
+int gq_paged_release(gq_ctx *ctx, int64_t batch, int64_t page_size, const int32_t *seq_lens, const int32_t *keep_lens,
+                     const int32_t *block_table, int64_t table_stride, int32_t *free_pages, int64_t n_pages,
+                     const int32_t *free_count, int32_t *free_left, int32_t *totals);
+
+/* Write t new key and value rows into their pages: row i of k (f32, heads * head_dim
+ * values at k + i * k_tok_stride; 0 = packed) and of v, rounded to the pages' type
+ * (nearest, ties to even; e4m3: value * (1 / scale) clamped to +-448, NaN stays NaN),
+ * goes to slots[i] (device int64). A negative slot skips the row; one past the pool
+ * skips it and raises GQ_DEVERR_PAGES. Two rows must not have the same slot. k and v
+ * 16-byte aligned, token strides multiples of 4. */
+int gq_paged_append(gq_ctx *ctx, const gq_kv_pages *pages, const float *k, const float *v, int64_t t,
+                    int64_t k_tok_stride, int64_t v_tok_stride, const int64_t *slots);
+
+/* Attention of one new token of each request over its pages (the paged form of
+ * gq_attention with t = 1): the query of request b is at position seq_lens[b] - 1 and
+ * sees positions j < seq_lens[b], the last sliding_window of them when that is not 0;
+ * scores scale * q . k, optional tanh soft-cap, softmax, weighted sum of v. q is
+ * [batch, hq, head_dim] f32 (token stride q_tok_stride, 0 = packed), out [batch, hq *
+ * head_dim] f32. A length of 0 or less gives zeros. hq is a multiple of the pages'
+ * heads, hq / heads <= 64. Rows of a page past the request's length are never read as
+ * numbers (they may hold NaN). A page id outside the pool raises GQ_DEVERR_PAGES and
+ * counts as a page of zero rows; a length past the table row raises it and is cut to
+ * the row: nothing outside the pool is read. Finite q and visible keys and values give f32 results (all sums in
+ * f32, products exact to 2^-21 or better); where one is not finite, its row may be NaN.
+ * Long requests are split over many CTAs, whose partial results (context workspace)
+ * are joined in the same launch in a fixed order: results do not vary from run to
+ * run. */
+int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const float *q, int64_t batch, int64_t hq,
+                       int64_t q_tok_stride, const int32_t *block_table, int64_t table_stride,
+                       const int32_t *seq_lens, float scale, uint32_t sliding_window, float attn_softcap, float *out);
+
+/* Per-request control of the logits [m, vocab] (row stride ld, 0 = vocab) before
+ * sampling, in one pass to y (row stride ldy; y may be logits with ldy = ld):
+ *   l = logits[r, c]
+ *   c among the row's tokens[r, 0 .. lens[r]):  l = l > 0 ? l / rep : l * rep
+ *   n = times c is among tokens[r, prompt_lens[r] .. lens[r])  (what was generated)
+ *   l = (l - frequency * n) - (n > 0 ? presence : 0)
+ *   l = l + bias   (row r's entries bias_offsets[r] .. bias_offsets[r + 1) of bias_ids
+ *                   / bias_values; the last entry of an id counts)
+ *   bit c % 32 of word c / 32 of the row's mask clear: l = -inf
+ * penalties is [m, 3] f32 (rep > 0, presence, frequency). tokens has row stride
+ * tok_stride, which also bounds lens; ids outside the vocabulary are ignored. The
+ * row's mask is masks[mask_rows[r]] (mask_stride words each); an index outside [0,
+ * n_masks) leaves the row unmasked; mask_rows NULL is row r's own mask r. tokens,
+ * bias_offsets and masks may be NULL (that step is left out); a row whose mask is
+ * empty becomes all -inf. All pointers are device pointers; arithmetic is f32, one
+ * rounding per operation. vocab < 2^28, m <= 65535. */
+int gq_process_logits(gq_ctx *ctx, const float *logits, int64_t m, int64_t vocab, int64_t ld, const int32_t *tokens,
+                      int64_t tok_stride, const int32_t *prompt_lens, const int32_t *lens, const float *penalties,
+                      const int32_t *bias_ids, const float *bias_values, const int32_t *bias_offsets,
+                      const uint32_t *masks, int64_t n_masks, int64_t mask_stride, const int32_t *mask_rows, float *y,
+                      int64_t ldy);
 
 #ifdef __cplusplus
 }
