@@ -18,6 +18,10 @@
 
 #include "paged_attn.cuh"
 
+// paged_attn_tc.cu
+bool gq_paged_attn_tc_supported(const gq_kv_pages *pages, int64_t page_stride);
+int gq_paged_attn_tc_launch(gq_ctx *ctx, const gq_kv_pages *pages, pattn::Args &a);
+
 namespace {
 
 using namespace pattn;
@@ -249,16 +253,10 @@ extern "C" int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const f
   a.v_scale = pages->v_scale;
   a.ctr = ctx->counters + kCtrBase;
   a.err = ctx->dev_err;
-  // no more CTAs than there can be tiles: the table bounds a length the host does not know
-  const int64_t keys = std::min<int64_t>(table_stride * pages->page_size, INT32_MAX);
-  const int64_t visible = a.window > 0 ? std::min<int64_t>(keys, (int64_t)a.window + kRowTile) : keys;
-  const int64_t tiles = batch * a.units_per_req * std::max<int64_t>(1, (visible + kRowTile - 1) / kRowTile);
-  const int grid = (int)std::min<int64_t>(tiles, std::min<int64_t>(kMaxGrid, 4 * (int64_t)ctx->num_sms));
-  void *ws = nullptr;
-  rc = gq_workspace(ctx, (size_t)grid * 2 * kHeads * (a.dim + 2) * 4, &ws);
+  if (gq_paged_attn_tc_supported(pages, a.page_stride)) return gq_paged_attn_tc_launch(ctx, pages, a);
+  const int grid = grid_for(a, kRowTile, 4 * ctx->num_sms);
+  rc = bind_workspace(ctx, grid, a);
   if (rc != GQ_OK) return rc;
-  a.part_o = static_cast<float *>(ws);
-  a.part_ml = a.part_o + (size_t)grid * 2 * kHeads * a.dim;
   switch (pages->type) {
     case GQ_KV_F32: GQ_CUDA_TRY(ctx, rows_launch<GQ_KV_F32>(ctx, grid, a)); break;
     case GQ_KV_F16: GQ_CUDA_TRY(ctx, rows_launch<GQ_KV_F16>(ctx, grid, a)); break;

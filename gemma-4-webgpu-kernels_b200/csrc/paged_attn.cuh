@@ -16,6 +16,8 @@
 // levels of 17 take 3.
 #pragma once
 
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace pattn {
@@ -136,6 +138,12 @@ __device__ __forceinline__ void unit_heads(const Args &a, int u, int &head0, int
   n = min(kHeads, a.group - s * kHeads);
 }
 
+// Barrier of the NT threads that compute (the first NT of the block).
+template <int NT>
+__device__ __forceinline__ void sync_compute() {
+  asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
+}
+
 // Join `n` parts (part i in slot slots(i)) and hand each (head, 4 columns) sum with its
 // maximum and sum of weights to `put`.
 template <int NT, typename Slots, typename Put>
@@ -144,7 +152,7 @@ __device__ __forceinline__ void join(const Args &a, int n, Slots slots, Put put)
   __shared__ float ms[kHeads], ls[kHeads];
   const int tid = threadIdx.x;
   for (int i = tid; i < n * kHeads; i += NT) wgt[i / kHeads][i % kHeads] = __ldcg(a.part_ml + (slots(i / kHeads) * kHeads + i % kHeads) * 2);
-  __syncthreads();
+  sync_compute<NT>();
   if (tid < kHeads) {
     float m = -INFINITY, l = 0.0f;
     for (int i = 0; i < n; ++i) m = fmaxf(m, wgt[i][tid]);
@@ -157,7 +165,7 @@ __device__ __forceinline__ void join(const Args &a, int n, Slots slots, Put put)
     ms[tid] = m;
     ls[tid] = l;
   }
-  __syncthreads();
+  sync_compute<NT>();
   const int per = a.dim / 4;
   for (int i = tid; i < kHeads * per; i += NT) {
     const int h = i / per, c = (i - h * per) * 4;
@@ -176,9 +184,10 @@ __device__ __forceinline__ void join(const Args &a, int n, Slots slots, Put put)
 }
 
 // True in every thread of the CTA that arrives last of n at the counter.
+template <int NT>
 __device__ __forceinline__ bool arrive_last(uint32_t *ctr, int n) {
   __shared__ int last;
-  __syncthreads();
+  sync_compute<NT>();
   if (threadIdx.x == 0) {
     __threadfence();
     last = atomicAdd(ctr, 1u) == (uint32_t)n - 1;
@@ -187,7 +196,7 @@ __device__ __forceinline__ bool arrive_last(uint32_t *ctr, int n) {
       __threadfence();
     }
   }
-  __syncthreads();
+  sync_compute<NT>();
   return last != 0;
 }
 
@@ -197,18 +206,15 @@ __device__ __forceinline__ float inv_or_zero(float l) { return l == 0.0f ? 0.0f 
 // of cut units, the one it begins in the middle of (or begins with) and its last.
 __device__ __forceinline__ int slot_of(const Cut &cut, int c, int64_t s0) { return 2 * c + (cut.start(c) < s0 ? 1 : 0); }
 
-// All threads of CTA blockIdx.x, after its part of unit (b, u) (tiles s0 .. s0 + nt of
+// The NT computing threads of CTA blockIdx.x, after its part of unit (b, u) (tiles s0 .. s0 + nt of
 // the whole row of tiles) is in its slot: join when this CTA is the last.
 template <int NT>
 __device__ __forceinline__ void finish_part(const Args &a, const Cut &cut, int b, int u, int64_t s0, int nt) {
   const int c0 = cut.at(s0), n = cut.at(s0 + nt - 1) - c0 + 1;
-  int g = n;
-  if (n > kOneLevel) {
-    g = (int)ceilf(sqrtf((float)n));
-  }
+  const int g = n > kOneLevel ? (int)ceilf(sqrtf((float)n)) : n;
   const int groups = (n + g - 1) / g, j = ((int)blockIdx.x - c0) / g;
   const int first = c0 + j * g, members = min(g, n - j * g);
-  if (!arrive_last(a.ctr + 2 * slot_of(cut, first, s0), members)) return;
+  if (!arrive_last<NT>(a.ctr + 2 * slot_of(cut, first, s0), members)) return;
   if (groups > 1) {
     const int to = slot_of(cut, first, s0);
     // the sums replace the group's first part, column by column where that was just read
@@ -220,7 +226,7 @@ __device__ __forceinline__ void finish_part(const Args &a, const Cut &cut, int b
                  a.part_ml[(to * kHeads + h) * 2 + 1] = l;
                }
              });
-    if (!arrive_last(a.ctr + 2 * slot_of(cut, c0, s0) + 1, groups)) return;
+    if (!arrive_last<NT>(a.ctr + 2 * slot_of(cut, c0, s0) + 1, groups)) return;
   }
   int head0, nh, kv;
   unit_heads(a, u, head0, nh, kv);
@@ -238,6 +244,26 @@ __device__ __forceinline__ float score_log2(const Args &a, float dot) {
   float s = dot * a.scale;
   if (a.softcap > 0.0f) s = a.softcap * tanhf(__fdiv_rn(s, a.softcap));
   return s * kLog2e;
+}
+
+// ---- host side
+
+// CTAs to launch: at most `most`, and no more than there can be tiles (the table bounds
+// the lengths, which the host does not know).
+inline int grid_for(const Args &a, int tile, int most) {
+  int64_t keys = std::min<int64_t>(a.table_stride * a.page_size, INT32_MAX);
+  if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + tile);
+  const int64_t tiles = (int64_t)a.batch * a.units_per_req * std::max<int64_t>(1, (keys + tile - 1) / tile);
+  return (int)std::min<int64_t>(tiles, std::min(kMaxGrid, most));
+}
+
+// Workspace for the parts: two per CTA.
+inline int bind_workspace(gq_ctx *ctx, int grid, Args &a) {
+  void *ws = nullptr;
+  const int rc = gq_workspace(ctx, (size_t)grid * 2 * kHeads * (a.dim + 2) * 4, &ws);
+  a.part_o = static_cast<float *>(ws);
+  a.part_ml = a.part_o + (size_t)grid * 2 * kHeads * a.dim;
+  return rc;
 }
 
 }  // namespace pattn

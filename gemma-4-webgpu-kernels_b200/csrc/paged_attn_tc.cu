@@ -1,0 +1,634 @@
+// paged_attn_tc.cu — the tiled kernel of gq_paged_attention: pages by TMA, products on
+// the tensor cores, f32 results.
+//
+// A tile is T keys of one unit (one request, up to 8 query heads of one key-value head).
+// One warp is the producer: it walks this CTA's tiles and issues, per page (or part of
+// a page), one 4-D TMA copy of the keys and one of the values into a ring of tiles
+// (128-byte swizzle, so the fragment loads below have no bank conflicts). Four warps
+// compute, tile by tile:
+//   S^T = K q^T        m16 = keys, n8 = heads, over head_dim: keys split over the warps
+//                      (and head_dim over KS warps where T < 64)
+//   p = 2^(s - m)      16 threads per head; running maximum and sum
+//   O^T += V^T p^T     m16 = head_dim columns, n8 = heads, over the T keys: columns
+//                      split over the warps
+// Transposed, the 8 heads fill the instruction's n = 8 exactly: no product is wasted,
+// and a key-value head's cache is read once for all of them. The m16n8 instructions
+// (mma.sync) are used, not tcgen05: at n = 8 the work is 16 products per cached value,
+// and the ring, not the tensor pipe, is the limit; a 128-row accumulator tile in tensor
+// memory would add a round trip per tile for a softmax over its rows.
+//
+// f32 results from 16-bit products: q and p (f32) are cut into parts that each fit the
+// type and add up to the number: bf16 3 parts (24 bits); f16 2 parts (22 bits, q scaled
+// per head to 2^13..2^14 and p to 2^14 so the second part stays normal); f32 pages use
+// tf32 with both operands in 2 parts, the product of the two low parts (2^-22) left out.
+// The cached 16- and 8-bit values are exact in their type (e4m3 in f16), products are
+// exact in f32, and sums are f32. The extra instructions are free here: 3 per 16 x 16
+// cached values, about a quarter of the legacy tensor pipe at full bandwidth.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "paged_attn.cuh"
+#include "tc_common.cuh"
+
+namespace {
+
+using namespace pattn;
+
+constexpr int kComputeWarps = 4;
+constexpr int kCompute = kComputeWarps * 32;
+constexpr int kThreads = kCompute + 32;
+constexpr int kRingBytes = 96 * 1024;  // two CTAs per SM
+constexpr int kMaxSlots = 8;
+
+__device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int c0, int c1, int c2, int c3, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          gqd::smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(gqd::smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ float lds32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// v = hi + lo: hi the nearest tf32 number, lo exact (the instruction reads its top 11 bits).
+__device__ __forceinline__ void split_tf32(float v, uint32_t &hi, uint32_t &lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(v));
+  lo = __float_as_uint(v - __uint_as_float(hi));
+}
+template <typename H2>
+__device__ __forceinline__ uint32_t bits(H2 v) {
+  return *reinterpret_cast<uint32_t *>(&v);
+}
+// Parts of a pair of f32 numbers as packed pairs.
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t (&part)[3]) {
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    part[i] = bits(h);
+    x -= __low2float(h);
+    y -= __high2float(h);
+  }
+}
+__device__ __forceinline__ void split_f16(float x, float y, uint32_t (&part)[2]) {
+  const __half2 h = __floats2half2_rn(x, y);
+  part[0] = bits(h);
+  part[1] = bits(__floats2half2_rn(x - __low2float(h), y - __high2float(h)));
+}
+// Two e4m3 codes (low 16 bits of u) to a pair of f16.
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t u) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(u));
+  return r;
+}
+
+// What a type and head_dim fix.
+template <int TYPE, int D>
+struct Tile {
+  static constexpr int kSize = TYPE == GQ_KV_F32 ? 4 : TYPE == GQ_KV_E4M3 ? 1 : 2;
+  // head_dim is split over KS warps where the q fragments of one warp would not fit its
+  // registers (2 parts of 256 columns or 3 of 256 at 16 bits, 2 of 128 at 32)
+  static constexpr int KS = TYPE == GQ_KV_F32 ? (D > 128 ? D / 128 : 1) : (D > 256 ? D / 256 : 1);
+  static constexpr int T = 16 * kComputeWarps / KS;
+  static constexpr int kRow = D * kSize;          // bytes of a key
+  static constexpr int kChunks = kRow / 128;      // 128-byte pieces of a key
+  static constexpr int kSlot = T * kRow;
+  static constexpr int kSlots = std::min(kMaxSlots, kRingBytes / kSlot);
+  static constexpr int kParts = TYPE == GQ_KV_BF16 ? 3 : 2;
+  static constexpr int kStep = TYPE == GQ_KV_F32 ? 8 : 16;      // head_dim columns (keys) per instruction
+  static constexpr int kQSteps = D / KS / kStep;
+  static constexpr int kMTiles = D / kComputeWarps / 16;        // 16-column tiles of the output per warp
+  static constexpr int kSStride = T + 4;                        // floats between heads' scores
+  static constexpr int kPStride = TYPE == GQ_KV_F32 ? (T + 4) * 4 : T * 2 + 16;  // bytes between heads' weights
+  static constexpr int kPBytes = (TYPE == GQ_KV_F32 ? 1 : kParts) * kHeads * kPStride;
+  static constexpr int kSmem = 1024 + kSlots * kSlot + KS * kHeads * kSStride * 4 + kPBytes;
+  static_assert(kRow % 128 == 0 && kSlots >= 3, "tile");
+};
+
+// A wait that gave up: report once, and let the CTA run to its end without waiting (what
+// it computes is dropped by the error; counters and barriers stay consistent).
+__device__ __forceinline__ void wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort, uint32_t *err) {
+  if (*abort) return;
+  if (!gqd::mbar_wait_bounded(bar, parity)) {
+    *abort = 1;
+    gqd::report(err, GQ_DEVERR_WAIT_TIMEOUT);
+  }
+}
+
+
+template <int TYPE, int D>
+__global__ void __launch_bounds__(kThreads, 2)
+    paged_tiles_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+  using C = Tile<TYPE, D>;
+  constexpr int T = C::T, KS = C::KS;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t full[kMaxSlots], empty[kMaxSlots];
+  __shared__ float fix[kHeads], sum[kHeads];
+  __shared__ int abort_flag;
+  uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float *sS = reinterpret_cast<float *>(ring + C::kSlots * C::kSlot);                       // [KS][head][key]
+  uint8_t *sP = reinterpret_cast<uint8_t *>(sS + KS * kHeads * C::kSStride);                // [part][head][key]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    for (int i = 0; i < C::kSlots; ++i) {
+      gqd::mbar_init(&full[i], 1);
+      gqd::mbar_init(&empty[i], kComputeWarps);
+    }
+    gqd::fence_mbar_init();
+    abort_flag = 0;
+  }
+  gqd::griddep_wait();
+  gqd::griddep_launch_dependents();
+  const Cut cut = find_cut<kThreads, T>(a);  // (its barriers also publish the mbarriers)
+  if (cut.w0 >= cut.w1) return;
+  const int rows_shift = min(a.page_shift, T == 64 ? 6 : T == 32 ? 5 : 4);  // log2 of the keys one copy brings
+  const int rows = 1 << rows_shift;
+
+  if (warp == kComputeWarps) {
+    // ---- producer: lane i owns the tile's i-th copy; the next tile's table entry is
+    // read before this tile's slots are waited for
+    const int boxes = T >> rows_shift;
+    int b = cut.b, u = cut.u, t = cut.t;
+    Range r = range_of<T>(a, b);
+    auto entry = [&](int j0) -> int {  // page of this lane's copy, -1: nothing to load
+      const int j = j0 + (lane << rows_shift);
+      if (lane >= boxes || j >= r.hi || j + rows <= r.lo) return -1;
+      const int page = a.table[b * a.table_stride + (j >> a.page_shift)];
+      if (page >= 0 && page < a.n_pages) return page;
+      gqd::report(a.err, GQ_DEVERR_PAGES);
+      return (int)a.n_pages;  // out of the tensor's bounds: reads as zeros
+    };
+    int j0 = (r.tile0 + t) * T, page = entry(j0);
+    uint32_t n = 0;  // ring position
+    for (int64_t w = cut.w0; w < cut.w1; ++w) {
+      const int load = page, jj = j0 + (lane << rows_shift), kvh = u / a.sub;
+      if (w + 1 < cut.w1) {
+        if (++t == r.nt) {
+          t = 0;
+          if (++u == a.units_per_req) {
+            u = 0;
+            ++b;
+            r = range_of<T>(a, b);
+          }
+        }
+        j0 = (r.tile0 + t) * T;
+        page = entry(j0);
+      }
+      const int copies = __popc(__ballot_sync(0xffffffffu, load >= 0));
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv, ++n) {
+        const int slot = n % C::kSlots;
+        if (lane == 0) {
+          if (n >= C::kSlots) wait_or_abort(&empty[slot], ((n / C::kSlots) & 1) ^ 1, &abort_flag, a.err);
+          gqd::mbar_arrive_expect_tx(&full[slot], (uint32_t)(copies * rows * C::kRow));
+        }
+        __syncwarp();
+        if (load >= 0)
+          tma_load_4d(ring + slot * C::kSlot + lane * rows * C::kRow, kv ? &vmap : &kmap, 0,
+                      (kvh << a.page_shift) + (jj & (a.page_size - 1)), 0, load, &full[slot]);
+      }
+    }
+    if (*(volatile int *)&abort_flag && lane == 0)  // copies still in flight end before the CTA's memory goes away
+      for (uint32_t i = n > C::kSlots ? n - C::kSlots : 0; i < n; ++i)
+        (void)gqd::mbar_wait_bounded(&full[i % C::kSlots], (i / C::kSlots) & 1, 100000000ull);
+    return;
+  }
+
+  // ---- compute
+  const int g = lane >> 2, q4 = lane & 3;  // fragment row / column group
+  const int ks = warp % KS, mt = warp / KS;
+  const int sh = tid >> 4, sl = tid & 15;  // softmax: head, thread of 16
+  constexpr int KPT = T / 16;              // keys per softmax thread
+  const uint32_t ring_u = gqd::smem_u32(ring);
+  const uint32_t box_bytes = (uint32_t)rows * C::kRow;
+  // byte of row `key` of a tile (first 128-byte piece); pieces are rows * 128 bytes apart
+  auto row_at = [&](int key) { return (uint32_t)(key >> rows_shift) * box_bytes + (uint32_t)(key & (rows - 1)) * 128u; };
+  const uint32_t piece = (uint32_t)rows * 128u;
+  // rows that this lane addresses in the fragment loads
+  const int krow = mt * 16 + (lane & 15);
+  const uint32_t kbase = row_at(krow), kswz = (uint32_t)(krow & 7);
+
+  uint32_t n = 0;
+  int b = cut.b, u = cut.u, t = cut.t;
+  for (int64_t w = cut.w0; w < cut.w1;) {
+    const Range r = range_of<T>(a, b);
+    const int tiles = (int)min((int64_t)(r.nt - t), cut.w1 - w);
+    int head0, nh, kvh;
+    unit_heads(a, u, head0, nh, kvh);
+
+    // q fragments of this warp's columns (head g of the unit), in parts
+    uint32_t qf[C::kQSteps][C::kParts][2];
+    float unscale0 = 1.0f, unscale1 = 1.0f;  // of heads 2 q4 and 2 q4 + 1
+    {
+      const float *qg = a.q + b * a.q_stride + (int64_t)(head0 + min(g, nh - 1)) * D + ks * (D / KS);
+      const bool real = g < nh;
+      if constexpr (TYPE == GQ_KV_F32) {
+#pragma unroll
+        for (int s = 0; s < C::kQSteps; ++s) {
+          const float x = real ? qg[s * 8 + q4] : 0.0f, y = real ? qg[s * 8 + q4 + 4] : 0.0f;
+          split_tf32(x, qf[s][0][0], qf[s][1][0]);
+          split_tf32(y, qf[s][0][1], qf[s][1][1]);
+        }
+      } else {
+        float2 v[C::kQSteps][2];
+        float top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < C::kQSteps; ++s) {
+          // e4m3: a thread's 4 bytes of a fragment are neighbours, so columns 4 q4 .. 4 q4 + 3
+          const int c0 = s * 16 + (TYPE == GQ_KV_E4M3 ? 4 * q4 : 2 * q4), c1 = c0 + (TYPE == GQ_KV_E4M3 ? 2 : 8);
+          v[s][0] = real ? *reinterpret_cast<const float2 *>(qg + c0) : make_float2(0.f, 0.f);
+          v[s][1] = real ? *reinterpret_cast<const float2 *>(qg + c1) : make_float2(0.f, 0.f);
+        }
+        if constexpr (TYPE != GQ_KV_BF16) {
+#pragma unroll
+          for (int s = 0; s < C::kQSteps; ++s)
+            top = fmaxf(top, fmaxf(fmaxf(fabsf(v[s][0].x), fabsf(v[s][0].y)), fmaxf(fabsf(v[s][1].x), fabsf(v[s][1].y))));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          // 2^e with top * 2^e in [2^13, 2^14); 1 where that has no answer
+          const int e = (int)((__float_as_uint(top) >> 23) & 255u);
+          const int up = e > 0 && e < 255 ? min(max(140 - e, -126), 126) : 0;
+          const float f = __uint_as_float((uint32_t)(127 + up) << 23), inv = __uint_as_float((uint32_t)(127 - up) << 23);
+          unscale0 = __shfl_sync(0xffffffffu, inv, q4 * 8);      // lane of head 2 q4: group 2 q4
+          unscale1 = __shfl_sync(0xffffffffu, inv, q4 * 8 + 4);
+#pragma unroll
+          for (int s = 0; s < C::kQSteps; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t part[2];
+              split_f16(v[s][i].x * f, v[s][i].y * f, part);
+              qf[s][0][i] = part[0];
+              qf[s][1][i] = part[1];
+            }
+        } else {
+#pragma unroll
+          for (int s = 0; s < C::kQSteps; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t part[3];
+              split_bf16(v[s][i].x, v[s][i].y, part);
+#pragma unroll
+              for (int p = 0; p < 3; ++p) qf[s][p % C::kParts][i] = part[p];
+            }
+        }
+      }
+    }
+    float acc[C::kMTiles][4];
+#pragma unroll
+    for (int i = 0; i < C::kMTiles; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[i][k] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+
+    for (int i = 0; i < tiles; ++i, n += 2) {
+      const int j0 = (r.tile0 + t + i) * T;
+      const int kslot = n % C::kSlots, vslot = (n + 1) % C::kSlots;
+      const uint32_t kpar = (n / C::kSlots) & 1, vpar = ((n + 1) / C::kSlots) & 1;
+      // ---- scores of 16 keys (and of this warp's columns)
+      wait_or_abort(&full[kslot], kpar, &abort_flag, a.err);
+      __syncwarp();
+      {
+        float c[3][4] = {};
+        const uint32_t at = ring_u + kslot * C::kSlot + kbase;
+#pragma unroll
+        for (int s = 0; s < (TYPE == GQ_KV_E4M3 ? C::kQSteps / 2 : C::kQSteps); ++s) {
+          uint32_t k4[4];
+          const int ch = ks * (C::kRow / KS / 16) + s * 2;  // 16-byte piece of the row (two per load)
+          ldsm4(k4, at + (uint32_t)(ch >> 3) * piece + ((((uint32_t)(ch & 7) + (lane >> 4)) ^ kswz) << 4));
+          if constexpr (TYPE == GQ_KV_F32) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) split_tf32(__uint_as_float(k4[x]), hi[x], lo[x]);
+            mma_tf32(c[0], hi, qf[s][0][0], qf[s][0][1]);
+            mma_tf32(c[1], hi, qf[s][1][0], qf[s][1][1]);
+            mma_tf32(c[2], lo, qf[s][0][0], qf[s][0][1]);
+          } else if constexpr (TYPE == GQ_KV_E4M3) {
+            const uint32_t a0[4] = {e4m3_pair(k4[0]), e4m3_pair(k4[1]), e4m3_pair(k4[0] >> 16), e4m3_pair(k4[1] >> 16)};
+            const uint32_t a1[4] = {e4m3_pair(k4[2]), e4m3_pair(k4[3]), e4m3_pair(k4[2] >> 16), e4m3_pair(k4[3] >> 16)};
+            mma_f16(c[0], a0, qf[2 * s][0][0], qf[2 * s][0][1]);
+            mma_f16(c[1], a0, qf[2 * s][1][0], qf[2 * s][1][1]);
+            mma_f16(c[0], a1, qf[2 * s + 1][0][0], qf[2 * s + 1][0][1]);
+            mma_f16(c[1], a1, qf[2 * s + 1][1][0], qf[2 * s + 1][1][1]);
+          } else if constexpr (TYPE == GQ_KV_F16) {
+            mma_f16(c[0], k4, qf[s][0][0], qf[s][0][1]);
+            mma_f16(c[1], k4, qf[s][1][0], qf[s][1][1]);
+          } else {
+#pragma unroll
+            for (int p = 0; p < C::kParts; ++p) mma_bf16(c[p], k4, qf[s][p][0], qf[s][p][1]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) gqt::mbar_arrive(&empty[kslot]);
+        float *to = sS + ks * kHeads * C::kSStride + 2 * q4 * C::kSStride + mt * 16 + g;
+        to[0] = (c[0][0] + (c[1][0] + c[2][0])) * unscale0;
+        to[C::kSStride] = (c[0][1] + (c[1][1] + c[2][1])) * unscale1;
+        to[8] = (c[0][2] + (c[1][2] + c[2][2])) * unscale0;
+        to[C::kSStride + 8] = (c[0][3] + (c[1][3] + c[2][3])) * unscale1;
+      }
+      sync_compute<kCompute>();
+
+      // ---- weights
+      const bool ragged = j0 < r.lo || j0 + T > r.hi;
+      {
+        float x[KPT], top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < KPT; ++k) {
+          const int key = sl * KPT + k;
+          float s = sS[sh * C::kSStride + key];
+#pragma unroll
+          for (int p = 1; p < KS; ++p) s += sS[(p * kHeads + sh) * C::kSStride + key];
+          s = score_log2(a, s);
+          x[k] = ragged && (j0 + key < r.lo || j0 + key >= r.hi) ? -INFINITY : s;
+          top = fmaxf(top, x[k]);
+        }
+#pragma unroll
+        for (int off = 8; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const float mn = fmaxf(m, top);
+        const float f = m == -INFINITY ? 0.0f : exp2f(m - mn);
+        // p = 2^(x - m), times 2^14 for the f16 parts (a common factor of every weight and sum)
+        const float base = TYPE == GQ_KV_F16 || TYPE == GQ_KV_E4M3 ? mn - 14.0f : mn;
+        float p[KPT];
+        l *= f;
+#pragma unroll
+        for (int k = 0; k < KPT; ++k) {
+          p[k] = x[k] == -INFINITY ? 0.0f : exp2f(x[k] - base);
+          l += p[k];
+        }
+        m = mn;
+        if (sl == 0) fix[sh] = f;
+        uint8_t *to = sP + sh * C::kPStride;
+        if constexpr (TYPE == GQ_KV_F32) {
+#pragma unroll
+          for (int k = 0; k < KPT; ++k) reinterpret_cast<float *>(to)[sl * KPT + k] = p[k];
+        } else {
+          static_assert(KPT % 2 == 0 || TYPE == GQ_KV_F32, "pairs of keys");
+#pragma unroll
+          for (int k = 0; k + 1 < KPT; k += 2) {
+            if constexpr (TYPE == GQ_KV_BF16) {
+              uint32_t part[3];
+              split_bf16(p[k], p[k + 1], part);
+#pragma unroll
+              for (int y = 0; y < 3; ++y)
+                *reinterpret_cast<uint32_t *>(to + y * kHeads * C::kPStride + (sl * KPT + k) * 2) = part[y];
+            } else {
+              uint32_t part[2];
+              split_f16(p[k], p[k + 1], part);
+#pragma unroll
+              for (int y = 0; y < 2; ++y)
+                *reinterpret_cast<uint32_t *>(to + y * kHeads * C::kPStride + (sl * KPT + k) * 2) = part[y];
+            }
+          }
+        }
+      }
+      wait_or_abort(&full[vslot], vpar, &abort_flag, a.err);
+      const uint32_t vat = ring_u + vslot * C::kSlot;
+      if (ragged) {
+        // rows that are not visible hold anything, NaN too, or an earlier tile: make them 0
+        for (int e = tid; e < T * C::kChunks * 8; e += kCompute) {
+          const int key = e / (C::kChunks * 8), ch = e - key * (C::kChunks * 8);
+          if (j0 + key >= r.lo && j0 + key < r.hi) continue;
+          *reinterpret_cast<uint4 *>(ring + vslot * C::kSlot + row_at(key) + (ch >> 3) * piece + (ch & 7) * 16) =
+              make_uint4(0, 0, 0, 0);
+        }
+        gqd::fence_proxy_async_smem();  // before the slot's next copy
+      }
+      sync_compute<kCompute>();
+
+      // ---- output columns warp * D/4 ..
+      {
+        const float f0 = fix[2 * q4], f1 = fix[2 * q4 + 1];
+#pragma unroll
+        for (int x = 0; x < C::kMTiles; ++x) {
+          acc[x][0] *= f0;
+          acc[x][1] *= f1;
+          acc[x][2] *= f0;
+          acc[x][3] *= f1;
+        }
+      }
+      const uint8_t *pg = sP + g * C::kPStride;
+#pragma unroll
+      for (int s = 0; s < T / C::kStep; ++s) {
+        if constexpr (TYPE == GQ_KV_F32) {
+          // the instruction's keys t, t + 4 are rows 2t, 2t + 1: four rows two apart lie on different banks
+          const float2 p = *reinterpret_cast<const float2 *>(pg + (s * 8 + 2 * q4) * 4);
+          uint32_t bh[2], bl[2];
+          split_tf32(p.x, bh[0], bl[0]);
+          split_tf32(p.y, bh[1], bl[1]);
+          const int k0 = s * 8 + 2 * q4;
+          const uint32_t r0 = vat + row_at(k0), r1 = vat + row_at(k0 + 1);
+          const uint32_t z0 = (uint32_t)(k0 & 7), z1 = (uint32_t)((k0 + 1) & 7);
+#pragma unroll
+          for (int x = 0; x < C::kMTiles; ++x) {
+            const int col = warp * (D / kComputeWarps) + x * 16 + g;  // and col + 8
+            const uint32_t c0 = (uint32_t)(col >> 2), c1 = c0 + 2, in = (uint32_t)(col & 3) * 4;
+            uint32_t hi[4], lo[4];
+            split_tf32(lds32(r0 + (c0 >> 3) * piece + (((c0 & 7) ^ z0) << 4) + in), hi[0], lo[0]);
+            split_tf32(lds32(r0 + (c1 >> 3) * piece + (((c1 & 7) ^ z0) << 4) + in), hi[1], lo[1]);
+            split_tf32(lds32(r1 + (c0 >> 3) * piece + (((c0 & 7) ^ z1) << 4) + in), hi[2], lo[2]);
+            split_tf32(lds32(r1 + (c1 >> 3) * piece + (((c1 & 7) ^ z1) << 4) + in), hi[3], lo[3]);
+            mma_tf32(acc[x], lo, bh[0], bh[1]);
+            mma_tf32(acc[x], hi, bl[0], bl[1]);
+            mma_tf32(acc[x], hi, bh[0], bh[1]);
+          }
+        } else {
+          uint32_t pf[C::kParts][2];
+#pragma unroll
+          for (int y = 0; y < C::kParts; ++y) {
+            pf[y][0] = *reinterpret_cast<const uint32_t *>(pg + y * kHeads * C::kPStride + (s * 16 + 2 * q4) * 2);
+            pf[y][1] = *reinterpret_cast<const uint32_t *>(pg + y * kHeads * C::kPStride + (s * 16 + 2 * q4 + 8) * 2);
+          }
+          if constexpr (TYPE == GQ_KV_E4M3) {
+            // two 16-column tiles per load: keys 0-7 and 8-15 of each. A transposed 8 x 8
+            // of byte pairs gives columns 2g and 2g + 1 of two keys: row g of the
+            // instruction is column 2g, row g + 8 column 2g + 1.
+            const int key = s * 16 + (lane & 15);
+            const uint32_t rb = vat + row_at(key), z = (uint32_t)(key & 7);
+#pragma unroll
+            for (int x = 0; x < C::kMTiles; x += 2) {
+              const uint32_t ch = (uint32_t)(warp * (D / kComputeWarps) / 16 + x + (lane >> 4));
+              uint32_t v4[4];
+              ldsm4_t(v4, rb + (ch >> 3) * piece + (((ch & 7) ^ z) << 4));
+#pragma unroll
+              for (int y = 0; y < 4; ++y) v4[y] = __byte_perm(v4[y], 0, 0x3120);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t af[4] = {e4m3_pair(v4[2 * h]), e4m3_pair(v4[2 * h] >> 16), e4m3_pair(v4[2 * h + 1]),
+                                        e4m3_pair(v4[2 * h + 1] >> 16)};
+                mma_f16(acc[x + h], af, pf[1][0], pf[1][1]);
+                mma_f16(acc[x + h], af, pf[0][0], pf[0][1]);
+              }
+            }
+          } else {
+            const int key = s * 16 + (lane & 7) + (lane >> 4) * 8;
+            const uint32_t rb = vat + row_at(key), z = (uint32_t)(key & 7);
+#pragma unroll
+            for (int x = 0; x < C::kMTiles; ++x) {
+              const uint32_t ch = (uint32_t)(warp * (D / kComputeWarps) / 8 + x * 2 + ((lane >> 3) & 1));
+              uint32_t v4[4];
+              ldsm4_t(v4, rb + (ch >> 3) * piece + (((ch & 7) ^ z) << 4));
+#pragma unroll
+              for (int y = C::kParts - 1; y >= 0; --y) {
+                if constexpr (TYPE == GQ_KV_BF16) mma_bf16(acc[x], v4, pf[y][0], pf[y][1]);
+                else mma_f16(acc[x], v4, pf[y][0], pf[y][1]);
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) gqt::mbar_arrive(&empty[vslot]);
+    }
+
+    // ---- the unit's output, or this CTA's part of it
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+    const bool whole = tiles == r.nt;
+    const int64_t s0 = w - t;
+    const int slot = whole ? 0 : slot_of(cut, blockIdx.x, s0);
+    if (sl == 0) {
+      sum[sh] = l;
+      if (!whole) {
+        a.part_ml[(slot * kHeads + sh) * 2] = m;
+        a.part_ml[(slot * kHeads + sh) * 2 + 1] = l;
+      }
+    }
+    sync_compute<kCompute>();
+    {
+      float *base = whole ? a.out + ((int64_t)b * a.hq + head0) * D : a.part_o + (int64_t)slot * kHeads * D;
+      const float f0 = whole ? inv_or_zero(sum[2 * q4]) * a.v_scale : 1.0f;
+      const float f1 = whole ? inv_or_zero(sum[2 * q4 + 1]) * a.v_scale : 1.0f;
+      const int most = whole ? nh : kHeads;
+#pragma unroll
+      for (int x = 0; x < C::kMTiles; ++x) {
+        const int col = warp * (D / kComputeWarps) + x * 16;
+        const int ca = TYPE == GQ_KV_E4M3 ? col + 2 * g : col + g, cb = TYPE == GQ_KV_E4M3 ? ca + 1 : ca + 8;
+        if (2 * q4 < most) {
+          base[(2 * q4) * D + ca] = acc[x][0] * f0;
+          base[(2 * q4) * D + cb] = acc[x][2] * f0;
+        }
+        if (2 * q4 + 1 < most) {
+          base[(2 * q4 + 1) * D + ca] = acc[x][1] * f1;
+          base[(2 * q4 + 1) * D + cb] = acc[x][3] * f1;
+        }
+      }
+    }
+    if (!whole) finish_part<kCompute>(a, cut, b, u, s0, r.nt);
+    w += tiles;
+    t = 0;
+    if (++u == a.units_per_req) {
+      u = 0;
+      ++b;
+    }
+  }
+}
+
+int log2_of(int64_t v) {
+  int s = 0;
+  while ((int64_t(1) << s) < v) ++s;
+  return s;
+}
+
+// A layer's pages as a 4-D tensor: 128-byte pieces of a row, rows of all heads of a
+// page, pieces of a row, pages. One copy brings `rows` rows whole, laid out piece by
+// piece with the 128-byte swizzle.
+int encode(gq_ctx *ctx, const gq_kv_pages *p, const void *base, int64_t page_stride, int rows, CUtensorMap *map) {
+  auto fn = gq_encode_fn();
+  if (!fn) return gq_fail(ctx, GQ_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled is not available");
+  const int size = gq_kv_size(p->type);
+  const int64_t row = p->head_dim * size;
+  const cuuint64_t dims[4] = {(cuuint64_t)(128 / size), (cuuint64_t)(p->heads * p->page_size), (cuuint64_t)(row / 128),
+                              (cuuint64_t)p->n_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)row, 128, (cuuint64_t)(page_stride * size)};
+  const cuuint32_t box[4] = {(cuuint32_t)(128 / size), (cuuint32_t)rows, (cuuint32_t)(row / 128), 1};
+  const cuuint32_t one[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type = size == 4   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : size == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  const CUresult e = fn(map, type, 4, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (e != CUDA_SUCCESS) return gq_fail(ctx, GQ_ERR_CUDA, "paged_attention: cuTensorMapEncodeTiled failed");
+  return GQ_OK;
+}
+
+template <int TYPE, int D>
+int launch(gq_ctx *ctx, const gq_kv_pages *p, Args &a) {
+  using C = Tile<TYPE, D>;
+  static bool attr_set[64] = {};
+  if (!attr_set[ctx->device & 63]) {
+    GQ_CUDA_TRY(ctx, cudaFuncSetAttribute(paged_tiles_kernel<TYPE, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+    attr_set[ctx->device & 63] = true;
+  }
+  a.page_shift = log2_of(p->page_size);
+  CUtensorMap kmap, vmap;
+  const int rows = (int)std::min<int64_t>(p->page_size, C::T);
+  int rc = encode(ctx, p, p->k, a.page_stride, rows, &kmap);
+  if (rc == GQ_OK) rc = encode(ctx, p, p->v, a.page_stride, rows, &vmap);
+  if (rc != GQ_OK) return rc;
+  const int grid = grid_for(a, C::T, 2 * ctx->num_sms);
+  rc = bind_workspace(ctx, grid, a);
+  if (rc != GQ_OK) return rc;
+  GQ_CUDA_TRY(ctx, gq_launch(ctx, paged_tiles_kernel<TYPE, D>, dim3(grid), dim3(kThreads), C::kSmem, a, kmap, vmap));
+  return GQ_OK;
+}
+
+template <int TYPE>
+int launch_dim(gq_ctx *ctx, const gq_kv_pages *p, Args &a) {
+  switch (p->head_dim) {
+    case 64:
+      if constexpr (TYPE != GQ_KV_E4M3) return launch<TYPE, 64>(ctx, p, a);
+      break;
+    case 128: return launch<TYPE, 128>(ctx, p, a);
+    case 256: return launch<TYPE, 256>(ctx, p, a);
+    case 512: return launch<TYPE, 512>(ctx, p, a);
+  }
+  return gq_fail(ctx, GQ_ERR_UNSUPPORTED, "paged_attention: no tiled kernel");
+}
+
+}  // namespace
+
+// Rows of whole 128-byte pieces at the instantiated head_dims, and pages that a tile is
+// a whole number of (or that are a whole number of tiles).
+bool gq_paged_attn_tc_supported(const gq_kv_pages *p, int64_t page_stride) {
+  const int size = gq_kv_size(p->type);
+  const int64_t d = p->head_dim;
+  return (d == 64 || d == 128 || d == 256 || d == 512) && d * size % 128 == 0 && p->page_size >= 8 &&
+         (p->page_size & (p->page_size - 1)) == 0 && page_stride * size % 16 == 0 &&
+         page_stride < (int64_t(1) << 36) && p->heads * p->page_size <= INT32_MAX && p->n_pages > 0;
+}
+
+int gq_paged_attn_tc_launch(gq_ctx *ctx, const gq_kv_pages *p, Args &a) {
+  switch (p->type) {
+    case GQ_KV_F32: return launch_dim<GQ_KV_F32>(ctx, p, a);
+    case GQ_KV_F16: return launch_dim<GQ_KV_F16>(ctx, p, a);
+    case GQ_KV_BF16: return launch_dim<GQ_KV_BF16>(ctx, p, a);
+    default: return launch_dim<GQ_KV_E4M3>(ctx, p, a);
+  }
+}
