@@ -59,7 +59,7 @@ struct gq_ctx {
   PeerDst peer_signal = {};
 };
 
-constexpr size_t kCtxCounters = 4096;
+constexpr size_t kCtxCounters = 16;
 
 struct gq_qweight {
   gq_ctx *ctx = nullptr;

@@ -64,9 +64,20 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const Args a) {
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
   const Cut cut = find_cut<kRowThreads, kRowTile>(a);
+  if (cut.w0 >= cut.w1) {
+    if (tid == 0) a.cut_units[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
   int b = cut.b, u = cut.u, t = cut.t;
-  for (int64_t w = cut.w0; w < cut.w1;) {
-    const Range r = range_of<kRowTile>(a, b);
+  for (int64_t w = cut.w0;;) {
+    const Range r = range_of<kRowTile>(a, visible(a, b));
+    if (t < 0) {  // the place ahead of the unit's tiles
+      t = 0;
+      if (++w == cut.w1) {  // its tiles are the next CTA's
+        if (tid == 0) a.cut_units[blockIdx.x] = make_int4(0, 0, 0, 0);
+        return;
+      }
+    }
     const int tiles = (int)min((int64_t)(r.nt - t), cut.w1 - w);
     int head0, nh, kvh;
     unit_heads(a, u, head0, nh, kvh);
@@ -168,7 +179,7 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const Args a) {
     for (int off = 8; off >= 1; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
     const bool whole = tiles == r.nt;
     const int64_t s0 = w - t;
-    const int slot = whole ? 0 : slot_of(cut, blockIdx.x, s0);
+    const int slot = whole ? 0 : slot_of(cut, s0);
     if (sl == 0) {
       sum[sh] = l;
       if (!whole) {
@@ -190,12 +201,133 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const Args a) {
         }
       }
     }
-    if (!whole) finish_part<kRowThreads>(a, cut, b, u, s0, r.nt);
     w += tiles;
-    t = 0;
+    if (w == cut.w1) {
+      if (tid == 0) put_cut_unit(a, cut, b, u, s0, r.nt);
+      return;
+    }
+    t = -1;
     if (++u == a.units_per_req) {
       u = 0;
       ++b;
+    }
+  }
+}
+
+// Adds up the parts of cut units. A CTA takes (unit, head, columns) in turn; its threads
+// are `wide` float4 columns times 256 / wide groups that share the parts, and the groups'
+// sums are added in order. wide is the most (up to a head's columns) that still gives
+// every CTA an item: many cut units of few parts are read in whole rows, a few long ones
+// by as many threads as there are. (Items of 128 columns for all: 11 us for 64 units of
+// 5 parts at head_dim 512.)
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinBatch = 8, kJoinNarrow = 8;
+
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Args a, int grid) {
+  constexpr int kEach = (kMaxGrid + kJoinThreads - 1) / kJoinThreads;
+  __shared__ int4 units[kMaxGrid];
+  __shared__ int counts[kJoinWarps];
+  __shared__ float4 sums[kJoinThreads];
+  __shared__ float2 group_ml[kJoinThreads / kJoinNarrow];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  gqd::griddep_wait();
+  gqd::griddep_launch_dependents();
+  // the list of cut units, in order of the CTAs they begin in
+  int4 mine[kEach];
+  int have = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int c = tid * kEach + i;
+    mine[i] = c < grid ? __ldcg(a.cut_units + c) : make_int4(0, 0, 0, 0);
+    have += mine[i].z > 0;
+  }
+  int incl = have;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 31) counts[warp] = incl;
+  __syncthreads();
+  int n = 0, at = incl - have;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    if (w < warp) at += counts[w];
+    n += counts[w];
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (mine[i].z > 0) units[at++] = mine[i];
+  __syncthreads();
+
+  const int cols = a.dim / 4;
+  int wide = kJoinThreads;
+  while (wide > kJoinNarrow && (wide >= 2 * cols || n * kHeads * ((cols + wide - 1) / wide) < (int)gridDim.x)) wide >>= 1;
+  const int groups = kJoinThreads / wide, group = tid / wide, slices = (cols + wide - 1) / wide, per_unit = kHeads * slices;
+  for (int item = blockIdx.x; item < n * per_unit; item += gridDim.x) {
+    const int4 unit = units[item / per_unit];
+    const int h = (item / slices) % kHeads, col = (item % slices) * wide + tid % wide;
+    int head0, nh, kvh;
+    unit_heads(a, unit.y, head0, nh, kvh);
+    if (h >= nh) continue;
+    const int parts = unit.z, first = unit.w, next = (first & ~1) + 2;  // slots: first, next, next + 2, ...
+    const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml);
+    const float4 *part = reinterpret_cast<const float4 *>(a.part_o);
+    // each group adds its parts to a maximum of its own, kJoinBatch parts' loads at a time
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = group; p0 < parts; p0 += groups * kJoinBatch) {
+      float2 x[kJoinBatch];
+      float4 v[kJoinBatch];
+#pragma unroll
+      for (int k = 0; k < kJoinBatch; ++k) {
+        const int p = p0 + k * groups;
+        x[k] = make_float2(-INFINITY, 0.0f);
+        v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p < parts) {
+          const int64_t s = (int64_t)(p == 0 ? first : next + 2 * (p - 1)) * kHeads + h;
+          x[k] = __ldcg(ml + s);
+          if (col < cols) v[k] = __ldcg(part + s * cols + col);
+        }
+      }
+      float top = m;
+#pragma unroll
+      for (int k = 0; k < kJoinBatch; ++k) top = fmaxf(top, x[k].x);
+      const float f = m == -INFINITY ? 0.0f : exp2f(m - top);
+      l *= f;
+      o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+#pragma unroll
+      for (int k = 0; k < kJoinBatch; ++k) {
+        const float w = x[k].x == -INFINITY ? 0.0f : exp2f(x[k].x - top);
+        l = fmaf(w, x[k].y, l);
+        o.x = fmaf(w, v[k].x, o.x);
+        o.y = fmaf(w, v[k].y, o.y);
+        o.z = fmaf(w, v[k].z, o.z);
+        o.w = fmaf(w, v[k].w, o.w);
+      }
+      m = top;
+    }
+    __syncthreads();  // the sums of the item before are read
+    sums[tid] = o;
+    if (tid % wide == 0) group_ml[group] = make_float2(m, l);
+    __syncthreads();
+    if (group == 0 && col < cols) {
+      m = -INFINITY;
+      for (int k = 0; k < groups; ++k) m = fmaxf(m, group_ml[k].x);
+      l = 0.0f;
+      o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < groups; ++k) {
+        const float2 x = group_ml[k];
+        const float4 v = sums[k * wide + tid];
+        const float f = x.x == -INFINITY ? 0.0f : exp2f(x.x - m);
+        l = fmaf(f, x.y, l);
+        o.x = fmaf(f, v.x, o.x);
+        o.y = fmaf(f, v.y, o.y);
+        o.z = fmaf(f, v.z, o.z);
+        o.w = fmaf(f, v.w, o.w);
+      }
+      const float s = inv_or_zero(l) * a.v_scale;
+      *reinterpret_cast<float4 *>(a.out + ((int64_t)unit.x * a.hq + head0 + h) * a.dim + col * 4) =
+          make_float4(o.x * s, o.y * s, o.z * s, o.w * s);
     }
   }
 }
@@ -206,6 +338,15 @@ cudaError_t rows_launch(gq_ctx *ctx, int grid, const Args &a) {
 }
 
 }  // namespace
+
+int gq_paged_join_launch(gq_ctx *ctx, const Args &a, int grid) {
+  if (grid <= 1) return GQ_OK;  // nothing can be cut
+  // two CTAs per SM, fewer where even the narrowest items of all possible cuts are fewer
+  const int64_t most = (int64_t)(grid - 1) * kHeads * ((a.dim / 4 + kJoinNarrow - 1) / kJoinNarrow);
+  const int items = (int)std::min<int64_t>(most, 2 * (int64_t)ctx->num_sms);
+  GQ_CUDA_TRY(ctx, gq_launch(ctx, paged_join_kernel, dim3(items), dim3(kJoinThreads), 0, a, grid));
+  return GQ_OK;
+}
 
 extern "C" int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const float *q, int64_t batch, int64_t hq,
                                   int64_t q_tok_stride, const int32_t *block_table, int64_t table_stride,
@@ -251,7 +392,6 @@ extern "C" int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const f
   a.scale = scale * pages->k_scale;
   a.softcap = attn_softcap;
   a.v_scale = pages->v_scale;
-  a.ctr = ctx->counters + kCtrBase;
   a.err = ctx->dev_err;
   if (gq_paged_attn_tc_supported(pages, a.page_stride)) return gq_paged_attn_tc_launch(ctx, pages, a);
   const int grid = grid_for(a, kRowTile, 4 * ctx->num_sms);
@@ -263,5 +403,5 @@ extern "C" int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const f
     case GQ_KV_BF16: GQ_CUDA_TRY(ctx, rows_launch<GQ_KV_BF16>(ctx, grid, a)); break;
     default: GQ_CUDA_TRY(ctx, rows_launch<GQ_KV_E4M3>(ctx, grid, a)); break;
   }
-  return GQ_OK;
+  return gq_paged_join_launch(ctx, a, grid);
 }

@@ -9,11 +9,11 @@
 //
 // Joining: softmax over a cut unit needs each part's maximum m, sum l and unnormalised
 // output o: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, m = max m_i. Parts go
-// to a workspace slot; the last CTA of a group of about sqrt(n) parts to arrive joins
-// the group, the last group joins the groups, always in part order, so the result does
-// not depend on who came last. Two levels because one CTA reads about 100 GB/s: the
-// 296 parts of one long request (8 KB each at head_dim 256) would take it 24 us, two
-// levels of 17 take 3.
+// to workspace slots and the second launch of the call, paged_join_kernel, adds them up
+// in part order, whichever CTA made them (results do not vary from run to run). A join
+// inside the first launch, by the last CTA to arrive, was measured slower: one CTA reads
+// its parts at some 15-100 GB/s, so the 99 parts of a 131072-key request (16 KB each)
+// kept it 40 us after the last key; the join kernel spreads them over the GPU.
 #pragma once
 
 #include <algorithm>
@@ -23,12 +23,7 @@
 namespace pattn {
 
 constexpr int kHeads = 8;       // query heads per unit
-constexpr int kMaxGrid = 1000;  // 4 counters per CTA
-constexpr int kCtrBase = 64;    // (paged.cu uses the counters below)
-constexpr int kOneLevel = 8;    // up to this many parts are joined at once
-constexpr int kMaxJoin = 32;    // >= ceil(sqrt(kMaxGrid))
-static_assert(kCtrBase + 4 * kMaxGrid <= (int)kCtxCounters, "counters");
-static_assert(kMaxJoin * kMaxJoin >= kMaxGrid, "two levels must reach every part");
+constexpr int kMaxGrid = 640;
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -43,7 +38,8 @@ struct Args {
   int32_t window;
   float scale, softcap, v_scale;  // scale: of the scores, the keys' scale included
   float *part_o, *part_ml;        // [2 grid][8][dim], [2 grid][8][2]
-  uint32_t *ctr, *err;
+  int4 *cut_units;                // [grid]: the cut unit that begins in a CTA: request, unit, parts (0: none), first slot
+  uint32_t *err;
 };
 
 struct Range {
@@ -56,38 +52,50 @@ __device__ __forceinline__ int visible(const Args &a, int b) {
   return (int)min(len, room);
 }
 template <int T>
-__device__ __forceinline__ Range range_of(const Args &a, int b) {
+__device__ __forceinline__ Range range_of(const Args &a, int keys) {
   Range r;
-  r.hi = visible(a, b);
+  r.hi = keys;
   r.lo = a.window > 0 && r.hi > a.window ? r.hi - a.window : 0;
   r.tile0 = r.lo / T;
   r.nt = max(1, (int)(((uint32_t)r.hi + T - 1) / T) - r.tile0);
   return r;
 }
 
-// This CTA's piece [w0, w1) of all tiles, and the unit and tile w0 lies in. The grid may
-// be larger than the work: CTAs at or past `grid` have none.
+__device__ __forceinline__ int64_t div_of(int64_t x, int64_t y) {  // x, y >= 0; the short division where it will do
+  return ((x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
+}
+
+// This CTA's piece [w0, w1) of all places, and the unit and tile w0 lies in (a unit is nt
+// + 1 places: t = -1 is the place ahead of its tiles). The first
+// `more` of `grid` pieces hold each + 1 tiles, the others each. (The grid may be larger
+// than the work: CTAs past `grid` have none.)
 struct Cut {
-  int64_t total, w0, w1;
-  int grid, b, u, t;  // request, unit of the request, tile of the unit
-  __device__ __forceinline__ int64_t start(int c) const { return c * total / grid; }
-  // the CTA whose piece holds tile w
-  __device__ __forceinline__ int at(int64_t w) const { return (int)(((w + 1) * grid - 1) / total); }
+  int64_t total, each, w0, w1;
+  int grid, more;
+  int b, u, t, keys;  // request, unit of the request, tile of the unit; the request's keys
+  __device__ __forceinline__ int64_t start(int c) const { return c * each + min(c, more); }
+  // the CTA whose piece holds place w
+  __device__ __forceinline__ int at(int64_t w) const {
+    const int64_t big = more * (each + 1);
+    return (int)(w < big ? div_of(w, each + 1) : more + div_of(w - big, each));
+  }
 };
 
 // Threads 0 .. NT - 1 (a whole block) take neighbouring requests each.
 template <int NT, int T>
 __device__ __forceinline__ Cut find_cut(const Args &a) {
   __shared__ int64_t sums[NT / 32];
-  __shared__ int found[3];
+  __shared__ int found[4];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.batch + NT - 1) / NT;
   const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
   int64_t mine = 0;
   bool past = false;
   for (int b = b0; b < b1; ++b) {
-    mine += (int64_t)range_of<T>(a, b).nt * a.units_per_req;
-    past |= a.lens[b] > a.table_stride * a.page_size;
+    const int len = a.lens[b];
+    const int64_t room = a.table_stride * a.page_size;
+    mine += (int64_t)(range_of<T>(a, (int)min((int64_t)max(len, 0), room)).nt + 1) * a.units_per_req;
+    past |= len > room;
   }
   if (past && blockIdx.x == 0) gqd::report(a.err, GQ_DEVERR_PAGES);
   int64_t incl = mine;
@@ -106,18 +114,22 @@ __device__ __forceinline__ Cut find_cut(const Args &a) {
     cut.total += sums[w];
   }
   cut.grid = (int)min((int64_t)gridDim.x, cut.total);
+  cut.each = div_of(cut.total, cut.grid);
+  cut.more = (int)(cut.total - cut.each * cut.grid);
   const int c = blockIdx.x;
   cut.w0 = c < cut.grid ? cut.start(c) : cut.total;
   cut.w1 = c < cut.grid ? cut.start(c + 1) : cut.total;
   if (cut.w0 >= incl - mine && cut.w0 < incl) {
     int64_t at = incl - mine;
     for (int b = b0; b < b1; ++b) {
-      const int nt = range_of<T>(a, b).nt;
-      const int64_t next = at + (int64_t)nt * a.units_per_req;
+      const int keys = visible(a, b), places = range_of<T>(a, keys).nt + 1;
+      const int64_t next = at + (int64_t)places * a.units_per_req;
       if (cut.w0 < next) {
+        const int u = (int)div_of(cut.w0 - at, places);
         found[0] = b;
-        found[1] = (int)((cut.w0 - at) / nt);
-        found[2] = (int)((cut.w0 - at) % nt);
+        found[1] = u;
+        found[2] = (int)(cut.w0 - at - (int64_t)u * places) - 1;
+        found[3] = keys;
         break;
       }
       at = next;
@@ -127,6 +139,7 @@ __device__ __forceinline__ Cut find_cut(const Args &a) {
   cut.b = found[0];
   cut.u = found[1];
   cut.t = found[2];
+  cut.keys = found[3];
   return cut;
 }
 
@@ -144,99 +157,19 @@ __device__ __forceinline__ void sync_compute() {
   asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
 }
 
-// Join `n` parts (part i in slot slots(i)) and hand each (head, 4 columns) sum with its
-// maximum and sum of weights to `put`.
-template <int NT, typename Slots, typename Put>
-__device__ __forceinline__ void join(const Args &a, int n, Slots slots, Put put) {
-  __shared__ float wgt[kMaxJoin][kHeads];
-  __shared__ float ms[kHeads], ls[kHeads];
-  const int tid = threadIdx.x;
-  for (int i = tid; i < n * kHeads; i += NT) wgt[i / kHeads][i % kHeads] = __ldcg(a.part_ml + (slots(i / kHeads) * kHeads + i % kHeads) * 2);
-  sync_compute<NT>();
-  if (tid < kHeads) {
-    float m = -INFINITY, l = 0.0f;
-    for (int i = 0; i < n; ++i) m = fmaxf(m, wgt[i][tid]);
-    for (int i = 0; i < n; ++i) {
-      const float mi = wgt[i][tid];
-      const float w = mi == -INFINITY ? 0.0f : exp2f(mi - m);
-      l = fmaf(w, __ldcg(a.part_ml + (slots(i) * kHeads + tid) * 2 + 1), l);
-      wgt[i][tid] = w;
-    }
-    ms[tid] = m;
-    ls[tid] = l;
-  }
-  sync_compute<NT>();
-  const int per = a.dim / 4;
-  for (int i = tid; i < kHeads * per; i += NT) {
-    const int h = i / per, c = (i - h * per) * 4;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int p = 0; p < n; ++p) {
-      const float w = wgt[p][h];
-      const float4 x = __ldcg(reinterpret_cast<const float4 *>(a.part_o + ((int64_t)slots(p) * kHeads + h) * a.dim + c));
-      o.x = fmaf(w, x.x, o.x);
-      o.y = fmaf(w, x.y, o.y);
-      o.z = fmaf(w, x.z, o.z);
-      o.w = fmaf(w, x.w, o.w);
-    }
-    put(h, c, o, ms[h], ls[h]);
-  }
-}
-
-// True in every thread of the CTA that arrives last of n at the counter.
-template <int NT>
-__device__ __forceinline__ bool arrive_last(uint32_t *ctr, int n) {
-  __shared__ int last;
-  sync_compute<NT>();
-  if (threadIdx.x == 0) {
-    __threadfence();
-    last = atomicAdd(ctr, 1u) == (uint32_t)n - 1;
-    if (last) {
-      *ctr = 0u;
-      __threadfence();
-    }
-  }
-  sync_compute<NT>();
-  return last != 0;
-}
-
 __device__ __forceinline__ float inv_or_zero(float l) { return l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l); }
 
-// Slot of CTA c's part of the unit that starts at tile s0: a CTA has at most two parts
-// of cut units, the one it begins in the middle of (or begins with) and its last.
-__device__ __forceinline__ int slot_of(const Cut &cut, int c, int64_t s0) { return 2 * c + (cut.start(c) < s0 ? 1 : 0); }
+// Slot of this CTA's part of a cut unit whose first tile is at place s0: a CTA has at most
+// two parts of cut units, the one it begins in the middle of (or begins with) and its last.
+__device__ __forceinline__ int slot_of(const Cut &cut, int64_t s0) { return 2 * blockIdx.x + (cut.w0 < s0 ? 1 : 0); }
 
-// The NT computing threads of CTA blockIdx.x, after its part of unit (b, u) (tiles s0 .. s0 + nt of
-// the whole row of tiles) is in its slot: join when this CTA is the last.
-template <int NT>
-__device__ __forceinline__ void finish_part(const Args &a, const Cut &cut, int b, int u, int64_t s0, int nt) {
-  const int c0 = cut.at(s0), n = cut.at(s0 + nt - 1) - c0 + 1;
-  const int g = n > kOneLevel ? (int)ceilf(sqrtf((float)n)) : n;
-  const int groups = (n + g - 1) / g, j = ((int)blockIdx.x - c0) / g;
-  const int first = c0 + j * g, members = min(g, n - j * g);
-  if (!arrive_last<NT>(a.ctr + 2 * slot_of(cut, first, s0), members)) return;
-  if (groups > 1) {
-    const int to = slot_of(cut, first, s0);
-    // the sums replace the group's first part, column by column where that was just read
-    join<NT>(a, members, [&](int i) { return slot_of(cut, first + i, s0); },
-             [&](int h, int c, float4 o, float m, float l) {
-               *reinterpret_cast<float4 *>(a.part_o + ((int64_t)to * kHeads + h) * a.dim + c) = o;
-               if (c == 0) {
-                 a.part_ml[(to * kHeads + h) * 2] = m;
-                 a.part_ml[(to * kHeads + h) * 2 + 1] = l;
-               }
-             });
-    if (!arrive_last<NT>(a.ctr + 2 * slot_of(cut, c0, s0) + 1, groups)) return;
-  }
-  int head0, nh, kv;
-  unit_heads(a, u, head0, nh, kv);
-  float *out = a.out + ((int64_t)b * a.hq + head0) * a.dim;
-  join<NT>(a, groups > 1 ? groups : n, [&](int i) { return slot_of(cut, c0 + (groups > 1 ? i * g : i), s0); },
-           [&](int h, int c, float4 o, float, float l) {
-             if (h >= nh) return;
-             const float s = inv_or_zero(l) * a.v_scale;
-             *reinterpret_cast<float4 *>(out + (int64_t)h * a.dim + c) = make_float4(o.x * s, o.y * s, o.z * s, o.w * s);
-           });
+// One thread of each CTA says which cut unit's first tile is in it (nt tiles from place
+// s0 on), or that none is. The unit's other parts are in the slots 2 c of the
+// CTAs that follow.
+__device__ __forceinline__ void put_cut_unit(const Args &a, const Cut &cut, int b, int u, int64_t s0, int nt) {
+  const bool begins = cut.w0 <= s0 && s0 < cut.w1 && s0 + nt > cut.w1;
+  const int parts = begins ? cut.at(s0 + nt - 1) - (int)blockIdx.x + 1 : 0;
+  a.cut_units[blockIdx.x] = make_int4(b, u, parts, slot_of(cut, s0));
 }
 
 // Score of one visible key in units of log2: the scaled, optionally capped product.
@@ -257,13 +190,17 @@ inline int grid_for(const Args &a, int tile, int most) {
   return (int)std::min<int64_t>(tiles, std::min(kMaxGrid, most));
 }
 
-// Workspace for the parts: two per CTA.
+// Workspace for the parts: two per CTA, and the list of cut units.
 inline int bind_workspace(gq_ctx *ctx, int grid, Args &a) {
   void *ws = nullptr;
-  const int rc = gq_workspace(ctx, (size_t)grid * 2 * kHeads * (a.dim + 2) * 4, &ws);
-  a.part_o = static_cast<float *>(ws);
+  const int rc = gq_workspace(ctx, (size_t)grid * (2 * kHeads * (a.dim + 2) * 4 + sizeof(int4)), &ws);
+  a.cut_units = static_cast<int4 *>(ws);
+  a.part_o = reinterpret_cast<float *>(a.cut_units + grid);
   a.part_ml = a.part_o + (size_t)grid * 2 * kHeads * a.dim;
   return rc;
 }
 
 }  // namespace pattn
+
+// The second launch: joins the units that the first one (of `grid` CTAs) cut.
+int gq_paged_join_launch(gq_ctx *ctx, const pattn::Args &a, int grid);

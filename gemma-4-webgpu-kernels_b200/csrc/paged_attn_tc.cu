@@ -65,17 +65,17 @@ __device__ __forceinline__ float lds32(uint32_t addr) {
   return v;
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -168,7 +168,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
   const Cut cut = find_cut<kThreads, T>(a);  // (its barriers also publish the mbarriers)
-  if (cut.w0 >= cut.w1) return;
+  if (cut.w0 >= cut.w1) {
+    if (tid == 0) a.cut_units[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
   const int rows_shift = min(a.page_shift, T == 64 ? 6 : T == 32 ? 5 : 4);  // log2 of the keys one copy brings
   const int rows = 1 << rows_shift;
 
@@ -177,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     // read before this tile's slots are waited for
     const int boxes = T >> rows_shift;
     int b = cut.b, u = cut.u, t = cut.t;
-    Range r = range_of<T>(a, b);
+    Range r = range_of<T>(a, cut.keys);
     auto entry = [&](int j0) -> int {  // page of this lane's copy, -1: nothing to load
       const int j = j0 + (lane << rows_shift);
       if (lane >= boxes || j >= r.hi || j + rows <= r.lo) return -1;
@@ -186,19 +189,27 @@ __global__ void __launch_bounds__(kThreads, 2)
       gqd::report(a.err, GQ_DEVERR_PAGES);
       return (int)a.n_pages;  // out of the tensor's bounds: reads as zeros
     };
-    int j0 = (r.tile0 + t) * T, page = entry(j0);
+    int64_t w = cut.w0;
+    if (t < 0) {
+      t = 0;
+      ++w;
+    }
+    int j0 = (r.tile0 + t) * T, page = w < cut.w1 ? entry(j0) : -1;
     uint32_t n = 0;  // ring position
-    for (int64_t w = cut.w0; w < cut.w1; ++w) {
+    while (w < cut.w1) {
       const int load = page, jj = j0 + (lane << rows_shift), kvh = u / a.sub;
-      if (w + 1 < cut.w1) {
-        if (++t == r.nt) {
-          t = 0;
+      ++w;
+      if (++t == r.nt) {
+        t = 0;
+        ++w;
+        if (w < cut.w1) {
           if (++u == a.units_per_req) {
             u = 0;
-            ++b;
-            r = range_of<T>(a, b);
+            r = range_of<T>(a, visible(a, ++b));
           }
         }
+      }
+      if (w < cut.w1) {
         j0 = (r.tile0 + t) * T;
         page = entry(j0);
       }
@@ -237,9 +248,16 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t kbase = row_at(krow), kswz = (uint32_t)(krow & 7);
 
   uint32_t n = 0;
-  int b = cut.b, u = cut.u, t = cut.t;
-  for (int64_t w = cut.w0; w < cut.w1;) {
-    const Range r = range_of<T>(a, b);
+  int b = cut.b, u = cut.u, t = cut.t, keys = cut.keys;
+  for (int64_t w = cut.w0;;) {
+    const Range r = range_of<T>(a, keys);
+    if (t < 0) {  // the place ahead of the unit's tiles
+      t = 0;
+      if (++w == cut.w1) {  // its tiles are the next CTA's
+        if (tid == 0) a.cut_units[blockIdx.x] = make_int4(0, 0, 0, 0);
+        break;
+      }
+    }
     const int tiles = (int)min((int64_t)(r.nt - t), cut.w1 - w);
     int head0, nh, kvh;
     unit_heads(a, u, head0, nh, kvh);
@@ -422,84 +440,102 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       sync_compute<kCompute>();
 
-      // ---- output columns warp * D/4 ..
+      // ---- output columns warp * D/4 ..: o = o 2^(m_old - m) + V^T p. The instruction
+      // truncates its sums, so it adds up one tile only; tiles are added in registers.
       {
         const float f0 = fix[2 * q4], f1 = fix[2 * q4 + 1];
+        const uint8_t *pg = sP + g * C::kPStride;
+        constexpr int kSteps = T / C::kStep;
+        uint32_t pf[kSteps][C::kParts][2];
 #pragma unroll
-        for (int x = 0; x < C::kMTiles; ++x) {
-          acc[x][0] *= f0;
-          acc[x][1] *= f1;
-          acc[x][2] *= f0;
-          acc[x][3] *= f1;
-        }
-      }
-      const uint8_t *pg = sP + g * C::kPStride;
-#pragma unroll
-      for (int s = 0; s < T / C::kStep; ++s) {
-        if constexpr (TYPE == GQ_KV_F32) {
-          // the instruction's keys t, t + 4 are rows 2t, 2t + 1: four rows two apart lie on different banks
-          const float2 p = *reinterpret_cast<const float2 *>(pg + (s * 8 + 2 * q4) * 4);
-          uint32_t bh[2], bl[2];
-          split_tf32(p.x, bh[0], bl[0]);
-          split_tf32(p.y, bh[1], bl[1]);
-          const int k0 = s * 8 + 2 * q4;
-          const uint32_t r0 = vat + row_at(k0), r1 = vat + row_at(k0 + 1);
-          const uint32_t z0 = (uint32_t)(k0 & 7), z1 = (uint32_t)((k0 + 1) & 7);
-#pragma unroll
-          for (int x = 0; x < C::kMTiles; ++x) {
-            const int col = warp * (D / kComputeWarps) + x * 16 + g;  // and col + 8
-            const uint32_t c0 = (uint32_t)(col >> 2), c1 = c0 + 2, in = (uint32_t)(col & 3) * 4;
-            uint32_t hi[4], lo[4];
-            split_tf32(lds32(r0 + (c0 >> 3) * piece + (((c0 & 7) ^ z0) << 4) + in), hi[0], lo[0]);
-            split_tf32(lds32(r0 + (c1 >> 3) * piece + (((c1 & 7) ^ z0) << 4) + in), hi[1], lo[1]);
-            split_tf32(lds32(r1 + (c0 >> 3) * piece + (((c0 & 7) ^ z1) << 4) + in), hi[2], lo[2]);
-            split_tf32(lds32(r1 + (c1 >> 3) * piece + (((c1 & 7) ^ z1) << 4) + in), hi[3], lo[3]);
-            mma_tf32(acc[x], lo, bh[0], bh[1]);
-            mma_tf32(acc[x], hi, bl[0], bl[1]);
-            mma_tf32(acc[x], hi, bh[0], bh[1]);
-          }
-        } else {
-          uint32_t pf[C::kParts][2];
-#pragma unroll
-          for (int y = 0; y < C::kParts; ++y) {
-            pf[y][0] = *reinterpret_cast<const uint32_t *>(pg + y * kHeads * C::kPStride + (s * 16 + 2 * q4) * 2);
-            pf[y][1] = *reinterpret_cast<const uint32_t *>(pg + y * kHeads * C::kPStride + (s * 16 + 2 * q4 + 8) * 2);
-          }
-          if constexpr (TYPE == GQ_KV_E4M3) {
-            // two 16-column tiles per load: keys 0-7 and 8-15 of each. A transposed 8 x 8
-            // of byte pairs gives columns 2g and 2g + 1 of two keys: row g of the
-            // instruction is column 2g, row g + 8 column 2g + 1.
-            const int key = s * 16 + (lane & 15);
-            const uint32_t rb = vat + row_at(key), z = (uint32_t)(key & 7);
-#pragma unroll
-            for (int x = 0; x < C::kMTiles; x += 2) {
-              const uint32_t ch = (uint32_t)(warp * (D / kComputeWarps) / 16 + x + (lane >> 4));
-              uint32_t v4[4];
-              ldsm4_t(v4, rb + (ch >> 3) * piece + (((ch & 7) ^ z) << 4));
-#pragma unroll
-              for (int y = 0; y < 4; ++y) v4[y] = __byte_perm(v4[y], 0, 0x3120);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t af[4] = {e4m3_pair(v4[2 * h]), e4m3_pair(v4[2 * h] >> 16), e4m3_pair(v4[2 * h + 1]),
-                                        e4m3_pair(v4[2 * h + 1] >> 16)};
-                mma_f16(acc[x + h], af, pf[1][0], pf[1][1]);
-                mma_f16(acc[x + h], af, pf[0][0], pf[0][1]);
-              }
-            }
+        for (int s = 0; s < kSteps; ++s) {
+          if constexpr (TYPE == GQ_KV_F32) {
+            const float2 p = *reinterpret_cast<const float2 *>(pg + (s * 8 + 2 * q4) * 4);
+            split_tf32(p.x, pf[s][0][0], pf[s][1][0]);
+            split_tf32(p.y, pf[s][0][1], pf[s][1][1]);
           } else {
-            const int key = s * 16 + (lane & 7) + (lane >> 4) * 8;
-            const uint32_t rb = vat + row_at(key), z = (uint32_t)(key & 7);
 #pragma unroll
-            for (int x = 0; x < C::kMTiles; ++x) {
-              const uint32_t ch = (uint32_t)(warp * (D / kComputeWarps) / 8 + x * 2 + ((lane >> 3) & 1));
-              uint32_t v4[4];
-              ldsm4_t(v4, rb + (ch >> 3) * piece + (((ch & 7) ^ z) << 4));
-#pragma unroll
-              for (int y = C::kParts - 1; y >= 0; --y) {
-                if constexpr (TYPE == GQ_KV_BF16) mma_bf16(acc[x], v4, pf[y][0], pf[y][1]);
-                else mma_f16(acc[x], v4, pf[y][0], pf[y][1]);
-              }
+            for (int y = 0; y < C::kParts; ++y) {
+              pf[s][y][0] = *reinterpret_cast<const uint32_t *>(pg + y * kHeads * C::kPStride + (s * 16 + 2 * q4) * 2);
+              pf[s][y][1] = *reinterpret_cast<const uint32_t *>(pg + y * kHeads * C::kPStride + (s * 16 + 2 * q4 + 8) * 2);
             }
+          }
+        }
+        // columns in groups of G 16-column tiles: their sums are independent, which hides
+        // the instruction's latency
+        constexpr int G = std::min(C::kMTiles, 4);
+#pragma unroll
+        for (int x0 = 0; x0 < C::kMTiles; x0 += G) {
+          float c[G][4] = {};
+#pragma unroll
+          for (int s = 0; s < kSteps; ++s) {
+            if constexpr (TYPE == GQ_KV_F32) {
+              // the instruction's keys t, t + 4 are rows 2t, 2t + 1: four rows two apart lie on different banks
+              const int k0 = s * 8 + 2 * q4;
+              const uint32_t r0 = vat + row_at(k0), r1 = vat + row_at(k0 + 1);
+              const uint32_t z0 = (uint32_t)(k0 & 7), z1 = (uint32_t)((k0 + 1) & 7);
+#pragma unroll
+              for (int x = 0; x < G; ++x) {
+                const int col = warp * (D / kComputeWarps) + (x0 + x) * 16 + g;  // and col + 8
+                const uint32_t c0 = (uint32_t)(col >> 2), c1 = c0 + 2, in = (uint32_t)(col & 3) * 4;
+                uint32_t hi[4], lo[4];
+                split_tf32(lds32(r0 + (c0 >> 3) * piece + (((c0 & 7) ^ z0) << 4) + in), hi[0], lo[0]);
+                split_tf32(lds32(r0 + (c1 >> 3) * piece + (((c1 & 7) ^ z0) << 4) + in), hi[1], lo[1]);
+                split_tf32(lds32(r1 + (c0 >> 3) * piece + (((c0 & 7) ^ z1) << 4) + in), hi[2], lo[2]);
+                split_tf32(lds32(r1 + (c1 >> 3) * piece + (((c1 & 7) ^ z1) << 4) + in), hi[3], lo[3]);
+                mma_tf32(c[x], lo, pf[s][0][0], pf[s][0][1]);
+                mma_tf32(c[x], hi, pf[s][1][0], pf[s][1][1]);
+                mma_tf32(c[x], hi, pf[s][0][0], pf[s][0][1]);
+              }
+            } else if constexpr (TYPE == GQ_KV_E4M3) {
+              // two 16-column tiles per load: keys 0-7 and 8-15 of each. A transposed 8 x 8
+              // of byte pairs gives columns 2g and 2g + 1 of two keys: row g of the
+              // instruction is column 2g, row g + 8 column 2g + 1.
+              const int key = s * 16 + (lane & 15);
+              const uint32_t rb = vat + row_at(key), z = (uint32_t)(key & 7);
+              uint32_t af[G][4];
+#pragma unroll
+              for (int x = 0; x < G; x += 2) {
+                const uint32_t ch = (uint32_t)(warp * (D / kComputeWarps) / 16 + x0 + x + (lane >> 4));
+                uint32_t v4[4];
+                ldsm4_t(v4, rb + (ch >> 3) * piece + (((ch & 7) ^ z) << 4));
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const uint32_t e = __byte_perm(v4[2 * h], 0, 0x3120), f = __byte_perm(v4[2 * h + 1], 0, 0x3120);
+                  af[x + h][0] = e4m3_pair(e);
+                  af[x + h][1] = e4m3_pair(e >> 16);
+                  af[x + h][2] = e4m3_pair(f);
+                  af[x + h][3] = e4m3_pair(f >> 16);
+                }
+              }
+#pragma unroll
+              for (int y = C::kParts - 1; y >= 0; --y)
+#pragma unroll
+                for (int x = 0; x < G; ++x) mma_f16(c[x], af[x], pf[s][y][0], pf[s][y][1]);
+            } else {
+              const int key = s * 16 + (lane & 7) + (lane >> 4) * 8;
+              const uint32_t rb = vat + row_at(key), z = (uint32_t)(key & 7);
+              uint32_t v4[G][4];
+#pragma unroll
+              for (int x = 0; x < G; ++x) {
+                const uint32_t ch = (uint32_t)(warp * (D / kComputeWarps) / 8 + (x0 + x) * 2 + ((lane >> 3) & 1));
+                ldsm4_t(v4[x], rb + (ch >> 3) * piece + (((ch & 7) ^ z) << 4));
+              }
+#pragma unroll
+              for (int y = C::kParts - 1; y >= 0; --y)
+#pragma unroll
+                for (int x = 0; x < G; ++x) {
+                  if constexpr (TYPE == GQ_KV_BF16) mma_bf16(c[x], v4[x], pf[s][y][0], pf[s][y][1]);
+                  else mma_f16(c[x], v4[x], pf[s][y][0], pf[s][y][1]);
+                }
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < G; ++x) {
+            acc[x0 + x][0] = fmaf(acc[x0 + x][0], f0, c[x][0]);
+            acc[x0 + x][1] = fmaf(acc[x0 + x][1], f1, c[x][1]);
+            acc[x0 + x][2] = fmaf(acc[x0 + x][2], f0, c[x][2]);
+            acc[x0 + x][3] = fmaf(acc[x0 + x][3], f1, c[x][3]);
           }
         }
       }
@@ -512,7 +548,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     for (int off = 8; off >= 1; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
     const bool whole = tiles == r.nt;
     const int64_t s0 = w - t;
-    const int slot = whole ? 0 : slot_of(cut, blockIdx.x, s0);
+    const int slot = whole ? 0 : slot_of(cut, s0);
     if (sl == 0) {
       sum[sh] = l;
       if (!whole) {
@@ -540,12 +576,15 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       }
     }
-    if (!whole) finish_part<kCompute>(a, cut, b, u, s0, r.nt);
     w += tiles;
-    t = 0;
+    if (w == cut.w1) {
+      if (tid == 0) put_cut_unit(a, cut, b, u, s0, r.nt);
+      break;
+    }
+    t = -1;
     if (++u == a.units_per_req) {
       u = 0;
-      ++b;
+      keys = visible(a, ++b);
     }
   }
 }
@@ -596,7 +635,7 @@ int launch(gq_ctx *ctx, const gq_kv_pages *p, Args &a) {
   rc = bind_workspace(ctx, grid, a);
   if (rc != GQ_OK) return rc;
   GQ_CUDA_TRY(ctx, gq_launch(ctx, paged_tiles_kernel<TYPE, D>, dim3(grid), dim3(kThreads), C::kSmem, a, kmap, vmap));
-  return GQ_OK;
+  return gq_paged_join_launch(ctx, a, grid);
 }
 
 template <int TYPE>
