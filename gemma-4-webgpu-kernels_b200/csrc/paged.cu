@@ -262,26 +262,46 @@ __device__ __forceinline__ void store4(void *base, int64_t elem, const float4 v,
   }
 }
 
-// Grid: x = pieces of four values of all rows, y = keys (0) or values (1).
+// A warp writes one token's row of keys (or values): what it needs of the slot is worked
+// out once, and a lane's kAppendLoads loads of 16 bytes are in flight together. Rows are
+// taken in turn by a grid that fills the GPU.
+constexpr int kAppendThreads = 256, kAppendLoads = 4;
+
 template <int TYPE>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendArgs a) {
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
-  const int kv = blockIdx.y;
-  const int per_head = a.head_dim / 4, per_row = a.heads * per_head;
-  const float *src = a.src[kv];
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < a.tokens * per_row; i += gridDim.x * 256ll) {
-    const int64_t t = i / per_row;
-    const int r = (int)(i - t * per_row), h = r / per_head, c = (r - h * per_head) * 4;
+  const int lane = threadIdx.x & 31;
+  const int per_head = a.head_dim / 4, pieces = a.heads * per_head;
+  const int64_t rows = 2 * a.tokens, step = (int64_t)gridDim.x * (kAppendThreads / 32);
+  for (int64_t r = blockIdx.x * (int64_t)(kAppendThreads / 32) + threadIdx.x / 32; r < rows; r += step) {
+    const int64_t t = r >> 1;
+    const int kv = (int)(r & 1);
     const int64_t slot = a.slots[t];
     if (slot < 0) continue;
     if (slot >= a.n_slots) {
-      gqd::report(a.err, GQ_DEVERR_PAGES);
+      if (lane == 0) gqd::report(a.err, GQ_DEVERR_PAGES);
       continue;
     }
-    const float4 v = *reinterpret_cast<const float4 *>(src + t * a.src_stride[kv] + (int64_t)r * 4);
-    const int64_t page = slot / a.page_size, row = slot - page * a.page_size;
-    store4<TYPE>(a.dst[kv], page * a.page_stride + (h * a.page_size + row) * a.head_dim + c, v, a.inv_scale[kv]);
+    const int64_t page = (slot >> 32) == 0 ? (int64_t)((uint32_t)slot / (uint32_t)a.page_size) : slot / a.page_size;
+    const int64_t base = page * a.page_stride + (slot - page * a.page_size) * a.head_dim;
+    const int64_t head = a.page_size * a.head_dim;  // elements between heads
+    const float4 *src = reinterpret_cast<const float4 *>(a.src[kv] + t * a.src_stride[kv]);
+    void *dst = a.dst[kv];
+    const float inv = a.inv_scale[kv];
+    for (int c0 = lane; c0 < pieces; c0 += 32 * kAppendLoads) {
+      float4 v[kAppendLoads];
+#pragma unroll
+      for (int i = 0; i < kAppendLoads; ++i)
+        if (c0 + 32 * i < pieces) v[i] = __ldcs(src + c0 + 32 * i);
+#pragma unroll
+      for (int i = 0; i < kAppendLoads; ++i) {
+        const int c = c0 + 32 * i;
+        if (c >= pieces) break;
+        const int h = a.heads == 1 ? 0 : c / per_head;
+        store4<TYPE>(dst, base + h * head + (c - h * per_head) * 4, v[i], inv);
+      }
+    }
   }
 }
 
@@ -428,13 +448,12 @@ extern "C" int gq_paged_append(gq_ctx *ctx, const gq_kv_pages *pages, const floa
   a.inv_scale[0] = 1.0f / pages->k_scale;
   a.inv_scale[1] = 1.0f / pages->v_scale;
   a.err = ctx->dev_err;
-  const int64_t pieces = t * (row / 4);
-  const dim3 grid((unsigned)std::min<int64_t>((pieces + 255) / 256, (int64_t)ctx->num_sms * 16), 2);
+  const dim3 grid((unsigned)std::min<int64_t>((2 * t + kAppendThreads / 32 - 1) / (kAppendThreads / 32), (int64_t)ctx->num_sms * 8));
   switch (pages->type) {
-    case GQ_KV_F32: GQ_CUDA_TRY(ctx, gq_launch(ctx, paged_append_kernel<GQ_KV_F32>, grid, dim3(256), 0, a)); break;
-    case GQ_KV_F16: GQ_CUDA_TRY(ctx, gq_launch(ctx, paged_append_kernel<GQ_KV_F16>, grid, dim3(256), 0, a)); break;
-    case GQ_KV_BF16: GQ_CUDA_TRY(ctx, gq_launch(ctx, paged_append_kernel<GQ_KV_BF16>, grid, dim3(256), 0, a)); break;
-    default: GQ_CUDA_TRY(ctx, gq_launch(ctx, paged_append_kernel<GQ_KV_E4M3>, grid, dim3(256), 0, a)); break;
+    case GQ_KV_F32: GQ_CUDA_TRY(ctx, gq_launch(ctx, paged_append_kernel<GQ_KV_F32>, grid, dim3(kAppendThreads), 0, a)); break;
+    case GQ_KV_F16: GQ_CUDA_TRY(ctx, gq_launch(ctx, paged_append_kernel<GQ_KV_F16>, grid, dim3(kAppendThreads), 0, a)); break;
+    case GQ_KV_BF16: GQ_CUDA_TRY(ctx, gq_launch(ctx, paged_append_kernel<GQ_KV_BF16>, grid, dim3(kAppendThreads), 0, a)); break;
+    default: GQ_CUDA_TRY(ctx, gq_launch(ctx, paged_append_kernel<GQ_KV_E4M3>, grid, dim3(kAppendThreads), 0, a)); break;
   }
   return GQ_OK;
 }
