@@ -2,14 +2,15 @@
 // logits (gq_process_logits), one pass over the rows.
 //
 // What bounds it: 8 bytes per logit (read and written once); the histories, biases and
-// mask bits are small beside that. The counts of a row's earlier tokens are made where
-// they are needed: a CTA owns a chunk of a row's columns, reads the row's whole history
-// and counts the tokens of its chunk in shared memory (whole numbers, so the order of
-// the atomic additions changes nothing), while its logits are on their way. A history
-// of 4096 tokens read once per 8192 columns adds 16 KB of L2 reads to 64 KB. Sharing the
-// scan over a cluster of 8 CTAs with counters in distributed shared memory read it 8
-// times less often and was slower: two cluster barriers per CTA, 67 us for 64 rows of
-// 262144 against NEW.
+// mask bits are small beside that, but each is a chain of dependent loads and barriers of
+// some microseconds. So a CTA owns many columns (16384): it copies them masked, which
+// waits for nothing, while it counts the tokens of its columns in shared memory (whole
+// numbers: the order of the atomic additions changes nothing), and then rewrites the few
+// columns that a penalty or a bias changes, one thread each.
+// Measured on 64 rows of 262144, histories up to 8192, 300 biases a row: penalties
+// applied where all columns are written, 47-67 us (their divisions run in nearly every
+// warp for a lane or two, and the logits wait in registers for the counts); a cluster of
+// 8 CTAs sharing the scan of the history, 53 us (cluster barriers); this way NEW us.
 #include <algorithm>
 
 #include "gq_internal.cuh"
@@ -17,9 +18,7 @@
 namespace {
 
 constexpr uint32_t kSeen = 0x80000000u;  // the token is in the prompt; below: times generated
-// Histories from here on are scanned once per 32768 columns (one CTA of 1024 threads per
-// SM) instead of once per 8192.
-constexpr int64_t kLongHistory = 32768;
+constexpr int kListed = 2048;
 
 struct LogitArgs {
   const float *x;
@@ -36,7 +35,6 @@ struct LogitArgs {
 };
 
 __device__ __forceinline__ float penalised(float l, uint32_t w, float rep, float presence, float frequency) {
-  if (w == 0) return l;
   l = l > 0.0f ? __fdiv_rn(l, rep) : __fmul_rn(l, rep);
   const uint32_t n = w & ~kSeen;
   if (n) l = __fsub_rn(__fsub_rn(l, __fmul_rn(frequency, (float)n)), presence);
@@ -52,15 +50,7 @@ __device__ __forceinline__ uint32_t mask_bits4(const uint32_t *mask, int c, int 
   return c < 0 ? bits << (uint32_t)(-c) : bits;
 }
 
-__device__ __forceinline__ void apply4(float4 &v, const uint32_t *words, float rep, float presence, float frequency) {
-  const uint4 w = *reinterpret_cast<const uint4 *>(words);
-  if (w.x | w.y | w.z | w.w) {
-    v.x = penalised(v.x, w.x, rep, presence, frequency);
-    v.y = penalised(v.y, w.y, rep, presence, frequency);
-    v.z = penalised(v.z, w.z, rep, presence, frequency);
-    v.w = penalised(v.w, w.w, rep, presence, frequency);
-  }
-}
+// A masked column is -inf whatever it was (a NaN, or -inf + inf, too).
 __device__ __forceinline__ void mask4(float4 &v, uint32_t bits) {
   if (!(bits & 1u)) v.x = -INFINITY;
   if (!(bits & 2u)) v.y = -INFINITY;
@@ -72,113 +62,154 @@ __device__ __forceinline__ void mask4(float4 &v, uint32_t bits) {
 // counted from the 16-byte boundary at or before the row's first logit, so that rows of
 // any stride are read in whole 16-byte pieces; `lead` columns lie before the row.
 template <int NT, int V, bool VEC>
-__global__ void __launch_bounds__(NT) logits_kernel(const LogitArgs a) {
-  constexpr int kCols = NT * V * 4;
-  extern __shared__ __align__(16) uint32_t words[];  // [kCols]
+__global__ void __launch_bounds__(NT, 1536 / NT) logits_kernel(const LogitArgs a) {
+  constexpr int kCols = NT * V * 4, kLoads = V < 4 ? V : 4, kTokens = 4;
+  static_assert(V % kLoads == 0 && kCols <= 65536, "whole batches, 16-bit columns");
+  extern __shared__ __align__(16) uint32_t words[];  // [kCols] counts, later owners of biases
+  __shared__ uint16_t counted[kListed];              // the first kListed columns that got a count
+  __shared__ int n_counted;
   const int tid = threadIdx.x, vocab = (int)a.vocab;
   const int64_t row = blockIdx.y;
   const float *x = a.x + row * a.ld;
   float *y = a.y + row * a.ldy;
   const int lead = VEC ? (int)((reinterpret_cast<uintptr_t>(x) >> 2) & 3u) : 0;
   const int col0 = (int)blockIdx.x * kCols - lead;  // column of words[0]
-  if (a.tokens)
+  const int lo = max(col0, 0), span = max(min(col0 + kCols, vocab) - lo, 0);
+  // (ids below lo, negative ones too, wrap past span: lo + span < 2^28)
+  auto here = [&](int id) { return (uint32_t)id - (uint32_t)lo < (uint32_t)span; };
+  if (a.tokens) {
 #pragma unroll
     for (int i = 0; i < V; ++i) reinterpret_cast<uint4 *>(words)[i * NT + tid] = make_uint4(0, 0, 0, 0);
+    if (tid == 0) n_counted = 0;
+  }
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
 
-  // the logits are requested first: the counting below runs while they arrive
-  const bool inside = VEC && col0 >= 0 && col0 + kCols <= vocab;  // every piece is whole
-  const int c0 = col0 + tid * 4;
-  float4 v[V];
-  if (inside) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = *reinterpret_cast<const float4 *>(x + c0 + j * NT * 4);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = c0 + j * NT * 4;
-      v[j].x = c >= 0 && c < vocab ? x[c] : 0.0f;
-      v[j].y = c + 1 >= 0 && c + 1 < vocab ? x[c + 1] : 0.0f;
-      v[j].z = c + 2 >= 0 && c + 2 < vocab ? x[c + 2] : 0.0f;
-      v[j].w = c + 3 >= 0 && c + 3 < vocab ? x[c + 3] : 0.0f;
-    }
-  }
+  // every chain of dependent loads begins here
+  int len = 0, prompt = 0, b0 = 0, biases = 0;
+  float rep = 1.0f, presence = 0.0f, frequency = 0.0f;
   const uint32_t *mask = nullptr;
+  if (a.tokens) {
+    len = a.lens[row];
+    prompt = a.prompt_lens[row];
+    rep = a.penalties[row * 3];
+    presence = a.penalties[row * 3 + 1];
+    frequency = a.penalties[row * 3 + 2];
+  }
+  if (a.bias_offsets) {
+    b0 = a.bias_offsets[row];
+    biases = a.bias_offsets[row + 1] - b0;
+  }
   if (a.masks) {
     const int64_t mr = a.mask_rows ? (int64_t)a.mask_rows[row] : row;
     if (mr >= 0 && mr < a.n_masks) mask = a.masks + mr * a.mask_stride;
   }
-
-  if (a.tokens) {
-    const float rep = a.penalties[row * 3], presence = a.penalties[row * 3 + 1], frequency = a.penalties[row * 3 + 2];
-    const int len = (int)min((int64_t)a.lens[row], a.tok_stride), prompt = a.prompt_lens[row];
-    const int32_t *tok = a.tokens + row * a.tok_stride;
-    const int lo = max(col0, 0), span = min(col0 + kCols, vocab) - lo;
-    __syncthreads();  // the counters are zero
-    for (int i = tid; i < len; i += NT * 4) {
-      int t[4];
+  const bool inside = VEC && col0 >= 0 && col0 + kCols <= vocab;  // every piece is whole
+  const int c0 = col0 + tid * 4;
+  float4 v[kLoads];
+  uint32_t bits[kLoads];
+  auto fetch = [&](int j0) {  // pieces j0 .. of this thread, and their mask bits
 #pragma unroll
-      for (int k = 0; k < 4; ++k) t[k] = i + k * NT < len ? tok[i + k * NT] : -1;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        // (ids below lo, negative ones too, wrap past span)
-        if ((uint32_t)t[k] - (uint32_t)lo >= (uint32_t)max(span, 0) || t[k] < 0) continue;
-        if (i + k * NT < prompt) atomicOr(&words[t[k] - col0], kSeen);
-        else atomicAdd(&words[t[k] - col0], 1u);
+    for (int j = 0; j < kLoads; ++j) {
+      const int c = c0 + (j0 + j) * NT * 4;
+      if (inside) {
+        v[j] = *reinterpret_cast<const float4 *>(x + c);
+      } else {
+        v[j].x = c >= 0 && c < vocab ? x[c] : 0.0f;
+        v[j].y = c + 1 >= 0 && c + 1 < vocab ? x[c + 1] : 0.0f;
+        v[j].z = c + 2 >= 0 && c + 2 < vocab ? x[c + 2] : 0.0f;
+        v[j].w = c + 3 >= 0 && c + 3 < vocab ? x[c + 3] : 0.0f;
       }
     }
-    __syncthreads();
 #pragma unroll
-    for (int j = 0; j < V; ++j) apply4(v[j], words + (j * NT + tid) * 4, rep, presence, frequency);
+    for (int j = 0; j < kLoads; ++j) {
+      const int c = c0 + (j0 + j) * NT * 4;
+      bits[j] = !mask || c + 3 < 0 || c >= vocab ? 15u : inside && lead == 0 ? mask[c >> 5] >> (c & 31) : mask_bits4(mask, c, vocab);
+    }
+  };
+  auto put = [&](int j0) {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int c = c0 + (j0 + j) * NT * 4;
+      mask4(v[j], bits[j]);
+      if (inside) {
+        *reinterpret_cast<float4 *>(y + c) = v[j];
+      } else {
+        if (c >= 0 && c < vocab) y[c] = v[j].x;
+        if (c + 1 >= 0 && c + 1 < vocab) y[c + 1] = v[j].y;
+        if (c + 2 >= 0 && c + 2 < vocab) y[c + 2] = v[j].z;
+        if (c + 3 >= 0 && c + 3 < vocab) y[c + 3] = v[j].w;
+      }
+    }
+  };
+  // the first logits are requested, then the history is counted while they arrive
+  fetch(0);
+  const int32_t *ids = a.bias_ids + b0;
+  const int id0 = tid < biases ? ids[tid] : -1;  // this thread's first entry
+  if (a.tokens) {
+    len = (int)min((int64_t)len, a.tok_stride);
+    const int32_t *tok = a.tokens + row * a.tok_stride;
+    __syncthreads();  // the counters are zero
+    for (int i = tid; i < len; i += NT * kTokens) {
+      int t[kTokens];
+#pragma unroll
+      for (int k = 0; k < kTokens; ++k) t[k] = i + k * NT < len ? tok[i + k * NT] : -1;
+#pragma unroll
+      for (int k = 0; k < kTokens; ++k) {
+        if (!here(t[k])) continue;
+        const int at = t[k] - col0;
+        const uint32_t before = i + k * NT < prompt ? atomicOr(&words[at], kSeen) : atomicAdd(&words[at], 1u);
+        if (before == 0) {
+          const int p = atomicAdd(&n_counted, 1);
+          if (p < kListed) counted[p] = (uint16_t)at;
+        }
+      }
+    }
   }
-  if (inside) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = c0 + j * NT * 4;
-      if (mask) mask4(v[j], lead == 0 ? mask[c >> 5] >> (c & 31) : mask_bits4(mask, c, vocab));
-      *reinterpret_cast<float4 *>(y + c) = v[j];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = c0 + j * NT * 4;
-      if (c + 3 < 0 || c >= vocab) continue;
-      if (mask) mask4(v[j], mask_bits4(mask, c, vocab));
-      if (c >= 0) y[c] = v[j].x;
-      if (c + 1 >= 0 && c + 1 < vocab) y[c + 1] = v[j].y;
-      if (c + 2 >= 0 && c + 2 < vocab) y[c + 2] = v[j].z;
-      if (c + 3 < vocab) y[c + 3] = v[j].w;
-    }
+  for (int j0 = 0; j0 < V; j0 += kLoads) {
+    put(j0);
+    if (j0 + kLoads < V) fetch(j0 + kLoads);
   }
 
-  if (a.bias_offsets) {
+  if (a.tokens) {
+    __syncthreads();  // counts are made, columns are written
+    const int n = n_counted;
+    auto rewrite = [&](int at) {
+      // (in place x[c] is what was just written: itself, unless it is masked)
+      const int c = col0 + at;
+      if (!mask || ((mask[c >> 5] >> (c & 31)) & 1u)) y[c] = penalised(x[c], words[at], rep, presence, frequency);
+    };
+    if (n <= kListed) {
+      for (int i = tid; i < n; i += NT) rewrite(counted[i]);
+    } else {  // more than the list holds: look at every column
+      for (int at = tid; at < kCols; at += NT)
+        if (words[at]) rewrite(at);
+    }
+  }
+  if (biases > 0) {
     // words now says which entry of the row's list owns a column: the last one
-    const int64_t b0 = a.bias_offsets[row];
-    const int n = a.bias_offsets[row + 1] - (int)b0;
-    const int32_t *ids = a.bias_ids + b0;
-    const int lo = max(col0, 0), hi = min(col0 + kCols, vocab);
+    auto each = [&](auto f) {
+      if (here(id0)) f(tid, id0);
+      for (int i = tid + NT; i < biases; i += NT) {
+        const int id = ids[i];
+        if (here(id)) f(i, id);
+      }
+    };
+    __syncthreads();  // words and y are done with
     bool any = false;
-    __syncthreads();  // words and y are written and read
-    for (int i = tid; i < n; i += NT) {
-      const int id = ids[i];
-      if (id < lo || id >= hi) continue;
+    each([&](int, int id) {
       words[id - col0] = 0;
       any = true;
-    }
+    });
     if (!__syncthreads_or(any)) return;
-    for (int i = tid; i < n; i += NT) {
-      const int id = ids[i];
-      if (id >= lo && id < hi) atomicMax(&words[id - col0], (uint32_t)(i + 1));
-    }
+    each([&](int i, int id) { atomicMax(&words[id - col0], (uint32_t)(i + 1)); });
     __syncthreads();
-    for (int i = tid; i < n; i += NT) {
-      const int id = ids[i];
-      if (id < lo || id >= hi || words[id - col0] != (uint32_t)(i + 1)) continue;
+    each([&](int i, int id) {
       // a masked column stays -inf whatever its bias (-inf + inf would be NaN)
-      if (mask && !((mask[id >> 5] >> (id & 31)) & 1u)) continue;
-      y[id] = __fadd_rn(y[id], a.bias_values[b0 + i]);
-    }
+      if (words[id - col0] == (uint32_t)(i + 1) && (!mask || ((mask[id >> 5] >> (id & 31)) & 1u)))
+        y[id] = __fadd_rn(y[id], a.bias_values[b0 + i]);
+    });
   }
 }
 
@@ -197,10 +228,9 @@ int logits_launch(gq_ctx *ctx, const LogitArgs &a, int64_t m, int64_t most_lead)
 
 template <bool VEC>
 int logits_dispatch(gq_ctx *ctx, const LogitArgs &a, int64_t m, int64_t most_lead) {
-  if (a.tokens && a.tok_stride >= kLongHistory) return logits_launch<1024, 8, VEC>(ctx, a, m, most_lead);
   // few rows: smaller chunks, so that more SMs take part
-  if (m * ((a.vocab + 8191) / 8192) < ctx->num_sms) return logits_launch<256, 2, VEC>(ctx, a, m, most_lead);
-  return logits_launch<256, 8, VEC>(ctx, a, m, most_lead);
+  if (m * ((a.vocab + 4095) / 4096) < ctx->num_sms) return logits_launch<256, 2, VEC>(ctx, a, m, most_lead);
+  return logits_launch<512, 8, VEC>(ctx, a, m, most_lead);
 }
 
 }  // namespace
