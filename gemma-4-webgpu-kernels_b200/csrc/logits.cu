@@ -2,11 +2,12 @@
 // logits (gq_process_logits), one pass over the rows.
 //
 // What bounds it: 8 bytes per logit (read and written once); the histories, biases and
-// mask bits are small beside that, but each is a chain of dependent loads and barriers of
-// some microseconds. So a CTA owns many columns (16384): it copies them masked, which
-// waits for nothing, while it counts the tokens of its columns in shared memory (whole
-// numbers: the order of the atomic additions changes nothing), and then rewrites the few
-// columns that a penalty or a bias changes, one thread each.
+// mask bits are small beside that, but the instructions they cost are not: the mask, the
+// look at each earlier token by each CTA of the row, and chains of dependent loads. So a
+// CTA owns many columns (16384): it copies them masked, which waits for nothing, while it
+// marks and counts the tokens of its columns in shared memory (whole numbers: the order
+// of the atomic operations changes nothing), and then rewrites the few columns that a
+// penalty or a bias changes, one thread each, from a list.
 // Measured on 64 rows of 262144, histories up to 8192, 300 biases a row: penalties
 // applied where all columns are written, 47-67 us (their divisions run in nearly every
 // warp for a lane or two, and the logits wait in registers for the counts); a cluster of
@@ -17,7 +18,7 @@
 
 namespace {
 
-constexpr uint32_t kSeen = 0x80000000u;  // the token is in the prompt; below: times generated
+constexpr uint32_t kOwner = 0x80000000u;  // a word that holds a bias entry, not a count (below 2^28)
 constexpr int kListed = 2048;
 
 struct LogitArgs {
@@ -34,9 +35,9 @@ struct LogitArgs {
   int64_t n_masks, mask_stride;
 };
 
-__device__ __forceinline__ float penalised(float l, uint32_t w, float rep, float presence, float frequency) {
+// A logit whose token was seen, n times among the generated ones.
+__device__ __forceinline__ float penalised(float l, uint32_t n, float rep, float presence, float frequency) {
   l = l > 0.0f ? __fdiv_rn(l, rep) : __fmul_rn(l, rep);
-  const uint32_t n = w & ~kSeen;
   if (n) l = __fsub_rn(__fsub_rn(l, __fmul_rn(frequency, (float)n)), presence);
   return l;
 }
@@ -62,12 +63,14 @@ __device__ __forceinline__ void mask4(float4 &v, uint32_t bits) {
 // counted from the 16-byte boundary at or before the row's first logit, so that rows of
 // any stride are read in whole 16-byte pieces; `lead` columns lie before the row.
 template <int NT, int V, bool VEC>
-__global__ void __launch_bounds__(NT, 1536 / NT) logits_kernel(const LogitArgs a) {
+__global__ void __launch_bounds__(NT, 1024 / NT) logits_kernel(const LogitArgs a) {
   constexpr int kCols = NT * V * 4, kLoads = V < 4 ? V : 4, kTokens = 4;
   static_assert(V % kLoads == 0 && kCols <= 65536, "whole batches, 16-bit columns");
+  static_assert(kCols / 32 <= NT && NT * 4 % 32 == 0, "a thread per bitmap word");
   extern __shared__ __align__(16) uint32_t words[];  // [kCols] counts, later owners of biases
-  __shared__ uint16_t counted[kListed];              // the first kListed columns that got a count
-  __shared__ int n_counted;
+  __shared__ uint32_t seen[kCols / 32];              // bit: the column's token was seen
+  __shared__ uint16_t listed[kListed];               // the first kListed of them
+  __shared__ int n_seen;
   const int tid = threadIdx.x, vocab = (int)a.vocab;
   const int64_t row = blockIdx.y;
   const float *x = a.x + row * a.ld;
@@ -77,10 +80,11 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logits_kernel(const LogitArgs a
   const int lo = max(col0, 0), span = max(min(col0 + kCols, vocab) - lo, 0);
   // (ids below lo, negative ones too, wrap past span: lo + span < 2^28)
   auto here = [&](int id) { return (uint32_t)id - (uint32_t)lo < (uint32_t)span; };
-  if (a.tokens) {
+  if (a.tokens || a.bias_offsets) {
 #pragma unroll
     for (int i = 0; i < V; ++i) reinterpret_cast<uint4 *>(words)[i * NT + tid] = make_uint4(0, 0, 0, 0);
-    if (tid == 0) n_counted = 0;
+    if (tid < kCols / 32) seen[tid] = 0;
+    if (tid == 0) n_seen = 0;
   }
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
@@ -108,30 +112,34 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logits_kernel(const LogitArgs a
   const int c0 = col0 + tid * 4;
   float4 v[kLoads];
   uint32_t bits[kLoads];
+  const uint32_t *mask0 = mask + (c0 >> 5);  // (read only where columns are inside the row)
   auto fetch = [&](int j0) {  // pieces j0 .. of this thread, and their mask bits
+    if (inside) {
 #pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int c = c0 + (j0 + j) * NT * 4;
-      if (inside) {
-        v[j] = *reinterpret_cast<const float4 *>(x + c);
-      } else {
+      for (int j = 0; j < kLoads; ++j) v[j] = *reinterpret_cast<const float4 *>(x + c0 + (j0 + j) * NT * 4);
+      if (mask && lead == 0)  // a piece's bits lie in one word, at the same place for all of a thread's pieces
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) bits[j] = mask0[(j0 + j) * (NT / 8)] >> (c0 & 31);
+      else if (mask)
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) bits[j] = mask_bits4(mask, c0 + (j0 + j) * NT * 4, vocab);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int c = c0 + (j0 + j) * NT * 4;
         v[j].x = c >= 0 && c < vocab ? x[c] : 0.0f;
         v[j].y = c + 1 >= 0 && c + 1 < vocab ? x[c + 1] : 0.0f;
         v[j].z = c + 2 >= 0 && c + 2 < vocab ? x[c + 2] : 0.0f;
         v[j].w = c + 3 >= 0 && c + 3 < vocab ? x[c + 3] : 0.0f;
+        bits[j] = !mask || c + 3 < 0 || c >= vocab ? 15u : mask_bits4(mask, c, vocab);
       }
-    }
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int c = c0 + (j0 + j) * NT * 4;
-      bits[j] = !mask || c + 3 < 0 || c >= vocab ? 15u : inside && lead == 0 ? mask[c >> 5] >> (c & 31) : mask_bits4(mask, c, vocab);
     }
   };
   auto put = [&](int j0) {
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int c = c0 + (j0 + j) * NT * 4;
-      mask4(v[j], bits[j]);
+      if (mask) mask4(v[j], bits[j]);
       if (inside) {
         *reinterpret_cast<float4 *>(y + c) = v[j];
       } else {
@@ -151,18 +159,15 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logits_kernel(const LogitArgs a
     const int32_t *tok = a.tokens + row * a.tok_stride;
     __syncthreads();  // the counters are zero
     for (int i = tid; i < len; i += NT * kTokens) {
-      int t[kTokens];
+      uint32_t t[kTokens];  // column in the chunk's part of the row
 #pragma unroll
-      for (int k = 0; k < kTokens; ++k) t[k] = i + k * NT < len ? tok[i + k * NT] : -1;
+      for (int k = 0; k < kTokens; ++k) t[k] = i + k * NT < len ? (uint32_t)tok[i + k * NT] - (uint32_t)lo : ~0u;
 #pragma unroll
       for (int k = 0; k < kTokens; ++k) {
-        if (!here(t[k])) continue;
-        const int at = t[k] - col0;
-        const uint32_t before = i + k * NT < prompt ? atomicOr(&words[at], kSeen) : atomicAdd(&words[at], 1u);
-        if (before == 0) {
-          const int p = atomicAdd(&n_counted, 1);
-          if (p < kListed) counted[p] = (uint16_t)at;
-        }
+        if (t[k] >= (uint32_t)span) continue;
+        const int at = (int)t[k] + lo - col0;
+        atomicOr(&seen[at >> 5], 1u << (at & 31));
+        if (i + k * NT >= prompt) atomicAdd(&words[at], 1u);
       }
     }
   }
@@ -174,17 +179,24 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logits_kernel(const LogitArgs a
 
   if (a.tokens) {
     __syncthreads();  // counts are made, columns are written
-    const int n = n_counted;
+    uint32_t set = tid < kCols / 32 ? seen[tid] : 0u;
+    if (set) {
+      int p = atomicAdd(&n_seen, __popc(set));
+      for (; set; set &= set - 1, ++p)
+        if (p < kListed) listed[p] = (uint16_t)(tid * 32 + __ffs(set) - 1);
+    }
+    __syncthreads();
+    const int n = n_seen;
     auto rewrite = [&](int at) {
       // (in place x[c] is what was just written: itself, unless it is masked)
       const int c = col0 + at;
       if (!mask || ((mask[c >> 5] >> (c & 31)) & 1u)) y[c] = penalised(x[c], words[at], rep, presence, frequency);
     };
     if (n <= kListed) {
-      for (int i = tid; i < n; i += NT) rewrite(counted[i]);
+      for (int i = tid; i < n; i += NT) rewrite(listed[i]);
     } else {  // more than the list holds: look at every column
       for (int at = tid; at < kCols; at += NT)
-        if (words[at]) rewrite(at);
+        if ((seen[at >> 5] >> (at & 31)) & 1u) rewrite(at);
     }
   }
   if (biases > 0) {
@@ -196,18 +208,12 @@ __global__ void __launch_bounds__(NT, 1536 / NT) logits_kernel(const LogitArgs a
         if (here(id)) f(i, id);
       }
     };
-    __syncthreads();  // words and y are done with
-    bool any = false;
-    each([&](int, int id) {
-      words[id - col0] = 0;
-      any = true;
-    });
-    if (!__syncthreads_or(any)) return;
-    each([&](int i, int id) { atomicMax(&words[id - col0], (uint32_t)(i + 1)); });
+    __syncthreads();  // counts are read, y is written
+    each([&](int i, int id) { atomicMax(&words[id - col0], kOwner + (uint32_t)i); });
     __syncthreads();
     each([&](int i, int id) {
       // a masked column stays -inf whatever its bias (-inf + inf would be NaN)
-      if (words[id - col0] == (uint32_t)(i + 1) && (!mask || ((mask[id >> 5] >> (id & 31)) & 1u)))
+      if (words[id - col0] == kOwner + (uint32_t)i && (!mask || ((mask[id >> 5] >> (id & 31)) & 1u)))
         y[id] = __fadd_rn(y[id], a.bias_values[b0 + i]);
     });
   }
