@@ -219,7 +219,10 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const Args a) {
 // sums are added in order. wide is the most (up to a head's columns) that still gives
 // every CTA an item: many cut units of few parts are read in whole rows, a few long ones
 // by as many threads as there are. (Items of 128 columns for all: 11 us for 64 units of
-// 5 parts at head_dim 512.)
+// 5 parts at head_dim 512.) A join inside the first launch was built two ways and was
+// slower: by the last CTA of a unit to arrive (up to 40 us after the last tile for a unit
+// of 99 parts of 16 KB), and by all CTAs of a cooperative launch, each waiting for its
+// units' parts and joining a share of their columns (4 us for 6 parts, 10-14 us for 300).
 constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinBatch = 8, kJoinNarrow = 8;
 
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Args a, int grid) {

@@ -2,15 +2,16 @@
 // the tensor cores, f32 results.
 //
 // A tile is T keys of one unit (one request, up to 8 query heads of one key-value head).
-// One warp is the producer: it walks this CTA's tiles and issues, per page (or part of
-// a page), one 4-D TMA copy of the keys and one of the values into a ring of tiles
-// (128-byte swizzle, so the fragment loads below have no bank conflicts). Four warps
-// compute, tile by tile:
+// Pages (or parts of pages) come by one 4-D TMA copy each into a ring of tiles (128-byte
+// swizzle, so the fragment loads below have no bank conflicts), issued by warp 0 as ring
+// slots become free. Four warps compute:
 //   S^T = K q^T        m16 = keys, n8 = heads, over head_dim: keys split over the warps
-//                      (and head_dim over KS warps where T < 64)
+//                      (and head_dim over KS warps where q would not fit the registers)
 //   p = 2^(s - m)      16 threads per head; running maximum and sum
 //   O^T += V^T p^T     m16 = head_dim columns, n8 = heads, over the T keys: columns
 //                      split over the warps
+// with the scores of tile i + 1 in the tensor pipe while the weights of tile i are made:
+// one barrier per tile.
 // Transposed, the 8 heads fill the instruction's n = 8 exactly: no product is wasted,
 // and a key-value head's cache is read once for all of them. The m16n8 instructions
 // (mma.sync) are used, not tcgen05: at n = 8 the work is 16 products per cached value,
@@ -38,8 +39,7 @@ using namespace pattn;
 
 constexpr int kComputeWarps = 4;
 constexpr int kCompute = kComputeWarps * 32;
-constexpr int kThreads = kCompute + 32;
-constexpr int kRingBytes = 96 * 1024;  // two CTAs per SM
+constexpr int kSmemBytes = 110 * 1024;  // two CTAs per SM
 constexpr int kMaxSlots = 8;
 
 __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int c0, int c1, int c2, int c3, uint64_t *bar) {
@@ -114,23 +114,29 @@ __device__ __forceinline__ uint32_t e4m3_pair(uint32_t u) {
 template <int TYPE, int D>
 struct Tile {
   static constexpr int kSize = TYPE == GQ_KV_F32 ? 4 : TYPE == GQ_KV_E4M3 ? 1 : 2;
+  static constexpr int kRow = D * kSize;          // bytes of a key
+  static constexpr int kChunks = kRow / 128;      // 128-byte pieces of a key
   // head_dim is split over KS warps where the q fragments of one warp would not fit its
   // registers (2 parts of 256 columns or 3 of 256 at 16 bits, 2 of 128 at 32)
   static constexpr int KS = TYPE == GQ_KV_F32 ? (D > 128 ? D / 128 : 1) : (D > 256 ? D / 256 : 1);
-  static constexpr int T = 16 * kComputeWarps / KS;
-  static constexpr int kRow = D * kSize;          // bytes of a key
-  static constexpr int kChunks = kRow / 128;      // 128-byte pieces of a key
+  // 16-key tiles per warp: two for rows of 128 bytes, whose tiles would be small beside
+  // what a tile costs whatever its size
+  static constexpr int MT = kRow == 128 ? 2 : 1;
+  static constexpr int T = 16 * kComputeWarps * MT / KS;
   static constexpr int kSlot = T * kRow;
-  static constexpr int kSlots = std::min(kMaxSlots, kRingBytes / kSlot);
   static constexpr int kParts = TYPE == GQ_KV_BF16 ? 3 : 2;
   static constexpr int kStep = TYPE == GQ_KV_F32 ? 8 : 16;      // head_dim columns (keys) per instruction
   static constexpr int kQSteps = D / KS / kStep;
   static constexpr int kMTiles = D / kComputeWarps / 16;        // 16-column tiles of the output per warp
   static constexpr int kSStride = T + 4;                        // floats between heads' scores
+  static constexpr int kSFloats = KS * kHeads * kSStride;
   static constexpr int kPStride = TYPE == GQ_KV_F32 ? (T + 4) * 4 : T * 2 + 16;  // bytes between heads' weights
   static constexpr int kPBytes = (TYPE == GQ_KV_F32 ? 1 : kParts) * kHeads * kPStride;
-  static constexpr int kSmem = 1024 + kSlots * kSlot + KS * kHeads * kSStride * 4 + kPBytes;
-  static_assert(kRow % 128 == 0 && kSlots >= 3, "tile");
+  static constexpr int kRest = 1024 + 2 * (kSFloats * 4 + kPBytes);  // scores and weights of two tiles
+  static constexpr int kSlots = std::min(kMaxSlots, (kSmemBytes - kRest) / kSlot);
+  static constexpr int kSmem = kRest + kSlots * kSlot;
+  static constexpr int kTShift = T == 128 ? 7 : T == 64 ? 6 : T == 32 ? 5 : 4;
+  static_assert(kRow % 128 == 0 && kSlots >= 3 && (1 << kTShift) == T && kPBytes % 16 == 0, "tile");
 };
 
 // A wait that gave up: report once, and let the CTA run to its end without waiting (what
@@ -144,98 +150,127 @@ __device__ __forceinline__ void wait_or_abort(uint64_t *bar, uint32_t parity, vo
 }
 
 
+// One tile of this CTA, as warp 0 sees it: lane i owns the tile's i-th copy.
+struct TileRef {
+  int page, row;      // of this lane's copy; page -1: nothing to load
+  bool valid, first;  // first: begins a unit's part
+};
+
 template <int TYPE, int D>
-__global__ void __launch_bounds__(kThreads, 2)
+__global__ void __launch_bounds__(kCompute, 2)
     paged_tiles_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using C = Tile<TYPE, D>;
-  constexpr int T = C::T, KS = C::KS;
+  constexpr int T = C::T, KS = C::KS, MT = C::MT;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t full[kMaxSlots], empty[kMaxSlots];
-  __shared__ float fix[kHeads], sum[kHeads];
+  __shared__ __align__(8) uint64_t full[kMaxSlots];
+  __shared__ float fix[2][kHeads], sum[kHeads];
   __shared__ int abort_flag;
   uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float *sS = reinterpret_cast<float *>(ring + C::kSlots * C::kSlot);                       // [KS][head][key]
-  uint8_t *sP = reinterpret_cast<uint8_t *>(sS + KS * kHeads * C::kSStride);                // [part][head][key]
+  float *sS = reinterpret_cast<float *>(ring + C::kSlots * C::kSlot);       // [2][KS][head][key]
+  uint8_t *sP = reinterpret_cast<uint8_t *>(sS + 2 * C::kSFloats);          // [2][part][head][key]
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
-    for (int i = 0; i < C::kSlots; ++i) {
-      gqd::mbar_init(&full[i], 1);
-      gqd::mbar_init(&empty[i], kComputeWarps);
-    }
+    for (int i = 0; i < C::kSlots; ++i) gqd::mbar_init(&full[i], 1);
     gqd::fence_mbar_init();
     abort_flag = 0;
   }
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
-  const Cut cut = find_cut<kThreads, T>(a);  // (its barriers also publish the mbarriers)
+  const Cut cut = find_cut<kCompute, T>(a);  // (its barriers also publish the mbarriers)
   if (cut.w0 >= cut.w1) {
     if (tid == 0) a.cut_units[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
   }
-  const int rows_shift = min(a.page_shift, T == 64 ? 6 : T == 32 ? 5 : 4);  // log2 of the keys one copy brings
-  const int rows = 1 << rows_shift;
+  const int rows_shift = min(a.page_shift, C::kTShift), rows = 1 << rows_shift;  // keys that one copy brings
+  const int boxes = T >> rows_shift;
 
-  if (warp == kComputeWarps) {
-    // ---- producer: lane i owns the tile's i-th copy; the next tile's table entry is
-    // read before this tile's slots are waited for
-    const int boxes = T >> rows_shift;
-    int b = cut.b, u = cut.u, t = cut.t;
-    Range r = range_of<T>(a, cut.keys);
-    auto entry = [&](int j0) -> int {  // page of this lane's copy, -1: nothing to load
-      const int j = j0 + (lane << rows_shift);
-      if (lane >= boxes || j >= r.hi || j + rows <= r.lo) return -1;
-      const int page = a.table[b * a.table_stride + (j >> a.page_shift)];
-      if (page >= 0 && page < a.n_pages) return page;
-      gqd::report(a.err, GQ_DEVERR_PAGES);
-      return (int)a.n_pages;  // out of the tensor's bounds: reads as zeros
-    };
-    int64_t w = cut.w0;
-    if (t < 0) {
-      t = 0;
-      ++w;
-    }
-    int j0 = (r.tile0 + t) * T, page = w < cut.w1 ? entry(j0) : -1;
-    uint32_t n = 0;  // ring position
-    while (w < cut.w1) {
-      const int load = page, jj = j0 + (lane << rows_shift), kvh = u / a.sub;
-      ++w;
-      if (++t == r.nt) {
-        t = 0;
-        ++w;
-        if (w < cut.w1) {
-          if (++u == a.units_per_req) {
-            u = 0;
-            r = range_of<T>(a, visible(a, ++b));
-          }
+  // ---- loads (warp 0). Order of the ring: the first keys of a part, then for each tile
+  // the next tile's keys and its own values. A tile's table entries are read two tiles
+  // before its copies are issued.
+  int lb = cut.b, lu = cut.u, lt = cut.t;
+  int64_t lw = cut.w0;
+  Range lr = range_of<T>(a, cut.keys);
+  auto advance = [&](bool begin) {
+    TileRef x;
+    x.valid = false;
+    x.first = begin;
+    x.page = -1;
+    x.row = 0;
+    if (!begin) {
+      if (lw >= cut.w1) return x;
+      ++lw;
+      ++lt;
+      if (lt == lr.nt) {
+        lt = -1;
+        if (lw >= cut.w1) return x;
+        if (++lu == a.units_per_req) {
+          lu = 0;
+          lr = range_of<T>(a, visible(a, ++lb));
         }
       }
-      if (w < cut.w1) {
-        j0 = (r.tile0 + t) * T;
-        page = entry(j0);
-      }
-      const int copies = __popc(__ballot_sync(0xffffffffu, load >= 0));
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv, ++n) {
-        const int slot = n % C::kSlots;
-        if (lane == 0) {
-          if (n >= C::kSlots) wait_or_abort(&empty[slot], ((n / C::kSlots) & 1) ^ 1, &abort_flag, a.err);
-          gqd::mbar_arrive_expect_tx(&full[slot], (uint32_t)(copies * rows * C::kRow));
-        }
-        __syncwarp();
-        if (load >= 0)
-          tma_load_4d(ring + slot * C::kSlot + lane * rows * C::kRow, kv ? &vmap : &kmap, 0,
-                      (kvh << a.page_shift) + (jj & (a.page_size - 1)), 0, load, &full[slot]);
+    }
+    if (lt < 0) {  // the place ahead of a unit's tiles
+      lt = 0;
+      ++lw;
+      x.first = true;
+    }
+    if (lw >= cut.w1) return x;
+    x.valid = true;
+    const int j = (lr.tile0 + lt) * T + (lane << rows_shift);
+    if (lane < boxes && j < lr.hi && j + rows > lr.lo) {
+      x.row = ((lu / a.sub) << a.page_shift) + (j & (a.page_size - 1));
+      x.page = a.table[lb * a.table_stride + (j >> a.page_shift)];
+      if (x.page < 0 || x.page >= a.n_pages) {
+        gqd::report(a.err, GQ_DEVERR_PAGES);
+        x.page = (int)a.n_pages;  // out of the tensor's bounds: reads as zeros
       }
     }
-    if (*(volatile int *)&abort_flag && lane == 0)  // copies still in flight end before the CTA's memory goes away
-      for (uint32_t i = n > C::kSlots ? n - C::kSlots : 0; i < n; ++i)
-        (void)gqd::mbar_wait_bounded(&full[i % C::kSlots], (i / C::kSlots) & 1, 100000000ull);
-    return;
+    return x;
+  };
+  TileRef cur, nxt;
+  uint32_t issued = 0;  // ring positions filled
+  int stage = 0;        // of the current tile: 0 its keys (if first), 1 the next tile's keys, 2 its values
+  auto copy = [&](const TileRef &x, const CUtensorMap *map) {
+    const int slot = issued % C::kSlots;
+    const int copies = __popc(__ballot_sync(0xffffffffu, x.page >= 0));
+    if (lane == 0) gqd::mbar_arrive_expect_tx(&full[slot], (uint32_t)(copies * rows * C::kRow));
+    __syncwarp();
+    if (x.page >= 0)
+      tma_load_4d(ring + slot * C::kSlot + lane * rows * C::kRow, map, 0, x.row, 0, x.page, &full[slot]);
+    ++issued;
+  };
+  auto fill = [&](uint32_t limit) {  // issue what there is, up to ring position `limit`
+    while (issued < limit && cur.valid) {
+      if (stage == 0) {
+        stage = 1;
+        if (cur.first) {
+          copy(cur, &kmap);
+          continue;
+        }
+      }
+      if (stage == 1) {
+        stage = 2;
+        if (nxt.valid && !nxt.first) {
+          copy(nxt, &kmap);
+          continue;
+        }
+      }
+      copy(cur, &vmap);
+      cur = nxt;
+      nxt = advance(false);
+      stage = 0;
+    }
+  };
+  if (warp == 0) {
+    cur = advance(true);
+    cur.first = true;
+    nxt = advance(false);
+    fill(C::kSlots);
   }
 
   // ---- compute
   const int g = lane >> 2, q4 = lane & 3;  // fragment row / column group
-  const int ks = warp % KS, mt = warp / KS;
+  const int ks = warp % KS, mt = warp / KS * MT;
   const int sh = tid >> 4, sl = tid & 15;  // softmax: head, thread of 16
   constexpr int KPT = T / 16;              // keys per softmax thread
   const uint32_t ring_u = gqd::smem_u32(ring);
@@ -243,11 +278,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   // byte of row `key` of a tile (first 128-byte piece); pieces are rows * 128 bytes apart
   auto row_at = [&](int key) { return (uint32_t)(key >> rows_shift) * box_bytes + (uint32_t)(key & (rows - 1)) * 128u; };
   const uint32_t piece = (uint32_t)rows * 128u;
-  // rows that this lane addresses in the fragment loads
-  const int krow = mt * 16 + (lane & 15);
-  const uint32_t kbase = row_at(krow), kswz = (uint32_t)(krow & 7);
 
-  uint32_t n = 0;
+  uint32_t n = 0;  // ring position of the next tile to read
   int b = cut.b, u = cut.u, t = cut.t, keys = cut.keys;
   for (int64_t w = cut.w0;;) {
     const Range r = range_of<T>(a, keys);
@@ -277,7 +309,6 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
       } else {
         float2 v[C::kQSteps][2];
-        float top = 0.0f;
 #pragma unroll
         for (int s = 0; s < C::kQSteps; ++s) {
           // e4m3: a thread's 4 bytes of a fragment are neighbours, so columns 4 q4 .. 4 q4 + 3
@@ -286,6 +317,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           v[s][1] = real ? *reinterpret_cast<const float2 *>(qg + c1) : make_float2(0.f, 0.f);
         }
         if constexpr (TYPE != GQ_KV_BF16) {
+          float top = 0.0f;
 #pragma unroll
           for (int s = 0; s < C::kQSteps; ++s)
             top = fmaxf(top, fmaxf(fmaxf(fabsf(v[s][0].x), fabsf(v[s][0].y)), fmaxf(fabsf(v[s][1].x), fabsf(v[s][1].y))));
@@ -295,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           const int e = (int)((__float_as_uint(top) >> 23) & 255u);
           const int up = e > 0 && e < 255 ? min(max(140 - e, -126), 126) : 0;
           const float f = __uint_as_float((uint32_t)(127 + up) << 23), inv = __uint_as_float((uint32_t)(127 - up) << 23);
-          unscale0 = __shfl_sync(0xffffffffu, inv, q4 * 8);      // lane of head 2 q4: group 2 q4
+          unscale0 = __shfl_sync(0xffffffffu, inv, q4 * 8);  // lane of head 2 q4: group 2 q4
           unscale1 = __shfl_sync(0xffffffffu, inv, q4 * 8 + 4);
 #pragma unroll
           for (int s = 0; s < C::kQSteps; ++s)
@@ -326,65 +358,87 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int k = 0; k < 4; ++k) acc[i][k] = 0.0f;
     float m = -INFINITY, l = 0.0f;
 
-    for (int i = 0; i < tiles; ++i, n += 2) {
-      const int j0 = (r.tile0 + t + i) * T;
-      const int kslot = n % C::kSlots, vslot = (n + 1) % C::kSlots;
-      const uint32_t kpar = (n / C::kSlots) & 1, vpar = ((n + 1) / C::kSlots) & 1;
-      // ---- scores of 16 keys (and of this warp's columns)
-      wait_or_abort(&full[kslot], kpar, &abort_flag, a.err);
+    // products of this warp's keys and columns with q: three (two) sums for the parts
+    float c[MT][3][4];
+    auto products = [&]() {
+      const int slot = n % C::kSlots;
+      wait_or_abort(&full[slot], (n / C::kSlots) & 1, &abort_flag, a.err);
       __syncwarp();
-      {
-        float c[3][4] = {};
-        const uint32_t at = ring_u + kslot * C::kSlot + kbase;
+      ++n;
+#pragma unroll
+      for (int x = 0; x < MT; ++x) {
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) c[x][p][k] = 0.0f;
+        const int krow = (mt + x) * 16 + (lane & 15);
+        const uint32_t at = ring_u + slot * C::kSlot + row_at(krow), swz = (uint32_t)(krow & 7);
 #pragma unroll
         for (int s = 0; s < (TYPE == GQ_KV_E4M3 ? C::kQSteps / 2 : C::kQSteps); ++s) {
           uint32_t k4[4];
           const int ch = ks * (C::kRow / KS / 16) + s * 2;  // 16-byte piece of the row (two per load)
-          ldsm4(k4, at + (uint32_t)(ch >> 3) * piece + ((((uint32_t)(ch & 7) + (lane >> 4)) ^ kswz) << 4));
+          ldsm4(k4, at + (uint32_t)(ch >> 3) * piece + ((((uint32_t)(ch & 7) + (lane >> 4)) ^ swz) << 4));
           if constexpr (TYPE == GQ_KV_F32) {
             uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) split_tf32(__uint_as_float(k4[x]), hi[x], lo[x]);
-            mma_tf32(c[0], hi, qf[s][0][0], qf[s][0][1]);
-            mma_tf32(c[1], hi, qf[s][1][0], qf[s][1][1]);
-            mma_tf32(c[2], lo, qf[s][0][0], qf[s][0][1]);
+            for (int y = 0; y < 4; ++y) split_tf32(__uint_as_float(k4[y]), hi[y], lo[y]);
+            mma_tf32(c[x][0], hi, qf[s][0][0], qf[s][0][1]);
+            mma_tf32(c[x][1], hi, qf[s][1][0], qf[s][1][1]);
+            mma_tf32(c[x][2], lo, qf[s][0][0], qf[s][0][1]);
           } else if constexpr (TYPE == GQ_KV_E4M3) {
             const uint32_t a0[4] = {e4m3_pair(k4[0]), e4m3_pair(k4[1]), e4m3_pair(k4[0] >> 16), e4m3_pair(k4[1] >> 16)};
             const uint32_t a1[4] = {e4m3_pair(k4[2]), e4m3_pair(k4[3]), e4m3_pair(k4[2] >> 16), e4m3_pair(k4[3] >> 16)};
-            mma_f16(c[0], a0, qf[2 * s][0][0], qf[2 * s][0][1]);
-            mma_f16(c[1], a0, qf[2 * s][1][0], qf[2 * s][1][1]);
-            mma_f16(c[0], a1, qf[2 * s + 1][0][0], qf[2 * s + 1][0][1]);
-            mma_f16(c[1], a1, qf[2 * s + 1][1][0], qf[2 * s + 1][1][1]);
+            mma_f16(c[x][0], a0, qf[2 * s][0][0], qf[2 * s][0][1]);
+            mma_f16(c[x][1], a0, qf[2 * s][1][0], qf[2 * s][1][1]);
+            mma_f16(c[x][0], a1, qf[2 * s + 1][0][0], qf[2 * s + 1][0][1]);
+            mma_f16(c[x][1], a1, qf[2 * s + 1][1][0], qf[2 * s + 1][1][1]);
           } else if constexpr (TYPE == GQ_KV_F16) {
-            mma_f16(c[0], k4, qf[s][0][0], qf[s][0][1]);
-            mma_f16(c[1], k4, qf[s][1][0], qf[s][1][1]);
+            mma_f16(c[x][0], k4, qf[s][0][0], qf[s][0][1]);
+            mma_f16(c[x][1], k4, qf[s][1][0], qf[s][1][1]);
           } else {
 #pragma unroll
-            for (int p = 0; p < C::kParts; ++p) mma_bf16(c[p], k4, qf[s][p][0], qf[s][p][1]);
+            for (int p = 0; p < 3; ++p) mma_bf16(c[x][p], k4, qf[s][p % C::kParts][0], qf[s][p % C::kParts][1]);
           }
         }
-        __syncwarp();
-        if (lane == 0) gqt::mbar_arrive(&empty[kslot]);
-        float *to = sS + ks * kHeads * C::kSStride + 2 * q4 * C::kSStride + mt * 16 + g;
-        to[0] = (c[0][0] + (c[1][0] + c[2][0])) * unscale0;
-        to[C::kSStride] = (c[0][1] + (c[1][1] + c[2][1])) * unscale1;
-        to[8] = (c[0][2] + (c[1][2] + c[2][2])) * unscale0;
-        to[C::kSStride + 8] = (c[0][3] + (c[1][3] + c[2][3])) * unscale1;
       }
-      sync_compute<kCompute>();
+    };
+    auto put_scores = [&](int buf) {
+#pragma unroll
+      for (int x = 0; x < MT; ++x) {
+        float *to = sS + buf * C::kSFloats + ks * kHeads * C::kSStride + 2 * q4 * C::kSStride + (mt + x) * 16 + g;
+        to[0] = (c[x][0][0] + (c[x][1][0] + c[x][2][0])) * unscale0;
+        to[C::kSStride] = (c[x][0][1] + (c[x][1][1] + c[x][2][1])) * unscale1;
+        to[8] = (c[x][0][2] + (c[x][1][2] + c[x][2][2])) * unscale0;
+        to[C::kSStride + 8] = (c[x][0][3] + (c[x][1][3] + c[x][2][3])) * unscale1;
+      }
+    };
 
-      // ---- weights
+    products();
+    put_scores(0);
+    sync_compute<kCompute>();
+    if (warp == 0) {  // every warp is done with what lies before ring position n
+      gqd::fence_proxy_async_smem();
+      fill(n + C::kSlots);
+    }
+
+    for (int i = 0; i < tiles; ++i) {
+      const int j0 = (r.tile0 + t + i) * T, buf = i & 1;
+      const bool more = i + 1 < tiles;
+      if (more) products();  // of tile i + 1
+
+      // ---- weights of tile i
       const bool ragged = j0 < r.lo || j0 + T > r.hi;
       {
+        const float *from = sS + buf * C::kSFloats + sh * C::kSStride + sl * KPT;
         float x[KPT], top = -INFINITY;
 #pragma unroll
         for (int k = 0; k < KPT; ++k) {
-          const int key = sl * KPT + k;
-          float s = sS[sh * C::kSStride + key];
+          float s = from[k];
 #pragma unroll
-          for (int p = 1; p < KS; ++p) s += sS[(p * kHeads + sh) * C::kSStride + key];
+          for (int p = 1; p < KS; ++p) s += from[p * kHeads * C::kSStride + k];
+          const int j = j0 + sl * KPT + k;
           s = score_log2(a, s);
-          x[k] = ragged && (j0 + key < r.lo || j0 + key >= r.hi) ? -INFINITY : s;
+          x[k] = ragged && (j < r.lo || j >= r.hi) ? -INFINITY : s;
           top = fmaxf(top, x[k]);
         }
 #pragma unroll
@@ -401,8 +455,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           l += p[k];
         }
         m = mn;
-        if (sl == 0) fix[sh] = f;
-        uint8_t *to = sP + sh * C::kPStride;
+        if (sl == 0) fix[buf][sh] = f;
+        uint8_t *to = sP + buf * C::kPBytes + sh * C::kPStride;
         if constexpr (TYPE == GQ_KV_F32) {
 #pragma unroll
           for (int k = 0; k < KPT; ++k) reinterpret_cast<float *>(to)[sl * KPT + k] = p[k];
@@ -426,7 +480,9 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
         }
       }
-      wait_or_abort(&full[vslot], vpar, &abort_flag, a.err);
+      if (more) put_scores(buf ^ 1);
+      const int vslot = n % C::kSlots;
+      wait_or_abort(&full[vslot], (n / C::kSlots) & 1, &abort_flag, a.err);
       const uint32_t vat = ring_u + vslot * C::kSlot;
       if (ragged) {
         // rows that are not visible hold anything, NaN too, or an earlier tile: make them 0
@@ -439,12 +495,17 @@ __global__ void __launch_bounds__(kThreads, 2)
         gqd::fence_proxy_async_smem();  // before the slot's next copy
       }
       sync_compute<kCompute>();
+      if (warp == 0) {  // every warp is done with what lies before the values of tile i
+        gqd::fence_proxy_async_smem();
+        fill(n + C::kSlots);
+      }
+      ++n;
 
       // ---- output columns warp * D/4 ..: o = o 2^(m_old - m) + V^T p. The instruction
       // truncates its sums, so it adds up one tile only; tiles are added in registers.
       {
-        const float f0 = fix[2 * q4], f1 = fix[2 * q4 + 1];
-        const uint8_t *pg = sP + g * C::kPStride;
+        const float f0 = fix[buf][2 * q4], f1 = fix[buf][2 * q4 + 1];
+        const uint8_t *pg = sP + buf * C::kPBytes + g * C::kPStride;
         constexpr int kSteps = T / C::kStep;
         uint32_t pf[kSteps][C::kParts][2];
 #pragma unroll
@@ -539,8 +600,6 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
         }
       }
-      __syncwarp();
-      if (lane == 0) gqt::mbar_arrive(&empty[vslot]);
     }
 
     // ---- the unit's output, or this CTA's part of it
@@ -587,6 +646,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       keys = visible(a, ++b);
     }
   }
+  if (warp == 0 && lane == 0 && *(volatile int *)&abort_flag)
+    // copies still in flight end before the CTA's memory goes away
+    for (uint32_t i = issued > C::kSlots ? issued - C::kSlots : 0; i < issued; ++i)
+      (void)gqd::mbar_wait_bounded(&full[i % C::kSlots], (i / C::kSlots) & 1, 100000000ull);
 }
 
 int log2_of(int64_t v) {
@@ -634,7 +697,7 @@ int launch(gq_ctx *ctx, const gq_kv_pages *p, Args &a) {
   const int grid = grid_for(a, C::T, 2 * ctx->num_sms);
   rc = bind_workspace(ctx, grid, a);
   if (rc != GQ_OK) return rc;
-  GQ_CUDA_TRY(ctx, gq_launch(ctx, paged_tiles_kernel<TYPE, D>, dim3(grid), dim3(kThreads), C::kSmem, a, kmap, vmap));
+  GQ_CUDA_TRY(ctx, gq_launch(ctx, paged_tiles_kernel<TYPE, D>, dim3(grid), dim3(kCompute), C::kSmem, a, kmap, vmap));
   return gq_paged_join_launch(ctx, a, grid);
 }
 
