@@ -119,9 +119,9 @@ struct Tile {
   // head_dim is split over KS warps where the q fragments of one warp would not fit its
   // registers (2 parts of 256 columns or 3 of 256 at 16 bits, 2 of 128 at 32)
   static constexpr int KS = TYPE == GQ_KV_F32 ? (D > 128 ? D / 128 : 1) : (D > 256 ? D / 256 : 1);
-  // 16-key tiles per warp: two for rows of 128 bytes, whose tiles would be small beside
-  // what a tile costs whatever its size
-  static constexpr int MT = kRow == 128 ? 2 : 1;
+  // 16-key tiles per warp: two where one would make a tile small beside what it costs
+  // whatever its size (barrier, softmax), and two leave room for three slots
+  static constexpr int MT = 16 * kComputeWarps / KS * kRow <= (KS > 1 ? 16384 : 8192) ? 2 : 1;
   static constexpr int T = 16 * kComputeWarps * MT / KS;
   static constexpr int kSlot = T * kRow;
   static constexpr int kParts = TYPE == GQ_KV_BF16 ? 3 : 2;
@@ -371,13 +371,15 @@ __global__ void __launch_bounds__(kCompute, 2)
         for (int p = 0; p < 3; ++p)
 #pragma unroll
           for (int k = 0; k < 4; ++k) c[x][p][k] = 0.0f;
+        // 16-byte pieces s * 2 and s * 2 + 1 of the rows; a piece's place in its 128 bytes is
+        // its number xor the row's, so steps of whole bits can be xor-ed on afterwards
         const int krow = (mt + x) * 16 + (lane & 15);
-        const uint32_t at = ring_u + slot * C::kSlot + row_at(krow), swz = (uint32_t)(krow & 7);
+        const uint32_t at = ring_u + slot * C::kSlot + row_at(krow) + (uint32_t)(ks * (C::kChunks / KS)) * piece +
+                            (((uint32_t)(lane >> 4) ^ (uint32_t)(krow & 7)) << 4);
 #pragma unroll
         for (int s = 0; s < (TYPE == GQ_KV_E4M3 ? C::kQSteps / 2 : C::kQSteps); ++s) {
           uint32_t k4[4];
-          const int ch = ks * (C::kRow / KS / 16) + s * 2;  // 16-byte piece of the row (two per load)
-          ldsm4(k4, at + (uint32_t)(ch >> 3) * piece + ((((uint32_t)(ch & 7) + (lane >> 4)) ^ swz) << 4));
+          ldsm4(k4, (at ^ (uint32_t)((s * 2 & 7) << 4)) + (uint32_t)(s >> 2) * piece);
           if constexpr (TYPE == GQ_KV_F32) {
             uint32_t hi[4], lo[4];
 #pragma unroll
@@ -531,19 +533,22 @@ __global__ void __launch_bounds__(kCompute, 2)
 #pragma unroll
           for (int s = 0; s < kSteps; ++s) {
             if constexpr (TYPE == GQ_KV_F32) {
-              // the instruction's keys t, t + 4 are rows 2t, 2t + 1: four rows two apart lie on different banks
+              // the instruction's keys t, t + 4 are rows 2t, 2t + 1: four rows two apart lie on
+              // different banks. Columns g and g + 8 of tile x are 16-byte pieces 4x + g/4 and
+              // two on of the warp's.
               const int k0 = s * 8 + 2 * q4;
-              const uint32_t r0 = vat + row_at(k0), r1 = vat + row_at(k0 + 1);
-              const uint32_t z0 = (uint32_t)(k0 & 7), z1 = (uint32_t)((k0 + 1) & 7);
+              constexpr int kWarpPieces = D / kComputeWarps / 4;
+              const uint32_t wp = (uint32_t)(warp * kWarpPieces), in = (wp >> 3) * piece + (uint32_t)(g & 3) * 4;
+              const uint32_t r0 = vat + row_at(k0) + in, r1 = vat + row_at(k0 + 1) + in;
+              const uint32_t c0 = (wp & 7) | (uint32_t)(g >> 2), z0 = (uint32_t)(2 * q4), z1 = z0 + 1;
+              const uint32_t at[4] = {r0 + ((c0 ^ z0) << 4), r0 + (((c0 ^ 2) ^ z0) << 4), r1 + ((c0 ^ z1) << 4),
+                                      r1 + (((c0 ^ 2) ^ z1) << 4)};
 #pragma unroll
               for (int x = 0; x < G; ++x) {
-                const int col = warp * (D / kComputeWarps) + (x0 + x) * 16 + g;  // and col + 8
-                const uint32_t c0 = (uint32_t)(col >> 2), c1 = c0 + 2, in = (uint32_t)(col & 3) * 4;
                 uint32_t hi[4], lo[4];
-                split_tf32(lds32(r0 + (c0 >> 3) * piece + (((c0 & 7) ^ z0) << 4) + in), hi[0], lo[0]);
-                split_tf32(lds32(r0 + (c1 >> 3) * piece + (((c1 & 7) ^ z0) << 4) + in), hi[1], lo[1]);
-                split_tf32(lds32(r1 + (c0 >> 3) * piece + (((c0 & 7) ^ z1) << 4) + in), hi[2], lo[2]);
-                split_tf32(lds32(r1 + (c1 >> 3) * piece + (((c1 & 7) ^ z1) << 4) + in), hi[3], lo[3]);
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                  split_tf32(lds32((at[y] ^ (uint32_t)(((x0 + x) & 1) << 6)) + (uint32_t)((x0 + x) >> 1) * piece), hi[y], lo[y]);
                 mma_tf32(c[x], lo, pf[s][0][0], pf[s][0][1]);
                 mma_tf32(c[x], hi, pf[s][1][0], pf[s][1][1]);
                 mma_tf32(c[x], hi, pf[s][0][0], pf[s][0][1]);
@@ -553,13 +558,14 @@ __global__ void __launch_bounds__(kCompute, 2)
               // of byte pairs gives columns 2g and 2g + 1 of two keys: row g of the
               // instruction is column 2g, row g + 8 column 2g + 1.
               const int key = s * 16 + (lane & 15);
-              const uint32_t rb = vat + row_at(key), z = (uint32_t)(key & 7);
+              constexpr int kWarpPieces = D / kComputeWarps / 16;
+              const uint32_t wp = (uint32_t)(warp * kWarpPieces);
+              const uint32_t at = vat + row_at(key) + (wp >> 3) * piece + ((((wp & 7) | (uint32_t)(lane >> 4)) ^ (uint32_t)(key & 7)) << 4);
               uint32_t af[G][4];
 #pragma unroll
               for (int x = 0; x < G; x += 2) {
-                const uint32_t ch = (uint32_t)(warp * (D / kComputeWarps) / 16 + x0 + x + (lane >> 4));
                 uint32_t v4[4];
-                ldsm4_t(v4, rb + (ch >> 3) * piece + (((ch & 7) ^ z) << 4));
+                ldsm4_t(v4, at ^ (uint32_t)((x0 + x) << 4));
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                   const uint32_t e = __byte_perm(v4[2 * h], 0, 0x3120), f = __byte_perm(v4[2 * h + 1], 0, 0x3120);
@@ -575,12 +581,13 @@ __global__ void __launch_bounds__(kCompute, 2)
                 for (int x = 0; x < G; ++x) mma_f16(c[x], af[x], pf[s][y][0], pf[s][y][1]);
             } else {
               const int key = s * 16 + (lane & 7) + (lane >> 4) * 8;
-              const uint32_t rb = vat + row_at(key), z = (uint32_t)(key & 7);
+              constexpr int kWarpPieces = D / kComputeWarps / 8;
+              const uint32_t wp = (uint32_t)(warp * kWarpPieces);
+              const uint32_t at = vat + row_at(key) + (wp >> 3) * piece + ((((wp & 7) | (uint32_t)((lane >> 3) & 1)) ^ (uint32_t)(key & 7)) << 4);
               uint32_t v4[G][4];
 #pragma unroll
               for (int x = 0; x < G; ++x) {
-                const uint32_t ch = (uint32_t)(warp * (D / kComputeWarps) / 8 + (x0 + x) * 2 + ((lane >> 3) & 1));
-                ldsm4_t(v4[x], rb + (ch >> 3) * piece + (((ch & 7) ^ z) << 4));
+                ldsm4_t(v4[x], (at ^ (uint32_t)(((x0 + x) * 2 & 7) << 4)) + (uint32_t)((x0 + x) >> 2) * piece);
               }
 #pragma unroll
               for (int y = C::kParts - 1; y >= 0; --y)
