@@ -214,65 +214,71 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const Args a) {
   }
 }
 
-// Adds up the parts of cut units. A CTA takes (unit, head, columns) in turn; its threads
-// are `wide` float4 columns times 256 / wide groups that share the parts, and the groups'
-// sums are added in order. wide is the most (up to a head's columns) that still gives
-// every CTA an item: many cut units of few parts are read in whole rows, a few long ones
-// by as many threads as there are. (Items of 128 columns for all: 11 us for 64 units of
-// 5 parts at head_dim 512.) A join inside the first launch was built two ways and was
-// slower: by the last CTA of a unit to arrive (up to 40 us after the last tile for a unit
-// of 99 parts of 16 KB), and by all CTAs of a cooperative launch, each waiting for its
-// units' parts and joining a share of their columns (4 us for 6 parts, 10-14 us for 300).
-constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinBatch = 8, kJoinNarrow = 8;
+// Adds up the parts of cut units. A CTA takes (unit, `wide` float4 columns of its heads)
+// in turn; its threads are wide columns times 256 / wide groups that share the parts, and
+// the groups' sums are added in order. wide is the most that leaves a thread no more parts
+// of the longest unit than it loads at once: one round of loads per item, and few items
+// (with items of 128 columns for all, 64 units of 5 parts took 11 us at head_dim 512).
+// A join inside the first launch was built two ways and was slower: by the last CTA of a
+// unit to arrive (up to 40 us after the last tile for a unit of 99 parts of 16 KB), and
+// by all CTAs of a cooperative launch, each waiting for its units' parts and joining a
+// share of their columns (4 us for 6 parts, 10-14 us for 300).
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinBatch = 8;
 
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Args a, int grid) {
   constexpr int kEach = (kMaxGrid + kJoinThreads - 1) / kJoinThreads;
   __shared__ int4 units[kMaxGrid];
-  __shared__ int counts[kJoinWarps];
+  __shared__ int counts[kJoinWarps], longest[kJoinWarps];
   __shared__ float4 sums[kJoinThreads];
-  __shared__ float2 group_ml[kJoinThreads / kJoinNarrow];
+  __shared__ float2 sum_ml[kJoinThreads];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
   // the list of cut units, in order of the CTAs they begin in
   int4 mine[kEach];
-  int have = 0;
+  int have = 0, most = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     const int c = tid * kEach + i;
     mine[i] = c < grid ? __ldcg(a.cut_units + c) : make_int4(0, 0, 0, 0);
     have += mine[i].z > 0;
+    most = max(most, mine[i].z);
   }
   int incl = have;
+  most = __reduce_max_sync(0xffffffffu, most);
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int up = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += up;
   }
-  if (lane == 31) counts[warp] = incl;
+  if (lane == 31) {
+    counts[warp] = incl;
+    longest[warp] = most;
+  }
   __syncthreads();
   int n = 0, at = incl - have;
 #pragma unroll
   for (int w = 0; w < kJoinWarps; ++w) {
     if (w < warp) at += counts[w];
     n += counts[w];
+    most = max(most, longest[w]);
   }
 #pragma unroll
   for (int i = 0; i < kEach; ++i)
     if (mine[i].z > 0) units[at++] = mine[i];
   __syncthreads();
 
-  const int cols = a.dim / 4;
-  int wide = kJoinThreads;
-  while (wide > kJoinNarrow && (wide >= 2 * cols || n * kHeads * ((cols + wide - 1) / wide) < (int)gridDim.x)) wide >>= 1;
-  const int groups = kJoinThreads / wide, group = tid / wide, slices = (cols + wide - 1) / wide, per_unit = kHeads * slices;
-  for (int item = blockIdx.x; item < n * per_unit; item += gridDim.x) {
-    const int4 unit = units[item / per_unit];
-    const int h = (item / slices) % kHeads, col = (item % slices) * wide + tid % wide;
+  int groups = 1;
+  while (groups * kJoinBatch < most && groups < kJoinThreads / 8) groups <<= 1;
+  const int wide = kJoinThreads / groups, group = tid / wide, cols = a.dim / 4;
+  const int slices = (kHeads * cols + wide - 1) / wide;
+  for (int item = blockIdx.x; item < n * slices; item += gridDim.x) {
+    const int4 unit = units[item / slices];
+    const int at = (item % slices) * wide + tid % wide, h = at / cols, col = at - h * cols;
     int head0, nh, kvh;
     unit_heads(a, unit.y, head0, nh, kvh);
-    if (h >= nh) continue;
-    const int parts = unit.z, first = unit.w, next = (first & ~1) + 2;  // slots: first, next, next + 2, ...
+    const bool real = h < nh;
+    const int parts = real ? unit.z : 0, first = unit.w, next = (first & ~1) + 2;  // slots: first, next, next + 2, ...
     const float2 *ml = reinterpret_cast<const float2 *>(a.part_ml);
     const float4 *part = reinterpret_cast<const float4 *>(a.part_o);
     // each group adds its parts to a maximum of its own, kJoinBatch parts' loads at a time
@@ -289,7 +295,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Args a, 
         if (p < parts) {
           const int64_t s = (int64_t)(p == 0 ? first : next + 2 * (p - 1)) * kHeads + h;
           x[k] = __ldcg(ml + s);
-          if (col < cols) v[k] = __ldcg(part + s * cols + col);
+          v[k] = __ldcg(part + s * cols + col);
         }
       }
       float top = m;
@@ -311,15 +317,14 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Args a, 
     }
     __syncthreads();  // the sums of the item before are read
     sums[tid] = o;
-    if (tid % wide == 0) group_ml[group] = make_float2(m, l);
+    sum_ml[tid] = make_float2(m, l);
     __syncthreads();
-    if (group == 0 && col < cols) {
-      m = -INFINITY;
-      for (int k = 0; k < groups; ++k) m = fmaxf(m, group_ml[k].x);
+    if (group == 0 && real) {
+      for (int k = 1; k < groups; ++k) m = fmaxf(m, sum_ml[k * wide + tid].x);
       l = 0.0f;
       o = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int k = 0; k < groups; ++k) {
-        const float2 x = group_ml[k];
+        const float2 x = sum_ml[k * wide + tid];
         const float4 v = sums[k * wide + tid];
         const float f = x.x == -INFINITY ? 0.0f : exp2f(x.x - m);
         l = fmaf(f, x.y, l);
@@ -345,7 +350,7 @@ cudaError_t rows_launch(gq_ctx *ctx, int grid, const Args &a) {
 int gq_paged_join_launch(gq_ctx *ctx, const Args &a, int grid) {
   if (grid <= 1) return GQ_OK;  // nothing can be cut
   // two CTAs per SM, fewer where even the narrowest items of all possible cuts are fewer
-  const int64_t most = (int64_t)(grid - 1) * kHeads * ((a.dim / 4 + kJoinNarrow - 1) / kJoinNarrow);
+  const int64_t most = (int64_t)(grid - 1) * ((kHeads * a.dim / 4 + 7) / 8);
   const int items = (int)std::min<int64_t>(most, 2 * (int64_t)ctx->num_sms);
   GQ_CUDA_TRY(ctx, gq_launch(ctx, paged_join_kernel, dim3(items), dim3(kJoinThreads), 0, a, grid));
   return GQ_OK;
