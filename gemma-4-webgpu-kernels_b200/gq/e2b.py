@@ -327,23 +327,7 @@ class Decoder:
             self.w[p + "ple_gate"] = qt(p + "ple_gate", P, H, c.ple_bits)
             self.w[p + "ple_proj"] = qt(p + "ple_proj", H, P, c.ple_bits)
 
-        # ---- KV caches of the source layers ----------------------------------------
-        self.kcache, self.vcache = {}, {}
-        for i in range(L):
-            if c.kv_source(i) != i:
-                continue
-            d = c.heads_kv * c.dh(i)
-            kc = torch.zeros(batch, self.capacity, d, dtype=f32, device=dev)
-            vc = torch.zeros(batch, self.capacity, d, dtype=f32, device=dev)
-            if cache_len:
-                if weights is not None and kv_device_seed is None:
-                    kk, vv = weights.kv_prefix(i, batch, cache_len)
-                    kc[:, :cache_len] = torch.from_numpy(kk).to(dev)
-                    vc[:, :cache_len] = torch.from_numpy(vv).to(dev)
-                else:
-                    kc[:, :cache_len].normal_(generator=kv_gen)
-                    vc[:, :cache_len].normal_(generator=kv_gen)
-            self.kcache[i], self.vcache[i] = kc, vc
+        self._make_kv(weights, kv_gen, kv_device_seed)
 
         # ---- activations and step inputs ------------------------------------------
         B = batch
@@ -374,6 +358,45 @@ class Decoder:
         self.position = -1
         self.set_position(cache_len)
 
+    # ---- the KV cache: what a decoder with another kind of cache overrides -------------
+    def _make_kv(self, weights, kv_gen, kv_device_seed) -> None:
+        """The caches of the source layers, with cache_len seeded rows."""
+        torch, c, batch, cache_len, dev = self.torch, self.cfg, self.batch, self.cache_len, self.g.torch_device
+        self.kcache, self.vcache = {}, {}
+        for i in range(c.layers):
+            if c.kv_source(i) != i:
+                continue
+            d = c.heads_kv * c.dh(i)
+            kc = torch.zeros(batch, self.capacity, d, dtype=torch.float32, device=dev)
+            vc = torch.zeros(batch, self.capacity, d, dtype=torch.float32, device=dev)
+            if cache_len:
+                if weights is not None and kv_device_seed is None:
+                    kk, vv = weights.kv_prefix(i, batch, cache_len)
+                    kc[:, :cache_len] = torch.from_numpy(kk).to(dev)
+                    vc[:, :cache_len] = torch.from_numpy(vv).to(dev)
+                else:
+                    kc[:, :cache_len].normal_(generator=kv_gen)
+                    vc[:, :cache_len].normal_(generator=kv_gen)
+            self.kcache[i], self.vcache[i] = kc, vc
+
+    def _begin_calls(self, add) -> None:
+        """Calls before the embeddings."""
+
+    def _end_calls(self, add) -> None:
+        """Calls after the lm_head."""
+
+    def _new_rows(self, src: int, p: int, kvd: int):
+        """Where source layer src's new key and value rows go: (k, v, stride between sequences)."""
+        kc, vc = self.kcache[src], self.vcache[src]
+        return c_void_p(kc.data_ptr() + 4 * p * kvd), c_void_p(vc.data_ptr() + 4 * p * kvd), self.capacity * kvd
+
+    def _attention_calls(self, add, pre: str, i: int, src: int, dh: int, p: int) -> None:
+        """Attention of layer i over source layer src's cache, into self.attn."""
+        c, V = self.cfg, lambda t: c_void_p(t.data_ptr())  # noqa: E731
+        add(pre + "attention", self.g.lib.gq_attention, self.g.ctx, V(self.qr), self.batch, 1, c.heads_q, dh,
+            V(self.kcache[src]), V(self.vcache[src]), p + 1, c.heads_kv, self.capacity * c.heads_kv * dh, V(self.pos),
+            None, 0, c_float(1.0), c.window_of(i), c_float(0.0), GQ_ATTN_KPOS_IDENTITY, V(self.attn))
+
     # ---- the step --------------------------------------------------------------------
     def set_position(self, p: int) -> None:
         """Steps write cache slot p (all sequences) and attend over slots [0, p]."""
@@ -397,13 +420,13 @@ class Decoder:
         calls = []
         add = lambda label, fn, *args: calls.append((label, fn, args))  # noqa: E731
 
+        self._begin_calls(add)
         # embeddings and per-layer inputs (rust/src/model.rs:152-177)
         add("embed", lib.gq_embed_rows, ctx, Q("embed"), V(self.ids), B, c_float(math.sqrt(H)), V(self.h))
         add("embed_ple", lib.gq_embed_rows, ctx, Q("embed_ple"), V(self.ids), B, c_float(math.sqrt(P)), V(self.emb))
         add("ple_model_proj", lib.gq_linear_bf16, ctx, V(self.h), B, H, F("ple_model_proj"), L * P, V(self.proj))
         add("ple_combine", lib.gq_add_rms_norm, ctx, V(self.emb), V(self.proj), B * L, P, F("ple_proj_norm"), eps,
             V(self.rsqrt2), V(self.ple))
-        S = p + 1
         # input norm of layer 0; later layers get theirs fused into the previous layer's last norm
         add("l0.input_norm", lib.gq_rms_norm, ctx, V(self.h), B, H, F("l0.input_ln"), eps, V(self.x), H)
         fuse = self.fuse_norms
@@ -421,9 +444,7 @@ class Decoder:
             dh = c.dh(i)
             theta, rot = c.rope(i)
             src = c.kv_source(i)
-            kc, vc = self.kcache[src], self.vcache[src]
             kvd = c.heads_kv * dh
-            cstride = self.capacity * kvd
             # attention block (rust/src/model.rs:214-219, 233-300)
             # the previous layer's closing norm (residual + PLE norm, layer scalar,
             # this layer's input norm), fused into this layer's first projection
@@ -438,10 +459,10 @@ class Decoder:
                           pre + "qkv_proj", None, None, 0, self.qkv)
                 else:
                     add(pre + "qkv_proj", lib.gq_linear, ctx, V(self.x), B, H, Q(pre + "qkv_proj"), V(self.qkv))
+                kp, vp, cstride = self._new_rows(i, p, kvd)
                 add(pre + "qkv_norm_rope", lib.gq_qkv_norm_rope, ctx, V(self.qkv), B, (c.heads_q + 2 * c.heads_kv) * dh,
                     c.heads_q, c.heads_kv, dh, F(pre + "q_norm"), F(pre + "k_norm"), eps, V(self.pos),
-                    c_float(theta), rot, V(self.qr), c.heads_q * dh, c_void_p(kc.data_ptr() + 4 * p * kvd), cstride,
-                    c_void_p(vc.data_ptr() + 4 * p * kvd), cstride)
+                    c_float(theta), rot, V(self.qr), c.heads_q * dh, kp, cstride, vp, cstride)
             else:
                 if pro:
                     fused(pre + "q_proj", 0, prev + "ple_norm", prev + "layer_scalar", pre + "input_ln",
@@ -450,9 +471,7 @@ class Decoder:
                     add(pre + "q_proj", lib.gq_linear, ctx, V(self.x), B, H, Q(pre + "q_proj"), V(self.q))
                 add(pre + "q_norm_rope", lib.gq_head_norm_rope, ctx, V(self.q), B, c.heads_q, dh, F(pre + "q_norm"),
                     eps, V(self.pos), c_float(theta), rot, V(self.qr), c.heads_q * dh)
-            add(pre + "attention", lib.gq_attention, ctx, V(self.qr), B, 1, c.heads_q, dh, V(kc), V(vc), S,
-                c.heads_kv, cstride, V(self.pos), None, 0, c_float(1.0), c.window_of(i), c_float(0.0),
-                GQ_ATTN_KPOS_IDENTITY, V(self.attn))
+            self._attention_calls(add, pre, i, src, dh, p)
             add(pre + "o_proj", lib.gq_linear, ctx, V(self.attn), B, c.heads_q * dh, Q(pre + "o_proj"), V(self.o))
             # h = h + post_attn_norm(o), then x = pre_ffn_norm(h): one pass (rust/src/model.rs:219, 223)
             # GeGLU MLP (rust/src/model.rs:221-227)
@@ -489,6 +508,7 @@ class Decoder:
                 V(self.logits), c.vocab, 0)
         else:  # this rank's vocab rows, stored into every rank's logits buffer `par` (set per step)
             self._lm_calls = [self.peer.device_calls(self.x.data_ptr(), B, H, par) for par in (0, 1)]
+        self._end_calls(add)
         return calls
 
     def run(self) -> None:

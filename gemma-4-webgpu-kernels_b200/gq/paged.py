@@ -1,0 +1,266 @@
+"""Decoding many requests of different lengths at once, over a paged KV cache.
+
+``PagedDecoder`` is the decode step of ``gq.e2b`` with the cache in pages: each of its
+``batch`` places holds a request with a length of its own, and a step
+
+* takes pages for the new tokens (``gq_paged_reserve``: positions and slots of the step),
+* writes each KV layer's new rows into their pages (``gq_paged_append``),
+* attends every request over its own pages (``gq_paged_attention``),
+* applies each request's penalties, biases and grammar mask to its logits
+  (``gq_process_logits``) and samples (``gq_sample_rows``),
+* takes back the pages of requests that have ended (``gq_paged_release``).
+
+Lengths, tables, free pages, histories and controls live on the device, so one recorded
+graph serves every step. No counterpart in the reference (one sequence, contiguous
+caches).
+
+    python -m gq.paged [--requests 64] [--steps 32] [--type bf16]
+
+decodes with synthetic E2B-shaped weights and prints the time of a step.
+"""
+from __future__ import annotations
+
+import argparse
+import ctypes
+import sys
+from ctypes import c_float, c_void_p
+from typing import Optional, Sequence
+
+import numpy as np
+
+from . import _abi, e2b
+from ._abi import GqError
+
+KEEP_ALL = 2 ** 31 - 1
+
+
+class PagedDecoder(e2b.Decoder):
+    """One decode step of ``batch`` requests through the C ABI, over pages.
+
+    max_len: the most tokens of a request (its block table row); page_size, kv_type
+    ("f32", "f16", "bf16", "e4m3" with k_scale / v_scale) and n_pages (default: enough
+    for every request at max_len) describe the pool that each source layer has. ``lens``
+    are the requests' lengths, filled by ``extend``; a place whose length is 0 and that
+    was ended idles: it decodes from an empty cache and gives its page back every step.
+
+    Controls, all device tensors that may be changed between steps: ``penalties``
+    [batch, 3] (repetition, presence, frequency), ``prompt_lens`` [batch], ``history``
+    [batch, max_len] (tokens by position), and, given at construction because their sizes
+    belong to the recorded step, ``bias`` (ids, values, offsets) and ``masks``
+    (words, rows); see gq_process_logits in include/gq.h. ``sample``: temperature, top_k,
+    top_p of gq_sample_rows."""
+
+    def __init__(self, g, cfg: e2b.Config, weights: Optional[e2b.Weights], batch: int, max_len: int, page_size: int = 16,
+                 kv_type: str = "bf16", n_pages: Optional[int] = None, k_scale: float = 1.0, v_scale: float = 1.0,
+                 sample=(0.0, 0, 1.0), bias=None, masks=None, seed: int = 1, device_init_seed: Optional[int] = None):
+        self.page_size, self.kv_type, self.width = page_size, kv_type, -(-max_len // page_size)
+        self.n_pages = n_pages if n_pages is not None else batch * self.width
+        self.k_scale, self.v_scale = k_scale, v_scale
+        self.bias, self.masks = bias, masks
+        self.opts = _abi.SampleOpts(float(sample[0]), int(sample[1]), float(sample[2]), 1.0)
+        self.seed = seed
+        super().__init__(g, cfg, weights, batch, cache_len=0, capacity=max_len, device_init_seed=device_init_seed,
+                         fuse_norms=False)
+        self.graph = None
+        self.torch.cuda.synchronize(g.torch_device)
+
+    # ---- the cache -------------------------------------------------------------------
+    def _make_kv(self, weights, kv_gen, kv_device_seed) -> None:
+        torch, c, g, B = self.torch, self.cfg, self.g, self.batch
+        dev, i32 = g.torch_device, torch.int32
+        dtypes = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "e4m3": torch.float8_e4m3fn}
+        if self.kv_type not in dtypes:
+            raise GqError(_abi.GQ_ERR_UNSUPPORTED, f"PagedDecoder: kv_type {self.kv_type}")
+        self.kcache, self.vcache, self.pages = {}, {}, {}
+        for i in range(c.layers):
+            if c.kv_source(i) == i:
+                shape = (self.n_pages, c.heads_kv, self.page_size, c.dh(i))
+                k, v = (torch.empty(shape, dtype=dtypes[self.kv_type], device=dev) for _ in range(2))
+                self.pages[i] = g.kv_pages(k, v, self.k_scale, self.v_scale)
+        self.table = torch.full((B, max(self.width, 1)), -1, dtype=i32, device=dev)
+        self.free = torch.arange(self.n_pages, dtype=i32, device=dev)
+        self.count = torch.tensor([self.n_pages], dtype=i32, device=dev)
+        self.lens = torch.zeros(B, dtype=i32, device=dev)
+        self.one = torch.ones(B, dtype=i32, device=dev)
+        self.keep = torch.full((B,), KEEP_ALL, dtype=i32, device=dev)
+        self.slots = torch.zeros(B, dtype=torch.int64, device=dev)
+        self.owners = torch.zeros(B, dtype=i32, device=dev)
+        d = c.heads_kv * c.global_head_dim
+        self.new_k, self.new_v = (torch.zeros(B, max(d, c.heads_kv * c.head_dim), device=dev) for _ in range(2))
+        # controls of the logits
+        self.history = torch.zeros(B, self.capacity, dtype=i32, device=dev)
+        self.prompt_lens = torch.zeros(B, dtype=i32, device=dev)
+        self.penalties = torch.tensor([[1.0, 0.0, 0.0]], device=dev).repeat(B, 1)
+        self.controlled = torch.empty(B, c.vocab, device=dev)
+        self.tokens = torch.zeros(B, dtype=i32, device=dev)
+        self.rng = torch.arange(self.seed, self.seed + B, dtype=torch.int64, device=dev)
+        torch.cuda.synchronize(dev)
+
+    def _stream(self):
+        return self.torch.cuda.ExternalStream(self.g.stream_ptr(), device=self.g.torch_device)
+
+    def extend(self, new_lens: Sequence[int], rows, tokens: Optional[Sequence[Sequence[int]]] = None) -> None:
+        """Add new_lens[b] tokens to request b without decoding (a prompt's cache made
+        elsewhere): rows(layer) gives their keys and values, f32 [sum, heads_kv *
+        head_dim] in request order, for each source layer; tokens, when given, each
+        request's ids (its prompt, for the penalties). Raises when the pages do not
+        suffice; nothing is taken then."""
+        torch, c, g = self.torch, self.cfg, self.g
+        dev, total = g.torch_device, int(np.sum(new_lens))
+        place = lambda dt: torch.empty(total, dtype=dt, device=dev)  # noqa: E731
+        before = self.lens.tolist()
+        new, slots = torch.tensor(list(new_lens), dtype=torch.int32, device=dev), place(torch.int64)
+        pos, owners = place(torch.int32), place(torch.int32)
+        kv = {i: rows(i) for i in self.pages} if total else {}
+        torch.cuda.synchronize(dev)  # (the rows are torch's, the calls go to the backend's stream)
+        g.paged_reserve(self.lens, new, self.page_size, self.table, self.free, self.count, slots, pos, owners, self.lens,
+                        self.count)
+        g.flush()
+        for i, (k, v) in kv.items():
+            g.paged_append(self.pages[i], k.view(total, c.heads_kv, c.dh(i)), v.view(total, c.heads_kv, c.dh(i)), slots)
+        g.flush()
+        if tokens is not None:
+            for b, ids in enumerate(tokens):
+                self.history[b, before[b]:before[b] + len(ids)] = torch.tensor(list(ids), dtype=torch.int32, device=dev)
+        self.prompt_lens.copy_(self.lens)
+        self.keep.masked_fill_(new > 0, KEEP_ALL)
+        torch.cuda.synchronize(dev)
+
+    def end(self, places: Sequence[int]) -> None:
+        """The requests at these places end: the next step gives their pages back."""
+        with self.torch.cuda.stream(self._stream()):
+            self.keep[self.torch.tensor(list(places), device=self.g.torch_device)] = 0
+
+    # ---- the step ----------------------------------------------------------------------
+    def set_position(self, p: int) -> None:
+        """(Every request has its own position; the calls are the same for every step.)"""
+        self._calls = self._build_calls(0)
+
+    def _begin_calls(self, add) -> None:
+        V = lambda t: c_void_p(t.data_ptr())  # noqa: E731
+        add("reserve", self.g.lib.gq_paged_reserve, self.g.ctx, self.batch, self.page_size, V(self.lens), V(self.one),
+            V(self.table), self.table.shape[1], V(self.free), self.n_pages, V(self.count), V(self.count), self.batch,
+            V(self.slots), V(self.pos), V(self.owners), V(self.lens))
+
+    def _new_rows(self, src: int, p: int, kvd: int):
+        return c_void_p(self.new_k.data_ptr()), c_void_p(self.new_v.data_ptr()), kvd
+
+    def _attention_calls(self, add, pre: str, i: int, src: int, dh: int, p: int) -> None:
+        c, V, lib, ctx = self.cfg, lambda t: c_void_p(t.data_ptr()), self.g.lib, self.g.ctx  # noqa: E731
+        pages = c_void_p(self.pages[src].ref)
+        if src == i:
+            add(pre + "append", lib.gq_paged_append, ctx, pages, V(self.new_k), V(self.new_v), self.batch, 0, 0,
+                V(self.slots))
+        add(pre + "attention", lib.gq_paged_attention, ctx, pages, V(self.qr), self.batch, c.heads_q, 0, V(self.table),
+            self.table.shape[1], V(self.lens), c_float(1.0), c.window_of(i), c_float(0.0), V(self.attn))
+
+    def _end_calls(self, add) -> None:
+        V = lambda t: c_void_p(t.data_ptr()) if t is not None else None  # noqa: E731
+        lib, ctx, B, vocab = self.g.lib, self.g.ctx, self.batch, self.cfg.vocab
+        ids, values, offsets = self.bias or (None, None, None)
+        words, rows = self.masks or (None, None)
+        add("process_logits", lib.gq_process_logits, ctx, V(self.logits), B, vocab, vocab, V(self.history), self.capacity,
+            V(self.prompt_lens), V(self.lens), V(self.penalties), V(ids), V(values), V(offsets), V(words),
+            words.shape[0] if words is not None else 0, words.shape[1] if words is not None else 0, V(rows),
+            V(self.controlled), vocab)
+        add("sample", lib.gq_sample_rows, ctx, V(self.controlled), B, vocab, vocab, ctypes.byref(self.opts), None, 0, 0,
+            V(self.rng), V(self.tokens))
+        add("release", lib.gq_paged_release, ctx, B, self.page_size, V(self.lens), V(self.keep), V(self.table),
+            self.table.shape[1], V(self.free), self.n_pages, V(self.count), V(self.count), V(self.lens))
+
+    def step(self, ids=None):
+        """Decode one token of every request: ids [batch] (default: the tokens that the last
+        step sampled) in, the sampled ``tokens`` [batch] out (a device tensor, valid until
+        the next step). Enqueued; a page shortage shows at the next ``g.flush()``."""
+        torch = self.torch
+        with torch.cuda.stream(self._stream()):
+            if ids is None:
+                self.ids.copy_(self.tokens)
+            else:
+                self.ids.copy_(torch.as_tensor(np.asarray(ids, dtype=np.int32).reshape(self.batch)))
+            at = self.lens.long().clamp(max=self.capacity - 1)[:, None]
+            self.history.scatter_(1, at, self.ids[:, None])
+        if self.graph is not None:
+            self.g.replay(self.graph)
+        else:
+            self.run()
+        return self.tokens
+
+    def record_steps(self) -> None:
+        """Record the step into a graph that ``step`` replays from now on (the backend must
+        own its stream). Runs one step first, which sizes the workspaces, and takes its
+        token back: lengths, pages and random states are as before."""
+        torch = self.torch
+        self.g.flush()
+        saved = [(t, t.clone()) for t in (self.lens, self.table, self.free, self.count, self.rng, self.tokens)]
+        torch.cuda.synchronize(self.g.torch_device)
+        self.run()
+        self.g.flush()
+        for t, old in saved:
+            t.copy_(old)
+        torch.cuda.synchronize(self.g.torch_device)
+        self.graph = self.g.record(self.run)
+
+    def close(self) -> None:
+        if self.graph is not None:
+            self.g.destroy_graph(self.graph)
+            self.graph = None
+        super().close()
+        self.pages.clear()
+
+    def kv_bytes(self) -> int:
+        """K and V bytes that a step's attention reads at the present lengths."""
+        c, size = self.cfg, {"f32": 4, "e4m3": 1}.get(self.kv_type, 2)
+        lens, tot = self.lens.tolist(), 0
+        for i in range(c.layers):
+            w = c.window_of(i)
+            tot += 2 * sum(min(n, w) if w else n for n in lens) * c.heads_kv * c.dh(i) * size
+        return tot
+
+
+def main(argv=None) -> int:
+    ap = argparse.ArgumentParser(prog="gq.paged")
+    ap.add_argument("--requests", type=int, default=64)
+    ap.add_argument("--max-len", type=int, default=2048)
+    ap.add_argument("--steps", type=int, default=32)
+    ap.add_argument("--type", choices=["f32", "f16", "bf16", "e4m3"], default="bf16")
+    args = ap.parse_args(argv)
+
+    import torch
+
+    from . import CudaBackend
+
+    g = CudaBackend(0, own_stream=True)
+    cfg, B = e2b.e2b_config(), args.requests
+    scales = dict(k_scale=1 / 32, v_scale=1 / 32) if args.type == "e4m3" else {}
+    dec = PagedDecoder(g, cfg, None, B, args.max_len, kv_type=args.type, sample=(1.0, 64, 0.95), device_init_seed=5, **scales)
+    gen = torch.Generator(device=g.torch_device)
+    gen.manual_seed(6)
+    room = max(1, args.max_len - args.steps - 4)
+    lens = np.random.default_rng(7).integers(1, room + 1, B)
+    total = int(lens.sum())
+
+    def rows(layer):
+        return [torch.randn(total, cfg.heads_kv * cfg.dh(layer), generator=gen, device=g.torch_device) for _ in range(2)]
+
+    dec.extend(lens, rows)
+    dec.penalties.copy_(torch.tensor([[1.1, 0.2, 0.1]], device=g.torch_device))
+    dec.record_steps()
+    dec.step(np.arange(B) % cfg.vocab)
+    g.flush()
+    t0, t1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    t0.record(dec._stream())
+    for _ in range(args.steps):
+        dec.step()
+    t1.record(dec._stream())
+    g.flush()
+    ms = t0.elapsed_time(t1) / args.steps
+    print(f"{B} requests of 1 to {room} tokens ({args.type} pages): {ms:.3f} ms per step, {B / ms * 1e3:.0f} tokens/s, "
+          f"{dec.kv_bytes() / 1e6:.0f} MB of keys and values read per step")
+    dec.close()
+    g.close()
+    return 0
+
+
+if __name__ == "__main__":
+    sys.exit(main())
