@@ -126,7 +126,9 @@ class KvPages:
     k: object
     v: object
     struct: object = field(repr=False, default=None)
-    ref: object = field(repr=False, default=None)
+    ref: int = 0       # address of struct
+    row: int = 0       # values of a token: heads * head_dim
+    head_dim: int = 0
 
 
 class Chain:
@@ -541,68 +543,73 @@ class CudaBackend:
             if t.numel() and (not t[0].is_contiguous() or (n > 1 and t.stride(0) != apart)):
                 raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "kv_pages: a page's values must be contiguous, k and v strided alike")
         st = _abi.KvPagesStruct(k.data_ptr(), v.data_ptr(), n, ps, h, d, apart, types[k.dtype], float(k_scale), float(v_scale))
-        return KvPages(k, v, st, ctypes.addressof(st))
+        return KvPages(k, v, st, ctypes.addressof(st), h * d, d)
 
-    def _dev(self, t, dtype, what: str, numel: Optional[int] = None) -> int:
-        """Pointer of a contiguous device tensor, checked."""
-        if t.dtype != dtype or t.device != self.torch_device or not t.is_contiguous():
-            raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, f"{what} must be a contiguous {dtype} tensor on the backend's device")
-        if numel is not None and t.numel() < numel:
-            raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, f"{what} has {t.numel()} elements, {numel} are needed")
+    # (Single calls of these ops take the GPU 2-9 us, as long as the checks and the
+    # conversions of 8-19 arguments take the host: the checks below ask for as little as
+    # they can, and only a failed one says what was wrong.)
+    def _dev(self, t, dtype, what: str, numel: int = 0) -> int:
+        """Pointer of a contiguous device tensor of at least numel elements, checked."""
+        if t.dtype is not dtype or t.get_device() != self.device or not t.is_contiguous() or t.numel() < numel:
+            raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT,
+                          f"{what} must be a contiguous {dtype} tensor of at least {numel} elements on the backend's device")
         return t.data_ptr()
 
-    def _rows(self, x, width: int, what: str):
-        """A f32 device tensor [rows, ...] as (tensor, rows, row stride): rows may lie apart,
-        a row's `width` values are contiguous."""
+    def _rows(self, x, rows: int, width: int, what: str):
+        """A f32 device tensor of `rows` rows as (pointer, row stride): rows may lie apart, a
+        row's `width` values are contiguous."""
         t = x.data if isinstance(x, GqTensor) else x
-        if t.dtype != self._torch.float32 or t.device != self.torch_device or t.dim() < 2:
-            raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, f"{what} must be a float32 tensor [rows, ...] on the backend's device")
-        rows = t.shape[0]
-        if t.numel() != rows * width or not (t.is_contiguous() or (t[0].is_contiguous() and t.stride(0) >= width)):
+        if t.dtype is not self._torch.float32 or t.get_device() != self.device or t.numel() != rows * width:
+            raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT,
+                          f"{what} must be {rows} rows of {width} float32 values on the backend's device")
+        if t.is_contiguous():
+            return t.data_ptr(), width
+        if t.dim() < 2 or t.shape[0] != rows or not t[0].is_contiguous() or t.stride(0) < width:
             raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, f"{what}: a row must be {width} contiguous values, rows apart")
-        return t, rows, (width if t.is_contiguous() else t.stride(0))
+        return t.data_ptr(), t.stride(0)
 
     def _table(self, block_table, batch: int, what: str):
-        i32 = self._torch.int32
-        if block_table.dim() != 2 or block_table.shape[0] < batch:
+        shape = block_table.shape
+        if len(shape) != 2 or shape[0] < batch:
             raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, f"{what}: block_table must be [batch, pages]")
-        return self._dev(block_table, i32, f"{what}: block_table"), block_table.shape[1]
+        return self._dev(block_table, self._torch.int32, "block_table"), shape[1]
 
     def paged_reserve(self, seq_lens, new_lens, page_size: int, block_table, free_pages, free_count, slots, positions,
                       owners, totals, free_left) -> None:
         """Take pages for each request's new tokens and number the tokens (gq_paged_reserve):
         int32 device tensors, slots int64; slots, positions and owners have one place per
         token of the (padded) step; totals may be seq_lens and free_left free_count."""
-        i32, n, m = self._torch.int32, seq_lens.numel(), slots.numel()
+        d, i32, n, m = self._dev, self._torch.int32, seq_lens.numel(), slots.numel()
         tp, width = self._table(block_table, n, "paged_reserve")
-        d = self._dev
-        self._check(self.lib.gq_paged_reserve(
+        rc = self.lib.gq_paged_reserve(
             self.ctx, n, page_size, d(seq_lens, i32, "seq_lens"), d(new_lens, i32, "new_lens", n), tp, width,
             d(free_pages, i32, "free_pages"), free_pages.numel(), d(free_count, i32, "free_count", 1),
             d(free_left, i32, "free_left", 1), m, d(slots, self._torch.int64, "slots"), d(positions, i32, "positions", m),
-            d(owners, i32, "owners", m), d(totals, i32, "totals", n)), "paged_reserve")
+            d(owners, i32, "owners", m), d(totals, i32, "totals", n))
+        if rc:
+            self._check(rc, "paged_reserve")
 
     def paged_release(self, seq_lens, keep_lens, page_size: int, block_table, free_pages, free_count, totals,
                       free_left) -> None:
         """Give back the pages past each request's keep_lens tokens (gq_paged_release)."""
-        i32, n = self._torch.int32, seq_lens.numel()
+        d, i32, n = self._dev, self._torch.int32, seq_lens.numel()
         tp, width = self._table(block_table, n, "paged_release")
-        d = self._dev
-        self._check(self.lib.gq_paged_release(
+        rc = self.lib.gq_paged_release(
             self.ctx, n, page_size, d(seq_lens, i32, "seq_lens"), d(keep_lens, i32, "keep_lens", n), tp, width,
             d(free_pages, i32, "free_pages"), free_pages.numel(), d(free_count, i32, "free_count", 1),
-            d(free_left, i32, "free_left", 1), d(totals, i32, "totals", n)), "paged_release")
+            d(free_left, i32, "free_left", 1), d(totals, i32, "totals", n))
+        if rc:
+            self._check(rc, "paged_release")
 
     def paged_append(self, pages: KvPages, k, v, slots) -> None:
         """Write rows k, v [T, heads, head_dim] f32 (token strides free) to slots [T] int64
         of the pages, rounded to their type (gq_paged_append)."""
-        width = pages.struct.heads * pages.struct.head_dim
-        kt, n, ks = self._rows(k, width, "paged_append: k")
-        vt, nv, vs = self._rows(v, width, "paged_append: v")
-        if n != nv or n != slots.numel():
-            raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "paged_append: k, v and slots must have as many rows")
-        self._check(self.lib.gq_paged_append(self.ctx, pages.ref, kt.data_ptr(), vt.data_ptr(), n, ks, vs,
-                                             self._dev(slots, self._torch.int64, "slots")), "paged_append")
+        n = slots.numel()
+        kp, ks = self._rows(k, n, pages.row, "paged_append: k")
+        vp, vs = self._rows(v, n, pages.row, "paged_append: v")
+        rc = self.lib.gq_paged_append(self.ctx, pages.ref, kp, vp, n, ks, vs, self._dev(slots, self._torch.int64, "slots"))
+        if rc:
+            self._check(rc, "paged_append")
 
     def paged_attention(self, pages: KvPages, q, block_table, seq_lens, scale: float = 1.0, sliding_window: int = 0,
                         attn_softcap: float = 0.0, out=None):
@@ -610,19 +617,20 @@ class CudaBackend:
         q [batch, hq, head_dim] f32 (token stride free), block_table [batch, pages] and
         seq_lens [batch] int32 -> [batch, hq * head_dim] (`out`, or a new tensor)."""
         t = q.data if isinstance(q, GqTensor) else q
-        batch = seq_lens.numel()
-        dim = pages.struct.head_dim
-        if t.dim() != 3 or t.shape[0] != batch or t.shape[2] != dim:
+        batch, shape = seq_lens.numel(), t.shape
+        if len(shape) != 3 or shape[0] != batch or shape[2] != pages.head_dim:
             raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "paged_attention: q must be [batch, hq, head_dim]")
-        hq = t.shape[1]
-        t, _, qs = self._rows(t, hq * dim, "paged_attention: q")
-        tp, width = self._table(block_table, batch, "paged_attention")
-        y = out if out is not None else self._alloc((batch, hq * dim))
+        hq = shape[1]
+        width = hq * shape[2]
+        qp, qs = self._rows(t, batch, width, "paged_attention: q")
+        tp, entries = self._table(block_table, batch, "paged_attention")
+        y = out if out is not None else self._alloc((batch, width))
         yt = y.data if isinstance(y, GqTensor) else y
-        self._check(self.lib.gq_paged_attention(
-            self.ctx, pages.ref, t.data_ptr(), batch, hq, qs, tp, width, self._dev(seq_lens, self._torch.int32, "seq_lens"),
-            scale, sliding_window, attn_softcap, self._dev(yt, self._torch.float32, "out", batch * hq * dim)),
-            "paged_attention")
+        rc = self.lib.gq_paged_attention(
+            self.ctx, pages.ref, qp, batch, hq, qs, tp, entries, self._dev(seq_lens, self._torch.int32, "seq_lens"), scale,
+            sliding_window, attn_softcap, self._dev(yt, self._torch.float32, "out", batch * width))
+        if rc:
+            self._check(rc, "paged_attention")
         return y
 
     def process_logits(self, logits, tokens=None, prompt_lens=None, lens=None, penalties=None, bias_ids=None,
@@ -635,34 +643,38 @@ class CudaBackend:
         torch, d = self._torch, self._dev
         i32, f32 = torch.int32, torch.float32
         lt = logits.data if isinstance(logits, GqTensor) else logits
-        if lt.dim() != 2:
+        shape = lt.shape
+        if len(shape) != 2:
             raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "process_logits: logits must be [m, vocab]")
-        m, vocab = lt.shape
-        lt, _, ld = self._rows(lt, vocab, "process_logits: logits")
+        m, vocab = shape
+        lp, ld = self._rows(lt, m, vocab, "process_logits: logits")
         y = out if out is not None else self._alloc((m, vocab))
         yt = y.data if isinstance(y, GqTensor) else y
-        if yt.shape != lt.shape:
+        if yt.shape != shape:
             raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "process_logits: out must have the logits' shape")
-        yt, _, ldy = self._rows(yt, vocab, "process_logits: out")
-        tok = n_tok = pl = ln = pen = bi = bv = bo = mk = mr = None
-        n_masks = words = 0
+        yp, ldy = self._rows(yt, m, vocab, "process_logits: out")
+        tok = pl = ln = pen = bi = bv = bo = mk = mr = None
+        n_tok = n_masks = words = 0
         if tokens is not None and tokens.numel():
-            if tokens.dim() != 2 or tokens.shape[0] != m or prompt_lens is None or lens is None or penalties is None:
+            ts = tokens.shape
+            if len(ts) != 2 or ts[0] != m or prompt_lens is None or lens is None or penalties is None:
                 raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT,
                               "process_logits: tokens must be [m, n], with prompt_lens, lens and penalties")
-            tok, n_tok = d(tokens, i32, "tokens"), tokens.shape[1]
+            tok, n_tok = d(tokens, i32, "tokens"), ts[1]
             pl, ln = d(prompt_lens, i32, "prompt_lens", m), d(lens, i32, "lens", m)
             pen = d(penalties, f32, "penalties", 3 * m)
-        if bias_offsets is not None and bias_ids is not None and bias_ids.numel():
-            bi, bv = d(bias_ids, i32, "bias_ids"), d(bias_values, f32, "bias_values", bias_ids.numel())
+        if bias_offsets is not None and bias_ids is not None and (n_bias := bias_ids.numel()):
+            bi, bv = d(bias_ids, i32, "bias_ids"), d(bias_values, f32, "bias_values", n_bias)
             bo = d(bias_offsets, i32, "bias_offsets", m + 1)
         if masks is not None and masks.numel():
             if masks.dim() != 2:
                 raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "process_logits: masks must be [k, words]")
             mk, (n_masks, words) = d(masks, i32, "masks"), masks.shape
             mr = d(mask_rows, i32, "mask_rows", m) if mask_rows is not None else None
-        self._check(self.lib.gq_process_logits(self.ctx, lt.data_ptr(), m, vocab, ld, tok, n_tok or 0, pl, ln, pen, bi, bv,
-                                               bo, mk, n_masks, words, mr, yt.data_ptr(), ldy), "process_logits")
+        rc = self.lib.gq_process_logits(self.ctx, lp, m, vocab, ld, tok, n_tok, pl, ln, pen, bi, bv, bo, mk, n_masks, words,
+                                        mr, yp, ldy)
+        if rc:
+            self._check(rc, "process_logits")
         return y
 
     # ---- sync / lifecycle (rust/src/backend.rs:169-179) ------------------------
