@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kCompute, 2)
     }
     return x;
   };
-  TileRef cur, nxt;
+  TileRef cur = {}, nxt = {};
   uint32_t issued = 0;  // ring positions filled
   int stage = 0;        // of the current tile: 0 its keys (if first), 1 the next tile's keys, 2 its values
   auto copy = [&](const TileRef &x, const CUtensorMap *map) {
@@ -261,12 +261,19 @@ __global__ void __launch_bounds__(kCompute, 2)
       stage = 0;
     }
   };
-  if (warp == 0) {
-    cur = advance(true);
-    cur.first = true;
-    nxt = advance(false);
-    fill(C::kSlots);
-  }
+  // The first fill comes after the first unit's q is requested: the ring holds some 3 us
+  // of this SM's share of the bandwidth, and what is asked for later arrives later.
+  bool filled = false;
+  auto first_fill = [&]() {
+    if (filled) return;
+    filled = true;
+    if (warp == 0) {
+      cur = advance(true);
+      cur.first = true;
+      nxt = advance(false);
+      fill(C::kSlots);
+    }
+  };
 
   // ---- compute
   const int g = lane >> 2, q4 = lane & 3;  // fragment row / column group
@@ -301,11 +308,17 @@ __global__ void __launch_bounds__(kCompute, 2)
       const float *qg = a.q + b * a.q_stride + (int64_t)(head0 + min(g, nh - 1)) * D + ks * (D / KS);
       const bool real = g < nh;
       if constexpr (TYPE == GQ_KV_F32) {
+        float v[C::kQSteps][2];
 #pragma unroll
         for (int s = 0; s < C::kQSteps; ++s) {
-          const float x = real ? qg[s * 8 + q4] : 0.0f, y = real ? qg[s * 8 + q4 + 4] : 0.0f;
-          split_tf32(x, qf[s][0][0], qf[s][1][0]);
-          split_tf32(y, qf[s][0][1], qf[s][1][1]);
+          v[s][0] = real ? qg[s * 8 + q4] : 0.0f;
+          v[s][1] = real ? qg[s * 8 + q4 + 4] : 0.0f;
+        }
+        first_fill();
+#pragma unroll
+        for (int s = 0; s < C::kQSteps; ++s) {
+          split_tf32(v[s][0], qf[s][0][0], qf[s][1][0]);
+          split_tf32(v[s][1], qf[s][0][1], qf[s][1][1]);
         }
       } else {
         float2 v[C::kQSteps][2];
@@ -316,6 +329,7 @@ __global__ void __launch_bounds__(kCompute, 2)
           v[s][0] = real ? *reinterpret_cast<const float2 *>(qg + c0) : make_float2(0.f, 0.f);
           v[s][1] = real ? *reinterpret_cast<const float2 *>(qg + c1) : make_float2(0.f, 0.f);
         }
+        first_fill();
         if constexpr (TYPE != GQ_KV_BF16) {
           float top = 0.0f;
 #pragma unroll
