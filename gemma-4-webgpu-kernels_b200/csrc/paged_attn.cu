@@ -139,11 +139,12 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const Args a) {
 #pragma unroll
       for (int off = 8; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
       const float mn = fmaxf(m, top);
-      const float f = m == -INFINITY ? 0.0f : exp2f(m - mn);
+      const float base = mn == -INFINITY ? 0.0f : mn;  // (no visible key yet)
+      const float f = exp2_of(m - base);
       l *= f;
 #pragma unroll
       for (int k = 0; k < kRowTile / 16; ++k) {
-        const float p = x[k] == -INFINITY ? 0.0f : exp2f(x[k] - mn);
+        const float p = exp2_of(x[k] - base);
         s[sh][k * 16 + sl] = p;
         l += p;
       }
@@ -399,6 +400,7 @@ extern "C" int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const f
   a.window = (int32_t)std::min<uint32_t>(sliding_window, INT32_MAX);
   a.scale = scale * pages->k_scale;
   a.softcap = attn_softcap;
+  a.inv_softcap = attn_softcap > 0.0f ? 1.0f / attn_softcap : 0.0f;
   a.v_scale = pages->v_scale;
   a.err = ctx->dev_err;
   if (gq_paged_attn_tc_supported(pages, a.page_stride)) return gq_paged_attn_tc_launch(ctx, pages, a);

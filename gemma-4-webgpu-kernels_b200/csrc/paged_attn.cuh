@@ -36,7 +36,7 @@ struct Args {
   int batch, hq, heads, group, sub, units_per_req;  // group = hq / heads, sub = blocks of 8 per key-value head
   int dim, page_size, page_shift;                   // page_shift: log2 page_size (tiled kernels)
   int32_t window;
-  float scale, softcap, v_scale;  // scale: of the scores, the keys' scale included
+  float scale, softcap, inv_softcap, v_scale;  // scale: of the scores, the keys' scale included
   float *part_o, *part_ml;        // [2 grid][8][dim], [2 grid][8][2]
   int4 *cut_units;                // [grid]: the cut unit that begins in a CTA: request, unit, parts (0: none), first slot
   uint32_t *err;
@@ -172,10 +172,18 @@ __device__ __forceinline__ void put_cut_unit(const Args &a, const Cut &cut, int 
   a.cut_units[blockIdx.x] = make_int4(b, u, parts, slot_of(cut, s0));
 }
 
+// 2^x, x at most a little above 0; -inf gives 0. (What is below 2^-126 of the largest
+// weight counts as 0; the instruction's error is 2^-22.)
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Score of one visible key in units of log2: the scaled, optionally capped product.
 __device__ __forceinline__ float score_log2(const Args &a, float dot) {
   float s = dot * a.scale;
-  if (a.softcap > 0.0f) s = a.softcap * tanhf(__fdiv_rn(s, a.softcap));
+  if (a.softcap > 0.0f) s = a.softcap * tanhf(s * a.inv_softcap);
   return s * kLog2e;
 }
 

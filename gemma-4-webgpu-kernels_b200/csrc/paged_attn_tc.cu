@@ -79,9 +79,10 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// v = hi + lo: hi the nearest tf32 number, lo exact (the instruction reads its top 11 bits).
+// v = hi + lo: hi the nearest tf32 number (two integer operations; the conversion
+// instruction costs four), lo exact (the tensor instruction reads its top 11 bits).
 __device__ __forceinline__ void split_tf32(float v, uint32_t &hi, uint32_t &lo) {
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(v));
+  hi = (__float_as_uint(v) + 0x1000u) & 0xffffe000u;
   lo = __float_as_uint(v - __uint_as_float(hi));
 }
 template <typename H2>
@@ -460,14 +461,15 @@ __global__ void __launch_bounds__(kCompute, 2)
 #pragma unroll
         for (int off = 8; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         const float mn = fmaxf(m, top);
-        const float f = m == -INFINITY ? 0.0f : exp2f(m - mn);
+        const float zero = mn == -INFINITY ? 0.0f : mn;  // (no visible key yet)
+        const float f = exp2_of(m - zero);
         // p = 2^(x - m), times 2^14 for the f16 parts (a common factor of every weight and sum)
-        const float base = TYPE == GQ_KV_F16 || TYPE == GQ_KV_E4M3 ? mn - 14.0f : mn;
+        const float base = TYPE == GQ_KV_F16 || TYPE == GQ_KV_E4M3 ? zero - 14.0f : zero;
         float p[KPT];
         l *= f;
 #pragma unroll
         for (int k = 0; k < KPT; ++k) {
-          p[k] = x[k] == -INFINITY ? 0.0f : exp2f(x[k] - base);
+          p[k] = exp2_of(x[k] - base);
           l += p[k];
         }
         m = mn;

@@ -582,8 +582,9 @@ int gq_paged_append(gq_ctx *ctx, const gq_kv_pages *pages, const float *k, const
  * heads, hq / heads <= 64. Rows of a page past the request's length are never read as
  * numbers (they may hold NaN). A page id outside the pool raises GQ_DEVERR_PAGES and
  * counts as a page of zero rows; a length past the table row raises it and is cut to
- * the row: nothing outside the pool is read. Finite q and visible keys and values give f32 results (all sums in
- * f32, products exact to 2^-21 or better); where one is not finite, its row may be NaN.
+ * the row: nothing outside the pool is read. Finite q and visible keys and values (below 2^127) give f32 results:
+ * all sums in f32, products exact to 2^-21 or better; where one is not finite, its row
+ * may be NaN.
  * Long requests are split over many CTAs, whose partial results (context workspace)
  * are joined in the same launch in a fixed order: results do not vary from run to
  * run. */
