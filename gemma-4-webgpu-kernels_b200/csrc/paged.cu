@@ -20,10 +20,12 @@
 namespace {
 
 constexpr int kPlanThreads = 512;
+constexpr int kPlanEach = 4;  // neighbouring requests per thread and round of loads
 constexpr int kMaxBatch = 16384;
 
 struct PlanArgs {
-  int64_t batch, page_size, table_stride, n_pages, max_tokens;
+  int64_t batch, table_stride, n_pages, max_tokens;
+  uint32_t page_size;
   const int32_t *seq_lens, *other_lens;  // other: new (reserve) or kept (release) tokens
   int32_t *table;                        // reserve writes it, release reads it
   int32_t *free_pages;                   // reserve reads it, release writes it
@@ -38,8 +40,10 @@ __device__ __forceinline__ int64_t len_of(const int32_t *p, int64_t b) {
   const int32_t v = p[b];
   return v > 0 ? (int64_t)v : 0;
 }
-__device__ __forceinline__ int64_t pages_of(int64_t tokens, int64_t page_size) {
-  return (tokens + page_size - 1) / page_size;
+// (two lengths add up to less than 2^32: the short division)
+__device__ __forceinline__ int64_t pages_of(int64_t tokens, uint32_t page_size) {
+  const uint32_t t = (uint32_t)tokens, full = t / page_size;
+  return full + (t != full * page_size);
 }
 
 // Inclusive scan over the block of two sums at once; red is 2 * 32 entries of scratch.
@@ -115,21 +119,35 @@ __global__ void __launch_bounds__(kPlanThreads) paged_reserve_kernel(const PlanA
   const int64_t count = min(max(listed, (int64_t)0), a.n_pages);
   int64_t tokens = 0, taken = 0;
   bool bad = listed != count;
-  for (int b0 = 0; b0 < n; b0 += kPlanThreads) {
-    const int b = b0 + tid;
-    int64_t add = 0, need = 0;
-    if (b < n) {
-      const int64_t len = len_of(a.seq_lens, b);
-      add = len_of(a.other_lens, b);
-      const int64_t have = pages_of(len + add, a.page_size);
-      need = have - pages_of(len, a.page_size);
-      bad |= have > a.table_stride;
+  for (int b0 = 0; b0 < n; b0 += kPlanThreads * kPlanEach) {
+    int64_t add[kPlanEach], need[kPlanEach], sa = 0, sn = 0, ta, tn;
+#pragma unroll
+    for (int i = 0; i < kPlanEach; ++i) {
+      const int b = b0 + tid * kPlanEach + i;
+      add[i] = need[i] = 0;
+      if (b < n) {
+        const int64_t len = len_of(a.seq_lens, b);
+        add[i] = len_of(a.other_lens, b);
+        const int64_t have = pages_of(len + add[i], a.page_size);
+        need[i] = have - pages_of(len, a.page_size);
+        bad |= have > a.table_stride || len + add[i] > INT32_MAX;
+      }
+      sa += add[i];
+      sn += need[i];
     }
-    int64_t sa = add, sn = need, ta, tn;
+    const int64_t mine_a = sa, mine_n = sn;
     block_scan2(sa, sn, red, ta, tn);
-    if (b < n) {  // (sums past 31 bits end up refused below: max_tokens and n_pages are smaller)
-      ends[b] = (int32_t)min(tokens + sa, (int64_t)INT32_MAX);
-      first[b] = (int32_t)min(taken + sn - need, (int64_t)INT32_MAX);
+    sa += tokens - mine_a;  // of the requests before this thread's
+    sn += taken - mine_n;
+#pragma unroll
+    for (int i = 0; i < kPlanEach; ++i) {
+      const int b = b0 + tid * kPlanEach + i;
+      sa += add[i];
+      if (b < n) {  // (sums past 31 bits end up refused below: max_tokens and n_pages are smaller)
+        ends[b] = (int32_t)min(sa, (int64_t)INT32_MAX);
+        first[b] = (int32_t)min(sn, (int64_t)INT32_MAX);
+      }
+      sn += need[i];
     }
     tokens += ta;
     taken += tn;
@@ -143,7 +161,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_reserve_kernel(const PlanA
       owner = owner_of(ends, n, (int32_t)t);
       const int64_t len = len_of(a.seq_lens, owner);
       const int64_t pos = len + (t - (owner ? ends[owner - 1] : 0));
-      const int64_t p = pos / a.page_size, row = pos - p * a.page_size, had = pages_of(len, a.page_size);
+      const int64_t p = (uint32_t)pos / a.page_size, row = pos - p * a.page_size, had = pages_of(len, a.page_size);
       int32_t *entry = a.table + owner * a.table_stride + p;
       int32_t page;
       if (p < had) {
@@ -186,33 +204,52 @@ __global__ void __launch_bounds__(kPlanThreads) paged_release_kernel(const PlanA
   const int64_t count = min(max(listed, (int64_t)0), a.n_pages);
   int64_t given = 0;
   bool bad = listed != count;
-  for (int b0 = 0; b0 < n; b0 += kPlanThreads) {
-    const int b = b0 + tid;
-    int64_t back = 0, keep_pages = 0;
-    if (b < n) {
-      const int64_t len = len_of(a.seq_lens, b);
-      const int64_t had = pages_of(len, a.page_size);
-      keep_pages = pages_of(min(len_of(a.other_lens, b), len), a.page_size);
-      back = had - keep_pages;
-      bad |= had > a.table_stride;
+  for (int b0 = 0; b0 < n; b0 += kPlanThreads * kPlanEach) {
+    int64_t back[kPlanEach], sb = 0, unused = 0, tb, tu;
+#pragma unroll
+    for (int i = 0; i < kPlanEach; ++i) {
+      const int b = b0 + tid * kPlanEach + i;
+      back[i] = 0;
+      if (b < n) {
+        const int64_t len = len_of(a.seq_lens, b);
+        const int64_t had = pages_of(len, a.page_size), keep = pages_of(min(len_of(a.other_lens, b), len), a.page_size);
+        back[i] = had - keep;
+        start[b] = (int32_t)keep;
+        bad |= had > a.table_stride;
+      }
+      sb += back[i];
     }
-    int64_t sb = back, unused = 0, tb, tu;
+    const int64_t mine = sb;
     block_scan2(sb, unused, red, tb, tu);
-    if (b < n) {
-      ends[b] = (int32_t)min(given + sb, (int64_t)INT32_MAX);
-      start[b] = (int32_t)keep_pages;
+    sb += given - mine;
+#pragma unroll
+    for (int i = 0; i < kPlanEach; ++i) {
+      const int b = b0 + tid * kPlanEach + i;
+      sb += back[i];
+      if (b < n) ends[b] = (int32_t)min(sb, (int64_t)INT32_MAX);
     }
     given += tb;
   }
   bad = __syncthreads_or(bad) || count + given > a.n_pages;
   bool wrong = false;  // a page id outside the pool
   if (!bad)
-    for (int64_t i = blockIdx.x * (int64_t)kPlanThreads + tid; i < given; i += (int64_t)gridDim.x * kPlanThreads) {
-      const int b = owner_of(ends, n, (int32_t)i);
-      const int64_t p = start[b] + (i - (b ? ends[b - 1] : 0));
-      const int32_t page = a.table[b * a.table_stride + p];
-      a.free_pages[count + given - 1 - i] = page;
-      wrong |= page < 0 || page >= a.n_pages;
+    for (int64_t i0 = blockIdx.x * (int64_t)kPlanThreads + tid; i0 < given; i0 += (int64_t)gridDim.x * kPlanThreads * kPlanEach) {
+      int32_t page[kPlanEach];
+#pragma unroll
+      for (int k = 0; k < kPlanEach; ++k) {
+        const int64_t i = i0 + (int64_t)k * gridDim.x * kPlanThreads;
+        page[k] = 0;
+        if (i >= given) continue;
+        const int b = owner_of(ends, n, (int32_t)i);
+        page[k] = a.table[b * a.table_stride + start[b] + (i - (b ? ends[b - 1] : 0))];
+      }
+#pragma unroll
+      for (int k = 0; k < kPlanEach; ++k) {
+        const int64_t i = i0 + (int64_t)k * gridDim.x * kPlanThreads;
+        if (i >= given) break;
+        a.free_pages[count + given - 1 - i] = page[k];
+        wrong |= page[k] < 0 || page[k] >= a.n_pages;
+      }
     }
   if (wrong) gqd::report(a.err, GQ_DEVERR_PAGES);
   if (last_cta(a.ctr)) {
@@ -374,7 +411,7 @@ extern "C" int gq_paged_reserve(gq_ctx *ctx, int64_t batch, int64_t page_size, c
     return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT, "paged_reserve: null pointer");
   PlanArgs a{};
   a.batch = batch;
-  a.page_size = page_size;
+  a.page_size = (uint32_t)page_size;
   a.table_stride = table_stride;
   a.n_pages = n_pages;
   a.max_tokens = max_tokens;
@@ -403,7 +440,7 @@ extern "C" int gq_paged_release(gq_ctx *ctx, int64_t batch, int64_t page_size, c
     return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT, "paged_release: null pointer");
   PlanArgs a{};
   a.batch = batch;
-  a.page_size = page_size;
+  a.page_size = (uint32_t)page_size;
   a.table_stride = table_stride;
   a.n_pages = n_pages;
   a.seq_lens = seq_lens;

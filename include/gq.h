@@ -541,7 +541,7 @@ typedef struct gq_kv_pages {
  * -1, position 0, owner -1. totals[b] = seq_lens[b] + new_lens[b], free_left[0] = what
  * remains of free_count[0]; they may be seq_lens and free_count themselves.
  * All or nothing: when the pool (n_pages entries of free_pages), a table row or
- * max_tokens is too small, no page is taken, every slot is -1, totals = seq_lens,
+ * max_tokens is too small (or a length passes 2^31 - 1), no page is taken, every slot is -1, totals = seq_lens,
  * free_left = free_count and GQ_DEVERR_PAGES is raised at the next gq_sync. A page id
  * outside [0, n_pages) in the table or the list gives slot -1 and the same error.
  * All pointers are device pointers. batch <= 16384, max_tokens < 2^31. */
