@@ -54,6 +54,7 @@ struct gq_ctx {
   // arrival counters of kernels whose last CTA finishes the work (the paged-cache ops):
   // zero between launches, the last CTA to arrive at one puts it back to zero
   uint32_t *counters = nullptr;
+  void *paged_ws = nullptr;  // parts of gq_paged_attention: made by its first call, never moved
   // set by gq_linear_softcap_peers(_signal) for the duration of one call
   PeerDst peers = {};
   PeerDst peer_signal = {};

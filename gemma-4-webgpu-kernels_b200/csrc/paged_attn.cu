@@ -389,6 +389,8 @@ extern "C" int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const f
   a.table_stride = table_stride;
   a.page_stride = pages->page_stride ? pages->page_stride : pages->heads * pages->page_size * pages->head_dim;
   a.n_pages = pages->n_pages;
+  // (the last tile's keys are numbered in 32 bits)
+  a.room = std::min<int64_t>(table_stride * pages->page_size, INT32_MAX - 1024);
   a.batch = (int)batch;
   a.hq = (int)hq;
   a.heads = (int)pages->heads;
@@ -404,8 +406,8 @@ extern "C" int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const f
   a.v_scale = pages->v_scale;
   a.err = ctx->dev_err;
   if (gq_paged_attn_tc_supported(pages, a.page_stride)) return gq_paged_attn_tc_launch(ctx, pages, a);
-  const int grid = grid_for(a, kRowTile, 4 * ctx->num_sms);
-  rc = bind_workspace(ctx, grid, a);
+  const int grid = grid_for(ctx, a, kRowTile);
+  rc = bind_parts(ctx, grid, a);
   if (rc != GQ_OK) return rc;
   switch (pages->type) {
     case GQ_KV_F32: GQ_CUDA_TRY(ctx, rows_launch<GQ_KV_F32>(ctx, grid, a)); break;

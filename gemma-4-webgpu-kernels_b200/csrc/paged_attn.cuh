@@ -33,6 +33,7 @@ struct Args {
   const void *k, *v;
   const int32_t *table, *lens;
   int64_t q_stride, table_stride, page_stride, n_pages;
+  int64_t room;                                     // tokens that a table row can hold
   int batch, hq, heads, group, sub, units_per_req;  // group = hq / heads, sub = blocks of 8 per key-value head
   int dim, page_size, page_shift;                   // page_shift: log2 page_size (tiled kernels)
   int32_t window;
@@ -48,8 +49,7 @@ struct Range {
 };
 
 __device__ __forceinline__ int visible(const Args &a, int b) {
-  const int64_t len = max(a.lens[b], 0), room = a.table_stride * a.page_size;
-  return (int)min(len, room);
+  return (int)min((int64_t)max(a.lens[b], 0), a.room);
 }
 template <int T>
 __device__ __forceinline__ Range range_of(const Args &a, int keys) {
@@ -92,10 +92,8 @@ __device__ __forceinline__ Cut find_cut(const Args &a) {
   int64_t mine = 0;
   bool past = false;
   for (int b = b0; b < b1; ++b) {
-    const int len = a.lens[b];
-    const int64_t room = a.table_stride * a.page_size;
-    mine += (int64_t)(range_of<T>(a, (int)min((int64_t)max(len, 0), room)).nt + 1) * a.units_per_req;
-    past |= len > room;
+    mine += (int64_t)(range_of<T>(a, visible(a, b)).nt + 1) * a.units_per_req;
+    past |= a.lens[b] > a.room;
   }
   if (past && blockIdx.x == 0) gqd::report(a.err, GQ_DEVERR_PAGES);
   int64_t incl = mine;
@@ -189,23 +187,31 @@ __device__ __forceinline__ float score_log2(const Args &a, float dot) {
 
 // ---- host side
 
-// CTAs to launch: at most `most`, and no more than there can be tiles (the table bounds
-// the lengths, which the host does not know).
-inline int grid_for(const Args &a, int tile, int most) {
-  int64_t keys = std::min<int64_t>(a.table_stride * a.page_size, INT32_MAX);
+// CTAs to launch: at most two per SM, and no more than there can be tiles (the table
+// bounds the lengths, which the host does not know).
+inline int grid_for(gq_ctx *ctx, const Args &a, int tile) {
+  int64_t keys = a.room;
   if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + tile);
   const int64_t tiles = (int64_t)a.batch * a.units_per_req * std::max<int64_t>(1, (keys + tile - 1) / tile);
-  return (int)std::min<int64_t>(tiles, std::min(kMaxGrid, most));
+  return (int)std::min<int64_t>(tiles, std::min(kMaxGrid, 2 * ctx->num_sms));
 }
 
-// Workspace for the parts: two per CTA, and the list of cut units.
-inline int bind_workspace(gq_ctx *ctx, int grid, Args &a) {
-  void *ws = nullptr;
-  const int rc = gq_workspace(ctx, (size_t)grid * (2 * kHeads * (a.dim + 2) * 4 + sizeof(int4)), &ws);
-  a.cut_units = static_cast<int4 *>(ws);
+// Memory for the parts (two per CTA) and the list of cut units: one block of the largest
+// size, made by the context's first call and kept, so that a recorded graph's addresses
+// stay good whatever is called after it (10 MB on 148 SMs).
+inline int bind_parts(gq_ctx *ctx, int grid, Args &a) {
+  constexpr size_t kPerCta = 2 * kHeads * (512 + 2) * 4 + sizeof(int4);
+  if (!ctx->paged_ws) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    GQ_CUDA_TRY(ctx, cudaStreamIsCapturing(ctx->stream, &st));
+    if (st != cudaStreamCaptureStatusNone)
+      return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT, "paged_attention: run the call once before recording (it allocates)");
+    GQ_CUDA_TRY(ctx, cudaMalloc(&ctx->paged_ws, (size_t)std::min(kMaxGrid, 2 * ctx->num_sms) * kPerCta));
+  }
+  a.cut_units = static_cast<int4 *>(ctx->paged_ws);
   a.part_o = reinterpret_cast<float *>(a.cut_units + grid);
   a.part_ml = a.part_o + (size_t)grid * 2 * kHeads * a.dim;
-  return rc;
+  return GQ_OK;
 }
 
 }  // namespace pattn

@@ -505,10 +505,9 @@ int gq_copy_rows(gq_ctx *ctx, const float *src, int64_t rows, int64_t cols, int6
  * and values live in pages of a pool shared by all of them, found through a block
  * table (row b, entry p: the page holding tokens p * page_size .. of request b).
  * Lengths, tables and the free list stay on the device, so one recorded step
- * (gq_graph_*) serves every following token. Calls that may
- * overlap on two streams need a context each (they share its workspace and arrival
- * counters). No counterpart in the reference (its caches are one contiguous tensor per
- * layer of one sequence). */
+ * (gq_graph_*) serves every following token. Calls that may overlap on two streams
+ * need a context each (they share its workspace and arrival counters). No counterpart in
+ * the reference (its caches are one contiguous tensor per layer of one sequence). */
 
 /* Storage of a page's values. An e4m3 code stands for code * k_scale (or v_scale). */
 #define GQ_KV_F32 0
@@ -541,9 +540,10 @@ typedef struct gq_kv_pages {
  * -1, position 0, owner -1. totals[b] = seq_lens[b] + new_lens[b], free_left[0] = what
  * remains of free_count[0]; they may be seq_lens and free_count themselves.
  * All or nothing: when the pool (n_pages entries of free_pages), a table row or
- * max_tokens is too small (or a length passes 2^31 - 1), no page is taken, every slot is -1, totals = seq_lens,
- * free_left = free_count and GQ_DEVERR_PAGES is raised at the next gq_sync. A page id
- * outside [0, n_pages) in the table or the list gives slot -1 and the same error.
+ * max_tokens is too small (or a length passes 2^31 - 1), no page is taken, every slot is
+ * -1, totals = seq_lens, free_left = free_count and GQ_DEVERR_PAGES is raised at the
+ * next gq_sync. A page id outside [0, n_pages) in the table or the list gives slot -1
+ * and the same error.
  * All pointers are device pointers. batch <= 16384, max_tokens < 2^31. */
 int gq_paged_reserve(gq_ctx *ctx, int64_t batch, int64_t page_size, const int32_t *seq_lens, const int32_t *new_lens,
                      int32_t *block_table, int64_t table_stride, const int32_t *free_pages, int64_t n_pages,
@@ -582,12 +582,12 @@ int gq_paged_append(gq_ctx *ctx, const gq_kv_pages *pages, const float *k, const
  * heads, hq / heads <= 64. Rows of a page past the request's length are never read as
  * numbers (they may hold NaN). A page id outside the pool raises GQ_DEVERR_PAGES and
  * counts as a page of zero rows; a length past the table row raises it and is cut to
- * the row: nothing outside the pool is read. Finite q and visible keys and values (below 2^127) give f32 results:
- * all sums in f32, products exact to 2^-21 or better; where one is not finite, its row
- * may be NaN.
- * Long requests are split over many CTAs, whose partial results (context workspace)
- * are joined in the same launch in a fixed order: results do not vary from run to
- * run. */
+ * the row: nothing outside the pool is read. Finite q and visible keys and values
+ * (below 2^127) give f32 results: all sums in f32, products exact to 2^-21 or better;
+ * where one is not finite, its row may be NaN. Long requests are split over many CTAs,
+ * whose partial results (10 MB that the context's first call allocates: not while the
+ * stream is captured) a second launch joins in a fixed order: results do not vary from
+ * run to run. */
 int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const float *q, int64_t batch, int64_t hq,
                        int64_t q_tok_stride, const int32_t *block_table, int64_t table_stride,
                        const int32_t *seq_lens, float scale, uint32_t sliding_window, float attn_softcap, float *out);

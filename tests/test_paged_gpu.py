@@ -413,6 +413,29 @@ def test_attention_in_a_graph_follows_the_device_lengths(g):
     own.close()
 
 
+def test_a_recorded_call_outlives_larger_ones(g):
+    """The memory of the partial results does not move when a later call needs more."""
+    torch = g._torch
+    own = CudaBackend(0, own_stream=True)
+    small = Cache(own, "bf16", [900], 1, 64, 16, seed=21)
+    q = torch.randn(1, 4, 64, device=own.torch_device)
+    out = torch.zeros(1, 4 * 64, device=own.torch_device)
+    fn = lambda: own.paged_attention(small.pages, q, small.table, small.lens, scale=0.125, out=out)  # noqa: E731
+    torch.cuda.synchronize()
+    fn()
+    graph = own.record(fn)
+    large = Cache(own, "bf16", [5000] * 40, 1, 512, 16, seed=22)
+    torch.cuda.synchronize()
+    check_attend(own, large, 8)
+    out.zero_()
+    torch.cuda.synchronize()
+    own.replay(graph)
+    own.flush()
+    assert rel_l2(out.cpu().numpy(), attend_ref(small, q, 0.125)) <= ATTN_REL_L2
+    own.destroy_graph(graph)
+    own.close()
+
+
 def test_attention_reports_bad_pages_and_long_lengths(g):
     torch = g._torch
     cache = Cache(g, "bf16", [40, 40], 1, 128, 16, seed=6)
