@@ -34,6 +34,7 @@ struct Args {
   const int32_t *table, *lens;
   int64_t q_stride, table_stride, page_stride, n_pages;
   int64_t room;                                     // tokens that a table row can hold
+  int cluster;                                      // CTAs per unit (one cluster), 0: units cut by find_cut
   int batch, hq, heads, group, sub, units_per_req;  // group = hq / heads, sub = blocks of 8 per key-value head
   int dim, page_size, page_shift;                   // page_shift: log2 page_size (tiled kernels)
   int32_t window;
@@ -187,12 +188,16 @@ __device__ __forceinline__ float score_log2(const Args &a, float dot) {
 
 // ---- host side
 
+// Most tiles a unit can have.
+inline int64_t most_tiles(const Args &a, int tile) {
+  const int64_t keys = a.window > 0 ? std::min<int64_t>(a.room, (int64_t)a.window + tile - 1) : a.room;
+  return std::max<int64_t>(1, (keys + tile - 1) / tile);
+}
+
 // CTAs to launch: at most two per SM, and no more than there can be tiles (the table
 // bounds the lengths, which the host does not know).
 inline int grid_for(gq_ctx *ctx, const Args &a, int tile) {
-  int64_t keys = a.room;
-  if (a.window > 0) keys = std::min<int64_t>(keys, (int64_t)a.window + tile);
-  const int64_t tiles = (int64_t)a.batch * a.units_per_req * std::max<int64_t>(1, (keys + tile - 1) / tile);
+  const int64_t tiles = (int64_t)a.batch * a.units_per_req * most_tiles(a, tile);
   return (int)std::min<int64_t>(tiles, std::min(kMaxGrid, 2 * ctx->num_sms));
 }
 

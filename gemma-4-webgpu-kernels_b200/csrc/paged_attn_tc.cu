@@ -32,6 +32,7 @@
 // of up to 131072 keys, e4m3, 249 MB: 58 us. 23 requests of up to 2501, f32, 4 heads of
 // 128, soft-cap, 127 MB: 33.6 us. With plain loads and CUDA-core products
 // (paged_rows_kernel): 324, 606 and 204 us. One request of 333 keys: 9.3 us replayed.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -158,6 +159,41 @@ __device__ __forceinline__ void wait_or_abort(uint64_t *bar, uint32_t parity, vo
 }
 
 
+// Join the parts of a cluster's unit, each in its CTA's shared memory (mine [8][D] and its
+// maxima and sums): every CTA adds up a share of the columns, in rank order.
+template <int D>
+__device__ __forceinline__ void join_cluster(const Args &a, const float *mine, const float2 *mine_ml, int b, int head0, int nh) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int n = a.cluster, rank = (int)cluster.block_rank(), items = nh * (D / 4);
+  cluster.sync();  // every part is written
+  for (int at = items * rank / n + (int)threadIdx.x; at < items * (rank + 1) / n; at += kCompute) {
+    const int h = at / (D / 4);
+    float m = -INFINITY, l = 0.0f;
+    float2 ml[8];
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      ml[p] = p < n ? cluster.map_shared_rank(mine_ml, p)[h] : make_float2(-INFINITY, 0.0f);
+      m = fmaxf(m, ml[p].x);
+    }
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      if (ml[p].x == -INFINITY) continue;  // no CTA, or one without a visible key: its columns are not written
+      const float4 v = reinterpret_cast<const float4 *>(cluster.map_shared_rank(mine, p))[at];
+      const float w = exp2_of(ml[p].x - m);
+      l = fmaf(w, ml[p].y, l);
+      o.x = fmaf(w, v.x, o.x);
+      o.y = fmaf(w, v.y, o.y);
+      o.z = fmaf(w, v.z, o.z);
+      o.w = fmaf(w, v.w, o.w);
+    }
+    const float s = inv_or_zero(l) * a.v_scale;
+    reinterpret_cast<float4 *>(a.out + ((int64_t)b * a.hq + head0) * D)[at] = make_float4(o.x * s, o.y * s, o.z * s, o.w * s);
+  }
+  cluster.sync();  // no CTA's memory goes away while it is read
+}
+
 // One tile of this CTA, as warp 0 sees it: lane i owns the tile's i-th copy.
 struct TileRef {
   int page, row;      // of this lane's copy; page -1: nothing to load
@@ -172,6 +208,7 @@ __global__ void __launch_bounds__(kCompute, 2)
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full[kMaxSlots];
   __shared__ float fix[2][kHeads], sum[kHeads];
+  __shared__ float2 share_ml[kHeads];
   __shared__ int abort_flag;
   uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float *sS = reinterpret_cast<float *>(ring + C::kSlots * C::kSlot);       // [2][KS][head][key]
@@ -184,8 +221,23 @@ __global__ void __launch_bounds__(kCompute, 2)
   }
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
-  const Cut cut = find_cut<kCompute, T>(a);  // (its barriers also publish the mbarriers)
-  if (cut.w0 >= cut.w1) {
+  Cut cut;
+  if (a.cluster) {
+    // a unit of few tiles: its cluster's CTAs take neighbouring tiles (the last may get none)
+    const int unit = blockIdx.x / a.cluster, rank = blockIdx.x - unit * a.cluster;
+    cut.b = unit / a.units_per_req;
+    cut.u = unit - cut.b * a.units_per_req;
+    cut.keys = visible(a, cut.b);
+    const int nt = range_of<T>(a, cut.keys).nt, each = (nt + a.cluster - 1) / a.cluster;
+    cut.t = min(rank * each, nt);
+    cut.w0 = 0;
+    cut.w1 = min(each, nt - cut.t);
+    if (tid == 0 && rank == 0 && a.lens[cut.b] > a.room) gqd::report(a.err, GQ_DEVERR_PAGES);
+    __syncthreads();  // the mbarriers
+  } else {
+    cut = find_cut<kCompute, T>(a);  // (its barriers also publish the mbarriers)
+  }
+  if (!a.cluster && cut.w0 >= cut.w1) {
     if (tid == 0) a.cut_units[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
   }
@@ -379,7 +431,7 @@ __global__ void __launch_bounds__(kCompute, 2)
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[i][k] = 0.0f;
     float m = -INFINITY, l = 0.0f;
-
+    if (tiles > 0) {  // (a cluster's last CTAs may have none)
     // products of this warp's keys and columns with q: three (two) sums for the parts
     float c[MT][3][4];
     auto products = [&]() {
@@ -632,22 +684,29 @@ __global__ void __launch_bounds__(kCompute, 2)
       }
     }
 
+    }
+
     // ---- the unit's output, or this CTA's part of it
 #pragma unroll
     for (int off = 8; off >= 1; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
-    const bool whole = tiles == r.nt;
+    const bool shared = a.cluster > 1, whole = !shared && tiles == r.nt;
     const int64_t s0 = w - t;
-    const int slot = whole ? 0 : slot_of(cut, s0);
+    const int slot = whole || shared ? 0 : slot_of(cut, s0);
     if (sl == 0) {
       sum[sh] = l;
-      if (!whole) {
+      if (shared) {
+        share_ml[sh] = make_float2(m, l);
+      } else if (!whole) {
         a.part_ml[(slot * kHeads + sh) * 2] = m;
         a.part_ml[(slot * kHeads + sh) * 2 + 1] = l;
       }
     }
     sync_compute<kCompute>();
     {
-      float *base = whole ? a.out + ((int64_t)b * a.hq + head0) * D : a.part_o + (int64_t)slot * kHeads * D;
+      // (the ring's tiles are read: a cluster's part takes its place)
+      float *base = shared  ? reinterpret_cast<float *>(ring)
+                    : whole ? a.out + ((int64_t)b * a.hq + head0) * D
+                            : a.part_o + (int64_t)slot * kHeads * D;
       const float f0 = whole ? inv_or_zero(sum[2 * q4]) * a.v_scale : 1.0f;
       const float f1 = whole ? inv_or_zero(sum[2 * q4 + 1]) * a.v_scale : 1.0f;
       const int most = whole ? nh : kHeads;
@@ -665,6 +724,11 @@ __global__ void __launch_bounds__(kCompute, 2)
         }
       }
     }
+    if (shared) {
+      join_cluster<D>(a, reinterpret_cast<const float *>(ring), share_ml, b, head0, nh);
+      break;
+    }
+    if (a.cluster) break;
     w += tiles;
     if (w == cut.w1) {
       if (tid == 0) put_cut_unit(a, cut, b, u, s0, r.nt);
@@ -724,6 +788,40 @@ int launch(gq_ctx *ctx, const gq_kv_pages *p, Args &a) {
   int rc = encode(ctx, p, p->k, a.page_stride, rows, &kmap);
   if (rc == GQ_OK) rc = encode(ctx, p, p->v, a.page_stride, rows, &vmap);
   if (rc != GQ_OK) return rc;
+  // Units that cannot have many tiles (a sliding window, a short table) get a cluster of
+  // CTAs each, as large as fills the GPU: no cut to work out, and a join in shared memory
+  // (some 4 us less, the time of two tiles). What it can cost is uneven work: tiles beyond
+  // an equal share, and lengths that differ (a window evens them out). Measured, cluster
+  // against cut, head_dim 256, bf16: window 512 and 1, 8, 64, 200, 500 requests 6.9 / 9.6,
+  // 9.2 / 12.4, 13.2 / 17.2, 28.4 / 34.5, 56 / 60 us; up to 1024 keys and 1, 16, 64
+  // requests 8.7 / 10.0, 9.4 / 12.8, 15.3 / 17.6; up to 2048 keys 13.1 / 10.0, 13.7 / 13.0,
+  // 26.5 / 24.1. (150 requests with the window, where a cluster is one CTA and half the
+  // GPU is idle: 27.5 / 27.0.)
+  const int64_t units = (int64_t)a.batch * a.units_per_req, tiles = most_tiles(a, C::T);
+  int cluster = 8;
+  while (cluster > 1 && (units * cluster > 2 * ctx->num_sms || cluster >= 2 * tiles)) cluster >>= 1;
+  const int64_t each = (tiles + cluster - 1) / cluster;
+  const int64_t equal = (units * tiles + 2 * ctx->num_sms - 1) / (2 * ctx->num_sms);
+  const bool even = a.window > 0;
+  if (each <= (even ? 9 : 4) && each <= equal + (even ? 2 : 1) && units * cluster <= INT32_MAX) {
+    a.cluster = cluster;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(units * cluster));
+    cfg.blockDim = dim3(kCompute);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ctx->pdl ? 2 : 1;
+    GQ_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, paged_tiles_kernel<TYPE, D>, (const Args)a, (const CUtensorMap)kmap, (const CUtensorMap)vmap));
+    return GQ_OK;
+  }
   const int grid = grid_for(ctx, a, C::T);
   rc = bind_parts(ctx, grid, a);
   if (rc != GQ_OK) return rc;

@@ -238,12 +238,12 @@ class Cache:
     """A paged cache with random contents: everything behind the requests' lengths, and
     every page of no request, is NaN."""
 
-    def __init__(self, g, name, lens, hkv, d, ps, seed, interleave=False, spare=3, k_scale=None, dtype_scale=(1 / 32, 1 / 24)):
+    def __init__(self, g, name, lens, hkv, d, ps, seed, interleave=False, spare=3, room=0, dtype_scale=(1 / 32, 1 / 24)):
         torch = g._torch
         rng = np.random.default_rng(seed)
         lens = np.asarray(lens)
         dt = tdtype(g, name)
-        width = max(1, -(-int(lens.max(initial=0)) // ps)) + 1
+        width = max(1, -(-max(int(lens.max(initial=0)), room) // ps)) + 1
         table, _, _, n = pool_state(rng, lens, ps, width, spare)
         self.k_scale, self.v_scale = dtype_scale if name == "e4m3" else (1.0, 1.0)
         gen = torch.Generator(device=g.torch_device)
@@ -264,7 +264,6 @@ class Cache:
         self.table_np, self.lens_np, self.ps, self.hkv, self.d = table, lens, ps, hkv, d
         self.table, self.lens = i32(g, table), i32(g, lens)
         self.pages = g.kv_pages(self.k, self.v, k_scale=self.k_scale, v_scale=self.v_scale)
-        self.q = 2.0 * torch.randn(len(lens), 0 or 1, 1, generator=gen, device=g.torch_device)
 
     def rows(self, b, lo, hi):
         """The visible keys and values of request b in 64 bits, [n, hkv, d]."""
@@ -320,9 +319,12 @@ LENS = [0, 1, 2, 15, 16, 17, 63, 64, 65, 130, 511, 513, 1000, -1]
 
 @pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("d,hkv,group", [(64, 1, 8), (128, 2, 4), (256, 1, 8), (512, 1, 8), (256, 3, 1), (128, 1, 16), (64, 2, 13)])
-@pytest.mark.parametrize("window,softcap", [(0, 0.0), (100, 0.0), (512, 30.0)])
-def test_attention_lengths_heads_and_types(g, name, d, hkv, group, window, softcap):
-    cache = Cache(g, name, LENS, hkv, d, 16, seed=d + hkv)
+@pytest.mark.parametrize("window,softcap", [(0, 0.0), (100, 0.0), (512, 30.0), (3000, 0.0)])
+@pytest.mark.parametrize("room", [0, 20000])
+def test_attention_lengths_heads_and_types(g, name, d, hkv, group, window, softcap, room):
+    """room: tokens the table rows could hold; long rows and windows are cut over the grid,
+    short ones go to a cluster each."""
+    cache = Cache(g, name, LENS, hkv, d, 16, seed=d + hkv, room=room)
     check_attend(g, cache, hkv * group, window, softcap)
 
 
@@ -335,8 +337,9 @@ def test_attention_other_head_dims(g, name, d):
 @pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("ps", [1, 3, 4, 8, 16, 24, 32, 64, 100, 128, 256])
 @pytest.mark.parametrize("d", [128, 512])
-def test_attention_page_sizes(g, name, ps, d):
-    check_attend(g, Cache(g, name, [1, 7, 100, 129, 600], 2, d, ps, seed=ps), 8, window=77)
+@pytest.mark.parametrize("window", [77, 0])
+def test_attention_page_sizes(g, name, ps, d, window):
+    check_attend(g, Cache(g, name, [1, 7, 100, 129, 600], 2, d, ps, seed=ps, room=0 if window else 20000), 8, window)
 
 
 @pytest.mark.parametrize("name", ["f32", "bf16", "e4m3"])
