@@ -406,7 +406,7 @@ extern "C" int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const f
   a.v_scale = pages->v_scale;
   a.err = ctx->dev_err;
   if (gq_paged_attn_tc_supported(pages, a.page_stride)) return gq_paged_attn_tc_launch(ctx, pages, a);
-  const int grid = grid_for(ctx, a, kRowTile);
+  const int grid = grid_for(a, kRowTile, 2 * ctx->num_sms);
   rc = bind_parts(ctx, grid, a);
   if (rc != GQ_OK) return rc;
   switch (pages->type) {

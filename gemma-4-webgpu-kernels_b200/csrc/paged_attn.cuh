@@ -194,18 +194,21 @@ inline int64_t most_tiles(const Args &a, int tile) {
   return std::max<int64_t>(1, (keys + tile - 1) / tile);
 }
 
-// CTAs to launch: at most two per SM, and no more than there can be tiles (the table
-// bounds the lengths, which the host does not know).
-inline int grid_for(gq_ctx *ctx, const Args &a, int tile) {
+// CTAs to launch: at most `slots`, and no more than there can be tiles (the table bounds
+// the lengths, which the host does not know).
+inline int grid_for(const Args &a, int tile, int slots) {
   const int64_t tiles = (int64_t)a.batch * a.units_per_req * most_tiles(a, tile);
-  return (int)std::min<int64_t>(tiles, std::min(kMaxGrid, 2 * ctx->num_sms));
+  return (int)std::min<int64_t>(tiles, std::min(kMaxGrid, slots));
 }
 
 // Memory for the parts (two per CTA) and the list of cut units: one block of the largest
 // size, made by the context's first call and kept, so that a recorded graph's addresses
-// stay good whatever is called after it (10 MB on 148 SMs).
+// stay good whatever is called after it (10 MB on 148 SMs: two CTAs per SM at head_dim
+// 512; where there are three, rows are at most half as long).
 inline int bind_parts(gq_ctx *ctx, int grid, Args &a) {
   constexpr size_t kPerCta = 2 * kHeads * (512 + 2) * 4 + sizeof(int4);
+  if ((size_t)grid * (2 * kHeads * (a.dim + 2) * 4 + sizeof(int4)) > (size_t)std::min(kMaxGrid, 2 * ctx->num_sms) * kPerCta)
+    return gq_fail(ctx, GQ_ERR_UNSUPPORTED, "paged_attention: more partial results than there is memory for");
   if (!ctx->paged_ws) {
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
     GQ_CUDA_TRY(ctx, cudaStreamIsCapturing(ctx->stream, &st));

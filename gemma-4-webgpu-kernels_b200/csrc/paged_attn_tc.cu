@@ -47,7 +47,6 @@ using namespace pattn;
 
 constexpr int kComputeWarps = 4;
 constexpr int kCompute = kComputeWarps * 32;
-constexpr int kSmemBytes = 110 * 1024;  // two CTAs per SM
 constexpr int kMaxSlots = 8;
 
 __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *map, int c0, int c1, int c2, int c3, uint64_t *bar) {
@@ -133,6 +132,12 @@ struct Tile {
   static constexpr int MT = 16 * kComputeWarps / KS * kRow <= (KS > 1 ? 16384 : 8192) ? 2 : 1;
   static constexpr int T = 16 * kComputeWarps * MT / KS;
   static constexpr int kSlot = T * kRow;
+  // CTAs per SM: three where rows are short, a tile is little work and 168 registers will
+  // do (225 requests of up to 62 keys, 8 heads of 64, bf16: 31.4 us with two, 24.5 with
+  // three; 10 of up to 40000, one head of 128: 35.3 and 33.8; e4m3 rows of 256 spill with
+  // three and lose 20 %)
+  static constexpr int kPerSm = kRow <= 256 && D <= 128 ? 3 : 2;
+  static constexpr int kSmemBytes = (kPerSm == 3 ? 72 : 110) * 1024;
   static constexpr int kParts = TYPE == GQ_KV_BF16 ? 3 : 2;
   static constexpr int kStep = TYPE == GQ_KV_F32 ? 8 : 16;      // head_dim columns (keys) per instruction
   static constexpr int kQSteps = D / KS / kStep;
@@ -201,7 +206,7 @@ struct TileRef {
 };
 
 template <int TYPE, int D>
-__global__ void __launch_bounds__(kCompute, 2)
+__global__ void __launch_bounds__(kCompute, (Tile<TYPE, D>::kPerSm))
     paged_tiles_kernel(const Args a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   using C = Tile<TYPE, D>;
   constexpr int T = C::T, KS = C::KS, MT = C::MT;
@@ -798,10 +803,11 @@ int launch(gq_ctx *ctx, const gq_kv_pages *p, Args &a) {
   // 26.5 / 24.1. (150 requests with the window, where a cluster is one CTA and half the
   // GPU is idle: 27.5 / 27.0.)
   const int64_t units = (int64_t)a.batch * a.units_per_req, tiles = most_tiles(a, C::T);
+  const int slots = C::kPerSm * ctx->num_sms;
   int cluster = 8;
-  while (cluster > 1 && (units * cluster > 2 * ctx->num_sms || cluster >= 2 * tiles)) cluster >>= 1;
+  while (cluster > 1 && (units * cluster > slots || cluster >= 2 * tiles)) cluster >>= 1;
   const int64_t each = (tiles + cluster - 1) / cluster;
-  const int64_t equal = (units * tiles + 2 * ctx->num_sms - 1) / (2 * ctx->num_sms);
+  const int64_t equal = (units * tiles + slots - 1) / slots;
   const bool even = a.window > 0;
   if (each <= (even ? 9 : 4) && each <= equal + (even ? 2 : 1) && units * cluster <= INT32_MAX) {
     a.cluster = cluster;
@@ -822,7 +828,7 @@ int launch(gq_ctx *ctx, const gq_kv_pages *p, Args &a) {
     GQ_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, paged_tiles_kernel<TYPE, D>, (const Args)a, (const CUtensorMap)kmap, (const CUtensorMap)vmap));
     return GQ_OK;
   }
-  const int grid = grid_for(ctx, a, C::T);
+  const int grid = grid_for(a, C::T, slots);
   rc = bind_parts(ctx, grid, a);
   if (rc != GQ_OK) return rc;
   GQ_CUDA_TRY(ctx, gq_launch(ctx, paged_tiles_kernel<TYPE, D>, dim3(grid), dim3(kCompute), C::kSmem, a, kmap, vmap));
