@@ -1,10 +1,10 @@
 // paged_attn.cu — attention of one new token per request over a paged key-value cache
 // (gq_paged_attention).
 //
-//   out_h = sum_j p_j v_j / sum_j p_j,  p_j = 2^(s_j - m),  s_j = log2(e) cap(scale q_h . k_j)
+//   out_h = sum_j p_j v_j / sum_j p_j,  p_j = e^(s_j - m),  s_j = cap(scale q_h . k_j)
 //
 // with m the running maximum: tiles of keys are read once, and when a tile raises m the
-// sum and the output so far are scaled by 2^(m_old - m). What bounds it: the bytes of
+// sum and the output so far are scaled by e^(m_old - m). What bounds it: the bytes of
 // the visible keys and values, each read once (the up to 8 query heads of a key-value
 // head share the read).
 //
@@ -133,18 +133,18 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const Args a) {
 #pragma unroll
       for (int k = 0; k < kRowTile / 16; ++k) {
         const int j = j0 + k * 16 + sl;
-        x[k] = j >= r.lo && j < r.hi ? score_log2(a, s[sh][k * 16 + sl]) : -INFINITY;
+        x[k] = j >= r.lo && j < r.hi ? score_of(a, s[sh][k * 16 + sl]) : -INFINITY;
         top = fmaxf(top, x[k]);
       }
 #pragma unroll
       for (int off = 8; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
       const float mn = fmaxf(m, top);
       const float base = mn == -INFINITY ? 0.0f : mn;  // (no visible key yet)
-      const float f = exp2_of(m - base);
+      const float f = exp_of(m - base);
       l *= f;
 #pragma unroll
       for (int k = 0; k < kRowTile / 16; ++k) {
-        const float p = exp2_of(x[k] - base);
+        const float p = exp_of(x[k] - base);
         s[sh][k * 16 + sl] = p;
         l += p;
       }
@@ -302,12 +302,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Args a, 
       float top = m;
 #pragma unroll
       for (int k = 0; k < kJoinBatch; ++k) top = fmaxf(top, x[k].x);
-      const float f = m == -INFINITY ? 0.0f : exp2f(m - top);
+      const float f = m == -INFINITY ? 0.0f : exp_of(m - top);
       l *= f;
       o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
 #pragma unroll
       for (int k = 0; k < kJoinBatch; ++k) {
-        const float w = x[k].x == -INFINITY ? 0.0f : exp2f(x[k].x - top);
+        const float w = x[k].x == -INFINITY ? 0.0f : exp_of(x[k].x - top);
         l = fmaf(w, x[k].y, l);
         o.x = fmaf(w, v[k].x, o.x);
         o.y = fmaf(w, v[k].y, o.y);
@@ -327,7 +327,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Args a, 
       for (int k = 0; k < groups; ++k) {
         const float2 x = sum_ml[k * wide + tid];
         const float4 v = sums[k * wide + tid];
-        const float f = x.x == -INFINITY ? 0.0f : exp2f(x.x - m);
+        const float f = x.x == -INFINITY ? 0.0f : exp_of(x.x - m);
         l = fmaf(f, x.y, l);
         o.x = fmaf(f, v.x, o.x);
         o.y = fmaf(f, v.y, o.y);

@@ -8,7 +8,7 @@
 // begin another. The lengths are on the device, so each CTA makes the cut itself.
 //
 // Joining: softmax over a cut unit needs each part's maximum m, sum l and unnormalised
-// output o: out = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i, m = max m_i. Parts go
+// output o: out = sum_i e^(m_i - m) o_i / sum_i e^(m_i - m) l_i, m = max m_i. Parts go
 // to workspace slots and the second launch of the call, paged_join_kernel, adds them up
 // in part order, whichever CTA made them (results do not vary from run to run). A join
 // inside the first launch, by the last CTA to arrive, was measured slower: one CTA reads
@@ -171,19 +171,19 @@ __device__ __forceinline__ void put_cut_unit(const Args &a, const Cut &cut, int 
   a.cut_units[blockIdx.x] = make_int4(b, u, parts, slot_of(cut, s0));
 }
 
-// 2^x, x at most a little above 0; -inf gives 0. (What is below 2^-126 of the largest
-// weight counts as 0; the instruction's error is 2^-22.)
-__device__ __forceinline__ float exp2_of(float x) {
+// e^x of a difference x <= 0 of two scores; -inf gives 0. (The difference is taken before it
+// is brought to powers of 2: of scores near the maximum, which weigh most, it is exact.
+// What is below 2^-126 counts as 0; the instruction's error is 2^-22.)
+__device__ __forceinline__ float exp_of(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * kLog2e));
   return y;
 }
 
-// Score of one visible key in units of log2: the scaled, optionally capped product.
-__device__ __forceinline__ float score_log2(const Args &a, float dot) {
-  float s = dot * a.scale;
-  if (a.softcap > 0.0f) s = a.softcap * tanhf(s * a.inv_softcap);
-  return s * kLog2e;
+// Score of one visible key: the scaled, optionally capped product.
+__device__ __forceinline__ float score_of(const Args &a, float dot) {
+  const float s = dot * a.scale;
+  return a.softcap > 0.0f ? a.softcap * tanhf(s * a.inv_softcap) : s;
 }
 
 // ---- host side

@@ -7,7 +7,7 @@
 // slots become free. Four warps compute:
 //   S^T = K q^T        m16 = keys, n8 = heads, over head_dim: keys split over the warps
 //                      (and head_dim over KS warps where q would not fit the registers)
-//   p = 2^(s - m)      16 threads per head; running maximum and sum
+//   p = e^(s - m)      16 threads per head; running maximum and sum
 //   O^T += V^T p^T     m16 = head_dim columns, n8 = heads, over the T keys: columns
 //                      split over the warps
 // with the scores of tile i + 1 in the tensor pipe while the weights of tile i are made:
@@ -186,7 +186,7 @@ __device__ __forceinline__ void join_cluster(const Args &a, const float *mine, c
     for (int p = 0; p < 8; ++p) {
       if (ml[p].x == -INFINITY) continue;  // no CTA, or one without a visible key: its columns are not written
       const float4 v = reinterpret_cast<const float4 *>(cluster.map_shared_rank(mine, p))[at];
-      const float w = exp2_of(ml[p].x - m);
+      const float w = exp_of(ml[p].x - m);
       l = fmaf(w, ml[p].y, l);
       o.x = fmaf(w, v.x, o.x);
       o.y = fmaf(w, v.y, o.y);
@@ -437,7 +437,9 @@ __global__ void __launch_bounds__(kCompute, (Tile<TYPE, D>::kPerSm))
       for (int k = 0; k < 4; ++k) acc[i][k] = 0.0f;
     float m = -INFINITY, l = 0.0f;
     if (tiles > 0) {  // (a cluster's last CTAs may have none)
-    // products of this warp's keys and columns with q: three (two) sums for the parts
+    // Products of this warp's keys and columns with q. The instruction truncates its sums,
+    // so the large products (with q's first part) go to two sums in turn, 0 and 2, and the
+    // small ones to 1: half the truncations in a row, half their error.
     float c[MT][3][4];
     auto products = [&]() {
       const int slot = n % C::kSlots;
@@ -463,22 +465,23 @@ __global__ void __launch_bounds__(kCompute, (Tile<TYPE, D>::kPerSm))
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int y = 0; y < 4; ++y) split_tf32(__uint_as_float(k4[y]), hi[y], lo[y]);
-            mma_tf32(c[x][0], hi, qf[s][0][0], qf[s][0][1]);
+            mma_tf32(c[x][s % 2 * 2], hi, qf[s][0][0], qf[s][0][1]);
             mma_tf32(c[x][1], hi, qf[s][1][0], qf[s][1][1]);
-            mma_tf32(c[x][2], lo, qf[s][0][0], qf[s][0][1]);
+            mma_tf32(c[x][1], lo, qf[s][0][0], qf[s][0][1]);
           } else if constexpr (TYPE == GQ_KV_E4M3) {
             const uint32_t a0[4] = {e4m3_pair(k4[0]), e4m3_pair(k4[1]), e4m3_pair(k4[0] >> 16), e4m3_pair(k4[1] >> 16)};
             const uint32_t a1[4] = {e4m3_pair(k4[2]), e4m3_pair(k4[3]), e4m3_pair(k4[2] >> 16), e4m3_pair(k4[3] >> 16)};
             mma_f16(c[x][0], a0, qf[2 * s][0][0], qf[2 * s][0][1]);
             mma_f16(c[x][1], a0, qf[2 * s][1][0], qf[2 * s][1][1]);
-            mma_f16(c[x][0], a1, qf[2 * s + 1][0][0], qf[2 * s + 1][0][1]);
+            mma_f16(c[x][2], a1, qf[2 * s + 1][0][0], qf[2 * s + 1][0][1]);
             mma_f16(c[x][1], a1, qf[2 * s + 1][1][0], qf[2 * s + 1][1][1]);
           } else if constexpr (TYPE == GQ_KV_F16) {
-            mma_f16(c[x][0], k4, qf[s][0][0], qf[s][0][1]);
+            mma_f16(c[x][s % 2 * 2], k4, qf[s][0][0], qf[s][0][1]);
             mma_f16(c[x][1], k4, qf[s][1][0], qf[s][1][1]);
           } else {
+            mma_bf16(c[x][s % 2 * 2], k4, qf[s][0][0], qf[s][0][1]);
 #pragma unroll
-            for (int p = 0; p < 3; ++p) mma_bf16(c[x][p], k4, qf[s][p % C::kParts][0], qf[s][p % C::kParts][1]);
+            for (int p = 1; p < C::kParts; ++p) mma_bf16(c[x][1], k4, qf[s][p][0], qf[s][p][1]);
           }
         }
       }
@@ -487,10 +490,10 @@ __global__ void __launch_bounds__(kCompute, (Tile<TYPE, D>::kPerSm))
 #pragma unroll
       for (int x = 0; x < MT; ++x) {
         float *to = sS + buf * C::kSFloats + ks * kHeads * C::kSStride + 2 * q4 * C::kSStride + (mt + x) * 16 + g;
-        to[0] = (c[x][0][0] + (c[x][1][0] + c[x][2][0])) * unscale0;
-        to[C::kSStride] = (c[x][0][1] + (c[x][1][1] + c[x][2][1])) * unscale1;
-        to[8] = (c[x][0][2] + (c[x][1][2] + c[x][2][2])) * unscale0;
-        to[C::kSStride + 8] = (c[x][0][3] + (c[x][1][3] + c[x][2][3])) * unscale1;
+        to[0] = ((c[x][0][0] + c[x][2][0]) + c[x][1][0]) * unscale0;
+        to[C::kSStride] = ((c[x][0][1] + c[x][2][1]) + c[x][1][1]) * unscale1;
+        to[8] = ((c[x][0][2] + c[x][2][2]) + c[x][1][2]) * unscale0;
+        to[C::kSStride + 8] = ((c[x][0][3] + c[x][2][3]) + c[x][1][3]) * unscale1;
       }
     };
 
@@ -518,22 +521,22 @@ __global__ void __launch_bounds__(kCompute, (Tile<TYPE, D>::kPerSm))
 #pragma unroll
           for (int p = 1; p < KS; ++p) s += from[p * kHeads * C::kSStride + k];
           const int j = j0 + sl * KPT + k;
-          s = score_log2(a, s);
+          s = score_of(a, s);
           x[k] = ragged && (j < r.lo || j >= r.hi) ? -INFINITY : s;
           top = fmaxf(top, x[k]);
         }
 #pragma unroll
         for (int off = 8; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         const float mn = fmaxf(m, top);
-        const float zero = mn == -INFINITY ? 0.0f : mn;  // (no visible key yet)
-        const float f = exp2_of(m - zero);
-        // p = 2^(x - m), times 2^14 for the f16 parts (a common factor of every weight and sum)
-        const float base = TYPE == GQ_KV_F16 || TYPE == GQ_KV_E4M3 ? zero - 14.0f : zero;
+        const float base = mn == -INFINITY ? 0.0f : mn;  // (no visible key yet)
+        const float f = exp_of(m - base);
+        // p = e^(x - m), times 2^14 for the f16 parts (a common factor of every weight and sum)
+        constexpr float kUp = TYPE == GQ_KV_F16 || TYPE == GQ_KV_E4M3 ? 16384.0f : 1.0f;
         float p[KPT];
         l *= f;
 #pragma unroll
         for (int k = 0; k < KPT; ++k) {
-          p[k] = exp2_of(x[k] - base);
+          p[k] = kUp * exp_of(x[k] - base);
           l += p[k];
         }
         m = mn;
@@ -583,7 +586,7 @@ __global__ void __launch_bounds__(kCompute, (Tile<TYPE, D>::kPerSm))
       }
       ++n;
 
-      // ---- output columns warp * D/4 ..: o = o 2^(m_old - m) + V^T p. The instruction
+      // ---- output columns warp * D/4 ..: o = o e^(m_old - m) + V^T p. The instruction
       // truncates its sums, so it adds up one tile only; tiles are added in registers.
       {
         const float f0 = fix[buf][2 * q4], f1 = fix[buf][2 * q4 + 1];
