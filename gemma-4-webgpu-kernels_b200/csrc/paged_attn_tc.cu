@@ -150,6 +150,7 @@ struct Tile {
   static constexpr int kSlots = std::min(kMaxSlots, (kSmemBytes - kRest) / kSlot);
   static constexpr int kSmem = kRest + kSlots * kSlot;
   static constexpr int kTShift = T == 128 ? 7 : T == 64 ? 6 : T == 32 ? 5 : 4;
+  static_assert(kQSteps % 4 == 0, "whole groups of products");
   static_assert(kRow % 128 == 0 && kSlots >= 3 && (1 << kTShift) == T && kPBytes % 16 == 0, "tile");
 };
 
@@ -437,9 +438,9 @@ __global__ void __launch_bounds__(kCompute, (Tile<TYPE, D>::kPerSm))
       for (int k = 0; k < 4; ++k) acc[i][k] = 0.0f;
     float m = -INFINITY, l = 0.0f;
     if (tiles > 0) {  // (a cluster's last CTAs may have none)
-    // Products of this warp's keys and columns with q. The instruction truncates its sums,
-    // so the large products (with q's first part) go to two sums in turn, 0 and 2, and the
-    // small ones to 1: half the truncations in a row, half their error.
+    // Products of this warp's keys and columns with q. The instruction truncates its sums:
+    // the large products (with q's first part) are added up four instructions at a time
+    // in 0, and those sums, rounded, in 2; the small ones go to 1.
     float c[MT][3][4];
     auto products = [&]() {
       const int slot = n % C::kSlots;
@@ -465,7 +466,7 @@ __global__ void __launch_bounds__(kCompute, (Tile<TYPE, D>::kPerSm))
             uint32_t hi[4], lo[4];
 #pragma unroll
             for (int y = 0; y < 4; ++y) split_tf32(__uint_as_float(k4[y]), hi[y], lo[y]);
-            mma_tf32(c[x][s % 2 * 2], hi, qf[s][0][0], qf[s][0][1]);
+            mma_tf32(c[x][0], hi, qf[s][0][0], qf[s][0][1]);
             mma_tf32(c[x][1], hi, qf[s][1][0], qf[s][1][1]);
             mma_tf32(c[x][1], lo, qf[s][0][0], qf[s][0][1]);
           } else if constexpr (TYPE == GQ_KV_E4M3) {
@@ -473,16 +474,22 @@ __global__ void __launch_bounds__(kCompute, (Tile<TYPE, D>::kPerSm))
             const uint32_t a1[4] = {e4m3_pair(k4[2]), e4m3_pair(k4[3]), e4m3_pair(k4[2] >> 16), e4m3_pair(k4[3] >> 16)};
             mma_f16(c[x][0], a0, qf[2 * s][0][0], qf[2 * s][0][1]);
             mma_f16(c[x][1], a0, qf[2 * s][1][0], qf[2 * s][1][1]);
-            mma_f16(c[x][2], a1, qf[2 * s + 1][0][0], qf[2 * s + 1][0][1]);
+            mma_f16(c[x][0], a1, qf[2 * s + 1][0][0], qf[2 * s + 1][0][1]);
             mma_f16(c[x][1], a1, qf[2 * s + 1][1][0], qf[2 * s + 1][1][1]);
           } else if constexpr (TYPE == GQ_KV_F16) {
-            mma_f16(c[x][s % 2 * 2], k4, qf[s][0][0], qf[s][0][1]);
+            mma_f16(c[x][0], k4, qf[s][0][0], qf[s][0][1]);
             mma_f16(c[x][1], k4, qf[s][1][0], qf[s][1][1]);
           } else {
-            mma_bf16(c[x][s % 2 * 2], k4, qf[s][0][0], qf[s][0][1]);
+            mma_bf16(c[x][0], k4, qf[s][0][0], qf[s][0][1]);
 #pragma unroll
             for (int p = 1; p < C::kParts; ++p) mma_bf16(c[x][1], k4, qf[s][p][0], qf[s][p][1]);
           }
+          if (s % (TYPE == GQ_KV_E4M3 ? 2 : 4) == (TYPE == GQ_KV_E4M3 ? 1 : 3))
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              c[x][2][k] += c[x][0][k];
+              c[x][0][k] = 0.0f;
+            }
         }
       }
     };
@@ -490,10 +497,10 @@ __global__ void __launch_bounds__(kCompute, (Tile<TYPE, D>::kPerSm))
 #pragma unroll
       for (int x = 0; x < MT; ++x) {
         float *to = sS + buf * C::kSFloats + ks * kHeads * C::kSStride + 2 * q4 * C::kSStride + (mt + x) * 16 + g;
-        to[0] = ((c[x][0][0] + c[x][2][0]) + c[x][1][0]) * unscale0;
-        to[C::kSStride] = ((c[x][0][1] + c[x][2][1]) + c[x][1][1]) * unscale1;
-        to[8] = ((c[x][0][2] + c[x][2][2]) + c[x][1][2]) * unscale0;
-        to[C::kSStride + 8] = ((c[x][0][3] + c[x][2][3]) + c[x][1][3]) * unscale1;
+        to[0] = (c[x][2][0] + c[x][1][0]) * unscale0;
+        to[C::kSStride] = (c[x][2][1] + c[x][1][1]) * unscale1;
+        to[8] = (c[x][2][2] + c[x][1][2]) * unscale0;
+        to[C::kSStride + 8] = (c[x][2][3] + c[x][1][3]) * unscale1;
       }
     };
 
