@@ -231,6 +231,25 @@ def test_append_to_interleaved_pages_and_past_the_pool(g):
     assert torch.equal(both, want)
 
 
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("t,h,d", [(20011, 1, 128), (20011, 3, 20), (5003, 1, 132)])
+def test_append_of_more_rows_than_the_grid_takes_at_once(g, name, t, h, d):
+    torch = g._torch
+    ps, dt = 16, tdtype(g, name)
+    n_pages = t // ps + 3
+    pools = [torch.zeros(n_pages, h, ps, d, device=g.torch_device).to(dt) for _ in range(2)]
+    gen = torch.Generator(device=g.torch_device).manual_seed(t + d)
+    xs = torch.randn(2, t, h, d, device=g.torch_device, generator=gen)
+    slots = torch.randperm(n_pages * ps, device=g.torch_device, generator=gen)[:t]
+    slots[::7] = -1
+    g.paged_append(g.kv_pages(*pools), xs[0], xs[1], slots)
+    assert sync_status(g) == _abi.GQ_OK
+    for got, rows in zip(pools, xs):
+        want = torch.zeros(n_pages * ps, h, d, device=g.torch_device).to(dt)
+        want[slots[slots >= 0]] = rows[slots >= 0].to(dt)
+        assert torch.equal(got, want.view(n_pages, ps, h, d).transpose(1, 2))
+
+
 # ---- attention ----------------------------------------------------------------------------------------
 
 
