@@ -103,7 +103,8 @@ class PagedDecoder(e2b.Decoder):
         """Add new_lens[b] tokens to request b without decoding (a prompt's cache made
         elsewhere): rows(layer) gives their keys and values, f32 [sum, heads_kv *
         head_dim] in request order, for each source layer; tokens, when given, each
-        request's ids (its prompt, for the penalties). Raises when the pages do not
+        request's ids (its prompt, for the penalties; all that an extended request holds
+        counts as its prompt from then on). Raises when the pages do not
         suffice; nothing is taken then."""
         torch, c, g = self.torch, self.cfg, self.g
         dev, total = g.torch_device, int(np.sum(new_lens))
@@ -122,7 +123,8 @@ class PagedDecoder(e2b.Decoder):
         if tokens is not None:
             for b, ids in enumerate(tokens):
                 self.history[b, before[b]:before[b] + len(ids)] = torch.tensor(list(ids), dtype=torch.int32, device=dev)
-        self.prompt_lens.copy_(self.lens)
+        # (requests that were not extended keep theirs: what they generated stays generated)
+        self.prompt_lens.copy_(torch.where(new > 0, self.lens, self.prompt_lens))
         self.keep.masked_fill_(new > 0, KEEP_ALL)
         torch.cuda.synchronize(dev)
 

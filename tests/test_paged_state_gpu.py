@@ -1,0 +1,87 @@
+"""What gq.paged.PagedDecoder keeps of its requests while others join, end and stand
+still (needs a B200). The tests keep each request's ids themselves; the step's
+controlled logits must equal the definition applied to its raw logits, operation by
+operation in f32 (every one rounds once on both sides)."""
+import numpy as np
+import pytest
+
+from gq import CudaBackend, e2b, paged
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def g():
+    be = CudaBackend(0, own_stream=True)
+    yield be
+    be.close()
+
+
+CFG = e2b.small_config()
+
+
+def seeded_rows(g, lens, seed=5):
+    """Keys and values of `lens` new tokens of each request, ~N(0, 1)."""
+    def rows(layer):
+        gen = g._torch.Generator(device=g.torch_device).manual_seed(seed + layer)
+        d = CFG.heads_kv * CFG.dh(layer)
+        return [g._torch.randn(sum(lens), d, generator=gen, device=g.torch_device) for _ in range(2)]
+    return rows
+
+
+def make(g, batch, max_len=64, seed=12, **kw):
+    return paged.PagedDecoder(g, CFG, e2b.Weights(CFG, seed=seed), batch, max_len=max_len, kv_type="f32", **kw)
+
+
+def set_penalties(g, dec, rep, presence, frequency):
+    dec.penalties.copy_(g._torch.tensor([[rep, presence, frequency]], device=g.torch_device).expand(dec.batch, 3))
+    g._torch.cuda.synchronize()
+
+
+def controlled(raw, prompt, made, rep, presence, frequency):
+    """The penalties' definition: ids of the prompt (None: not known) and the ids decoded since."""
+    f, y = np.float32, np.array(raw, dtype=np.float32)
+    for c in {t for t in list(prompt) + list(made) if t is not None}:
+        y[c] = y[c] / f(rep) if y[c] > 0 else y[c] * f(rep)
+        n = list(made).count(c)
+        if n:
+            y[c] = (y[c] - f(frequency) * f(n)) - f(presence)
+    return y
+
+
+PENALTIES = (1.25, 0.75, 0.5)
+
+
+def check_controlled(dec, prompts, made, places):
+    raw, got = dec.read(dec.logits), dec.read(dec.controlled)
+    for b in places:
+        np.testing.assert_array_equal(got[b], controlled(raw[b], prompts[b], made[b], *PENALTIES), err_msg=f"request {b}")
+
+
+def test_a_request_that_joins_leaves_the_others_penalties_alone(g):
+    """What running requests have generated stays generated: their presence and frequency
+    penalties count it after another request joins."""
+    dec = make(g, 3)
+    set_penalties(g, dec, *PENALTIES)
+    prompts, made = [[1, 2, 3], [7] * 20, []], [[], [], []]
+    dec.extend([3, 20, 0], seeded_rows(g, [3, 20]), tokens=[prompts[0], prompts[1], []])
+    for ids in ([5, 9, 11], [5, 7, 12], [6, 8, 12]):
+        dec.step(ids)
+        g.flush()
+        for b in range(3):
+            made[b].append(ids[b])
+        check_controlled(dec, prompts, made, range(3))
+    dec.end([2])
+    dec.step([6, 6, 6])
+    g.flush()
+    prompts[2], made[2] = [30, 31, 32, 33, 34], []
+    for b in (0, 1):
+        made[b].append(6)
+    dec.extend([0, 0, 5], seeded_rows(g, [5], seed=9), tokens=[[], [], prompts[2]])
+    assert dec.prompt_lens.tolist() == [3, 20, 5]
+    dec.step([5, 7, 30])
+    g.flush()
+    for b, t in enumerate([5, 7, 30]):
+        made[b].append(t)
+    check_controlled(dec, prompts, made, range(3))
+    dec.close()
