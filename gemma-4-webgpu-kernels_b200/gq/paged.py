@@ -103,7 +103,7 @@ class PagedDecoder(e2b.Decoder):
         """Add new_lens[b] tokens to request b without decoding (a prompt's cache made
         elsewhere): rows(layer) gives their keys and values, f32 [sum, heads_kv *
         head_dim] in request order, for each source layer; tokens, when given, each
-        request's ids (its prompt, for the penalties; all that an extended request holds
+        request's ids, as many as are known (its prompt, for the penalties; all that an extended request holds
         counts as its prompt from then on). Raises when the pages do not
         suffice; nothing is taken then."""
         torch, c, g = self.torch, self.cfg, self.g
@@ -120,6 +120,9 @@ class PagedDecoder(e2b.Decoder):
         for i, (k, v) in kv.items():
             g.paged_append(self.pages[i], k.view(total, c.heads_kv, c.dh(i)), v.view(total, c.heads_kv, c.dh(i)), slots)
         g.flush()
+        # ids that are not given are -1, which the penalties ignore
+        at, first = torch.arange(self.capacity, device=dev)[None], torch.tensor(before, device=dev)[:, None]
+        self.history.masked_fill_((at >= first) & (at < first + new[:, None]), -1)
         if tokens is not None:
             for b, ids in enumerate(tokens):
                 self.history[b, before[b]:before[b] + len(ids)] = torch.tensor(list(ids), dtype=torch.int32, device=dev)

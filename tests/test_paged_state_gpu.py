@@ -85,3 +85,26 @@ def test_a_request_that_joins_leaves_the_others_penalties_alone(g):
         made[b].append(t)
     check_controlled(dec, prompts, made, range(3))
     dec.close()
+
+
+def test_a_prompt_without_ids_is_not_penalised(g):
+    """A prompt whose ids are not given counts as no id: not as zeros, and not as what the
+    place's former request said."""
+    dec = make(g, 2)
+    set_penalties(g, dec, *PENALTIES)
+    dec.extend([4, 20], seeded_rows(g, [4, 20]), tokens=[[1, 2, 3, 4], list(range(40, 60))])
+    dec.step([5, 60])
+    g.flush()
+    dec.end([1])
+    dec.step([6, 61])
+    g.flush()
+    dec.extend([0, 12], seeded_rows(g, [12], seed=9))
+    dec.step([7, 8])
+    g.flush()
+    check_controlled(dec, [[1, 2, 3, 4], []], [[5, 6, 7], [8]], range(2))
+    # ids of a part of the prompt: the rest is not known
+    dec.extend([0, 6], seeded_rows(g, [6], seed=10), tokens=[[], [21, 22]])
+    dec.step([8, 9])
+    g.flush()
+    check_controlled(dec, [[1, 2, 3, 4], [8, 21, 22]], [[5, 6, 7, 8], [9]], range(2))
+    dec.close()
