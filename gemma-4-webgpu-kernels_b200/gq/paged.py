@@ -109,6 +109,7 @@ class PagedDecoder(e2b.Decoder):
         torch, c, g = self.torch, self.cfg, self.g
         dev, total = g.torch_device, int(np.sum(new_lens))
         place = lambda dt: torch.empty(total, dtype=dt, device=dev)  # noqa: E731
+        self._stream().synchronize()  # steps in flight change the lengths
         before = self.lens.tolist()
         new, slots = torch.tensor(list(new_lens), dtype=torch.int32, device=dev), place(torch.int64)
         pos, owners = place(torch.int32), place(torch.int32)
@@ -216,6 +217,7 @@ class PagedDecoder(e2b.Decoder):
     def kv_bytes(self) -> int:
         """K and V bytes that a step's attention reads at the present lengths."""
         c, size = self.cfg, {"f32": 4, "e4m3": 1}.get(self.kv_type, 2)
+        self._stream().synchronize()
         lens, tot = self.lens.tolist(), 0
         for i in range(c.layers):
             w = c.window_of(i)

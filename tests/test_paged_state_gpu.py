@@ -108,3 +108,32 @@ def test_a_prompt_without_ids_is_not_penalised(g):
     g.flush()
     check_controlled(dec, [[1, 2, 3, 4], [8, 21, 22]], [[5, 6, 7, 8], [9]], range(2))
     dec.close()
+
+
+def hold(g, dec, ms=60):
+    """Keep the backend's stream busy for some milliseconds, so that what is enqueued next
+    is still to come when the host goes on."""
+    with g._torch.cuda.stream(dec._stream()):
+        g._torch.cuda._sleep(int(ms * 1.9e6))
+
+
+def test_extend_sees_the_steps_still_in_flight(g):
+    """A request takes the place of one that ended in a step not yet done: its ids go to the
+    start of the place's history."""
+    dec = make(g, 2)
+    set_penalties(g, dec, *PENALTIES)
+    dec.extend([4, 20], seeded_rows(g, [4, 20]), tokens=[[1, 2, 3, 4], list(range(40, 60))])
+    hold(g, dec)
+    dec.end([1])
+    dec.step([5, 60])
+    dec.extend([0, 3], seeded_rows(g, [3], seed=9), tokens=[[], [30, 31, 32]])
+    assert dec.lens.tolist() == [5, 3]
+    assert dec.history[1, :3].tolist() == [30, 31, 32]
+    hold(g, dec)
+    dec.step([6, 33])
+    size = 2 * CFG.heads_kv * 4
+    want = sum(size * CFG.dh(i) * min(n, CFG.window_of(i) or n) for n in (6, 4) for i in range(CFG.layers))
+    assert dec.kv_bytes() == want
+    g.flush()
+    check_controlled(dec, [[1, 2, 3, 4], [30, 31, 32]], [[5, 6], [33]], range(2))
+    dec.close()
