@@ -105,11 +105,11 @@ class PagedDecoder(e2b.Decoder):
         head_dim] in request order, for each source layer; tokens, when given, each
         request's ids, as many as are known (its prompt, for the penalties; all that an extended request holds
         counts as its prompt from then on). Raises when the pages do not
-        suffice; nothing is taken then."""
+        suffice, and what earlier steps left to raise; nothing is taken then."""
         torch, c, g = self.torch, self.cfg, self.g
         dev, total = g.torch_device, int(np.sum(new_lens))
         place = lambda dt: torch.empty(total, dtype=dt, device=dev)  # noqa: E731
-        self._stream().synchronize()  # steps in flight change the lengths
+        g.flush()  # steps in flight change the lengths; their errors are raised before anything is taken
         before = self.lens.tolist()
         new, slots = torch.tensor(list(new_lens), dtype=torch.int32, device=dev), place(torch.int64)
         pos, owners = place(torch.int32), place(torch.int32)

@@ -5,7 +5,7 @@ operation in f32 (every one rounds once on both sides)."""
 import numpy as np
 import pytest
 
-from gq import CudaBackend, e2b, paged
+from gq import CudaBackend, GqError, _abi, e2b, paged
 
 pytestmark = pytest.mark.gpu
 
@@ -136,4 +136,24 @@ def test_extend_sees_the_steps_still_in_flight(g):
     assert dec.kv_bytes() == want
     g.flush()
     check_controlled(dec, [[1, 2, 3, 4], [30, 31, 32]], [[5, 6], [33]], range(2))
+    dec.close()
+
+
+def test_an_earlier_steps_error_takes_nothing(g):
+    """An error that a step left behind is raised before extend takes pages: its rows are
+    not left out of pages that it took."""
+    dec = make(g, 2, n_pages=3)
+    dec.extend([32, 0], seeded_rows(g, [32]))
+    dec.step([1, 2])  # one page is left, two are needed
+    with pytest.raises(GqError) as e:
+        dec.extend([0, 5], seeded_rows(g, [5], seed=9))
+    assert e.value.status == _abi.GQ_ERR_DEVICE
+    assert dec.lens.tolist() == [32, 0] and int(dec.count[0]) == 1
+    rows = seeded_rows(g, [5], seed=9)
+    dec.extend([0, 5], rows)
+    assert dec.lens.tolist() == [32, 5] and int(dec.count[0]) == 0
+    for layer, pages in dec.pages.items():
+        k, v = rows(layer)
+        at = dec.table[1, 0].long()
+        assert g._torch.equal(pages.k[at, 0, :5], k) and g._torch.equal(pages.v[at, 0, :5], v)
     dec.close()
