@@ -105,13 +105,20 @@ class PagedDecoder(e2b.Decoder):
         head_dim] in request order, for each source layer; tokens, when given, each
         request's ids, as many as are known (its prompt, for the penalties; all that an extended request holds
         counts as its prompt from then on). Raises when the pages do not
-        suffice, and what earlier steps left to raise; nothing is taken then."""
+        suffice, and what earlier steps left to raise; nothing is taken then. A place whose request was
+        ended begins anew, whether a step has come between or not."""
         torch, c, g = self.torch, self.cfg, self.g
         dev, total = g.torch_device, int(np.sum(new_lens))
         place = lambda dt: torch.empty(total, dtype=dt, device=dev)  # noqa: E731
         g.flush()  # steps in flight change the lengths; their errors are raised before anything is taken
-        before = self.lens.tolist()
         new, slots = torch.tensor(list(new_lens), dtype=torch.int32, device=dev), place(torch.int64)
+        anew = (new > 0) & (self.keep == 0)  # places whose end no step has carried out yet: it is now
+        if bool(anew.any()):
+            keep = torch.where(anew, 0, KEEP_ALL).to(torch.int32)
+            torch.cuda.synchronize(dev)
+            g.paged_release(self.lens, keep, self.page_size, self.table, self.free, self.count, self.lens, self.count)
+            g.flush()
+        before = self.lens.tolist()
         pos, owners = place(torch.int32), place(torch.int32)
         kv = {i: rows(i) for i in self.pages} if total else {}
         torch.cuda.synchronize(dev)  # (the rows are torch's, the calls go to the backend's stream)

@@ -1,13 +1,17 @@
 """What gq.paged.PagedDecoder keeps of its requests while others join, end and stand
 still (needs a B200). The tests keep each request's ids themselves; the step's
 controlled logits must equal the definition applied to its raw logits, operation by
-operation in f32 (every one rounds once on both sides)."""
+operation in f32 (every one rounds once on both sides). Logits of two decoders of the
+same step agree to relative L2 1e-4, the bound of the whole-step tests."""
 import numpy as np
 import pytest
 
 from gq import CudaBackend, GqError, _abi, e2b, paged
+from numerics import rel_l2
 
 pytestmark = pytest.mark.gpu
+
+STEP_REL = 1e-4
 
 
 @pytest.fixture(scope="module")
@@ -156,4 +160,42 @@ def test_an_earlier_steps_error_takes_nothing(g):
         k, v = rows(layer)
         at = dec.table[1, 0].long()
         assert g._torch.equal(pages.k[at, 0, :5], k) and g._torch.equal(pages.v[at, 0, :5], v)
+    dec.close()
+
+
+def alone(g, rows, ids):
+    """Logits of decoding `ids` after the cache `rows` of one request, in a decoder of its own."""
+    dec = make(g, 1)
+    n = rows(0)[0].shape[0]
+    dec.extend([n], rows)
+    for t in ids:
+        dec.step([t])
+    g.flush()
+    out = dec.read(dec.logits)[0].copy()
+    dec.close()
+    return out
+
+
+def test_a_request_that_takes_an_ended_place_at_once(g):
+    """end, then extend with no step between: the place begins anew, and the former
+    request's pages are back."""
+    dec = make(g, 2, n_pages=4)
+    dec.extend([40, 3], seeded_rows(g, [40, 3]), tokens=[[9] * 40, [1, 2, 3]])
+    assert int(dec.count[0]) == 0
+    dec.end([0])
+    rows = seeded_rows(g, [18], seed=9)
+    dec.extend([18, 0], rows, tokens=[[5] * 18, []])
+    assert dec.lens.tolist() == [18, 3] and int(dec.count[0]) == 1
+    assert dec.history[0, :18].tolist() == [5] * 18
+    dec.step([7, 8])
+    g.flush()
+    assert dec.lens.tolist() == [19, 4] and dec.prompt_lens.tolist() == [18, 3]
+    assert rel_l2(dec.read(dec.logits)[0], alone(g, rows, [7])) <= STEP_REL
+    # a place that ended and is not extended still waits for its step
+    dec.end([1])
+    dec.extend([2, 0], seeded_rows(g, [2], seed=11))
+    assert dec.lens.tolist() == [21, 4]
+    dec.step([7, 8])
+    g.flush()
+    assert dec.lens.tolist() == [22, 0]
     dec.close()
