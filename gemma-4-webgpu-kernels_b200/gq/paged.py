@@ -23,6 +23,7 @@ from __future__ import annotations
 import argparse
 import ctypes
 import sys
+from contextlib import contextmanager
 from ctypes import c_float, c_void_p
 from typing import Optional, Sequence
 
@@ -43,8 +44,9 @@ class PagedDecoder(e2b.Decoder):
     are the requests' lengths, filled by ``extend``; a place whose length is 0 and that
     was ended idles: it decodes from an empty cache and gives its page back every step.
 
-    Controls, all device tensors that may be changed between steps: ``penalties``
-    [batch, 3] (repetition, presence, frequency), ``prompt_lens`` [batch], ``history``
+    Controls, all device tensors that may be changed between steps on torch's current
+    stream, which a step comes after and which goes on after it (whatever stream the
+    backend has): ``penalties`` [batch, 3] (repetition, presence, frequency), ``prompt_lens`` [batch], ``history``
     [batch, max_len] (tokens by position), and, given at construction because their sizes
     belong to the recorded step, ``bias`` (ids, values, offsets) and ``masks``
     (words, rows); see gq_process_logits in include/gq.h. ``sample``: temperature, top_k,
@@ -99,6 +101,21 @@ class PagedDecoder(e2b.Decoder):
     def _stream(self):
         return self.torch.cuda.ExternalStream(self.g.stream_ptr(), device=self.g.torch_device)
 
+    @contextmanager
+    def _ordered(self):
+        """Work on the backend's stream that comes after what torch's current stream was given
+        so far, and before what it is given next."""
+        mine, callers = self._stream(), self.torch.cuda.current_stream(self.g.torch_device)
+        apart = (callers.cuda_stream or 1) != mine.cuda_stream  # (1: the legacy default stream, as the backend has it)
+        if apart:
+            mine.wait_stream(callers)
+        try:
+            with self.torch.cuda.stream(mine):
+                yield
+        finally:
+            if apart:
+                callers.wait_stream(mine)
+
     def extend(self, new_lens: Sequence[int], rows, tokens: Optional[Sequence[Sequence[int]]] = None) -> None:
         """Add new_lens[b] tokens to request b without decoding (a prompt's cache made
         elsewhere): rows(layer) gives their keys and values, f32 [sum, heads_kv *
@@ -141,7 +158,7 @@ class PagedDecoder(e2b.Decoder):
 
     def end(self, places: Sequence[int]) -> None:
         """The requests at these places end: the next step gives their pages back."""
-        with self.torch.cuda.stream(self._stream()):
+        with self._ordered():
             self.keep[self.torch.tensor(list(places), device=self.g.torch_device)] = 0
 
     # ---- the step ----------------------------------------------------------------------
@@ -186,17 +203,17 @@ class PagedDecoder(e2b.Decoder):
         step sampled) in, the sampled ``tokens`` [batch] out (a device tensor, valid until
         the next step). Enqueued; a page shortage shows at the next ``g.flush()``."""
         torch = self.torch
-        with torch.cuda.stream(self._stream()):
+        with self._ordered():
             if ids is None:
                 self.ids.copy_(self.tokens)
             else:
                 self.ids.copy_(torch.as_tensor(np.asarray(ids, dtype=np.int32).reshape(self.batch)))
             at = self.lens.long().clamp(max=self.capacity - 1)[:, None]
             self.history.scatter_(1, at, self.ids[:, None])
-        if self.graph is not None:
-            self.g.replay(self.graph)
-        else:
-            self.run()
+            if self.graph is not None:
+                self.g.replay(self.graph)
+            else:
+                self.run()
         return self.tokens
 
     def record_steps(self) -> None:

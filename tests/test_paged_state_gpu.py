@@ -199,3 +199,48 @@ def test_a_request_that_takes_an_ended_place_at_once(g):
     g.flush()
     assert dec.lens.tolist() == [22, 0]
     dec.close()
+
+
+def test_controls_and_tokens_follow_the_callers_stream(g):
+    """What torch's current stream does before a step is in it, what it does after comes
+    after it, and it sees the step's tokens and lengths, all without a synchronisation."""
+    torch = g._torch
+    dec = make(g, 2)
+    dec.extend([3, 4], seeded_rows(g, [3, 4]), tokens=[[1, 2, 3], [4, 5, 6, 7]])
+    new = torch.tensor([PENALTIES] * 2, device=g.torch_device)
+    prompts, made, tokens = [[1, 2, 3], [4, 5, 6, 7]], [[], []], [8, 9]
+    dec.tokens.copy_(torch.tensor(tokens, device=g.torch_device))
+    for record in (False, True):
+        if record:
+            dec.record_steps()
+        dec.penalties.copy_(torch.tensor([[1.0, 0.0, 0.0]] * 2, device=g.torch_device))
+        torch.cuda.synchronize()
+        torch.cuda._sleep(100_000_000)  # the change below is still to come when step returns
+        dec.penalties.copy_(new)
+        dec.step()
+        for b in range(2):
+            made[b].append(tokens[b])
+        tokens = dec.tokens.tolist()
+        g.flush()
+        check_controlled(dec, prompts, made, range(2))
+        hold(g, dec)
+        dec.step()
+        dec.penalties.fill_(2.0)  # the step, still in flight, does not see it
+        for b in range(2):
+            made[b].append(tokens[b])
+        tokens = dec.tokens.tolist()
+        assert dec.lens.tolist() == [3 + len(made[0]), 4 + len(made[1])]
+        g.flush()
+        check_controlled(dec, prompts, made, range(2))
+        assert tokens == np.argmax(dec.read(dec.controlled), 1).tolist()
+    # a change on another stream of the caller's
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        dec.penalties.copy_(new)
+        dec.step()
+    for b in range(2):
+        made[b].append(tokens[b])
+    g.flush()
+    check_controlled(dec, prompts, made, range(2))
+    dec.close()
