@@ -83,6 +83,8 @@ class PagedDecoder(e2b.Decoder):
         self.free = torch.arange(self.n_pages, dtype=i32, device=dev)
         self.count = torch.tensor([self.n_pages], dtype=i32, device=dev)
         self.lens = torch.zeros(B, dtype=i32, device=dev)
+        self.now = torch.zeros(B, dtype=i32, device=dev)  # the lengths with the step's tokens
+        self.took = torch.zeros(B, dtype=torch.bool, device=dev)
         self.one = torch.ones(B, dtype=i32, device=dev)
         self.keep = torch.full((B,), KEEP_ALL, dtype=i32, device=dev)
         self.slots = torch.zeros(B, dtype=torch.int64, device=dev)
@@ -96,6 +98,7 @@ class PagedDecoder(e2b.Decoder):
         self.controlled = torch.empty(B, c.vocab, device=dev)
         self.tokens = torch.zeros(B, dtype=i32, device=dev)
         self.rng = torch.arange(self.seed, self.seed + B, dtype=torch.int64, device=dev)
+        self.drawn, self.rng_after = torch.zeros_like(self.tokens), torch.zeros_like(self.rng)  # of the step
         torch.cuda.synchronize(dev)
 
     def _stream(self):
@@ -170,7 +173,7 @@ class PagedDecoder(e2b.Decoder):
         V = lambda t: c_void_p(t.data_ptr())  # noqa: E731
         add("reserve", self.g.lib.gq_paged_reserve, self.g.ctx, self.batch, self.page_size, V(self.lens), V(self.one),
             V(self.table), self.table.shape[1], V(self.free), self.n_pages, V(self.count), V(self.count), self.batch,
-            V(self.slots), V(self.pos), V(self.owners), V(self.lens))
+            V(self.slots), V(self.pos), V(self.owners), V(self.now))
 
     def _new_rows(self, src: int, p: int, kvd: int):
         return c_void_p(self.new_k.data_ptr()), c_void_p(self.new_v.data_ptr()), kvd
@@ -182,7 +185,7 @@ class PagedDecoder(e2b.Decoder):
             add(pre + "append", lib.gq_paged_append, ctx, pages, V(self.new_k), V(self.new_v), self.batch, 0, 0,
                 V(self.slots))
         add(pre + "attention", lib.gq_paged_attention, ctx, pages, V(self.qr), self.batch, c.heads_q, 0, V(self.table),
-            self.table.shape[1], V(self.lens), c_float(1.0), c.window_of(i), c_float(0.0), V(self.attn))
+            self.table.shape[1], V(self.now), c_float(1.0), c.window_of(i), c_float(0.0), V(self.attn))
 
     def _end_calls(self, add) -> None:
         V = lambda t: c_void_p(t.data_ptr()) if t is not None else None  # noqa: E731
@@ -190,18 +193,39 @@ class PagedDecoder(e2b.Decoder):
         ids, values, offsets = self.bias or (None, None, None)
         words, rows = self.masks or (None, None)
         add("process_logits", lib.gq_process_logits, ctx, V(self.logits), B, vocab, vocab, V(self.history), self.capacity,
-            V(self.prompt_lens), V(self.lens), V(self.penalties), V(ids), V(values), V(offsets), V(words),
+            V(self.prompt_lens), V(self.now), V(self.penalties), V(ids), V(values), V(offsets), V(words),
             words.shape[0] if words is not None else 0, words.shape[1] if words is not None else 0, V(rows),
             V(self.controlled), vocab)
+        if self.opts.temperature > 0:
+            add("rng", self._torch_call, lambda: self.rng_after.copy_(self.rng))
         add("sample", lib.gq_sample_rows, ctx, V(self.controlled), B, vocab, vocab, ctypes.byref(self.opts), None, 0, 0,
-            V(self.rng), V(self.tokens))
-        add("release", lib.gq_paged_release, ctx, B, self.page_size, V(self.lens), V(self.keep), V(self.table),
+            V(self.rng_after), V(self.drawn))
+        add("keep", self._torch_call, self._take_tokens)
+        add("release", lib.gq_paged_release, ctx, B, self.page_size, V(self.now), V(self.keep), V(self.table),
             self.table.shape[1], V(self.free), self.n_pages, V(self.count), V(self.count), V(self.lens))
+
+    def _torch_call(self, fn) -> int:
+        """One of the step's calls that is torch's: on the backend's stream, into tensors that
+        are there already (the step is recorded)."""
+        with self.torch.cuda.stream(self._stream()):
+            fn()
+        return _abi.GQ_OK
+
+    def _take_tokens(self) -> None:
+        """The drawn tokens become the requests', except where the step placed no token."""
+        torch = self.torch
+        torch.ne(self.now, self.lens, out=self.took)
+        torch.where(self.took, self.drawn, self.tokens, out=self.tokens)
+        if self.opts.temperature > 0:  # (a greedy step draws no numbers)
+            torch.where(self.took, self.rng_after, self.rng, out=self.rng)
 
     def step(self, ids=None):
         """Decode one token of every request: ids [batch] (default: the tokens that the last
         step sampled) in, the sampled ``tokens`` [batch] out (a device tensor, valid until
-        the next step). Enqueued; a page shortage shows at the next ``g.flush()``."""
+        the next step). Enqueued; a page shortage shows at the next ``g.flush()``: the step
+        then decoded nothing. Lengths, tokens and random states are as they were, and only
+        the pages of requests that were ended have gone back, so that it can be repeated.
+        ``took`` [batch] tells which requests the last step has decoded a token of."""
         torch = self.torch
         with self._ordered():
             if ids is None:
@@ -222,13 +246,15 @@ class PagedDecoder(e2b.Decoder):
         token back: lengths, pages and random states are as before."""
         torch = self.torch
         self.g.flush()
-        saved = [(t, t.clone()) for t in (self.lens, self.table, self.free, self.count, self.rng, self.tokens)]
+        saved = [(t, t.clone()) for t in (self.lens, self.table, self.free, self.count, self.rng, self.tokens, self.took)]
         torch.cuda.synchronize(self.g.torch_device)
-        self.run()
-        self.g.flush()
-        for t, old in saved:
-            t.copy_(old)
-        torch.cuda.synchronize(self.g.torch_device)
+        try:
+            self.run()
+            self.g.flush()
+        finally:
+            for t, old in saved:
+                t.copy_(old)
+            torch.cuda.synchronize(self.g.torch_device)
         self.graph = self.g.record(self.run)
 
     def close(self) -> None:

@@ -244,3 +244,42 @@ def test_controls_and_tokens_follow_the_callers_stream(g):
     g.flush()
     check_controlled(dec, prompts, made, range(2))
     dec.close()
+
+
+@pytest.mark.parametrize("recorded", [False, True])
+def test_a_refused_step_can_be_repeated(g, recorded):
+    """Too few pages for a step: tokens, random states, lengths and pages are as before, and
+    the next step that fits goes on from there."""
+    dec = make(g, 2, n_pages=4, sample=(1.0, 8, 0.95))
+    rows = seeded_rows(g, [31])
+    dec.extend([31, 0], rows)
+    dec.extend([0, 15], seeded_rows(g, [15], seed=9))
+    if recorded:
+        dec.record_steps()
+    assert dec.took.tolist() == [False, False]
+    dec.step([5, 6])
+    g.flush()
+    state = lambda: [t.tolist() for t in (dec.tokens, dec.rng, dec.lens, dec.count)]  # noqa: E731
+    before = state()
+    assert before[2] == [32, 16] and before[3] == [1] and dec.took.tolist() == [True, True]
+    for _ in range(2):  # two pages are needed
+        dec.step()
+        with pytest.raises(GqError) as e:
+            g.flush()
+        assert e.value.status == _abi.GQ_ERR_DEVICE
+        assert state() == before and dec.took.tolist() == [False, False]
+    if not recorded:
+        with pytest.raises(GqError):
+            dec.record_steps()
+        assert state() == before
+    dec.end([1])
+    dec.step()  # refused too, and gives the ended request's page back
+    with pytest.raises(GqError):
+        g.flush()
+    assert state() == [before[0], before[1], [32, 0], [2]]
+    dec.step()
+    g.flush()
+    assert dec.lens.tolist()[0] == 33 and dec.took.tolist()[0]
+    assert dec.history[0, 31:33].tolist() == [5, before[0][0]]
+    assert rel_l2(dec.read(dec.logits)[0], alone(g, rows, [5, before[0][0]])) <= STEP_REL
+    dec.close()
