@@ -41,8 +41,9 @@ class PagedDecoder(e2b.Decoder):
     max_len: the most tokens of a request (its block table row); page_size, kv_type
     ("f32", "f16", "bf16", "e4m3" with k_scale / v_scale) and n_pages (default: enough
     for every request at max_len) describe the pool that each source layer has. ``lens``
-    are the requests' lengths, filled by ``extend``; a place whose length is 0 and that
-    was ended idles: it decodes from an empty cache and gives its page back every step.
+    are the requests' lengths, filled by ``extend``. A place whose request has ended idles,
+    and a request of max_len tokens stands still: a step takes no page for them, leaves
+    their token as it is, and their rows of the logits mean nothing.
 
     Controls, all device tensors that may be changed between steps on torch's current
     stream, which a step comes after and which goes on after it (whatever stream the
@@ -85,10 +86,19 @@ class PagedDecoder(e2b.Decoder):
         self.lens = torch.zeros(B, dtype=i32, device=dev)
         self.now = torch.zeros(B, dtype=i32, device=dev)  # the lengths with the step's tokens
         self.took = torch.zeros(B, dtype=torch.bool, device=dev)
-        self.one = torch.ones(B, dtype=i32, device=dev)
         self.keep = torch.full((B,), KEEP_ALL, dtype=i32, device=dev)
+        # a place below its limit takes a token: max_len, and 0 where no request is
+        self.limit = torch.full((B,), self.capacity, dtype=i32, device=dev)
+        self.new = torch.zeros(B, dtype=i32, device=dev)
+        self.ending = set()  # places that were ended and whose last step is still to come
+        # the step's tokens in the order of gq_paged_reserve, which leaves out places without
+        # one, and then by place (one more: what is left over goes there)
         self.slots = torch.zeros(B, dtype=torch.int64, device=dev)
+        self.positions = torch.zeros(B, dtype=i32, device=dev)
         self.owners = torch.zeros(B, dtype=i32, device=dev)
+        self.place = torch.zeros(B, dtype=torch.int64, device=dev)
+        self.place_slots = torch.full((B + 1,), -1, dtype=torch.int64, device=dev)
+        self.place_pos = torch.zeros(B + 1, dtype=i32, device=dev)
         d = c.heads_kv * c.global_head_dim
         self.new_k, self.new_v = (torch.zeros(B, max(d, c.heads_kv * c.head_dim), device=dev) for _ in range(2))
         # controls of the logits
@@ -157,23 +167,38 @@ class PagedDecoder(e2b.Decoder):
         # (requests that were not extended keep theirs: what they generated stays generated)
         self.prompt_lens.copy_(torch.where(new > 0, self.lens, self.prompt_lens))
         self.keep.masked_fill_(new > 0, KEEP_ALL)
+        self.limit.masked_fill_(new > 0, self.capacity)
+        self.ending -= {b for b, n in enumerate(new_lens) if n > 0}
         torch.cuda.synchronize(dev)
 
     def end(self, places: Sequence[int]) -> None:
-        """The requests at these places end: the next step gives their pages back."""
+        """The requests at these places end: the next step is their last, and gives their pages
+        back. The places idle from then on, until ``extend`` gives them a request."""
         with self._ordered():
             self.keep[self.torch.tensor(list(places), device=self.g.torch_device)] = 0
+        self.ending |= set(places)
 
     # ---- the step ----------------------------------------------------------------------
     def set_position(self, p: int) -> None:
         """(Every request has its own position; the calls are the same for every step.)"""
+        self.pos = self.place_pos[:self.batch]
         self._calls = self._build_calls(0)
 
     def _begin_calls(self, add) -> None:
         V = lambda t: c_void_p(t.data_ptr())  # noqa: E731
-        add("reserve", self.g.lib.gq_paged_reserve, self.g.ctx, self.batch, self.page_size, V(self.lens), V(self.one),
+        add("new", self._torch_call, lambda: self.torch.gt(self.limit, self.lens, out=self.new))
+        add("reserve", self.g.lib.gq_paged_reserve, self.g.ctx, self.batch, self.page_size, V(self.lens), V(self.new),
             V(self.table), self.table.shape[1], V(self.free), self.n_pages, V(self.count), V(self.count), self.batch,
-            V(self.slots), V(self.pos), V(self.owners), V(self.now))
+            V(self.slots), V(self.positions), V(self.owners), V(self.now))
+        add("place", self._torch_call, self._place_tokens)
+
+    def _place_tokens(self) -> None:
+        """Slots and positions by place: -1 (no row is written) and any position where the step
+        has no token of the place."""
+        self.torch.remainder(self.owners, self.batch + 1, out=self.place)  # (no owner, -1: the place past the last)
+        self.place_slots.fill_(-1)
+        self.place_slots.scatter_(0, self.place, self.slots)
+        self.place_pos.scatter_(0, self.place, self.positions)
 
     def _new_rows(self, src: int, p: int, kvd: int):
         return c_void_p(self.new_k.data_ptr()), c_void_p(self.new_v.data_ptr()), kvd
@@ -183,7 +208,7 @@ class PagedDecoder(e2b.Decoder):
         pages = c_void_p(self.pages[src].ref)
         if src == i:
             add(pre + "append", lib.gq_paged_append, ctx, pages, V(self.new_k), V(self.new_v), self.batch, 0, 0,
-                V(self.slots))
+                V(self.place_slots))
         add(pre + "attention", lib.gq_paged_attention, ctx, pages, V(self.qr), self.batch, c.heads_q, 0, V(self.table),
             self.table.shape[1], V(self.now), c_float(1.0), c.window_of(i), c_float(0.0), V(self.attn))
 
@@ -220,7 +245,7 @@ class PagedDecoder(e2b.Decoder):
             torch.where(self.took, self.rng_after, self.rng, out=self.rng)
 
     def step(self, ids=None):
-        """Decode one token of every request: ids [batch] (default: the tokens that the last
+        """Decode one token of every request (of less than max_len tokens): ids [batch] (default: the tokens that the last
         step sampled) in, the sampled ``tokens`` [batch] out (a device tensor, valid until
         the next step). Enqueued; a page shortage shows at the next ``g.flush()``: the step
         then decoded nothing. Lengths, tokens and random states are as they were, and only
@@ -238,6 +263,9 @@ class PagedDecoder(e2b.Decoder):
                 self.g.replay(self.graph)
             else:
                 self.run()
+            if self.ending:
+                self.limit[torch.tensor(sorted(self.ending), device=self.g.torch_device)] = 0
+                self.ending.clear()
         return self.tokens
 
     def record_steps(self) -> None:

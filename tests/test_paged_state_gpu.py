@@ -283,3 +283,44 @@ def test_a_refused_step_can_be_repeated(g, recorded):
     assert dec.history[0, 31:33].tolist() == [5, before[0][0]]
     assert rel_l2(dec.read(dec.logits)[0], alone(g, rows, [5, before[0][0]])) <= STEP_REL
     dec.close()
+
+
+@pytest.mark.parametrize("recorded", [False, True])
+def test_places_without_a_token_take_no_page(g, recorded):
+    """In a full pool an idle place and a request at max_len do not stop the others, whose
+    rows go to their own places; the idle ones' tokens and random states stay."""
+    lens = [5, 47, 31, 17]
+    dec = make(g, 4, max_len=48, n_pages=8, sample=(1.0, 8, 0.95))
+    rows = [seeded_rows(g, [n], seed=20 + n) for n in lens]
+    for b, n in enumerate(lens):
+        dec.extend([n if i == b else 0 for i in range(4)], rows[b])
+    assert int(dec.count[0]) == 0
+    if recorded:
+        dec.record_steps()
+    dec.end([0])
+    dec.step([1, 2, 3, 4])
+    g.flush()
+    assert dec.lens.tolist() == [0, 48, 32, 18] and dec.took.tolist() == [True] * 4 and int(dec.count[0]) == 1
+    said, tokens, states = [[3], [4]], dec.tokens.tolist(), dec.rng.tolist()
+    for i in range(10):  # the first takes the last page
+        dec.step()
+        g.flush()
+        assert dec.lens.tolist() == [0, 48, 33 + i, 19 + i] and dec.took.tolist() == [False, False, True, True]
+        for k, b in enumerate((2, 3)):
+            said[k].append(tokens[b])
+        now = dec.tokens.tolist()
+        assert now[:2] == tokens[:2] and dec.rng.tolist()[:2] == states[:2]
+        tokens = now
+    assert int(dec.count[0]) == 0
+    logits = dec.read(dec.logits)
+    for k, b in enumerate((2, 3)):
+        assert rel_l2(logits[b], alone(g, rows[b], said[k])) <= STEP_REL
+    dec.end([1])
+    dec.step()  # (a full request has no last step to take)
+    g.flush()
+    assert dec.lens.tolist() == [0, 0, 43, 29] and int(dec.count[0]) == 3
+    dec.extend([17, 0, 0, 0], seeded_rows(g, [17], seed=60))
+    dec.step()
+    g.flush()
+    assert dec.lens.tolist() == [18, 0, 44, 30] and dec.took.tolist() == [True, False, True, True]
+    dec.close()
