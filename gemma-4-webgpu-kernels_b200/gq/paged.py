@@ -102,7 +102,9 @@ class PagedDecoder(e2b.Decoder):
         d = c.heads_kv * c.global_head_dim
         self.new_k, self.new_v = (torch.zeros(B, max(d, c.heads_kv * c.head_dim), device=dev) for _ in range(2))
         # controls of the logits
-        self.history = torch.zeros(B, self.capacity, dtype=i32, device=dev)
+        # (a column more: a request that stands still at max_len puts its id there)
+        self.ids_at = torch.zeros(B, self.capacity + 1, dtype=i32, device=dev)
+        self.history = self.ids_at[:, :self.capacity]
         self.prompt_lens = torch.zeros(B, dtype=i32, device=dev)
         self.penalties = torch.tensor([[1.0, 0.0, 0.0]], device=dev).repeat(B, 1)
         self.controlled = torch.empty(B, c.vocab, device=dev)
@@ -135,14 +137,21 @@ class PagedDecoder(e2b.Decoder):
         head_dim] in request order, for each source layer; tokens, when given, each
         request's ids, as many as are known (its prompt, for the penalties; all that an extended request holds
         counts as its prompt from then on). Raises when the pages do not
-        suffice, and what earlier steps left to raise; nothing is taken then. A place whose request was
+        suffice, when a request would pass max_len, and what earlier steps left to raise; nothing is taken then. A place whose request was
         ended begins anew, whether a step has come between or not."""
         torch, c, g = self.torch, self.cfg, self.g
-        dev, total = g.torch_device, int(np.sum(new_lens))
+        new_lens = [int(n) for n in new_lens]
+        if len(new_lens) != self.batch or min(new_lens) < 0:
+            raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, f"extend: new_lens must be {self.batch} lengths")
+        if tokens is not None and (len(tokens) > self.batch or any(len(ids) > n for ids, n in zip(tokens, new_lens))):
+            raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "extend: more ids than new tokens")
+        dev, total = g.torch_device, sum(new_lens)
         place = lambda dt: torch.empty(total, dtype=dt, device=dev)  # noqa: E731
         g.flush()  # steps in flight change the lengths; their errors are raised before anything is taken
-        new, slots = torch.tensor(list(new_lens), dtype=torch.int32, device=dev), place(torch.int64)
+        new, slots = torch.tensor(new_lens, dtype=torch.int32, device=dev), place(torch.int64)
         anew = (new > 0) & (self.keep == 0)  # places whose end no step has carried out yet: it is now
+        if bool((torch.where(anew, 0, self.lens) + new > self.capacity).any()):
+            raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, f"extend: a request would hold more than {self.capacity} tokens")
         if bool(anew.any()):
             keep = torch.where(anew, 0, KEEP_ALL).to(torch.int32)
             torch.cuda.synchronize(dev)
@@ -217,7 +226,7 @@ class PagedDecoder(e2b.Decoder):
         lib, ctx, B, vocab = self.g.lib, self.g.ctx, self.batch, self.cfg.vocab
         ids, values, offsets = self.bias or (None, None, None)
         words, rows = self.masks or (None, None)
-        add("process_logits", lib.gq_process_logits, ctx, V(self.logits), B, vocab, vocab, V(self.history), self.capacity,
+        add("process_logits", lib.gq_process_logits, ctx, V(self.logits), B, vocab, vocab, V(self.ids_at), self.capacity + 1,
             V(self.prompt_lens), V(self.now), V(self.penalties), V(ids), V(values), V(offsets), V(words),
             words.shape[0] if words is not None else 0, words.shape[1] if words is not None else 0, V(rows),
             V(self.controlled), vocab)
@@ -257,8 +266,7 @@ class PagedDecoder(e2b.Decoder):
                 self.ids.copy_(self.tokens)
             else:
                 self.ids.copy_(torch.as_tensor(np.asarray(ids, dtype=np.int32).reshape(self.batch)))
-            at = self.lens.long().clamp(max=self.capacity - 1)[:, None]
-            self.history.scatter_(1, at, self.ids[:, None])
+            self.ids_at.scatter_(1, self.lens.long()[:, None], self.ids[:, None])
             if self.graph is not None:
                 self.g.replay(self.graph)
             else:

@@ -327,3 +327,32 @@ def test_places_without_a_token_take_no_page(g, recorded):
     g.flush()
     assert dec.lens.tolist() == [18, 0, 44, 30] and dec.took.tolist() == [True, False, True, True]
     dec.close()
+
+
+def test_no_request_passes_max_len(g):
+    """max_len is the limit where the last page could hold more, in steps and in extend; the
+    ids of a request that stands still there are not written over."""
+    dec = make(g, 2, max_len=20)  # pages of 16
+    set_penalties(g, dec, *PENALTIES)
+    prompt, said = list(range(40, 58)), [[60, 61], [1, 2]]
+    dec.extend([18, 0], seeded_rows(g, [18]), tokens=[prompt, []])
+    for ids in zip(*said):
+        dec.step(list(ids))
+    for i in range(3):
+        dec.step([70 + i, 3 + i])
+        said[1].append(3 + i)
+    g.flush()
+    assert dec.lens.tolist() == [20, 5] and dec.history[0].tolist() == prompt + said[0]
+    check_controlled(dec, [prompt, []], said, range(2))
+    for lens, tokens in (([1, 0], None), ([0, 16], None), ([0], None), ([0, 0, 0], None), ([0, -1], None),
+                         ([0, 2], [[], [1, 2, 3]]), ([0, 0], [[], [], []])):
+        with pytest.raises(GqError) as e:
+            dec.extend(lens, seeded_rows(g, [sum(lens)]), tokens=tokens)
+        assert e.value.status == _abi.GQ_ERR_INVALID_ARGUMENT
+    assert dec.lens.tolist() == [20, 5]
+    dec.extend([0, 15], seeded_rows(g, [15], seed=8))
+    assert dec.lens.tolist() == [20, 20]
+    dec.end([0])
+    dec.extend([20, 0], seeded_rows(g, [20], seed=8))  # the ended request's tokens do not count
+    assert dec.lens.tolist() == [20, 20]
+    dec.close()
