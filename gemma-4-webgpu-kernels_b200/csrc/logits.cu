@@ -31,6 +31,7 @@ struct LogitArgs {
   const float *penalties;
   const int32_t *bias_ids, *bias_offsets;
   const float *bias_values;
+  int64_t n_bias;  // entries of bias_ids, -1: as many as the last offset says
   const uint32_t *masks;
   const int32_t *mask_rows;
   int64_t n_masks, mask_stride;
@@ -102,8 +103,10 @@ __global__ void __launch_bounds__(NT, 1024 / NT) logits_kernel(const LogitArgs a
     frequency = a.penalties[row * 3 + 2];
   }
   if (a.bias_offsets) {
-    b0 = a.bias_offsets[row];
-    biases = a.bias_offsets[row + 1] - b0;
+    // (offsets are cut to the entries there are: nothing past bias_ids is read)
+    const int entries = a.n_bias >= 0 ? (int)a.n_bias : min(max(a.bias_offsets[gridDim.y], 0), INT32_MAX / 2);
+    b0 = min(max(a.bias_offsets[row], 0), entries);
+    biases = min(max(a.bias_offsets[row + 1], 0), entries) - b0;
   }
   if (a.masks) {
     const int64_t mr = a.mask_rows ? (int64_t)a.mask_rows[row] : row;
@@ -241,13 +244,11 @@ int logits_dispatch(gq_ctx *ctx, const LogitArgs &a, int64_t m, int64_t most_lea
   return logits_launch<512, 8, VEC>(ctx, a, m, most_lead);
 }
 
-}  // namespace
-
-extern "C" int gq_process_logits(gq_ctx *ctx, const float *logits, int64_t m, int64_t vocab, int64_t ld,
-                                 const int32_t *tokens, int64_t tok_stride, const int32_t *prompt_lens,
-                                 const int32_t *lens, const float *penalties, const int32_t *bias_ids,
-                                 const float *bias_values, const int32_t *bias_offsets, const uint32_t *masks,
-                                 int64_t n_masks, int64_t mask_stride, const int32_t *mask_rows, float *y, int64_t ldy) {
+int process_logits(gq_ctx *ctx, const float *logits, int64_t m, int64_t vocab, int64_t ld, const int32_t *tokens,
+                   int64_t tok_stride, const int32_t *prompt_lens, const int32_t *lens, const float *penalties,
+                   const int32_t *bias_ids, const float *bias_values, const int32_t *bias_offsets, int64_t n_bias,
+                   const uint32_t *masks, int64_t n_masks, int64_t mask_stride, const int32_t *mask_rows, float *y,
+                   int64_t ldy) {
   if (!ctx) return GQ_ERR_INVALID_ARGUMENT;
   int rc = gq_enter_ctx(ctx);
   if (rc != GQ_OK) return rc;
@@ -281,6 +282,7 @@ extern "C" int gq_process_logits(gq_ctx *ctx, const float *logits, int64_t m, in
   a.penalties = penalties;
   a.bias_ids = bias_ids;
   a.bias_values = bias_values;
+  a.n_bias = n_bias;
   a.bias_offsets = bias_offsets;
   a.masks = masks;
   a.n_masks = n_masks;
@@ -290,4 +292,27 @@ extern "C" int gq_process_logits(gq_ctx *ctx, const float *logits, int64_t m, in
   const bool vec = ((uintptr_t)logits - (uintptr_t)y) % 16 == 0 && (m == 1 || (ld - ldy) % 4 == 0);
   const int64_t most_lead = (uintptr_t)logits % 16 == 0 && (m == 1 || ld % 4 == 0) ? 0 : 3;
   return vec ? logits_dispatch<true>(ctx, a, m, most_lead) : logits_dispatch<false>(ctx, a, m, 0);
+}
+
+}  // namespace
+
+extern "C" int gq_process_logits(gq_ctx *ctx, const float *logits, int64_t m, int64_t vocab, int64_t ld,
+                                 const int32_t *tokens, int64_t tok_stride, const int32_t *prompt_lens,
+                                 const int32_t *lens, const float *penalties, const int32_t *bias_ids,
+                                 const float *bias_values, const int32_t *bias_offsets, const uint32_t *masks,
+                                 int64_t n_masks, int64_t mask_stride, const int32_t *mask_rows, float *y, int64_t ldy) {
+  return process_logits(ctx, logits, m, vocab, ld, tokens, tok_stride, prompt_lens, lens, penalties, bias_ids, bias_values,
+                        bias_offsets, -1, masks, n_masks, mask_stride, mask_rows, y, ldy);
+}
+
+extern "C" int gq_process_logits_bounded(gq_ctx *ctx, const float *logits, int64_t m, int64_t vocab, int64_t ld,
+                                         const int32_t *tokens, int64_t tok_stride, const int32_t *prompt_lens,
+                                         const int32_t *lens, const float *penalties, const int32_t *bias_ids,
+                                         const float *bias_values, const int32_t *bias_offsets, int64_t n_bias,
+                                         const uint32_t *masks, int64_t n_masks, int64_t mask_stride,
+                                         const int32_t *mask_rows, float *y, int64_t ldy) {
+  if (ctx && (n_bias < 0 || n_bias > INT32_MAX / 2))
+    return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT, "process_logits: the number of bias entries must be below 2^30");
+  return process_logits(ctx, logits, m, vocab, ld, tokens, tok_stride, prompt_lens, lens, penalties, bias_ids, bias_values,
+                        bias_offsets, n_bias, masks, n_masks, mask_stride, mask_rows, y, ldy);
 }

@@ -654,7 +654,7 @@ class CudaBackend:
             raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "process_logits: out must have the logits' shape")
         yp, ldy = self._rows(yt, m, vocab, "process_logits: out")
         tok = pl = ln = pen = bi = bv = bo = mk = mr = None
-        n_tok = n_masks = words = 0
+        n_tok = n_masks = words = n_bias = 0
         if tokens is not None and tokens.numel():
             ts = tokens.shape
             if len(ts) != 2 or ts[0] != m or prompt_lens is None or lens is None or penalties is None:
@@ -671,8 +671,8 @@ class CudaBackend:
                 raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "process_logits: masks must be [k, words]")
             mk, (n_masks, words) = d(masks, i32, "masks"), masks.shape
             mr = d(mask_rows, i32, "mask_rows", m) if mask_rows is not None else None
-        rc = self.lib.gq_process_logits(self.ctx, lp, m, vocab, ld, tok, n_tok, pl, ln, pen, bi, bv, bo, mk, n_masks, words,
-                                        mr, yp, ldy)
+        rc = self.lib.gq_process_logits_bounded(self.ctx, lp, m, vocab, ld, tok, n_tok, pl, ln, pen, bi, bv, bo, n_bias, mk,
+                                                n_masks, words, mr, yp, ldy)
         if rc:
             self._check(rc, "process_logits")
         return y

@@ -171,6 +171,9 @@ SIGNATURES = {
     "gq_process_logits": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
                                   c_void_p, c_int64]),
+    "gq_process_logits_bounded": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p,
+                                          c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_int64,
+                                          c_int64, c_void_p, c_void_p, c_int64]),
 }
 
 GQ_ATTN_KPOS_ASCENDING = 0x1

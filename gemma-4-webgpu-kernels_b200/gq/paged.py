@@ -226,8 +226,9 @@ class PagedDecoder(e2b.Decoder):
         lib, ctx, B, vocab = self.g.lib, self.g.ctx, self.batch, self.cfg.vocab
         ids, values, offsets = self.bias or (None, None, None)
         words, rows = self.masks or (None, None)
-        add("process_logits", lib.gq_process_logits, ctx, V(self.logits), B, vocab, vocab, V(self.ids_at), self.capacity + 1,
-            V(self.prompt_lens), V(self.now), V(self.penalties), V(ids), V(values), V(offsets), V(words),
+        add("process_logits", lib.gq_process_logits_bounded, ctx, V(self.logits), B, vocab, vocab, V(self.ids_at),
+            self.capacity + 1, V(self.prompt_lens), V(self.now), V(self.penalties), V(ids), V(values), V(offsets),
+            ids.numel() if ids is not None else 0, V(words),
             words.shape[0] if words is not None else 0, words.shape[1] if words is not None else 0, V(rows),
             V(self.controlled), vocab)
         if self.opts.temperature > 0:

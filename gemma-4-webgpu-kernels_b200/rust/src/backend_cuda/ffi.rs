@@ -227,4 +227,8 @@ extern "C" {
         tok_stride: i64, prompt_lens: *const i32, lens: *const i32, penalties: *const f32, bias_ids: *const i32,
         bias_values: *const f32, bias_offsets: *const i32, masks: *const u32, n_masks: i64, mask_stride: i64,
         mask_rows: *const i32, y: *mut f32, ldy: i64) -> c_int;
+    pub fn gq_process_logits_bounded(ctx: *mut GqCtx, logits: *const f32, m: i64, vocab: i64, ld: i64,
+        tokens: *const i32, tok_stride: i64, prompt_lens: *const i32, lens: *const i32, penalties: *const f32,
+        bias_ids: *const i32, bias_values: *const f32, bias_offsets: *const i32, n_bias: i64, masks: *const u32,
+        n_masks: i64, mask_stride: i64, mask_rows: *const i32, y: *mut f32, ldy: i64) -> c_int;
 }

@@ -614,6 +614,16 @@ int gq_process_logits(gq_ctx *ctx, const float *logits, int64_t m, int64_t vocab
                       const uint32_t *masks, int64_t n_masks, int64_t mask_stride, const int32_t *mask_rows, float *y,
                       int64_t ldy);
 
+/* The same with the number of entries of bias_ids and bias_values: offsets, which are on
+ * the device, are cut to [0, n_bias], so whatever they hold, nothing past the entries is
+ * read (n_bias below 2^30). gq_process_logits takes bias_offsets[m] for that number. */
+int gq_process_logits_bounded(gq_ctx *ctx, const float *logits, int64_t m, int64_t vocab, int64_t ld,
+                              const int32_t *tokens, int64_t tok_stride, const int32_t *prompt_lens,
+                              const int32_t *lens, const float *penalties, const int32_t *bias_ids,
+                              const float *bias_values, const int32_t *bias_offsets, int64_t n_bias,
+                              const uint32_t *masks, int64_t n_masks, int64_t mask_stride, const int32_t *mask_rows,
+                              float *y, int64_t ldy);
+
 #ifdef __cplusplus
 }
 #endif
