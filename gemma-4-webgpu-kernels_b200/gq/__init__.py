@@ -663,7 +663,11 @@ class CudaBackend:
             tok, n_tok = d(tokens, i32, "tokens"), ts[1]
             pl, ln = d(prompt_lens, i32, "prompt_lens", m), d(lens, i32, "lens", m)
             pen = d(penalties, f32, "penalties", 3 * m)
-        if bias_offsets is not None and bias_ids is not None and (n_bias := bias_ids.numel()):
+        if bias_ids is not None or bias_values is not None or bias_offsets is not None:
+            if bias_ids is None or bias_values is None or bias_offsets is None:
+                raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "process_logits: biases are bias_ids, bias_values and bias_offsets")
+            n_bias = bias_ids.numel()
+        if n_bias:
             bi, bv = d(bias_ids, i32, "bias_ids"), d(bias_values, f32, "bias_values", n_bias)
             bo = d(bias_offsets, i32, "bias_offsets", m + 1)
         if masks is not None and masks.numel():

@@ -3,7 +3,7 @@ the definition: every operation rounds once in f32 on both sides."""
 import numpy as np
 import pytest
 
-from gq import CudaBackend, _abi
+from gq import CudaBackend, GqError, _abi
 from test_logits_gpu import dev
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +48,16 @@ def test_bias_offsets_are_cut_to_the_entries(g, offsets, rows):
     assert g.lib.gq_process_logits_bounded(g.ctx, t[0].data_ptr(), 3, 100, 0, None, 0, None, None, None, t[1].data_ptr(),
                                            t[2].data_ptr(), t[3].data_ptr(), -1, None, 0, 0, None, y.data_ptr(),
                                            0) == _abi.GQ_ERR_INVALID_ARGUMENT
+
+
+def test_biases_need_all_three_tensors(g):
+    x = g._torch.zeros(2, 64, device=g.torch_device)
+    all3 = dict(bias_ids=dev(g, [1], np.int32), bias_values=dev(g, [1], np.float32), bias_offsets=dev(g, [0, 1, 1], np.int32))
+    for left_out in [("bias_ids",), ("bias_values",), ("bias_offsets",), ("bias_ids", "bias_values"), ("bias_values", "bias_offsets"),
+                     ("bias_ids", "bias_offsets")]:
+        with pytest.raises(GqError) as e:
+            g.process_logits(x, **{k: v for k, v in all3.items() if k not in left_out})
+        assert e.value.status == _abi.GQ_ERR_INVALID_ARGUMENT
+    assert g.process_logits(x, **all3).data[0, 1] == 1.0
+    none = dict(bias_ids=dev(g, [], np.int32), bias_values=dev(g, [], np.float32), bias_offsets=dev(g, [0, 0, 0], np.int32))
+    assert (g.process_logits(x, **none).data == 0).all()
