@@ -222,15 +222,24 @@ class PagedDecoder(e2b.Decoder):
             self.table.shape[1], V(self.now), c_float(1.0), c.window_of(i), c_float(0.0), V(self.attn))
 
     def _end_calls(self, add) -> None:
-        V = lambda t: c_void_p(t.data_ptr()) if t is not None else None  # noqa: E731
+        V = lambda t: c_void_p(t.data_ptr())  # noqa: E731
         lib, ctx, B, vocab = self.g.lib, self.g.ctx, self.batch, self.cfg.vocab
-        ids, values, offsets = self.bias or (None, None, None)
-        words, rows = self.masks or (None, None)
+        d, i32, n_bias, n_masks, mask_words = self.g._dev, self.torch.int32, 0, 0, 0
+        ids = values = offsets = words = rows = None
+        if self.bias is not None:
+            n_bias = self.bias[0].numel()
+            ids, offsets = d(self.bias[0], i32, "bias: ids"), d(self.bias[2], i32, "bias: offsets", B + 1)
+            values = d(self.bias[1], self.torch.float32, "bias: values", n_bias)
+        if self.masks is not None:
+            if self.masks[0].dim() != 2:
+                raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "masks: words must be [k, words]")
+            words, (n_masks, mask_words) = d(self.masks[0], i32, "masks: words"), self.masks[0].shape
+            if mask_words < -(-vocab // 32) or (self.masks[1] is None and n_masks < B):
+                raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "masks: too few words of a row, or rows")
+            rows = d(self.masks[1], i32, "masks: rows", B) if self.masks[1] is not None else None
         add("process_logits", lib.gq_process_logits_bounded, ctx, V(self.logits), B, vocab, vocab, V(self.ids_at),
-            self.capacity + 1, V(self.prompt_lens), V(self.now), V(self.penalties), V(ids), V(values), V(offsets),
-            ids.numel() if ids is not None else 0, V(words),
-            words.shape[0] if words is not None else 0, words.shape[1] if words is not None else 0, V(rows),
-            V(self.controlled), vocab)
+            self.capacity + 1, V(self.prompt_lens), V(self.now), V(self.penalties), ids, values, offsets, n_bias, words,
+            n_masks, mask_words, rows, V(self.controlled), vocab)
         if self.opts.temperature > 0:
             add("rng", self._torch_call, lambda: self.rng_after.copy_(self.rng))
         add("sample", lib.gq_sample_rows, ctx, V(self.controlled), B, vocab, vocab, ctypes.byref(self.opts), None, 0, 0,

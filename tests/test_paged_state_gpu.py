@@ -356,3 +356,22 @@ def test_no_request_passes_max_len(g):
     dec.extend([20, 0], seeded_rows(g, [20], seed=8))  # the ended request's tokens do not count
     assert dec.lens.tolist() == [20, 20]
     dec.close()
+
+
+def test_biases_and_masks_of_a_decoder_are_checked(g):
+    """Too short for the batch, of another type or on the host: refused when the decoder is
+    made, not read past when it steps."""
+    torch, dev = g._torch, g.torch_device
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device=dev)  # noqa: E731
+    ids, values, offsets = i32(5, 6), torch.tensor([30.0, 1.0], device=dev), i32(0, 1, 2)
+    words, rows = torch.full((2, CFG.vocab // 32), -1, dtype=torch.int32, device=dev), i32(0, 1)
+    for kw in (dict(bias=(ids, values, offsets[:2])), dict(bias=(ids, values[:1], offsets)), dict(bias=(ids.long(), values, offsets)),
+               dict(bias=(ids, values, offsets.cpu())), dict(masks=(words, rows[:1])), dict(masks=(words[:, 1:], rows)),
+               dict(masks=(words[:1], None)), dict(masks=(words[:, :-1].contiguous(), rows)), dict(masks=(words[0], rows))):
+        with pytest.raises(GqError) as e:
+            make(g, 2, **kw)
+        assert e.value.status == _abi.GQ_ERR_INVALID_ARGUMENT
+    dec = make(g, 2, bias=(ids, 1000 * values, offsets), masks=(words, rows))
+    assert dec.step([1, 1]).tolist() == [5, 6]
+    g.flush()
+    dec.close()
