@@ -127,22 +127,24 @@ def test_extend_sees_the_steps_still_in_flight(g):
     dec = make(g, 2)
     set_penalties(g, dec, *PENALTIES)
     dec.extend([4, 20], seeded_rows(g, [4, 20]), tokens=[[1, 2, 3, 4], list(range(40, 60))])
-    dec.tokens.copy_(g._torch.tensor([5, 60], device=g.torch_device))
+    dec.step([5, 60])  # (a first step allocates, which waits for the device)
+    g.flush()
+    dec.tokens.copy_(g._torch.tensor([6, 61], device=g.torch_device))
     dec.end([1])
     hold(g, dec)
     dec.step()  # (ids from the host would wait for the stream)
     dec.extend([0, 3], seeded_rows(g, [3], seed=9), tokens=[[], [30, 31, 32]])
-    assert dec.lens.tolist() == [5, 3]
+    assert dec.lens.tolist() == [6, 3]
     assert dec.history[1, :3].tolist() == [30, 31, 32]
-    dec.tokens.copy_(g._torch.tensor([6, 33], device=g.torch_device))
+    dec.tokens.copy_(g._torch.tensor([7, 33], device=g.torch_device))
     g._torch.cuda.synchronize()
     hold(g, dec)
     dec.step()
     size = 2 * CFG.heads_kv * 4
-    want = sum(size * CFG.dh(i) * min(n, CFG.window_of(i) or n) for n in (6, 4) for i in range(CFG.layers))
+    want = sum(size * CFG.dh(i) * min(n, CFG.window_of(i) or n) for n in (7, 4) for i in range(CFG.layers))
     assert dec.kv_bytes() == want
     g.flush()
-    check_controlled(dec, [[1, 2, 3, 4], [30, 31, 32]], [[5, 6], [33]], range(2))
+    check_controlled(dec, [[1, 2, 3, 4], [30, 31, 32]], [[5, 6, 7], [33]], range(2))
     dec.close()
 
 
