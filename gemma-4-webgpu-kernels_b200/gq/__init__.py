@@ -542,6 +542,8 @@ class CudaBackend:
         for t in (k, v):
             if t.numel() and (not t[0].is_contiguous() or (n > 1 and t.stride(0) != apart)):
                 raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "kv_pages: a page's values must be contiguous, k and v strided alike")
+        if apart < h * ps * d:  # (an expanded tensor's stride 0 would mean packed pages to the library)
+            raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "kv_pages: pages lie on one another")
         st = _abi.KvPagesStruct(k.data_ptr(), v.data_ptr(), n, ps, h, d, apart, types[k.dtype], float(k_scale), float(v_scale))
         return KvPages(k, v, st, ctypes.addressof(st), h * d, d)
 
