@@ -607,6 +607,10 @@ class CudaBackend:
         """Write rows k, v [T, heads, head_dim] f32 (token strides free) to slots [T] int64
         of the pages, rounded to their type (gq_paged_append)."""
         n = slots.numel()
+        for x in (k, v):  # (rows of heads * head_dim, or of one head after another)
+            shape = x.shape
+            if len(shape) > 2 and shape[-1] * shape[-2] != pages.row:
+                raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "paged_append: k and v must be [T, heads, head_dim]")
         kp, ks = self._rows(k, n, pages.row, "paged_append: k")
         vp, vs = self._rows(v, n, pages.row, "paged_append: v")
         rc = self.lib.gq_paged_append(self.ctx, pages.ref, kp, vp, n, ks, vs, self._dev(slots, self._torch.int64, "slots"))

@@ -29,3 +29,20 @@ def test_pages_that_share_memory_are_refused(g):
         with pytest.raises(GqError) as e:
             g.kv_pages(k, k)
         assert e.value.status == _abi.GQ_ERR_INVALID_ARGUMENT
+
+
+def test_append_refuses_rows_by_head(g):
+    """[heads, T, head_dim] holds as many values as [T, heads, head_dim], in another order."""
+    calls = []
+    g.device, g.lib = -1, type("Lib", (), {"gq_paged_append": lambda self, *a: calls.append(a) or 0})()
+    pages = g.kv_pages(torch.zeros(4, 2, 16, 64), torch.zeros(4, 2, 16, 64))
+    ok, slots = torch.zeros(5, 2, 64), torch.zeros(5, dtype=torch.int64)
+    for rows in (ok, ok.view(5, 128), ok.view(-1), ok[None], torch.zeros(5, 256)[:, :128]):
+        g.paged_append(pages, rows, ok, slots)
+    assert len(calls) == 5
+    by_head = torch.zeros(2, 5, 64)
+    for k, v in ((by_head, ok), (ok, by_head)):
+        with pytest.raises(GqError) as e:
+            g.paged_append(pages, k, v, slots)
+        assert e.value.status == _abi.GQ_ERR_INVALID_ARGUMENT
+    assert len(calls) == 5
