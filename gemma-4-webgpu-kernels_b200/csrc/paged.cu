@@ -429,8 +429,9 @@ int gq_check_kv_pages(gq_ctx *ctx, const char *op, const gq_kv_pages *p) {
     return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT, who + ": k and v pages must be 16-byte aligned");
   const bool scaled = p->type == GQ_KV_E4M3;
   for (const float s : {p->k_scale, p->v_scale})
-    if (!(s > 0.0f) || !std::isfinite(s) || (!scaled && s != 1.0f))
-      return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT, who + ": scales must be positive and finite, and 1 unless the type is e4m3");
+    if (!(s > 0.0f) || !std::isfinite(s) || !std::isfinite(1.0f / s) || (!scaled && s != 1.0f))
+      return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT,
+                     who + ": scales must be positive, finite with a finite reciprocal, and 1 unless the type is e4m3");
   return GQ_OK;
 }
 

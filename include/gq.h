@@ -520,8 +520,8 @@ int gq_copy_rows(gq_ctx *ctx, const float *src, int64_t rows, int64_t cols, int6
  * (page_stride = 0: heads * page_size * head_dim, packed; a larger stride lets keys
  * and values, or several layers, interleave in one allocation). head_dim a multiple
  * of 4 up to 512, page_size 1 .. 65536, heads up to 65535, k and v 16-byte aligned,
- * page_stride a multiple of 4. k_scale and v_scale are positive and finite
- * for GQ_KV_E4M3 and 1 for the other types. */
+ * page_stride a multiple of 4. k_scale and v_scale are positive and finite,
+ * their reciprocals too, for GQ_KV_E4M3, and 1 for the other types. */
 typedef struct gq_kv_pages {
   void *k, *v;
   int64_t n_pages, page_size, heads, head_dim, page_stride;
