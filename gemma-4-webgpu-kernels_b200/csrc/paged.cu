@@ -490,7 +490,7 @@ extern "C" int gq_paged_release(gq_ctx *ctx, int64_t batch, int64_t page_size, c
   a.free_left = free_left;
   a.totals = totals;
   // the pages given back are known on the device only: at most every entry of the pool or the table
-  return plan_launch(ctx, false, a, std::min(n_pages, batch * table_stride));
+  return plan_launch(ctx, false, a, std::min(n_pages, batch * std::min<int64_t>(table_stride, INT32_MAX)));
 }
 
 extern "C" int gq_paged_append(gq_ctx *ctx, const gq_kv_pages *pages, const float *k, const float *v, int64_t t,

@@ -389,8 +389,8 @@ extern "C" int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const f
   a.table_stride = table_stride;
   a.page_stride = pages->page_stride ? pages->page_stride : pages->heads * pages->page_size * pages->head_dim;
   a.n_pages = pages->n_pages;
-  // (the last tile's keys are numbered in 32 bits)
-  a.room = std::min<int64_t>(table_stride * pages->page_size, INT32_MAX - 1024);
+  // (the last tile's keys are numbered in 32 bits; the product is kept inside 64)
+  a.room = std::min<int64_t>(std::min<int64_t>(table_stride, INT32_MAX) * pages->page_size, INT32_MAX - 1024);
   a.batch = (int)batch;
   a.hq = (int)hq;
   a.heads = (int)pages->heads;
