@@ -28,6 +28,12 @@ using namespace pattn;
 
 constexpr int kRowThreads = 128;
 constexpr int kRowTile = 64;
+// CTAs per SM: a warp has one key's loads in flight, so warps make up for it. Two against
+// four, replayed, 64 requests of up to 4096 keys: e4m3 rows of 64 184.9 / 116.7 us, bf16
+// rows of 96 371.7 / 205.5, bf16 rows of 512 on pages of 24 575.3 / 316.9; 225 of up to 62
+// keys, 8 heads of 96 in bf16, 160.7 / 129.1; one of 333 keys 27.5 / 27.4.
+constexpr int kRowPerSm = 4;
+static_assert(kRowPerSm <= kMostPerSm, "memory for the parts");
 
 template <int TYPE>
 __device__ __forceinline__ float4 load4(const void *base, int64_t elem) {
@@ -406,7 +412,7 @@ extern "C" int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const f
   a.v_scale = pages->v_scale;
   a.err = ctx->dev_err;
   if (gq_paged_attn_tc_supported(pages, a.page_stride)) return gq_paged_attn_tc_launch(ctx, pages, a);
-  const int grid = grid_for(a, kRowTile, 2 * ctx->num_sms);
+  const int grid = grid_for(a, kRowTile, kRowPerSm * ctx->num_sms);
   rc = bind_parts(ctx, grid, a);
   if (rc != GQ_OK) return rc;
   switch (pages->type) {

@@ -24,6 +24,7 @@ namespace pattn {
 
 constexpr int kHeads = 8;       // query heads per unit
 constexpr int kMaxGrid = 640;
+constexpr int kMostPerSm = 4;   // CTAs per SM of any of the kernels
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -203,18 +204,19 @@ inline int grid_for(const Args &a, int tile, int slots) {
 
 // Memory for the parts (two per CTA) and the list of cut units: one block of the largest
 // size, made by the context's first call and kept, so that a recorded graph's addresses
-// stay good whatever is called after it (10 MB on 148 SMs: two CTAs per SM at head_dim
-// 512; where there are three, rows are at most half as long).
+// stay good whatever is called after it (20 MB on 148 SMs: four CTAs per SM, the most any
+// kernel has, at head_dim 512).
 inline int bind_parts(gq_ctx *ctx, int grid, Args &a) {
   constexpr size_t kPerCta = 2 * kHeads * (512 + 2) * 4 + sizeof(int4);
-  if ((size_t)grid * (2 * kHeads * (a.dim + 2) * 4 + sizeof(int4)) > (size_t)std::min(kMaxGrid, 2 * ctx->num_sms) * kPerCta)
+  const size_t bytes = (size_t)std::min(kMaxGrid, kMostPerSm * ctx->num_sms) * kPerCta;
+  if ((size_t)grid * (2 * kHeads * (a.dim + 2) * 4 + sizeof(int4)) > bytes)
     return gq_fail(ctx, GQ_ERR_UNSUPPORTED, "paged_attention: more partial results than there is memory for");
   if (!ctx->paged_ws) {
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
     GQ_CUDA_TRY(ctx, cudaStreamIsCapturing(ctx->stream, &st));
     if (st != cudaStreamCaptureStatusNone)
       return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT, "paged_attention: run the call once before recording (it allocates)");
-    GQ_CUDA_TRY(ctx, cudaMalloc(&ctx->paged_ws, (size_t)std::min(kMaxGrid, 2 * ctx->num_sms) * kPerCta));
+    GQ_CUDA_TRY(ctx, cudaMalloc(&ctx->paged_ws, bytes));
   }
   a.cut_units = static_cast<int4 *>(ctx->paged_ws);
   a.part_o = reinterpret_cast<float *>(a.cut_units + grid);

@@ -585,7 +585,7 @@ int gq_paged_append(gq_ctx *ctx, const gq_kv_pages *pages, const float *k, const
  * the row: nothing outside the pool is read. Finite q and visible keys and values
  * (below 2^127) give f32 results: all sums in f32, products exact to 2^-21 or better;
  * where one is not finite, its row may be NaN. Long requests are split over many CTAs,
- * whose partial results (10 MB that the context's first call allocates: not while the
+ * whose partial results (20 MB that the context's first call allocates: not while the
  * stream is captured) a second launch joins in a fixed order: results do not vary from
  * run to run. */
 int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const float *q, int64_t batch, int64_t hq,
