@@ -157,18 +157,6 @@ __device__ __forceinline__ void sync_compute() {
   asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory");
 }
 
-// The same, and whether p holds in any of them.
-template <int NT>
-__device__ __forceinline__ bool any_compute(bool p) {
-  uint32_t any;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(any)
-      : "r"((uint32_t)p), "n"(NT)
-      : "memory");
-  return any != 0;
-}
-
 __device__ __forceinline__ float inv_or_zero(float l) { return l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l); }
 
 // Slot of this CTA's part of a cut unit whose first tile is at place s0: a CTA has at most

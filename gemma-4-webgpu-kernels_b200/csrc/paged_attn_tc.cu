@@ -156,14 +156,22 @@ struct Tile {
   static_assert(kRow % 128 == 0 && kSlots >= 3 && (1 << kTShift) == T && kPBytes % 16 == 0, "tile");
 };
 
-// A wait that gave up: report it, and let the CTA run to its end without waiting and
-// without further copies (what it computes is dropped by the error).
+// Wait of a whole warp; false in all its lanes where one's gave up, or did not wait because
+// another's had. It is reported, and the CTA runs to its end without waiting (what it
+// computes is dropped by the error). Warp 0 then asks for no more copies: the slot's last
+// one may still be in flight, and its barrier's phase is not over. (The vote in place of a
+// warp barrier: 64 requests of up to 4096 keys in bf16 58.3 -> 58.4 us; the vote in each
+// tile's block barrier, or on the flag before each copy, 58.7 and 58.8.)
 __device__ __forceinline__ bool wait_or_abort(uint64_t *bar, uint32_t parity, volatile int *abort, uint32_t *err) {
-  if (*abort) return false;
-  if (gqd::mbar_wait_bounded(bar, parity)) return true;
-  *abort = 1;
-  gqd::report(err, GQ_DEVERR_WAIT_TIMEOUT);
-  return false;
+  bool ok = !*abort;
+  if (ok) {
+    ok = gqd::mbar_wait_bounded(bar, parity);
+    if (!ok) {
+      *abort = 1;
+      gqd::report(err, GQ_DEVERR_WAIT_TIMEOUT);
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
 }
 
 
@@ -298,7 +306,6 @@ __global__ void __launch_bounds__(kCompute, (Tile<TYPE, D>::kPerSm))
   TileRef cur = {}, nxt = {};
   uint32_t issued = 0;  // ring positions filled
   int stage = 0;        // of the current tile: 0 its keys (if first), 1 the next tile's keys, 2 its values
-  bool gave_up = false; // a wait of this thread has
   auto copy = [&](const TileRef &x, const CUtensorMap *map) {
     const int slot = issued % C::kSlots;
     const int copies = __popc(__ballot_sync(0xffffffffu, x.page >= 0));
@@ -447,8 +454,7 @@ __global__ void __launch_bounds__(kCompute, (Tile<TYPE, D>::kPerSm))
     float c[MT][3][4];
     auto products = [&]() {
       const int slot = n % C::kSlots;
-      gave_up |= !wait_or_abort(&full[slot], (n / C::kSlots) & 1, &abort_flag, a.err);
-      __syncwarp();
+      if (!wait_or_abort(&full[slot], (n / C::kSlots) & 1, &abort_flag, a.err)) cur.valid = false;
       ++n;
 #pragma unroll
       for (int x = 0; x < MT; ++x) {
@@ -509,7 +515,7 @@ __global__ void __launch_bounds__(kCompute, (Tile<TYPE, D>::kPerSm))
 
     products();
     put_scores(0);
-    if (any_compute<kCompute>(gave_up)) cur.valid = false;
+    sync_compute<kCompute>();
     if (warp == 0) {  // every warp is done with what lies before ring position n
       gqd::fence_proxy_async_smem();
       fill(n + C::kSlots);
@@ -577,7 +583,7 @@ __global__ void __launch_bounds__(kCompute, (Tile<TYPE, D>::kPerSm))
       }
       if (more) put_scores(buf ^ 1);
       const int vslot = n % C::kSlots;
-      gave_up |= !wait_or_abort(&full[vslot], (n / C::kSlots) & 1, &abort_flag, a.err);
+      if (!wait_or_abort(&full[vslot], (n / C::kSlots) & 1, &abort_flag, a.err)) cur.valid = false;
       const uint32_t vat = ring_u + vslot * C::kSlot;
       if (ragged) {
         // rows that are not visible hold anything, NaN too, or an earlier tile: make them 0
@@ -589,8 +595,7 @@ __global__ void __launch_bounds__(kCompute, (Tile<TYPE, D>::kPerSm))
         }
         gqd::fence_proxy_async_smem();  // before the slot's next copy
       }
-      // (after a wait that gave up a slot's last copy may be in flight: none gets another)
-      if (any_compute<kCompute>(gave_up)) cur.valid = false;
+      sync_compute<kCompute>();
       if (warp == 0) {  // every warp is done with what lies before the values of tile i
         gqd::fence_proxy_async_smem();
         fill(n + C::kSlots);
