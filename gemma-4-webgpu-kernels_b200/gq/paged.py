@@ -157,6 +157,9 @@ class PagedDecoder(e2b.Decoder):
             torch.cuda.synchronize(dev)
             g.paged_release(self.lens, keep, self.page_size, self.table, self.free, self.count, self.lens, self.count)
             g.flush()
+            # (whatever becomes of what follows, the place is idle now)
+            self.limit.masked_fill_(anew, 0)
+            self.ending -= {b for b, n in enumerate(new_lens) if n > 0}
         before = self.lens.tolist()
         pos, owners = place(torch.int32), place(torch.int32)
         kv = {i: rows(i) for i in self.pages} if total else {}

@@ -377,3 +377,23 @@ def test_biases_and_masks_of_a_decoder_are_checked(g):
     assert dec.step([1, 1]).tolist() == [5, 6]
     g.flush()
     dec.close()
+
+
+def test_a_refused_extend_of_an_ended_place_leaves_it_idle(g):
+    """The ended request's pages have gone back; the place takes none of them until a request
+    has it."""
+    dec = make(g, 2, n_pages=4)
+    dec.extend([20, 31], seeded_rows(g, [20, 31]))
+    dec.end([0])
+    with pytest.raises(GqError):
+        dec.extend([48, 0], seeded_rows(g, [48]))  # three pages, two are back
+    assert dec.lens.tolist() == [0, 31] and int(dec.count[0]) == 2
+    for n in (32, 33):
+        dec.step([1, 2])
+        g.flush()
+        assert dec.lens.tolist() == [0, n] and dec.took.tolist() == [False, True]
+    dec.extend([5, 0], seeded_rows(g, [5]))
+    dec.step([1, 2])
+    g.flush()
+    assert dec.lens.tolist() == [6, 34] and dec.took.tolist() == [True, True]
+    dec.close()
