@@ -1,8 +1,8 @@
 // logits.cu — penalties for repeated tokens, biases and grammar masks on a step's
 // logits (gq_process_logits), one pass over the rows.
 //
-// What bounds it: 8 bytes per logit (read and written once); the histories, biases and
-// mask bits are small beside that, but the instructions they cost are not: the mask, the
+// What it has to move: 8 bytes per logit (read and written once). The histories, biases and
+// mask bits are small beside that, but what bounds it is the latency of what they cost: the
 // look at each earlier token by each CTA of the row, and chains of dependent loads. So a
 // CTA owns many columns (16384): it copies them masked, which waits for nothing, while it
 // marks and counts the tokens of its columns in shared memory (whole numbers: the order
@@ -19,7 +19,7 @@
 
 namespace {
 
-constexpr uint32_t kOwner = 0x80000000u;  // a word that holds a bias entry, not a count (below 2^28)
+constexpr uint32_t kOwner = 0x80000000u;  // a word that holds a bias entry, not a count (below 2^30, as tok_stride)
 constexpr int kListed = 2048;  // columns of a CTA's list; past that it looks at every column
 
 struct LogitArgs {
@@ -31,7 +31,7 @@ struct LogitArgs {
   const float *penalties;
   const int32_t *bias_ids, *bias_offsets;
   const float *bias_values;
-  int64_t n_bias;  // entries of bias_ids, -1: as many as the last offset says
+  int n_bias;  // entries of bias_ids, where the call is told (COUNTED)
   const uint32_t *masks;
   const int32_t *mask_rows;
   int64_t n_masks, mask_stride;
@@ -64,7 +64,9 @@ __device__ __forceinline__ void mask4(float4 &v, uint32_t bits) {
 // Grid: x = chunks of a row, y = rows; NT threads of V pieces of 4 columns. Columns are
 // counted from the 16-byte boundary at or before the row's first logit, so that rows of
 // any stride are read in whole 16-byte pieces; `lead` columns lie before the row.
-template <int NT, int V, bool VEC>
+// COUNTED: the number of bias entries is an argument, not the last offset (which costs a
+// branch and a load: 64 rows 34.6 / 34.8 us; without any bound 34.2).
+template <int NT, int V, bool VEC, bool COUNTED>
 __global__ void __launch_bounds__(NT, 1024 / NT) logits_kernel(const LogitArgs a) {
   constexpr int kCols = NT * V * 4, kLoads = V < 4 ? V : 4, kTokens = 4;
   static_assert(V % kLoads == 0 && kCols <= 65536, "whole batches, 16-bit columns");
@@ -104,7 +106,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) logits_kernel(const LogitArgs a
   }
   if (a.bias_offsets) {
     // (offsets are cut to the entries there are: nothing past bias_ids is read)
-    const int entries = a.n_bias >= 0 ? (int)a.n_bias : min(max(a.bias_offsets[gridDim.y], 0), INT32_MAX / 2);
+    const int entries = COUNTED ? a.n_bias : min(max(a.bias_offsets[gridDim.y], 0), INT32_MAX / 2);
     b0 = min(max(a.bias_offsets[row], 0), entries);
     biases = min(max(a.bias_offsets[row + 1], 0), entries) - b0;
   }
@@ -224,24 +226,28 @@ __global__ void __launch_bounds__(NT, 1024 / NT) logits_kernel(const LogitArgs a
   }
 }
 
-template <int NT, int V, bool VEC>
+template <int NT, int V, bool VEC, bool COUNTED>
 int logits_launch(gq_ctx *ctx, const LogitArgs &a, int64_t m, int64_t most_lead) {
   constexpr int kCols = NT * V * 4;
   static bool attr_set[64] = {};
   if (kCols * 4 > 32768 && !attr_set[ctx->device & 63]) {
-    GQ_CUDA_TRY(ctx, cudaFuncSetAttribute(logits_kernel<NT, V, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCols * 4));
+    GQ_CUDA_TRY(ctx, cudaFuncSetAttribute(logits_kernel<NT, V, VEC, COUNTED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCols * 4));
     attr_set[ctx->device & 63] = true;
   }
   const dim3 grid((unsigned)((a.vocab + most_lead + kCols - 1) / kCols), (unsigned)m);
-  GQ_CUDA_TRY(ctx, gq_launch(ctx, logits_kernel<NT, V, VEC>, grid, dim3(NT), kCols * 4, a));
+  GQ_CUDA_TRY(ctx, gq_launch(ctx, logits_kernel<NT, V, VEC, COUNTED>, grid, dim3(NT), kCols * 4, a));
   return GQ_OK;
 }
 
-template <bool VEC>
+template <bool VEC, bool COUNTED>
 int logits_dispatch(gq_ctx *ctx, const LogitArgs &a, int64_t m, int64_t most_lead) {
-  // few rows: smaller chunks, so that more SMs take part (one row of 262144: 2.8 us replayed)
-  if (m * ((a.vocab + 4095) / 4096) < ctx->num_sms) return logits_launch<256, 2, VEC>(ctx, a, m, most_lead);
-  return logits_launch<512, 8, VEC>(ctx, a, m, most_lead);
+  // Chunks of 2048 columns while chunks of 4096 would not give every SM one (rows of 262144:
+  // up to 2): more SMs take part, but each looks at its rows' whole histories. 2048 against
+  // 16384, us replayed, 300 biases, histories up to 900: 1 row 3.4 / 4.8, 2 3.6 / 4.8, 3
+  // 3.9 / 5.0, 4 4.0 / 4.8, 8 6.9 / 5.3, 16 13.9 / 9.0, 64 47.2 / 29.0; up to 8192: 5.9 / 6.5,
+  // 6.2 / 6.5, 6.3 / 6.5, 6.6 / 6.5, 10.6 / 6.7, 20.7 / 10.6, 77.2 / 33.9.
+  if (m * ((a.vocab + 4095) / 4096) < ctx->num_sms) return logits_launch<256, 2, VEC, COUNTED>(ctx, a, m, most_lead);
+  return logits_launch<512, 8, VEC, COUNTED>(ctx, a, m, most_lead);
 }
 
 int process_logits(gq_ctx *ctx, const float *logits, int64_t m, int64_t vocab, int64_t ld, const int32_t *tokens,
@@ -282,7 +288,7 @@ int process_logits(gq_ctx *ctx, const float *logits, int64_t m, int64_t vocab, i
   a.penalties = penalties;
   a.bias_ids = bias_ids;
   a.bias_values = bias_values;
-  a.n_bias = n_bias;
+  a.n_bias = (int)n_bias;
   a.bias_offsets = bias_offsets;
   a.masks = masks;
   a.n_masks = n_masks;
@@ -291,7 +297,8 @@ int process_logits(gq_ctx *ctx, const float *logits, int64_t m, int64_t vocab, i
   // 16-byte pieces need input and output rows on the same phase of a 16-byte boundary
   const bool vec = ((uintptr_t)logits - (uintptr_t)y) % 16 == 0 && (m == 1 || (ld - ldy) % 4 == 0);
   const int64_t most_lead = (uintptr_t)logits % 16 == 0 && (m == 1 || ld % 4 == 0) ? 0 : 3;
-  return vec ? logits_dispatch<true>(ctx, a, m, most_lead) : logits_dispatch<false>(ctx, a, m, 0);
+  if (n_bias >= 0) return vec ? logits_dispatch<true, true>(ctx, a, m, most_lead) : logits_dispatch<false, true>(ctx, a, m, 0);
+  return vec ? logits_dispatch<true, false>(ctx, a, m, most_lead) : logits_dispatch<false, false>(ctx, a, m, 0);
 }
 
 }  // namespace
