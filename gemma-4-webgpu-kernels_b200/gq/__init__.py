@@ -524,8 +524,8 @@ class CudaBackend:
         return KvAppend(tensor=self.concat_rows(existing, add), dead=existing)
 
     # ---- paged cache and logits of many requests (include/gq.h) -------------------
-    # Device tensors here are torch tensors (f32 ones may be GqTensors); the calls check
-    # types, devices and shapes, and the library the rest.
+    # Device tensors here are torch tensors (rows of f32, i.e. k, v, q, logits and out, may be
+    # GqTensors); the calls check types, devices and shapes, and the library the rest.
     def kv_pages(self, k, v, k_scale: float = 1.0, v_scale: float = 1.0) -> KvPages:
         """Describe one layer's pages: k, v [n_pages, heads, page_size, head_dim] of the same
         shape, strides and type; a page's values are contiguous, pages may lie apart."""
@@ -607,10 +607,11 @@ class CudaBackend:
         """Write rows k, v [T, heads, head_dim] f32 (token strides free) to slots [T] int64
         of the pages, rounded to their type (gq_paged_append)."""
         n = slots.numel()
-        for x in (k, v):  # (rows of heads * head_dim, or of one head after another)
-            shape = x.shape
-            if len(shape) > 2 and shape[-1] * shape[-2] != pages.row:
-                raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "paged_append: k and v must be [T, heads, head_dim]")
+        if pages.row != pages.head_dim:  # (several heads: rows by head would be in another order)
+            for x in (k, v):
+                shape = x.shape
+                if len(shape) > 2 and shape[-1] * shape[-2] != pages.row:
+                    raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "paged_append: k and v must be [T, heads, head_dim]")
         kp, ks = self._rows(k, n, pages.row, "paged_append: k")
         vp, vs = self._rows(v, n, pages.row, "paged_append: v")
         rc = self.lib.gq_paged_append(self.ctx, pages.ref, kp, vp, n, ks, vs, self._dev(slots, self._torch.int64, "slots"))
@@ -669,13 +670,12 @@ class CudaBackend:
             tok, n_tok = d(tokens, i32, "tokens"), ts[1]
             pl, ln = d(prompt_lens, i32, "prompt_lens", m), d(lens, i32, "lens", m)
             pen = d(penalties, f32, "penalties", 3 * m)
-        if bias_ids is not None or bias_values is not None or bias_offsets is not None:
-            if bias_ids is None or bias_values is None or bias_offsets is None:
-                raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "process_logits: biases are bias_ids, bias_values and bias_offsets")
-            n_bias = bias_ids.numel()
-        if n_bias:
-            bi, bv = d(bias_ids, i32, "bias_ids"), d(bias_values, f32, "bias_values", n_bias)
-            bo = d(bias_offsets, i32, "bias_offsets", m + 1)
+        if bias_offsets is not None and bias_ids is not None and bias_values is not None:
+            if n_bias := bias_ids.numel():
+                bi, bv = d(bias_ids, i32, "bias_ids"), d(bias_values, f32, "bias_values", n_bias)
+                bo = d(bias_offsets, i32, "bias_offsets", m + 1)
+        elif bias_offsets is not None or bias_ids is not None or bias_values is not None:
+            raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "process_logits: biases are bias_ids, bias_values and bias_offsets")
         if masks is not None and masks.numel():
             if masks.dim() != 2:
                 raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "process_logits: masks must be [k, words]")
