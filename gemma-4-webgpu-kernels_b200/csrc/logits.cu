@@ -12,7 +12,7 @@
 // applied where all columns are written, 47-67 us (their divisions run in nearly every
 // warp for a lane or two, and the logits wait in registers for the counts); a cluster of
 // 4 or 8 CTAs sharing the scan of the history, 38-53 us (cluster scheduling and barriers);
-// this way 34.4 us (floor 20.8; 23.4 without history, biases and masks).
+// this way 34.8 us (floor 20.8; 23.4 without history, biases and masks).
 #include <algorithm>
 
 #include "gq_internal.cuh"

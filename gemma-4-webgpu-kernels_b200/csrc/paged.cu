@@ -305,8 +305,10 @@ __device__ __forceinline__ void store4(void *base, int64_t elem, const float4 v,
 
 // A warp writes one token's row of keys (or values): what it needs of the slot is worked
 // out once, and a lane's kAppendLoads loads of 16 bytes are in flight together. Rows are
-// taken in turn by a grid that fills the GPU. HBM-bound: 16411 rows of 512 to e4m3, 84 MB,
-// 17.5 us, 4.8 TB/s (a thread per 4 values, each with its own slot and divisions: 34 us).
+// taken in turn by a grid of eight CTAs per SM, of which some 48 registers a thread let
+// five be resident; the arguments that are indexed by key or value lie in local memory (a
+// frame of 112 bytes). HBM-bound: 16411 rows of 512 to e4m3, 84 MB, 17.5 us, 4.8 TB/s (a
+// thread per 4 values, each with its own slot and divisions: 34 us).
 constexpr int kAppendThreads = 256, kAppendLoads = 4;
 
 template <int TYPE>

@@ -11,8 +11,11 @@
 //   O^T += V^T p^T     m16 = head_dim columns, n8 = heads, over the T keys: columns
 //                      split over the warps
 // with the scores of tile i + 1 in the tensor pipe while the weights of tile i are made:
-// one barrier per tile. Transposed, the 8 heads fill the instruction's n = 8 exactly: no product is wasted,
-// and a key-value head's cache is read once for all of them. The m16n8 instructions
+// one barrier per tile. Transposed, the 8 heads fill the instruction's n = 8 exactly: no
+// product is wasted, and a key-value head's cache is read once for all of them. More than 8
+// heads are more units, each of which reads it (L2 may still have it: 64 requests of up to
+// 4096 keys in bf16, 8 against 16 heads of 512 59 / 91 us, 8 against 64 heads of 128 24 / 121
+// us, replayed). The m16n8 instructions
 // (mma.sync) are used, not tcgen05: at n = 8 the work is 16 products per cached value,
 // and the ring, not the tensor pipe, is the limit; a 128-row accumulator tile in tensor
 // memory would add a round trip per tile for a softmax over its rows.
@@ -27,12 +30,12 @@
 // cached values, a fifth to a third of the legacy tensor pipe at the rates below.
 //
 // Measured (B200, a call among others, both launches): 64 requests of up to 4096 keys,
-// head_dim 512, bf16, 279 MB: 58.6 us, 4.8 TB/s, the tiles themselves 41 us at 6.8 TB/s
+// head_dim 512, bf16, 279 MB: 59 us, 4.7 TB/s, the tiles themselves 41 us at 6.8 TB/s
 // (the rest: 4 us from the start to the first keys, which come through two dependent
 // loads, lengths and table, and 12 us for the join and two kernel boundaries). 3 requests
-// of up to 131072 keys, e4m3, 249 MB: 57.4 us. 23 requests of up to 2501, f32, 4 heads of
-// 128, soft-cap, 127 MB: 33.8 us. With plain loads and CUDA-core products
-// (paged_rows_kernel): 324, 606 and 204 us. One request of 333 keys (a cluster of 8): 6.7
+// of up to 131072 keys, e4m3, 249 MB: 58 us. 23 requests of up to 2501, f32, 4 heads of
+// 128, soft-cap, 127 MB: 34 us. With plain loads and CUDA-core products
+// (paged_rows_kernel, replayed): 318, 528 and 202 us. One request of 333 keys (a cluster of 8): 6.7
 // us replayed.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -137,7 +140,7 @@ struct Tile {
   // CTAs per SM: three where rows are short, a tile is little work and 168 registers will
   // do (225 requests of up to 62 keys, 8 heads of 64, bf16: 31.4 us with two, 24.5 with
   // three; 10 of up to 40000, one head of 128: 35.3 and 33.8; e4m3 rows of 256 spill with
-  // three and lose 20 %)
+  // three and lose 20 %). (With two, e4m3 rows of 512 spill 16 bytes at the head.)
   static constexpr int kPerSm = kRow <= 256 && D <= 128 ? 3 : 2;
   static constexpr int kSmemBytes = (kPerSm == 3 ? 72 : 110) * 1024;
   static constexpr int kParts = TYPE == GQ_KV_BF16 ? 3 : 2;
@@ -815,12 +818,17 @@ int launch(gq_ctx *ctx, const gq_kv_pages *p, Args &a) {
   // Units that cannot have many tiles (a sliding window, a short table) get a cluster of
   // CTAs each, as large as fills the GPU: no cut to work out, and a join in shared memory
   // (some 4 us less, the time of two tiles). What it can cost is uneven work: tiles beyond
-  // an equal share, and lengths that differ (a window evens them out). Measured, cluster
-  // against cut, head_dim 256, bf16: window 512 and 1, 8, 64, 200, 500 requests 6.9 / 9.6,
-  // 9.2 / 12.4, 13.2 / 17.2, 28.4 / 34.5, 56 / 60 us; up to 1024 keys and 1, 16, 64
-  // requests 8.7 / 10.0, 9.4 / 12.8, 15.3 / 17.6; up to 2048 keys 13.1 / 10.0, 13.7 / 13.0,
-  // 26.5 / 24.1. (150 requests with the window, where a cluster is one CTA and half the
-  // GPU is idle: 27.5 / 27.0.)
+  // an equal share, and lengths that differ (a window evens them out). The bounds below come
+  // from head_dim 256 in bf16 (tiles of 64 keys), cluster against cut, us: window 512 and 1,
+  // 8, 64, 200, 500 requests 6.9 / 9.6, 9.2 / 12.4, 13.2 / 17.2, 28.4 / 34.5, 56 / 60; up to
+  // 1024 keys and 1, 16, 64 requests 8.7 / 10.0, 9.4 / 12.8, 15.3 / 17.6; up to 2048 keys
+  // 13.1 / 10.0, 13.7 / 13.0, 26.5 / 24.1. (150 requests with the window, where a cluster is
+  // one CTA and half the GPU is idle: 27.5 / 27.0.) Elsewhere, where they choose clusters:
+  // 225 requests of up to 62 keys, 8 heads of 64, bf16 24.7 / 26.8; 256 of up to 60, 4 heads
+  // of 128 16.1 / 19.1; 200 of up to 200, 8 heads of 128 35.1 / 37.1; 53 of one key, 8 heads
+  // of 512, f16 11.1 / 14.3; 100 of up to 300, 8 heads of 64, f32 29.3 / 29.0, of 128, e4m3
+  // 21.2 / 23.8; 39 of up to 2017, one head of 64, f32 13.8 / 14.7; 64 of up to 1024,
+  // head_dim 256, e4m3 14.7 / 16.6; 256 of up to 100, head_dim 256, bf16 9.5 / 17.3.
   const int64_t units = (int64_t)a.batch * a.units_per_req, tiles = most_tiles(a, C::T);
   const int slots = C::kPerSm * ctx->num_sms;
   int cluster = 8;

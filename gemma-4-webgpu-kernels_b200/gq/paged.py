@@ -3,7 +3,8 @@
 ``PagedDecoder`` is the decode step of ``gq.e2b`` with the cache in pages: each of its
 ``batch`` places holds a request with a length of its own, and a step
 
-* takes pages for the new tokens (``gq_paged_reserve``: positions and slots of the step),
+* takes pages for the new tokens (``gq_paged_reserve``: positions and slots of the step,
+  brought to their places, since places without a request get none),
 * writes each KV layer's new rows into their pages (``gq_paged_append``),
 * attends every request over its own pages (``gq_paged_attention``),
 * applies each request's penalties, biases and grammar mask to its logits
@@ -46,12 +47,13 @@ class PagedDecoder(e2b.Decoder):
     their token as it is, and their rows of the logits mean nothing.
 
     Controls, all device tensors that may be changed between steps on torch's current
-    stream, which a step comes after and which goes on after it (whatever stream the
-    backend has): ``penalties`` [batch, 3] (repetition, presence, frequency), ``prompt_lens`` [batch], ``history``
-    [batch, max_len] (tokens by position), and, given at construction because their sizes
-    belong to the recorded step, ``bias`` (ids, values, offsets) and ``masks``
-    (words, rows); see gq_process_logits in include/gq.h. ``sample``: temperature, top_k,
-    top_p of gq_sample_rows."""
+    stream (whatever stream the backend has, a step comes after what that stream was given
+    before it, and the stream goes on after the step): ``penalties`` [batch, 3]
+    (repetition, presence, frequency), ``prompt_lens`` [batch], ``history`` [batch,
+    max_len] (tokens by position, -1 where they are not known), and, given at construction
+    because their sizes belong to the recorded step, ``bias`` (ids, values, offsets) and
+    ``masks`` (words, rows); see gq_process_logits in include/gq.h. ``sample``: temperature,
+    top_k, top_p of gq_sample_rows."""
 
     def __init__(self, g, cfg: e2b.Config, weights: Optional[e2b.Weights], batch: int, max_len: int, page_size: int = 16,
                  kv_type: str = "bf16", n_pages: Optional[int] = None, k_scale: float = 1.0, v_scale: float = 1.0,
@@ -135,10 +137,11 @@ class PagedDecoder(e2b.Decoder):
         """Add new_lens[b] tokens to request b without decoding (a prompt's cache made
         elsewhere): rows(layer) gives their keys and values, f32 [sum, heads_kv *
         head_dim] in request order, for each source layer; tokens, when given, each
-        request's ids, as many as are known (its prompt, for the penalties; all that an extended request holds
-        counts as its prompt from then on). Raises when the pages do not
-        suffice, when a request would pass max_len, and what earlier steps left to raise; nothing is taken then. A place whose request was
-        ended begins anew, whether a step has come between or not."""
+        request's ids, as many as are known (its prompt, for the penalties; all that an
+        extended request holds counts as its prompt from then on). A place whose request
+        was ended begins anew, whether a step has come between or not. Raises when the
+        pages do not suffice, when a request would pass max_len, and what earlier steps
+        left to raise; no page is taken then."""
         torch, c, g = self.torch, self.cfg, self.g
         new_lens = [int(n) for n in new_lens]
         if len(new_lens) != self.batch or min(new_lens) < 0:

@@ -540,9 +540,11 @@ typedef struct gq_kv_pages {
  * -1, position 0, owner -1. totals[b] = seq_lens[b] + new_lens[b], free_left[0] = what
  * remains of free_count[0]; they may be seq_lens and free_count themselves.
  * All or nothing: when the pool (n_pages entries of free_pages), a table row or
- * max_tokens is too small (or a length passes 2^31 - 1), no page is taken, every slot is
- * -1, totals = seq_lens, free_left = free_count and GQ_DEVERR_PAGES is raised at the
- * next gq_sync. A page id outside [0, n_pages) in the table or the list gives slot -1
+ * max_tokens is too small (or a length passes 2^31 - 1, or free_count is outside [0,
+ * n_pages]), no page is taken, every slot is -1, totals = seq_lens (negative ones 0),
+ * free_left = free_count cut to [0, n_pages], and GQ_DEVERR_PAGES is raised at the next
+ * gq_sync. Requests that add no token have no place among the step's tokens: owners tells
+ * which request each belongs to. A page id outside [0, n_pages) in the table or the list gives slot -1
  * and the same error.
  * All pointers are device pointers. batch <= 16384, max_tokens < 2^31. */
 int gq_paged_reserve(gq_ctx *ctx, int64_t batch, int64_t page_size, const int32_t *seq_lens, const int32_t *new_lens,
@@ -558,7 +560,8 @@ int gq_paged_reserve(gq_ctx *ctx, int64_t batch, int64_t page_size, const int32_
  * free_count[0] + R; they may be seq_lens and free_count. The block table is not
  * changed (entries past a request's length mean nothing). All or nothing: when the
  * list would outgrow its n_pages entries, or a length its row, nothing is given back,
- * totals = seq_lens, free_left = free_count, and GQ_DEVERR_PAGES is raised.
+ * totals = seq_lens, free_left = free_count (both cut as above), and GQ_DEVERR_PAGES is
+ * raised. A page id outside the pool is listed as it is and raises the error too.
  * batch <= 16384. */
 int gq_paged_release(gq_ctx *ctx, int64_t batch, int64_t page_size, const int32_t *seq_lens, const int32_t *keep_lens,
                      const int32_t *block_table, int64_t table_stride, int32_t *free_pages, int64_t n_pages,
@@ -582,9 +585,11 @@ int gq_paged_append(gq_ctx *ctx, const gq_kv_pages *pages, const float *k, const
  * heads, hq / heads <= 64. Rows of a page past the request's length are never read as
  * numbers (they may hold NaN). A page id outside the pool raises GQ_DEVERR_PAGES and
  * counts as a page of zero rows; a length past the table row raises it and is cut to
- * the row: nothing outside the pool is read. Finite q and visible keys and values
- * (below 2^127) give f32 results: all sums in f32, products exact to 2^-21 or better;
- * where one is not finite, its row may be NaN. Long requests are split over many CTAs,
+ * the row: nothing outside the pool is read. All sums are f32, products exact to 2^-21
+ * or better, and the weighted sum of the values is divided at its end: results are f32's
+ * while the sums q . k, and the number of visible keys times the largest |v| (as stored;
+ * f16 and e4m3 never get there), stay below 2^127; where a q, key, value or such a sum
+ * is not finite, the row may be NaN. Long requests are split over many CTAs,
  * whose partial results (20 MB that the context's first call allocates: not while the
  * stream is captured) a second launch joins in a fixed order: results do not vary from
  * run to run. */
