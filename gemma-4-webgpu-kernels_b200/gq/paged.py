@@ -189,8 +189,11 @@ class PagedDecoder(e2b.Decoder):
     def end(self, places: Sequence[int]) -> None:
         """The requests at these places end: the next step is their last, and gives their pages
         back. The places idle from then on, until ``extend`` gives them a request."""
+        places = [int(b) for b in places]
+        if any(not 0 <= b < self.batch for b in places):  # (on the device an index past the end is a fault)
+            raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, f"end: places are 0 to {self.batch - 1}")
         with self._ordered():
-            self.keep[self.torch.tensor(list(places), device=self.g.torch_device)] = 0
+            self.keep[self.torch.tensor(places, dtype=self.torch.int64, device=self.g.torch_device)] = 0
         self.ending |= set(places)
 
     # ---- the step ----------------------------------------------------------------------

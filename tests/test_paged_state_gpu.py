@@ -397,3 +397,17 @@ def test_a_refused_extend_of_an_ended_place_leaves_it_idle(g):
     g.flush()
     assert dec.lens.tolist() == [6, 34] and dec.took.tolist() == [True, True]
     dec.close()
+
+
+def test_places_that_are_not_there_cannot_end(g):
+    dec = make(g, 2)
+    dec.extend([3, 4], seeded_rows(g, [3, 4]))
+    for places in ([2], [-1], [0, 5]):
+        with pytest.raises(GqError) as e:
+            dec.end(places)
+        assert e.value.status == _abi.GQ_ERR_INVALID_ARGUMENT
+    dec.end([])
+    dec.step([1, 2])
+    g.flush()
+    assert dec.lens.tolist() == [4, 5]
+    dec.close()
