@@ -417,23 +417,25 @@ int check_plan(gq_ctx *ctx, const char *op, int64_t batch, int64_t page_size, in
 int gq_check_kv_pages(gq_ctx *ctx, const char *op, const gq_kv_pages *p) {
   const std::string who(op);
   if (!p) return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT, who + ": null pages");
-  if (p->type < GQ_KV_F32 || p->type > GQ_KV_E4M3) return gq_fail(ctx, GQ_ERR_UNSUPPORTED, who + ": unknown page type");
+  if (p->type < GQ_KV_F32 || p->type > GQ_KV_E2M1) return gq_fail(ctx, GQ_ERR_UNSUPPORTED, who + ": unknown page type");
   if (p->n_pages < 0 || p->n_pages > INT32_MAX || p->page_size < 1 || p->page_size > 65536 || p->heads < 1 ||
       p->heads > 65535 || p->head_dim < 1)
     return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT, who + ": bad n_pages, page_size, heads or head_dim");
   if (p->head_dim % 4 != 0 || p->head_dim > 512)
     return gq_fail(ctx, GQ_ERR_UNSUPPORTED, who + ": head_dim must be a multiple of 4, at most 512");
-  const int64_t packed = p->heads * p->page_size * p->head_dim, stride = p->page_stride ? p->page_stride : packed;
-  if (stride < packed || stride % 4 != 0)
+  if (p->type == GQ_KV_E2M1 && p->head_dim % 16 != 0)
+    return gq_fail(ctx, GQ_ERR_UNSUPPORTED, who + ": head_dim of e2m1 pages must be a multiple of 16");
+  const int64_t packed = p->heads * p->page_size * gq_kv_row(p), stride = gq_kv_page_stride(p);
+  if (stride < packed || (p->type != GQ_KV_E2M1 && stride % 4 != 0))
     return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT, who + ": page_stride below a page's size, or not a multiple of 4");
   if (p->n_pages > 0 && (!p->k || !p->v)) return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT, who + ": null page pool");
   if (((uintptr_t)p->k | (uintptr_t)p->v) % 16 != 0)
     return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT, who + ": k and v pages must be 16-byte aligned");
-  const bool scaled = p->type == GQ_KV_E4M3;
+  const bool scaled = p->type == GQ_KV_E4M3 || p->type == GQ_KV_E2M1;
   for (const float s : {p->k_scale, p->v_scale})
     if (!(s > 0.0f) || !std::isfinite(s) || !std::isfinite(1.0f / s) || (!scaled && s != 1.0f))
       return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT,
-                     who + ": scales must be positive, finite with a finite reciprocal, and 1 unless the type is e4m3");
+                     who + ": scales must be positive, finite with a finite reciprocal, and 1 unless the type is e4m3 or e2m1");
   return GQ_OK;
 }
 
@@ -509,6 +511,7 @@ extern "C" int gq_paged_append(gq_ctx *ctx, const gq_kv_pages *pages, const floa
   if (!k || !v || !slots) return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT, "paged_append: null pointer");
   if (((uintptr_t)k | (uintptr_t)v) % 16 != 0)
     return gq_fail(ctx, GQ_ERR_INVALID_ARGUMENT, "paged_append: k and v must be 16-byte aligned");
+  if (pages->type == GQ_KV_E2M1) return gq_paged_append_e2m1(ctx, pages, k, v, t, k_tok_stride, v_tok_stride, slots);
   AppendArgs a{};
   a.src[0] = k;
   a.src[1] = v;

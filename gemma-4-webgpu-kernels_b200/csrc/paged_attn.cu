@@ -16,6 +16,7 @@
 
 #include <algorithm>
 
+#include "e2m1.cuh"
 #include "paged_attn.cuh"
 
 // paged_attn_tc.cu
@@ -55,6 +56,20 @@ __device__ __forceinline__ float4 load4(const void *base, int64_t elem) {
       const float2 b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
       return make_float4(a.x, a.y, b.x, b.y);
     }
+  }
+}
+
+// Columns c .. c + 3 of the row that begins at element e.
+template <int TYPE>
+__device__ __forceinline__ float4 columns(const Args &a, const void *base, int64_t e, int c) {
+  if constexpr (TYPE == GQ_KV_E2M1) {
+    const uint8_t *row = static_cast<const uint8_t *>(base) + e;
+    const uint32_t u = row[c >> 1] | ((uint32_t)row[(c >> 1) + 1] << 8);
+    const float s = e4m3_value(row[(a.dim >> 1) + (c >> 4)]);
+    const float2 x = __half22float2(e2m1_pair(u)), y = __half22float2(e2m1_pair(u >> 8));
+    return make_float4(x.x * s, x.y * s, y.x * s, y.y * s);
+  } else {
+    return load4<TYPE>(base, e + c);
   }
 }
 
@@ -105,7 +120,7 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const Args a) {
         if (j >= r.lo && j < r.hi) {
           const int page = a.table[b * a.table_stride + j / a.page_size];
           if (page >= 0 && page < a.n_pages)
-            e = page * a.page_stride + ((int64_t)kvh * a.page_size + j % a.page_size) * a.dim;
+            e = page * a.page_stride + ((int64_t)kvh * a.page_size + j % a.page_size) * (TYPE == GQ_KV_E2M1 ? a.row : a.dim);
           else
             gqd::report(a.err, GQ_DEVERR_PAGES);
         }
@@ -119,7 +134,7 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const Args a) {
         for (int h = 0; h < kHeads; ++h) dot[h] = 0.0f;
         if (e >= 0)
           for (int c = lane * 4; c < a.dim; c += 128) {
-            const float4 k = load4<TYPE>(a.k, e + c);
+            const float4 k = columns<TYPE>(a, a.k, e, c);
 #pragma unroll
             for (int h = 0; h < kHeads; ++h) {
               const float4 qv = *reinterpret_cast<const float4 *>(&q[h][c]);
@@ -169,7 +184,7 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const Args a) {
         for (int kk = 0; kk < kRowTile; ++kk) {
           const int64_t e = elem[kk];
           if (e < 0) continue;
-          const float4 v = load4<TYPE>(a.v, e + tid * 4);
+          const float4 v = columns<TYPE>(a, a.v, e, tid * 4);
 #pragma unroll
           for (int h = 0; h < kHeads; ++h) {
             const float p = s[h][kk];
@@ -393,7 +408,8 @@ extern "C" int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const f
   a.lens = seq_lens;
   a.q_stride = q_tok_stride;
   a.table_stride = table_stride;
-  a.page_stride = pages->page_stride ? pages->page_stride : pages->heads * pages->page_size * pages->head_dim;
+  a.page_stride = gq_kv_page_stride(pages);
+  a.row = (int)gq_kv_row(pages);
   a.n_pages = pages->n_pages;
   // (the last tile's keys are numbered in 32 bits; the product is kept inside 64)
   a.room = std::min<int64_t>(std::min<int64_t>(table_stride, INT32_MAX) * pages->page_size, INT32_MAX - 1024);
@@ -419,6 +435,7 @@ extern "C" int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const f
     case GQ_KV_F32: GQ_CUDA_TRY(ctx, rows_launch<GQ_KV_F32>(ctx, grid, a)); break;
     case GQ_KV_F16: GQ_CUDA_TRY(ctx, rows_launch<GQ_KV_F16>(ctx, grid, a)); break;
     case GQ_KV_BF16: GQ_CUDA_TRY(ctx, rows_launch<GQ_KV_BF16>(ctx, grid, a)); break;
+    case GQ_KV_E2M1: GQ_CUDA_TRY(ctx, rows_launch<GQ_KV_E2M1>(ctx, grid, a)); break;
     default: GQ_CUDA_TRY(ctx, rows_launch<GQ_KV_E4M3>(ctx, grid, a)); break;
   }
   return gq_paged_join_launch(ctx, a, grid);

@@ -38,6 +38,7 @@ struct Args {
   int cluster;                                      // CTAs per unit (one cluster), 0: units cut by find_cut
   int batch, hq, heads, group, sub, units_per_req;  // group = hq / heads, sub = blocks of 8 per key-value head
   int dim, page_size, page_shift;                   // page_shift: log2 page_size (tiled kernels)
+  int row;                                          // elements from a row of a page to the next (bytes of e2m1 rows)
   int32_t window;
   float scale, softcap, inv_softcap, v_scale;  // scale: of the scores, the keys' scale included
   float *part_o, *part_ml;        // [2 grid][8][dim], [2 grid][8][2]

@@ -880,6 +880,7 @@ int launch_dim(gq_ctx *ctx, const gq_kv_pages *p, Args &a) {
 // Rows of whole 128-byte pieces at the instantiated head_dims, and pages that a tile is
 // a whole number of (or that are a whole number of tiles).
 bool gq_paged_attn_tc_supported(const gq_kv_pages *p, int64_t page_stride) {
+  if (p->type == GQ_KV_E2M1) return false;
   const int size = gq_kv_size(p->type);
   const int64_t d = p->head_dim;
   return (d == 64 || d == 128 || d == 256 || d == 512) && d * size % 128 == 0 && p->page_size >= 8 &&

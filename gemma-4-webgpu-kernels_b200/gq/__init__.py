@@ -18,7 +18,7 @@ names, argument meaning and error behaviour follow the trait:
   ``head_norm_rope`` (:137-154), and ``linear`` with a bf16-stored plain weight
 * the paged cache and the logits of a step that serves many requests (no counterpart in
   the trait): ``kv_pages``, ``paged_reserve``, ``paged_release``, ``paged_append``,
-  ``paged_attention``, ``process_logits``
+  ``paged_read``, ``paged_attention``, ``process_logits``, ``sample_requests``
 
 Ops enqueue on the backend's stream (torch's current stream of the device) and
 return immediately; ``readback`` blocks, like the reference. Failures raise
@@ -120,7 +120,8 @@ class KvAppend:
 class KvPages:
     """One layer's pages of a paged key-value cache (gq_kv_pages, include/gq.h): ``k`` and
     ``v`` are cuda tensors [n_pages, heads, page_size, head_dim] of one type (float32,
-    float16, bfloat16 or float8_e4m3fn), kept alive here. Made by
+    float16, bfloat16 or float8_e4m3fn), or [n_pages, heads, page_size, head_dim / 16 * 9]
+    uint8 (rows of 4-bit values and their scales, GQ_KV_E2M1), kept alive here. Made by
     ``CudaBackend.kv_pages``."""
 
     k: object
@@ -528,10 +529,11 @@ class CudaBackend:
     # GqTensors); the calls check types, devices and shapes, and the library the rest.
     def kv_pages(self, k, v, k_scale: float = 1.0, v_scale: float = 1.0) -> KvPages:
         """Describe one layer's pages: k, v [n_pages, heads, page_size, head_dim] of the same
-        shape, strides and type; a page's values are contiguous, pages may lie apart."""
+        shape, strides and type; a page's values are contiguous, pages may lie apart. uint8:
+        4-bit values, rows of head_dim / 16 * 9 bytes (GQ_KV_E2M1)."""
         torch = self._torch
         types = {torch.float32: _abi.GQ_KV_F32, torch.float16: _abi.GQ_KV_F16, torch.bfloat16: _abi.GQ_KV_BF16,
-                 torch.float8_e4m3fn: _abi.GQ_KV_E4M3}
+                 torch.float8_e4m3fn: _abi.GQ_KV_E4M3, torch.uint8: _abi.GQ_KV_E2M1}
         if k.dtype not in types or v.dtype != k.dtype:
             raise GqError(_abi.GQ_ERR_UNSUPPORTED, f"kv_pages: types {k.dtype} and {v.dtype}")
         if k.dim() != 4 or k.shape != v.shape or k.device != self.torch_device or v.device != self.torch_device:
@@ -544,6 +546,10 @@ class CudaBackend:
                 raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "kv_pages: a page's values must be contiguous, k and v strided alike")
         if apart < h * ps * d:  # (an expanded tensor's stride 0 would mean packed pages to the library)
             raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "kv_pages: pages lie on one another")
+        if k.dtype == torch.uint8:
+            if d % 9 != 0:
+                raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "kv_pages: rows of 4-bit values are head_dim / 16 * 9 bytes")
+            d = d // 9 * 16
         st = _abi.KvPagesStruct(k.data_ptr(), v.data_ptr(), n, ps, h, d, apart, types[k.dtype], float(k_scale), float(v_scale))
         return KvPages(k, v, st, ctypes.addressof(st), h * d, d)
 
@@ -618,6 +624,25 @@ class CudaBackend:
         if rc:
             self._check(rc, "paged_append")
 
+    def paged_read(self, pages: KvPages, slots, k_out=None, v_out=None):
+        """The rows at slots [T] int64 of the pages as f32 k, v [T, heads, head_dim]
+        (gq_paged_read): `k_out` and `v_out` (token strides free), whose rows of negative
+        slots stay as they are, or new tensors, where such rows are 0."""
+        n, heads = slots.numel(), pages.row // pages.head_dim
+        new = lambda: self._torch.zeros(n, heads, pages.head_dim, dtype=self._torch.float32, device=self.torch_device)  # noqa: E731
+        k, v = k_out if k_out is not None else new(), v_out if v_out is not None else new()
+        if pages.row != pages.head_dim:  # (as in paged_append)
+            for x in (k, v):
+                shape = x.shape
+                if len(shape) > 2 and shape[-1] * shape[-2] != pages.row:
+                    raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "paged_read: k_out and v_out must be [T, heads, head_dim]")
+        kp, ks = self._rows(k, n, pages.row, "paged_read: k_out")
+        vp, vs = self._rows(v, n, pages.row, "paged_read: v_out")
+        rc = self.lib.gq_paged_read(self.ctx, pages.ref, self._dev(slots, self._torch.int64, "slots"), n, kp, vp, ks, vs)
+        if rc:
+            self._check(rc, "paged_read")
+        return k, v
+
     def paged_attention(self, pages: KvPages, q, block_table, seq_lens, scale: float = 1.0, sliding_window: int = 0,
                         attn_softcap: float = 0.0, out=None):
         """Attention of one new token per request over its pages (gq_paged_attention):
@@ -686,6 +711,34 @@ class CudaBackend:
         if rc:
             self._check(rc, "process_logits")
         return y
+
+    def sample_requests(self, logits, temperature=None, top_k=None, top_p=None, min_p=None, uniforms=None, rng_state=None,
+                        tokens=None, probs=None):
+        """A token for each row of logits [m, vocab], drawn with the row's own options
+        (gq_sample_requests): temperature, top_p and min_p [m] f32, top_k [m] int32 (None:
+        off), and uniforms [m] f64 in [0, 1) or rng_state [m] int64 (splitmix64 states,
+        advanced). -> tokens [m] int32 (`tokens`, or a new tensor); `probs` [m] f32, when
+        given, receives the probabilities that they were drawn with."""
+        torch, d = self._torch, self._dev
+        f32 = torch.float32
+        lt = logits.data if isinstance(logits, GqTensor) else logits
+        shape = lt.shape
+        if len(shape) != 2:
+            raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, "sample_requests: logits must be [m, vocab]")
+        m, vocab = shape
+        lp, ld = self._rows(lt, m, vocab, "sample_requests: logits")
+        if tokens is None:
+            tokens = torch.empty(m, dtype=torch.int32, device=self.torch_device)
+        rc = self.lib.gq_sample_requests(
+            self.ctx, lp, m, vocab, ld, d(temperature, f32, "temperature", m) if temperature is not None else None,
+            d(top_k, torch.int32, "top_k", m) if top_k is not None else None,
+            d(top_p, f32, "top_p", m) if top_p is not None else None, d(min_p, f32, "min_p", m) if min_p is not None else None,
+            d(uniforms, torch.float64, "uniforms", m) if uniforms is not None else None,
+            d(rng_state, torch.int64, "rng_state", m) if rng_state is not None else None, d(tokens, torch.int32, "tokens", m),
+            d(probs, f32, "probs", m) if probs is not None else None)
+        if rc:
+            self._check(rc, "sample_requests")
+        return tokens
 
     # ---- sync / lifecycle (rust/src/backend.rs:169-179) ------------------------
     def readback(self, t: GqTensor) -> np.ndarray:

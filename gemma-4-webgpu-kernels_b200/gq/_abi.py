@@ -27,6 +27,7 @@ GQ_KV_F32 = 0
 GQ_KV_F16 = 1
 GQ_KV_BF16 = 2
 GQ_KV_E4M3 = 3
+GQ_KV_E2M1 = 4
 
 
 class SampleOpts(ctypes.Structure):
@@ -168,6 +169,9 @@ SIGNATURES = {
     "gq_paged_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p]),
     "gq_paged_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p,
                                    c_float, c_uint32, c_float, c_void_p]),
+    "gq_paged_read": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64]),
+    "gq_sample_requests": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_void_p]),
     "gq_process_logits": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
                                   c_void_p, c_int64]),

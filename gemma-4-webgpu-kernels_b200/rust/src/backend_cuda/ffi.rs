@@ -82,6 +82,7 @@ pub const GQ_KV_F32: i32 = 0;
 pub const GQ_KV_F16: i32 = 1;
 pub const GQ_KV_BF16: i32 = 2;
 pub const GQ_KV_E4M3: i32 = 3;
+pub const GQ_KV_E2M1: i32 = 4;
 pub const GQ_ATTN_KPOS_ASCENDING: u32 = 0x1;
 pub const GQ_ATTN_KPOS_IDENTITY: u32 = 0x2;
 
@@ -220,6 +221,11 @@ extern "C" {
         free_left: *mut i32, totals: *mut i32) -> c_int;
     pub fn gq_paged_append(ctx: *mut GqCtx, pages: *const GqKvPages, k: *const f32, v: *const f32, t: i64,
         k_tok_stride: i64, v_tok_stride: i64, slots: *const i64) -> c_int;
+    pub fn gq_paged_read(ctx: *mut GqCtx, pages: *const GqKvPages, slots: *const i64, t: i64, k: *mut f32, v: *mut f32,
+        k_tok_stride: i64, v_tok_stride: i64) -> c_int;
+    pub fn gq_sample_requests(ctx: *mut GqCtx, logits: *const f32, m: i64, vocab: i64, ld: i64, temperature: *const f32,
+        top_k: *const i32, top_p: *const f32, min_p: *const f32, uniforms: *const f64, rng_state: *mut u64,
+        tokens: *mut i32, probs: *mut f32) -> c_int;
     pub fn gq_paged_attention(ctx: *mut GqCtx, pages: *const GqKvPages, q: *const f32, batch: i64, hq: i64,
         q_tok_stride: i64, block_table: *const i32, table_stride: i64, seq_lens: *const i32, scale: f32,
         sliding_window: u32, attn_softcap: f32, out: *mut f32) -> c_int;

@@ -509,11 +509,16 @@ int gq_copy_rows(gq_ctx *ctx, const float *src, int64_t rows, int64_t cols, int6
  * need a context each (they share its workspace and arrival counters). No counterpart in
  * the reference (its caches are one contiguous tensor per layer of one sequence). */
 
-/* Storage of a page's values. An e4m3 code stands for code * k_scale (or v_scale). */
+/* Storage of a page's values. An e4m3 code stands for code * k_scale (or v_scale). A row
+ * of GQ_KV_E2M1 values is head_dim / 2 bytes of 4-bit codes (two exponent and one
+ * fraction bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6, and 8 more for the negatives; value 2i in the
+ * low half of byte i), then head_dim / 16 bytes of e4m3 scales, one for every 16
+ * neighbouring values: a value is code * scale * k_scale (or v_scale). */
 #define GQ_KV_F32 0
 #define GQ_KV_F16 1
 #define GQ_KV_BF16 2
 #define GQ_KV_E4M3 3
+#define GQ_KV_E2M1 4
 
 /* One layer's pages, in caller-owned device memory: value (page, head, row, c) of the
  * keys is element page * page_stride + (head * page_size + row) * head_dim + c of k
@@ -521,7 +526,9 @@ int gq_copy_rows(gq_ctx *ctx, const float *src, int64_t rows, int64_t cols, int6
  * and values, or several layers, interleave in one allocation). head_dim a multiple
  * of 4 up to 512, page_size 1 .. 65536, heads up to 65535, k and v 16-byte aligned,
  * page_stride a multiple of 4. k_scale and v_scale are positive and finite,
- * their reciprocals too, for GQ_KV_E4M3, and 1 for the other types. */
+ * their reciprocals too, for GQ_KV_E4M3 and GQ_KV_E2M1, and 1 for the other types.
+ * GQ_KV_E2M1: head_dim a multiple of 16; rows of head_dim / 16 * 9 bytes take the place of
+ * rows of head_dim values, and page_stride is bytes, any number from a page's size on. */
 typedef struct gq_kv_pages {
   void *k, *v;
   int64_t n_pages, page_size, heads, head_dim, page_stride;
@@ -569,12 +576,24 @@ int gq_paged_release(gq_ctx *ctx, int64_t batch, int64_t page_size, const int32_
 
 /* Write t new key and value rows into their pages: row i of k (f32, heads * head_dim
  * values at k + i * k_tok_stride; 0 = packed) and of v, rounded to the pages' type
- * (nearest, ties to even; e4m3: value * (1 / scale) clamped to +-448, NaN stays NaN),
+ * (nearest, ties to even; e4m3: value * (1 / scale) clamped to +-448, NaN stays NaN;
+ * e2m1: x = value * (1 / scale) in f32, the scale of 16 neighbours the e4m3 number nearest
+ * max|x| / 6 and at most 448, a code the number nearest x / (that scale) and at most 6 in
+ * size, both quotients exact; a NaN makes its 16 neighbours NaN),
  * goes to slots[i] (device int64). A negative slot skips the row; one past the pool
  * skips it and raises GQ_DEVERR_PAGES. Two rows must not have the same slot. k and v
  * 16-byte aligned, token strides multiples of 4. */
 int gq_paged_append(gq_ctx *ctx, const gq_kv_pages *pages, const float *k, const float *v, int64_t t,
                     int64_t k_tok_stride, int64_t v_tok_stride, const int64_t *slots);
+
+/* Read t rows back: the keys and values at slots[i] (device int64) of pages of any type, as
+ * f32, times k_scale and v_scale, become row i of k and of v (heads * head_dim values at k +
+ * i * k_tok_stride; 0 = packed). A negative slot leaves its row of k and v as it was; one
+ * past the pool does too and raises GQ_DEVERR_PAGES. A slot may be read any number of
+ * times. k and v 16-byte aligned, token strides multiples of 4, the rows of k and v apart
+ * from the pages and from one another. */
+int gq_paged_read(gq_ctx *ctx, const gq_kv_pages *pages, const int64_t *slots, int64_t t, float *k, float *v,
+                  int64_t k_tok_stride, int64_t v_tok_stride);
 
 /* Attention of one new token of each request over its pages (the paged form of
  * gq_attention with t = 1): the query of request b is at position seq_lens[b] - 1 and
@@ -628,6 +647,29 @@ int gq_process_logits_bounded(gq_ctx *ctx, const float *logits, int64_t m, int64
                               const float *bias_values, const int32_t *bias_offsets, int64_t n_bias,
                               const uint32_t *masks, int64_t n_masks, int64_t mask_stride, const int32_t *mask_rows,
                               float *y, int64_t ldy);
+
+/* A token for each of m rows of logits [m, vocab] (row stride ld, 0 = vocab), every row
+ * with options of its own (device arrays of m entries; NULL: the option is off, a
+ * temperature of 1):
+ *   w_i = e^((l_i - max l) / temperature)
+ *   in the order of the logits, largest first, ties to the smaller id: the first top_k
+ *   (0 or less: all); of those the shortest run from the first on whose mass reaches top_p
+ *   of theirs (1 and up: all; at least one token); of those the ones with w_i >= min_p
+ *   (above 1 counts as 1)
+ *   tokens[r]: the first kept id, in the order of the ids, at which the running sum of w
+ *   passes u times the sum of all kept
+ * A temperature that is not above 0 is greedy: the first of the largest. u is uniforms[r]
+ * (f64, cut to [0, 1), NaN counts as 0) or, with rng_state in its place, the next number of
+ * the row's splitmix64 state as gq_sample_rows draws it (advanced by every row that is not
+ * greedy). probs[r] (f32, may be NULL) is the probability the token was drawn with, its w
+ * over the sum (greedy: 1). A NaN is never drawn, nor is -inf; where there is nothing else
+ * the token is -1 and its probability 0. +inf: only such tokens are drawn. Weights are
+ * f64 and added up as multiples of 2^-44 of the largest: a weight below half of that
+ * counts as 0. The logits are not modified. vocab <= 524288 (GQ_ERR_UNSUPPORTED beyond).
+ * Uses no workspace: calls on several streams and recorded ones do not meet. */
+int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, int64_t vocab, int64_t ld, const float *temperature,
+                       const int32_t *top_k, const float *top_p, const float *min_p, const double *uniforms,
+                       uint64_t *rng_state, int32_t *tokens, float *probs);
 
 #ifdef __cplusplus
 }

@@ -46,3 +46,31 @@ def test_append_refuses_rows_by_head(g):
             g.paged_append(pages, k, v, slots)
         assert e.value.status == _abi.GQ_ERR_INVALID_ARGUMENT
     assert len(calls) == 5
+
+
+def test_rows_of_4_bit_values(g):
+    """uint8 rows: head_dim / 2 bytes of codes and head_dim / 16 of scales."""
+    pool = torch.zeros(6, 2, 3, 16, 144, dtype=torch.uint8)
+    pages = g.kv_pages(pool[:, 0], pool[:, 1], 1 / 32, 1 / 32)
+    st = pages.struct
+    assert (st.type, st.head_dim, st.page_stride, pages.row, pages.head_dim) == (_abi.GQ_KV_E2M1, 256, 2 * 3 * 16 * 144, 3 * 256, 256)
+    for bytes_of_row in (128, 136, 145):
+        with pytest.raises(GqError) as e:
+            g.kv_pages(*(torch.zeros(2, 1, 16, bytes_of_row, dtype=torch.uint8),) * 2)
+        assert e.value.status == _abi.GQ_ERR_INVALID_ARGUMENT
+    with pytest.raises(GqError) as e:
+        g.kv_pages(pool[:, 0], pool[:, 0].float())
+    assert e.value.status == _abi.GQ_ERR_UNSUPPORTED
+
+
+def test_read_refuses_rows_by_head(g):
+    calls = []
+    g.device, g.lib = -1, type("Lib", (), {"gq_paged_read": lambda self, *a: calls.append(a) or 0})()
+    pages = g.kv_pages(torch.zeros(4, 2, 16, 64), torch.zeros(4, 2, 16, 64))
+    ok, slots = torch.zeros(5, 2, 64), torch.zeros(5, dtype=torch.int64)
+    for rows in (ok, ok.view(5, 128), torch.zeros(5, 256)[:, :128], None):
+        k, v = g.paged_read(pages, slots, rows, ok)
+        assert k.numel() == 640 and v is ok
+    with pytest.raises(GqError) as e:
+        g.paged_read(pages, slots, torch.zeros(2, 5, 64), ok)
+    assert e.value.status == _abi.GQ_ERR_INVALID_ARGUMENT and len(calls) == 4
