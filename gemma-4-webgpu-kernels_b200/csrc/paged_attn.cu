@@ -22,6 +22,9 @@
 // paged_attn_tc.cu
 bool gq_paged_attn_tc_supported(const gq_kv_pages *pages, int64_t page_stride);
 int gq_paged_attn_tc_launch(gq_ctx *ctx, const gq_kv_pages *pages, pattn::Args &a);
+// paged_attn_q4.cu
+bool gq_paged_attn_q4_supported(const gq_kv_pages *pages);
+int gq_paged_attn_q4_launch(gq_ctx *ctx, const gq_kv_pages *pages, pattn::Args &a);
 
 namespace {
 
@@ -428,6 +431,7 @@ extern "C" int gq_paged_attention(gq_ctx *ctx, const gq_kv_pages *pages, const f
   a.v_scale = pages->v_scale;
   a.err = ctx->dev_err;
   if (gq_paged_attn_tc_supported(pages, a.page_stride)) return gq_paged_attn_tc_launch(ctx, pages, a);
+  if (gq_paged_attn_q4_supported(pages)) return gq_paged_attn_q4_launch(ctx, pages, a);
   const int grid = grid_for(a, kRowTile, kRowPerSm * ctx->num_sms);
   rc = bind_parts(ctx, grid, a);
   if (rc != GQ_OK) return rc;
