@@ -32,20 +32,20 @@ constexpr int kKeys = 32;  // keys of a tile
 
 template <int D>
 struct Conf {
-  static constexpr int PS = D > 256 ? 2 : 1;     // warps that share a tile's columns (a team)
+  static constexpr int PS = D > 128 ? D / 128 : 1;  // warps that share a tile's columns (a team)
   static constexpr int DW = D / PS;              // columns of a warp
   static constexpr int kRow = D / 16 * 9;        // bytes of a key's row
   static constexpr int CB = DW / 16;             // bytes of codes that a lane takes at once
   static constexpr int NC = DW / (8 * CB);       // times it does for K
   static constexpr int W = CB / 4;               // words of it
-  static constexpr int kWarps = 4;
+  static constexpr int kWarps = D > 128 ? 8 : 4;
   static constexpr int kTeams = kWarps / PS;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kSlot = 2 * kKeys * kRow;
-  static constexpr int kStages = D <= 128 ? 3 : 2;
-  static constexpr int kPerSm = D <= 128 ? 3 : 2;
+  static constexpr int kStages = 2;
+  static constexpr int kPerSm = D > 128 ? 2 : 4;
   static constexpr int kQBytes = D / 16 * 32 * 16;
-  static constexpr int kSwap = PS > 1 ? kTeams * 2 * 2 * 32 * 8 * 4 : 0;
+  static constexpr int kSwap = PS > 1 ? kTeams * 2 * PS * 32 * 8 * 4 : 0;
   static constexpr int kSmem = kTeams * kStages * kSlot + kQBytes + kSwap;
   static_assert(kSlot >= 8 * D * 4, "a team's part of the output fits a slot");
 };
@@ -54,9 +54,10 @@ struct Conf {
 // neighbouring n; V: every other key) then lie on different banks.
 template <int D>
 __device__ __forceinline__ int key_at(int r, int n) {
-  if constexpr (D == 256) return 16 * (r >> 1) + (r & 1) + (n & 1 ? (n + 11) - (n > 3 ? 8 : 0) : n);
-  if constexpr (D == 512) return 8 * r + (n >> 1) + (n & 1 ? (n > 3 ? 2 : 6) : 0);
-  if constexpr (D == 128) return r + 4 * (n < 4 ? n : (n ^ 1));
+  const int e = n < 4 ? n : n ^ 1;
+  if constexpr (D == 512) return 8 * r + e;
+  if constexpr (D == 256) return 16 * (r >> 1) + (r & 1) + 2 * e;
+  if constexpr (D == 128) return r + 4 * e;
   return r + 4 * n;
 }
 
@@ -90,6 +91,12 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32
   const __half2 h = __floats2half2_rn(x, y);
   hi = *reinterpret_cast<const uint32_t *>(&h);
   lo = pack2(x - __low2float(h), y - __high2float(h));
+}
+// The bits of x where the mask has ones, of y where it has none.
+__device__ __forceinline__ uint32_t select(uint32_t mask, uint32_t x, uint32_t y) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xca;" : "=r"(r) : "r"(mask), "r"(x), "r"(y));
+  return r;
 }
 template <int W>
 __device__ __forceinline__ void lds(const uint8_t *p, uint32_t (&w)[W]) {
@@ -159,13 +166,19 @@ __device__ __forceinline__ void join_cluster(const Args &a, const float *mine, c
   cluster.sync();  // no CTA's memory goes away while it is read
 }
 
+// The power of two that brings a number whose bits these are to 2^13 .. 2^14, 0 where that has no answer.
+__device__ __forceinline__ int up_of(uint32_t bits) {
+  const int e = (int)(bits >> 23);
+  return e > 0 && e < 255 ? min(max(140 - e, -126), 126) : 0;
+}
+
 template <int D>
 __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_kernel(const Args a) {
   using C = Conf<D>;
   constexpr int PS = C::PS, DW = C::DW, CB = C::CB, NC = C::NC, W = C::W, TEAMS = C::kTeams, S = C::kStages, ROW = C::kRow;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t full[TEAMS][S];
-  __shared__ float unscale[kHeads], upscale[kHeads];
+  __shared__ uint32_t head_top[kHeads];  // the largest |q| of a head (bits)
   __shared__ float2 ml[TEAMS][kHeads], share_ml[kHeads];
   __shared__ int part_slot[TEAMS];  // the slot of a team's part, -1: none
   __shared__ int abort_flag;
@@ -181,6 +194,7 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
     gqd::fence_mbar_init();
     abort_flag = 0;
   }
+  if (tid < kHeads) head_top[tid] = 0;
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
   Cut cut;
@@ -212,7 +226,8 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
   int64_t lw = cut.w0;
   Range lr = range_of<kKeys>(a, cut.keys);
   bool more = true;        // the cursor is on a tile
-  int page = -1, row = 0;  // of this lane's copy; page -1: nothing to load, -2: rows of zeros
+  bool has = false;        // this lane has a copy of it
+  int page = 0, row = 0;   // of this lane's copy
   auto step = [&](int n) {  // n tiles on
     if (lt < 0) {
       lt = 0;
@@ -231,16 +246,13 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
     lt += n;
     lw += n;
     more = lw < cut.w1;
-    page = -1;
+    has = false;
     if (!more) return;
     const int j = (lr.tile0 + lt) * kKeys + (lane << rows_shift);
     if (lane < boxes && j < lr.hi && j + rows > lr.lo) {
       row = ((lu / a.sub) << a.page_shift) + (j & (a.page_size - 1));
-      page = a.table[lb * a.table_stride + (j >> a.page_shift)];
-      if (page < 0 || page >= a.n_pages) {
-        gqd::report(a.err, GQ_DEVERR_PAGES);
-        page = -2;
-      }
+      page = a.table[lb * a.table_stride + (j >> a.page_shift)];  // (not looked at before its copy is due)
+      has = true;
     }
   };
   uint32_t issued = 0;
@@ -249,9 +261,11 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
     const int slot = issued % S;
     uint8_t *to = ring + slot * C::kSlot;
     const uint32_t bytes = (uint32_t)rows * ROW;
-    const int copies = __popc(__ballot_sync(0xffffffffu, page >= 0));
-    const uint32_t bad = __ballot_sync(0xffffffffu, page == -2);
-    if (bad) {
+    const bool good = has && page >= 0 && page < a.n_pages;
+    const int copies = __popc(__ballot_sync(0xffffffffu, good));
+    const uint32_t bad = __ballot_sync(0xffffffffu, has && !good);
+    if (bad) {  // rows of zeros
+      if (lane == 0) gqd::report(a.err, GQ_DEVERR_PAGES);
       for (int i = 0; i < boxes; ++i)
         if (bad >> i & 1)
           for (int at = lane * 4; at < (int)bytes; at += 128) {
@@ -262,7 +276,7 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
     }
     if (lane == 0) gqd::mbar_arrive_expect_tx(&full[team][slot], (uint32_t)copies * 2 * bytes);
     __syncwarp();
-    if (page >= 0) {
+    if (good) {
       const int64_t at = page * a.page_stride + (int64_t)row * ROW;
       gqd::bulk_g2s(to + lane * bytes, static_cast<const uint8_t *>(a.k) + at, bytes, &full[team][slot]);
       gqd::bulk_g2s(to + kKeys * ROW + lane * bytes, static_cast<const uint8_t *>(a.v) + at, bytes, &full[team][slot]);
@@ -270,6 +284,8 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
     ++issued;
     step(TEAMS);
   };
+
+  if (half == 0) step(team);
 
   // ---- compute
   uint32_t n = 0;    // tiles that this team has read
@@ -289,44 +305,48 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
     int head0, nh, kvh;
     unit_heads(a, u, head0, nh, kvh);
 
-    // ---- q: per head scaled to 2^13 .. 2^14, so that the second part stays normal, and cut in two
-    const float *qg = a.q + b * a.q_stride + (int64_t)head0 * D;
-    for (int h = warp; h < kHeads; h += C::kWarps) {
-      float top = 0.0f;
-      if (h < nh)
+    // ---- q: per head scaled to 2^13 .. 2^14, so that the second part stays normal, and cut in two. Asked
+    // for before the first keys, which come later.
+    constexpr int kItems = D / 16 * 32 / C::kThreads;
+    const int ig = (tid >> 2) & 7;  // the head of this thread's items: 4 columns each
+    float4 qv[kItems];
+    {
+      const float *qg = a.q + b * a.q_stride + (int64_t)(head0 + ig) * D + (tid & 3) * (2 * CB);
 #pragma unroll
-        for (int i = 0; i < D; i += 32) top = fmaxf(top, fabsf(qg[h * D + i + lane]));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const int e = (int)((__float_as_uint(top) >> 23) & 255u);
-      const int up = e > 0 && e < 255 ? min(max(140 - e, -126), 126) : 0;
-      if (lane == 0) {
-        upscale[h] = __uint_as_float((uint32_t)(127 + up) << 23);
-        unscale[h] = __uint_as_float((uint32_t)(127 - up) << 23);
+      for (int i = 0; i < kItems; ++i) {
+        const int st = (tid >> 5) + i * C::kWarps, k = st % (DW / 16);
+        qv[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (ig < nh) qv[i] = *reinterpret_cast<const float4 *>(qg + st / (DW / 16) * DW + k / (CB / 2) * (8 * CB) + k % (CB / 2) * 4);
       }
     }
     if (!begun) {
       begun = true;
-      if (half == 0) {
-        step(team);
+      if (half == 0)
         for (int i = 0; i < S; ++i) issue();
-      }
+    }
+    {
+      float top = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kItems; ++i)
+        top = fmaxf(top, fmaxf(fmaxf(fabsf(qv[i].x), fabsf(qv[i].y)), fmaxf(fabsf(qv[i].z), fabsf(qv[i].w))));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      if (q4 == 0) atomicMax(&head_top[ig], __float_as_uint(top));
     }
     __syncthreads();  // (also: everyone is done with the unit before)
-    for (int i = tid; i < D / 16 * 32; i += C::kThreads) {
-      const int st = i >> 5, ig = (i >> 2) & 7, i4 = i & 3;
-      const int hf = st / (DW / 16), k = st % (DW / 16), c = k / (CB / 2), s = k % (CB / 2);
-      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (ig < nh) v = *reinterpret_cast<const float4 *>(qg + ig * D + hf * DW + c * (8 * CB) + i4 * (2 * CB) + 4 * s);
-      const float f = upscale[ig];
-      uint4 x;
-      split_f16(v.x * f, v.y * f, x.x, x.y);
-      split_f16(v.z * f, v.w * f, x.z, x.w);
-      qs[i] = x;
+    {
+      const float f = __uint_as_float((uint32_t)(127 + up_of(head_top[ig])) << 23);
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        uint4 v;
+        split_f16(qv[i].x * f, qv[i].y * f, v.x, v.y);
+        split_f16(qv[i].z * f, qv[i].w * f, v.z, v.w);
+        qs[tid + i * C::kThreads] = v;
+      }
     }
+    const float un = __uint_as_float((uint32_t)(127 - up_of(head_top[g])) << 23) * a.scale;
     __syncthreads();
 
-    const float un = unscale[g];
     float acc[CB][4];
 #pragma unroll
     for (int i = 0; i < CB; ++i)
@@ -392,15 +412,23 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
           x[y][1] += c[y][3];
         }
       }
-      if constexpr (PS > 1) {  // the other warp's columns
-        float4 *put = swap + ((team * 2 + (n & 1)) * 2 + half) * 64 + lane;
-        put[0] = make_float4(x[0][0], x[0][1], x[1][0], x[1][1]);
-        put[32] = make_float4(x[2][0], x[2][1], x[3][0], x[3][1]);
+      if constexpr (PS > 1) {  // the other warps' columns
+        float4 *at = swap + (team * 2 + (n & 1)) * (PS * 64) + lane;
+        at[half * 64] = make_float4(x[0][0], x[0][1], x[1][0], x[1][1]);
+        at[half * 64 + 32] = make_float4(x[2][0], x[2][1], x[3][0], x[3][1]);
         team_sync<PS>(team);  // (the team is done with the tile before, too)
-        const float4 *get = swap + ((team * 2 + (n & 1)) * 2 + (half ^ 1)) * 64 + lane;
-        const float4 o0 = get[0], o1 = get[32];
-        x[0][0] += o0.x, x[0][1] += o0.y, x[1][0] += o0.z, x[1][1] += o0.w;
-        x[2][0] += o1.x, x[2][1] += o1.y, x[3][0] += o1.z, x[3][1] += o1.w;
+        // (in the same order in every warp: their weights are the same)
+#pragma unroll
+        for (int h = 0; h < PS; ++h) {
+          const float4 o0 = at[h * 64], o1 = at[h * 64 + 32];
+          if (h == 0) {
+            x[0][0] = o0.x, x[0][1] = o0.y, x[1][0] = o0.z, x[1][1] = o0.w;
+            x[2][0] = o1.x, x[2][1] = o1.y, x[3][0] = o1.z, x[3][1] = o1.w;
+          } else {
+            x[0][0] += o0.x, x[0][1] += o0.y, x[1][0] += o0.z, x[1][1] += o0.w;
+            x[2][0] += o1.x, x[2][1] += o1.y, x[3][0] += o1.z, x[3][1] += o1.w;
+          }
+        }
         if (mine >= 0 && half == 0) {
           gqd::fence_proxy_async_smem();
           __syncwarp();
@@ -413,17 +441,29 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
       // ---- weights
       const bool ragged = j0 < r.lo || j0 + kKeys > r.hi;
       float top = -INFINITY;
+      if (a.softcap > 0.0f) {
 #pragma unroll
-      for (int y = 0; y < 4; ++y)
+        for (int y = 0; y < 4; ++y)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          x[y][e] = score_of(a, x[y][e] * un);
-          if (ragged) {
+          for (int e = 0; e < 2; ++e) x[y][e] = a.softcap * tanhf(x[y][e] * un * a.inv_softcap);
+      } else {
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) x[y][e] *= un;
+      }
+      if (ragged) {
+        asm volatile("");  // (a branch: most tiles are whole)
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
             const int j = j0 + key_at<D>(y, 2 * q4 + e);
             if (j < r.lo || j >= r.hi) x[y][e] = -INFINITY;
           }
-          top = fmaxf(top, x[y][e]);
-        }
+      }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) top = fmaxf(top, fmaxf(x[y][0], x[y][1]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn, f = exp_of(m - base);
@@ -441,21 +481,26 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
 
       // ---- output: 16 columns by 8 heads per instruction, over 16 keys
       const uint8_t *vt = kt + kKeys * ROW;
-      uint32_t vw[8][W], sp[4][W == 4 ? 2 : 1];
+      uint32_t vw[8][W], sb[8], sp[4][W == 4 ? 2 : 1];
+#pragma unroll
+      for (int y = 0; y < 8; ++y) {
+        const uint8_t *vr = vt + key_at<D>(y >> 1, 2 * q4 + (y & 1)) * ROW;
+        lds<W>(vr + half * (DW / 2) + g * CB, vw[y]);
+        const uint8_t *vs = vr + D / 2 + half * (DW / 16);
+        if constexpr (W == 4) sb[y] = *reinterpret_cast<const uint16_t *>(vs + g * 2);
+        else sb[y] = vs[g * CB / 8];
+      }
+      if (ragged) {
+        asm volatile("");
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const int j = j0 + key_at<D>(y >> 1, 2 * q4 + (y & 1));
+          if (j < r.lo || j >= r.hi) sb[y] = 0;
+        }
+      }
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
-        uint32_t sb[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = key_at<D>(y, 2 * q4 + e);
-          const uint8_t *vr = vt + key * ROW;
-          lds<W>(vr + half * (DW / 2) + g * CB, vw[2 * y + e]);
-          const uint8_t *vs = vr + D / 2 + half * (DW / 16);
-          if constexpr (W == 4) sb[e] = *reinterpret_cast<const uint16_t *>(vs + g * 2);
-          else sb[e] = vs[g * CB / 8];
-          if (ragged && (j0 + key < r.lo || j0 + key >= r.hi)) sb[e] = 0;
-        }
-        const uint32_t pairs = __byte_perm(sb[0], sb[1], 0x5140);
+        const uint32_t pairs = __byte_perm(sb[2 * y], sb[2 * y + 1], 0x5140);
         sp[y][0] = e4m3_pair(pairs);
         if constexpr (W == 4) sp[y][W == 4 ? 1 : 0] = e4m3_pair(pairs >> 16);
       }
@@ -470,8 +515,8 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
             const uint32_t v0 = vw[4 * ks + 2 * y][wd], v1 = vw[4 * ks + 2 * y + 1][wd];
-            e2m1_word((v0 & 0x0f0f0f0fu) | ((v1 << 4) & 0xf0f0f0f0u), ev[y]);
-            e2m1_word(((v0 >> 4) & 0x0f0f0f0fu) | (v1 & 0xf0f0f0f0u), od[y]);
+            e2m1_word(select(0x0f0f0f0fu, v0, v1 << 4), ev[y]);
+            e2m1_word(select(0x0f0f0f0fu, v0 >> 4, v1), od[y]);
             const uint32_t s = sp[2 * ks + y][W == 4 ? wd / 2 : 0];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -564,6 +609,7 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
       if (tid == 0) put_cut_unit(a, cut, b, u, s0, r.nt);
       break;
     }
+    if (tid < kHeads) head_top[tid] = 0;
     __syncthreads();  // the parts are read
     if (mine >= 0 && half == 0) {
       gqd::fence_proxy_async_smem();
