@@ -9,7 +9,9 @@
 // All three options keep a beginning of the order, so what is left is one border: a logit and an id,
 // together a key of 64 bits. It is found without sorting the row: a histogram of counts (top-k) or masses
 // (top-p) says in which of 2048 bins the border lies, and the keys of that bin alone are sorted; where
-// they are too many (equal logits, far outliers) the bin's keys are cut into 2048 bins again.
+// they are too many (equal logits, far outliers) the bin's keys are cut into 2048 bins again. Where
+// few tokens may be enough (a small top_k, a top_p that they reach) each CTA gives its own largest to the
+// first one, which does all of this with some hundreds of keys.
 // Masses are whole numbers, w * 2^44 rounded: their sums (vocab <= 2^19) fit 64 bits and do not depend on
 // the order of additions, so atomics may add them up. The weights are made in f64: with f32's 2^-24 a
 // draw over 262144 tokens would land on a neighbour of the right token every few hundred rows; 2^-45
@@ -36,7 +38,9 @@ constexpr int kLimb = 15;         // bits of a mass that one 32-bit sum takes: a
 constexpr int kMaxShare = 32768;  // columns of a CTA
 constexpr int kTwoPerSm = 16384;  // columns of a CTA that leave room for two on an SM
 constexpr int kList = 2048;       // keys that are sorted
-constexpr int kTable = 128;
+constexpr int kFew = 128;         // keys that are compared with one another in place of that
+constexpr int kGiven = 1024;      // keys that a cluster's CTAs give together where few may be enough
+constexpr int kTable = 16;
 constexpr int64_t kMaxVocab = (int64_t)kMaxShare * kMaxCluster;
 
 struct Args {
@@ -57,19 +61,23 @@ struct Shared {
   union {
     uint32_t limb[3][kBins];  // sums of a mass's bits 0-14, 15-29 and 30-44 (counts: the first)
     uint64_t bin[kBins];      // the same as one number
-    uint64_t list[kList];     // of the first CTA: the keys of the border's bin
+    struct {                  // the keys of the border's bin, and the masses of few
+      uint64_t list[kList];
+      uint64_t mass[kFew];
+    };
   };
-  double table[kTable];           // 2^(j / 128)
+  uint64_t whole[kBins];  // the bins of the whole row, written by every CTA of the cluster
+  uint64_t part[kThreads];
+  double table[kTable];   // 2^(j / 16): 128 bytes, a lane's entry is on banks of its own
   uint64_t warp_sum[kWarps];
-  // written by every CTA of the cluster, in every CTA:
-  uint64_t cta_sum[2][kMaxCluster], low[kMaxCluster], high[kMaxCluster];
+  uint64_t cta_sum[kMaxCluster];  // written by every CTA, as these:
   float top[kMaxCluster], bottom[kMaxCluster];
-  // written by one CTA, in every CTA:
+  uint32_t listed[2];  // of the first CTA: keys in the lists, in this round and the next
+  float from[kMaxCluster];
   uint64_t border, need;
-  uint32_t bin_at;
-  uint32_t listed;  // of the first CTA: keys of the border's bin
+  uint32_t bin_at, count, given, known;
   float warp_top[kWarps], warp_bottom[kWarps];
-  uint64_t warp_low[kWarps], warp_high[kWarps];
+  uint64_t low[kWarps], high[kWarps];
 };
 
 // Order of the logits as an order of numbers (no logit is NaN here, and no zero negative).
@@ -84,29 +92,51 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
 // Of a logit and its id: larger logits first, then smaller ids.
 __device__ __forceinline__ uint64_t rank_key(float v, uint32_t id) { return ((uint64_t)key_of(v) << 32) | (uint32_t)~id; }
 
+// A row's largest logit (a number here), and what a weight is made with.
 struct Row {
-  float top, bins_per_logit;
-  double scale;  // 128 log2(e) / T
+  float top, least;  // from `least` down a mass is 0
+  bool far;          // `least` is -inf: -inf has to be told apart
+  double scale;      // 16 log2(e) / T
 };
+__device__ __forceinline__ Row row_of(float top, float t) {  // t > 0, or 0 for the limit
+  Row row;
+  row.top = top;
+  // the largest number that is 32 T and more below: e^-32 * 2^44 is below 1/2
+  row.least = top - 33.0f * t;
+  if ((double)top - (double)row.least < 32.0 * (double)t || t == 0.0f) row.least = nextafterf(row.least, -INFINITY);
+  row.far = row.least == -INFINITY;
+  const double gap = (double)top - (double)row.least;
+  row.scale = kTable * 1.4426950408889634074 / (double)t;
+  // (where a rounding of `top` is much more than T, nothing lies between the two)
+  if (!row.far && gap > 128.0 * (double)t) row.scale = 48.0 * kTable / gap;
+  if (row.far && t == 0.0f) row.scale = 0.0;
+  return row;
+}
 
-// w * 2^44 to the nearest whole number: 2^(t / 128), t = j + r with |r| <= 1/2, is 2^(j / 128) from a table
-// times a Taylor polynomial (its next term is below 2^-48).
-__device__ __forceinline__ uint64_t mass_of(const Shared &s, const Row &row, float v) {
-  if (v == row.top) return 1ull << kOne;  // (infinities too)
-  const double t = ((double)v - (double)row.top) * row.scale;
-  if (!(t > -128.0 * (kOne + 2))) return 0;  // (-inf; a NaN of two infinities)
+// 2^52 plus w * 2^44 to the nearest whole number: 2^(t / 16), t = j + r with |r| <= 1/2, is 2^(j / 16) from a
+// table times a Taylor polynomial of degree 6 (its next term is below 2^-50). The last addition rounds.
+constexpr double kWhole = 4503599627370496.0;
+__device__ __forceinline__ double rounded_mass(const double *table, const Row &row, float v) {
   constexpr double kRound = 6755399441055744.0;  // 1.5 * 2^52
-  const double shifted = t + kRound;
-  const int j = __double2loint(shifted);
-  const double x = (t - (shifted - kRound)) * (0.69314718055994530942 / 128);
-  double p = fma(x, 1.0 / 24, 1.0 / 6);
-  p = fma(x, p, 0.5);
-  p = fma(x, p, 1.0);
-  p = fma(x, p, 1.0);
-  p *= s.table[j & (kTable - 1)];
-  p = __hiloint2double(__double2hiint(p) + ((j >> 7) + kOne) * (1 << 20), __double2loint(p));
-  const double whole = p + 4503599627370496.0;  // 2^52: the sum's fraction is p rounded
-  return ((uint64_t)(__double2hiint(whole) & 0xfffff) << 32) | (uint32_t)__double2loint(whole);
+  constexpr double c = 0.69314718055994530942 / kTable;
+  const double x = (double)fmaxf(v, row.least) - (double)row.top;
+  const double whole = fma(x, row.scale, kRound);
+  const int j = __double2loint(whole);
+  const double r = fma(x, row.scale, kRound - whole);
+  double p = fma(r, c * c * c * c * c * c / 720, c * c * c * c * c / 120);
+  p = fma(r, p, c * c * c * c / 24);
+  p = fma(r, p, c * c * c / 6);
+  p = fma(r, p, c * c / 2);
+  p = fma(r, p, c);
+  p = fma(r, p, 1.0);
+  p *= table[j & (kTable - 1)];
+  p = __hiloint2double(__double2hiint(p) + ((j >> 4) + kOne) * (1 << 20), __double2loint(p));
+  return p + kWhole;
+}
+__device__ __forceinline__ uint64_t mass_of(const double *table, const Row &row, float v) {
+  const double m = rounded_mass(table, row, v);
+  const uint64_t w = ((uint64_t)(__double2hiint(m) & 0xfffff) << 32) | (uint32_t)__double2loint(m);
+  return row.far && v == -INFINITY ? 0 : w;
 }
 
 __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
@@ -155,185 +185,545 @@ __device__ void sort_down(uint64_t *k, int n) {
   __syncthreads();
 }
 
-// This CTA's columns, four at a time: f(logit, id) in the order of the warp's run, lanes in turn.
-template <typename F>
-__device__ __forceinline__ void each(const Args &a, const float *vals, uint32_t id0, F f) {
-  const int lane = threadIdx.x & 31, c0 = (threadIdx.x >> 5) * a.run + lane * 4;
-  for (int c = 0; c < a.run; c += 128) {
-    const float4 v = *reinterpret_cast<const float4 *>(vals + c0 + c);
-    f(v.x, id0 + c0 + c);
-    f(v.y, id0 + c0 + c + 1);
-    f(v.z, id0 + c0 + c + 2);
-    f(v.w, id0 + c0 + c + 3);
+// Of two logits and ids: whether the first is at or ahead of the second in the order.
+__device__ __forceinline__ bool from_on(float v, uint32_t id, float v0, uint32_t id0) { return v > v0 || (v == v0 && id <= id0); }
+
+// A lane's columns: four from v[0] on, whose first id is `id`, four from v[32] on, ... (n times). The passes
+// over them are functions of their own, so that each has the registers that it needs.
+struct Columns {
+  const float4 *v;
+  int n;
+  uint32_t id;
+};
+
+// Where the border may be, and the bin of a logit there.
+struct Span {
+  float low_v, high_v;  // the last and the first key, as logit and id
+  uint32_t low_id, high_id;
+  uint64_t high;
+  int shift;            // -1: bins by the distance from the largest logit; else by (high - key) >> shift
+  float top, per_logit;
+  // (rounded by the addition; only the order matters, and that equal logits have equal bins)
+  __device__ __forceinline__ uint32_t first_bin(float v) const {
+    return __float_as_uint(fminf((top - v) * per_logit, (float)(kBins - 1)) + 8388608.0f) & (kBins - 1);
   }
+  __device__ __forceinline__ bool has(float v, uint32_t id) const {
+    return from_on(v, id, low_v, low_id) && v > -INFINITY && from_on(high_v, high_id, v, id);
+  }
+  __device__ __forceinline__ uint32_t key_bin(float v, uint32_t id) const { return (uint32_t)((high - rank_key(v, id)) >> shift); }
+};
+
+__device__ __forceinline__ void add_mass(uint32_t (*limb)[kBins], uint32_t b, uint64_t w) {
+  const uint32_t rest = (uint32_t)(w >> kLimb);
+  if (w) atomicAdd(&limb[0][b], (uint32_t)w & ((1u << kLimb) - 1));
+  if (rest & ((1u << kLimb) - 1)) atomicAdd(&limb[1][b], rest & ((1u << kLimb) - 1));
+  if (rest >> kLimb) atomicAdd(&limb[2][b], rest >> kLimb);
+}
+
+// The first round's bins: all numbers (counts), or those from a border on (masses).
+__device__ __noinline__ void count_bins(const Columns c, const Span p, uint32_t *count) {
+#pragma unroll 2
+  for (int i = 0; i < c.n; ++i) {
+    const float4 x = c.v[i * 32];
+    const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (v[k] > -INFINITY) atomicAdd(&count[p.first_bin(v[k])], 1u);
+  }
+}
+__device__ __noinline__ void mass_bins(const Columns c, const Span p, const Row row, const double *table, uint32_t (*limb)[kBins]) {
+#pragma unroll 1
+  for (int i = 0; i < c.n; ++i) {
+    const float4 x = c.v[i * 32];
+    float v[4] = {x.x, x.y, x.z, x.w};
+    const uint32_t id = c.id + i * 128;
+    bool any = false;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (p.low_v > -INFINITY && !from_on(v[k], id + k, p.low_v, p.low_id)) v[k] = -INFINITY;
+      any |= v[k] > row.least;
+    }
+    if (!__any_sync(0xffffffffu, any)) continue;
+    double m[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m[k] = rounded_mass(table, row, v[k]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (v[k] > row.least) add_mass(limb, p.first_bin(v[k]), ((uint64_t)(__double2hiint(m[k]) & 0xfffff) << 32) | (uint32_t)__double2loint(m[k]));
+  }
+}
+// A later round's.
+template <bool MASS>
+__device__ __noinline__ void key_bins(const Columns c, const Span p, const Row row, const double *table, uint32_t (*limb)[kBins]) {
+#pragma unroll 1
+  for (int i = 0; i < c.n; ++i) {
+    const float4 x = c.v[i * 32];
+    const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll 1
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t id = c.id + i * 128 + k;
+      const float l = k == 0 ? v[0] : k == 1 ? v[1] : k == 2 ? v[2] : v[3];
+      if (!p.has(l, id)) continue;
+      if (MASS) add_mass(limb, p.key_bin(l, id), mass_of(table, row, l));
+      else atomicAdd(&limb[0][p.key_bin(l, id)], 1u);
+    }
+  }
+}
+// A bin's keys to the lists of all CTAs (kList at most; the first CTA counts them).
+template <bool FIRST>
+__device__ __noinline__ void collect(const Columns c, const Span p, uint32_t bin, uint64_t *my_list, uint32_t *my_listed) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = (int)cluster.num_blocks(), lane = threadIdx.x & 31;
+  uint32_t *listed = cluster.map_shared_rank(my_listed, 0);
+#pragma unroll 1
+  for (int i = 0; i < c.n; ++i) {
+    const float4 x = c.v[i * 32];
+    const float v[4] = {x.x, x.y, x.z, x.w};
+    const uint32_t id = c.id + i * 128;
+    uint32_t in = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (FIRST) in |= (uint32_t)(p.first_bin(v[k]) == bin) << k;
+      else in |= (uint32_t)(p.has(v[k], id + k) && p.key_bin(v[k], id + k) == bin) << k;
+    }
+    if (!__any_sync(0xffffffffu, in)) continue;
+#pragma unroll 1
+    for (int k = 0; k < 4; ++k) {
+      const float l = k == 0 ? v[0] : k == 1 ? v[1] : k == 2 ? v[2] : v[3];
+      const bool mine = (in >> k & 1) && (!FIRST || (l > -INFINITY && from_on(l, id + k, p.low_v, p.low_id)));
+      const uint32_t who = __ballot_sync(0xffffffffu, mine);
+      if (who == 0) continue;
+      uint32_t at = 0;
+      if (lane == __ffs(who) - 1) at = atomicAdd(listed, (uint32_t)__popc(who));
+      at = __shfl_sync(0xffffffffu, at, __ffs(who) - 1) + __popc(who & ((1u << lane) - 1));
+      if (mine && at < (uint32_t)kList)
+        for (int r = 0; r < ctas; ++r) cluster.map_shared_rank(my_list, r)[at] = rank_key(l, id + k);
+    }
+  }
+}
+
+// The key of the list at which the sum of masses (or the number), from the largest key on, reaches `need`.
+template <bool MASS>
+__device__ __noinline__ uint64_t border_of(Shared &s, int n, const Row row, uint64_t need) {
+  const int tid = threadIdx.x;
+  if (n <= kFew) {
+    // few: thread t adds up what is at or ahead of its key
+    const uint64_t key = tid < n ? s.list[tid] : 0, w = MASS ? mass_of(s.table, row, logit_of(key)) : 1ull;
+    if (tid < n) s.mass[tid] = w;
+    __syncthreads();
+    if (tid < n) {
+      uint64_t run = 0;
+      for (int i = 0; i < n; ++i) run += s.list[i] >= key ? s.mass[i] : 0;
+      if (run >= need && run - w < need) s.border = key;
+    }
+  } else {
+    int n2 = 1;
+    while (n2 < n) n2 <<= 1;
+    for (int i = n + tid; i < n2; i += kThreads) s.list[i] = 0;
+    sort_down(s.list, n2);
+    // thread t has neighbouring keys; the one whose sum reaches what is needed says so
+    const int e = (n2 + kThreads - 1) / kThreads;
+    uint64_t sum = 0;
+    for (int i = 0; i < e; ++i) {
+      const int p = tid * e + i;
+      if (p < n) sum += MASS ? mass_of(s.table, row, logit_of(s.list[p])) : 1ull;
+    }
+    uint64_t whole;
+    uint64_t run = block_scan(sum, s.warp_sum, whole) - sum;
+    if (need > run && need <= run + sum)
+      for (int i = 0; i < e; ++i) {
+        const int p = tid * e + i;
+        run += MASS ? mass_of(s.table, row, logit_of(s.list[p])) : 1ull;
+        if (run >= need) {
+          s.border = s.list[p];
+          break;
+        }
+      }
+  }
+  __syncthreads();
+  return s.border;
+}
+
+// One number for each of this CTA's bins.
+template <bool MASS>
+__device__ __forceinline__ void join_limbs(Shared &s) {
+  uint64_t w[kBins / kThreads];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kBins / kThreads; ++i) {
+    const int b = threadIdx.x + i * kThreads;
+    w[i] = MASS ? s.limb[0][b] + ((uint64_t)s.limb[1][b] << kLimb) + ((uint64_t)s.limb[2][b] << (2 * kLimb)) : s.limb[0][b];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kBins / kThreads; ++i) s.bin[threadIdx.x + i * kThreads] = w[i];
+}
+
+// The bin in which the sum of bins, from the first on, reaches what is needed, and what is needed of it.
+// `wanted(total)` is asked once.
+template <typename F>
+__device__ __forceinline__ void find_bin(Shared &s, const uint64_t *bins, F wanted, uint32_t &bin, uint64_t &need) {
+  constexpr int kEach = kBins / kThreads;
+  uint64_t w[kEach], mine = 0, total;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) mine += w[i] = bins[threadIdx.x * kEach + i];
+  uint64_t at = block_scan(mine, s.warp_sum, total) - mine;
+  need = wanted(total);
+  if (need > at && need <= at + mine)
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (need > at && need <= at + w[i]) {
+        s.bin_at = threadIdx.x * kEach + i;
+        s.need = need - at;
+      }
+      at += w[i];
+    }
+  __syncthreads();
+  bin = s.bin_at;
+  need = s.need;
 }
 
 // The border of the shortest beginning of the order (of the keys from `above` on) whose mass reaches `share`
 // of the whole, or whose number reaches `count`: the key of its last member.
 template <bool MASS>
-__device__ uint64_t find_border(cg::cluster_group &cluster, Shared &s, const Args &a, const Row &row, const float *vals, uint32_t id0,
-                                uint64_t above, double share, uint64_t count) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+__device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, const Row row, float per_logit, uint64_t above, double share,
+                                             uint64_t count, int &round) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x;
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  uint64_t low = above, high = ~0ull, need = count;
-  int shift = -1;  // -1: bins by the distance from the largest logit; else by (key - low) >> shift, the largest first
-  for (;;) {
+  uint64_t need = count;
+  Span span;
+  span.low_v = above ? logit_of(above) : -INFINITY;
+  span.low_id = ~(uint32_t)above;
+  span.high_v = INFINITY;
+  span.high_id = 0;
+  span.high = ~0ull;
+  span.shift = -1;
+  span.top = row.top;
+  span.per_logit = per_logit;
+  for (;; ++round) {
+    __syncthreads();  // (what was in the bins' place is read)
     for (int i = tid; i < kBins * (MASS ? 3 : 1); i += kThreads) (&s.limb[0][0])[i] = 0;
-    if (tid == 0) s.listed = 0;
     __syncthreads();
-    auto bin_of = [&](float v, uint64_t key) -> uint32_t {
-      if (shift < 0) {
-        const float d = (row.top - v) * row.bins_per_logit;  // (NaN: two infinities)
-        return d > 0.0f ? (uint32_t)fminf(d, (float)(kBins - 1)) : 0u;
-      }
-      return (uint32_t)((high - key) >> shift);
-    };
-    each(a, vals, id0, [&](float v, uint32_t id) {
-      const uint64_t key = rank_key(v, id);
-      if (key < low || key > high || v == -INFINITY) return;
-      const uint32_t b = bin_of(v, key);
-      if constexpr (MASS) {
-        const uint64_t w = mass_of(s, row, v);
-        if (w == 0) return;
-        atomicAdd(&s.limb[0][b], (uint32_t)w & ((1u << kLimb) - 1));
-        const uint32_t rest = (uint32_t)(w >> kLimb);
-        if (rest & ((1u << kLimb) - 1)) atomicAdd(&s.limb[1][b], rest & ((1u << kLimb) - 1));
-        if (rest >> kLimb) atomicAdd(&s.limb[2][b], rest >> kLimb);
-      } else {
-        atomicAdd(&s.limb[0][b], 1u);
-      }
-    });
-    __syncthreads();
-    {  // one number for each bin
-      uint64_t w[kBins / kThreads];
+    if (span.shift >= 0) key_bins<MASS>(columns, span, row, s.table, s.limb);
+    else if (MASS) mass_bins(columns, span, row, s.table, s.limb);
+    else count_bins(columns, span, s.limb[0]);
+    join_limbs<MASS>(s);
+    cluster.sync();
+    // every CTA adds up a share of the bins and gives it to all: `parts` threads a bin, some CTAs each
+    {
+      const int per = kBins / ctas, parts = max(1, kThreads / per), each = ctas / min(parts, ctas);
+      const int b0 = tid % min(per, kThreads), part = tid / min(per, kThreads);
+      for (int b = b0; b < per; b += kThreads) {
+        uint64_t x[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < kBins / kThreads; ++i) {
-        const int b = tid + i * kThreads;
-        w[i] = MASS ? s.limb[0][b] + ((uint64_t)s.limb[1][b] << kLimb) + ((uint64_t)s.limb[2][b] << (2 * kLimb)) : s.limb[0][b];
+        for (int r = 0; r < 4; ++r)
+          if (r < each && part * each + r < ctas) x[r] = cluster.map_shared_rank(s.bin, part * each + r)[rank * per + b];
+        uint64_t sum = (x[0] + x[1]) + (x[2] + x[3]);
+        if (parts > 1) {
+          s.part[tid] = sum;
+          __syncthreads();
+          sum = 0;
+          for (int i = 0; i < parts; ++i) sum += s.part[i * per + b];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (r < each && part * each + r < ctas) cluster.map_shared_rank(s.whole, part * each + r)[rank * per + b] = sum;
+      }
+    }
+    cluster.sync();
+    uint32_t bin;
+    const bool first = span.shift < 0;
+    find_bin(s, s.whole, [&](uint64_t all) -> uint64_t {
+      if (MASS && first) {
+        const double x = ceil(share * (double)all);
+        return min(x >= 1.0 ? (uint64_t)x : (uint64_t)1, all);
+      }
+      return min(need, all);
+    }, bin, need);
+    if (rank == 0 && tid == 0) s.listed[(round + 1) & 1] = 0;
+    if (first) collect<true>(columns, span, bin, s.list, &s.listed[round & 1]);
+    else collect<false>(columns, span, bin, s.list, &s.listed[round & 1]);
+    cluster.sync();
+    const uint32_t n = *cluster.map_shared_rank(&s.listed[round & 1], 0);
+    if (n <= (uint32_t)kList) {
+      const uint64_t border = border_of<MASS>(s, (int)n, row, need);
+      ++round;
+      return border;
+    }
+    // too many: their range, from the few that are listed and the bin's own
+    if (first) {
+      // the smallest and the largest key whose bin it is
+      uint64_t lo = ~0ull, hi = 0;
+      for (int i = 0; i < columns.n; ++i) {
+        const float4 x = columns.v[i * 32];
+        const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t id = columns.id + i * 128 + k;
+          if (span.first_bin(v[k]) != bin || !span.has(v[k], id)) continue;
+          lo = min(lo, rank_key(v[k], id));
+          hi = max(hi, rank_key(v[k], id));
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+      }
+      if ((tid & 31) == 0) {
+        s.low[tid >> 5] = lo;
+        s.high[tid >> 5] = hi;
       }
       __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kBins / kThreads; ++i) s.bin[tid + i * kThreads] = w[i];
-    }
-    cluster.sync();
-    // every CTA adds up a share of the bins: thread t has one of them, or none
-    const int per = (kBins + ctas - 1) / ctas;  // (a power of two: 128 to 2048)
-    uint64_t w[kBins / kThreads];
-    uint64_t mine = 0;
-    const int each_bins = (per + kThreads - 1) / kThreads;
-#pragma unroll
-    for (int i = 0; i < kBins / kThreads; ++i) {
-      w[i] = 0;
-      const int in = tid * each_bins + i;
-      if (i < each_bins && in < per)
-        for (int r = 0; r < ctas; ++r) w[i] += cluster.map_shared_rank(s.bin, r)[rank * per + in];
-      mine += w[i];
-    }
-    uint64_t total;
-    uint64_t incl = block_scan(mine, s.warp_sum, total);
-    if (tid < ctas) cluster.map_shared_rank(s.cta_sum[0], tid)[rank] = total;
-    cluster.sync();
-    uint64_t before = 0, all = 0;
-    for (int r = 0; r < ctas; ++r) {
-      if (r < rank) before += s.cta_sum[0][r];
-      all += s.cta_sum[0][r];
-    }
-    if (shift < 0) {
-      if constexpr (MASS) {
-        const double x = ceil(share * (double)all);
-        need = x >= 1.0 ? (uint64_t)x : 1ull;
-      }
-      need = min(need, all);
-    }
-    uint64_t at = before + incl - mine;
-#pragma unroll
-    for (int i = 0; i < kBins / kThreads; ++i) {
-      if (need > at && need <= at + w[i]) {
-        for (int r = 0; r < ctas; ++r) {
-          *cluster.map_shared_rank(&s.bin_at, r) = (uint32_t)(rank * per + tid * each_bins + i);
-          *cluster.map_shared_rank(&s.need, r) = need - at;
-        }
-      }
-      at += w[i];
-    }
-    cluster.sync();
-    const uint32_t bin = s.bin_at;
-    need = s.need;
-    // the bin's keys to the first CTA, and the smallest and largest of them
-    uint64_t lo = ~0ull, hi = 0;
-    uint64_t *list = cluster.map_shared_rank(s.list, 0);
-    uint32_t *listed = cluster.map_shared_rank(&s.listed, 0);
-    each(a, vals, id0, [&](float v, uint32_t id) {
-      const uint64_t key = rank_key(v, id);
-      const bool in = key >= low && key <= high && v != -INFINITY && bin_of(v, key) == bin;
-      const uint32_t who = __ballot_sync(0xffffffffu, in);
-      if (who == 0) return;
-      uint32_t i = 0;
-      if (lane == __ffs(who) - 1) i = atomicAdd(listed, (uint32_t)__popc(who));
-      i = __shfl_sync(0xffffffffu, i, __ffs(who) - 1) + __popc(who & ((1u << lane) - 1));
-      if (in) {
-        lo = min(lo, key);
-        hi = max(hi, key);
-        if (i < (uint32_t)kList) list[i] = key;
-      }
-    });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    if (lane == 0) {
-      s.warp_low[warp] = lo;
-      s.warp_high[warp] = hi;
-    }
-    __syncthreads();
-    if (tid < ctas) {
       for (int i = 0; i < kWarps; ++i) {
-        lo = min(lo, s.warp_low[i]);
-        hi = max(hi, s.warp_high[i]);
+        lo = min(lo, s.low[i]);
+        hi = max(hi, s.high[i]);
       }
-      cluster.map_shared_rank(s.low, tid)[rank] = lo;
-      cluster.map_shared_rank(s.high, tid)[rank] = hi;
-    }
-    cluster.sync();
-    const uint32_t n = *listed;
-    if (n <= (uint32_t)kList) {
-      if (rank == 0) {
-        int n2 = 1;
-        while (n2 < (int)n) n2 <<= 1;
-        for (int i = n + tid; i < n2; i += kThreads) s.list[i] = 0;
-        sort_down(s.list, n2);
-        // thread t has neighbouring keys; the one whose sum reaches what is needed says so
-        const int e = (n2 + kThreads - 1) / kThreads;
-        uint64_t sum = 0;
-        for (int i = 0; i < e; ++i) {
-          const int p = tid * e + i;
-          if (p < (int)n) sum += MASS ? mass_of(s, row, logit_of(s.list[p])) : 1ull;
-        }
-        uint64_t whole;
-        uint64_t run = block_scan(sum, s.warp_sum, whole) - sum;
-        if (need > run && need <= run + sum)
-          for (int i = 0; i < e; ++i) {
-            const int p = tid * e + i;
-            run += MASS ? mass_of(s, row, logit_of(s.list[p])) : 1ull;
-            if (run >= need) {
-              for (int r = 0; r < ctas; ++r) *cluster.map_shared_rank(&s.border, r) = s.list[p];
-              break;
-            }
-          }
+      if (tid < ctas) {
+        cluster.map_shared_rank(s.whole, tid)[2 * rank] = lo;
+        cluster.map_shared_rank(s.whole, tid)[2 * rank + 1] = hi;
       }
       cluster.sync();
-      return s.border;
+      for (int r = 0; r < ctas; ++r) {
+        lo = min(lo, s.whole[2 * r]);
+        hi = max(hi, s.whole[2 * r + 1]);
+      }
+      span.high = hi;
+      span.low_v = logit_of(lo);
+      span.low_id = ~(uint32_t)lo;
+      span.shift = max(0, 64 - __clzll((long long)(hi - lo)) - 11);
+      cluster.sync();  // (before the bins of the next round are written there)
+    } else {
+      // the bin's own range of keys
+      span.high -= (uint64_t)bin << span.shift;
+      const uint64_t lo = span.high - ((1ull << span.shift) - 1);
+      if (lo > rank_key(span.low_v, span.low_id)) {
+        span.low_v = logit_of(lo);
+        span.low_id = ~(uint32_t)lo;
+      }
+      span.shift = max(0, span.shift - 11);
     }
-    for (int r = 0; r < ctas; ++r) {
-      lo = min(lo, s.low[r]);
-      hi = max(hi, s.high[r]);
-    }
-    cluster.sync();  // everyone has read what the next round writes
-    low = lo;
-    high = hi;
-    shift = max(0, 64 - __clzll((long long)(hi - lo)) - 11);
+    span.high_v = logit_of(span.high);
+    span.high_id = ~(uint32_t)span.high;
   }
+}
+
+// What the options leave: logits from a border on (LIMIT: of a mass of `least` and up). A lane's four
+// masses, as 2^52 plus each; false where the whole warp has none.
+struct Kept {
+  float v;
+  uint32_t id;
+  double least;
+  template <bool BORDER, bool LIMIT>
+  __device__ __forceinline__ bool masses(const float4 x, uint32_t at, const Row &row, const double *table, double (&m)[4]) const {
+    float l[4] = {x.x, x.y, x.z, x.w};
+    if (BORDER) {
+      bool any = false;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (!from_on(l[k], at + k, v, id)) l[k] = -INFINITY;
+        any |= l[k] > -INFINITY;
+      }
+      if (!__any_sync(0xffffffffu, any)) return false;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m[k] = rounded_mass(table, row, l[k]);
+    if (LIMIT)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m[k] = m[k] >= least ? m[k] : kWhole;
+    if (row.far)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m[k] = l[k] > -INFINITY ? m[k] : kWhole;
+    return true;
+  }
+};
+template <bool BORDER, bool LIMIT>
+__device__ __noinline__ uint64_t sum_kept(const Columns c, const Kept kept, const Row row, const double *table) {
+  double sum = 0.0;  // (64 multiples of 1 up to 2^44 at most: exact)
+#pragma unroll 1
+  for (int i = 0; i < c.n; ++i) {
+    double m[4];
+    if (kept.masses<BORDER, LIMIT>(c.v[i * 32], c.id + i * 128, row, table, m))
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum += m[k] - kWhole;
+  }
+  return (uint64_t)sum;
+}
+
+// find_border over a list of keys in this CTA alone: `need` of their masses or number, from `low` on.
+template <bool MASS>
+__device__ __noinline__ uint64_t list_border(Shared &s, const uint64_t *keys, int n, const Row row, float per_logit, uint64_t low, uint64_t need) {
+  Span span;
+  span.top = row.top;
+  span.per_logit = per_logit;
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins * (MASS ? 3 : 1); i += kThreads) (&s.limb[0][0])[i] = 0;
+  if (threadIdx.x == 0) s.count = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    if (keys[i] < low) continue;
+    const float v = logit_of(keys[i]);
+    if (MASS) add_mass(s.limb, span.first_bin(v), mass_of(s.table, row, v));
+    else atomicAdd(&s.limb[0][span.first_bin(v)], 1u);
+  }
+  join_limbs<MASS>(s);
+  __syncthreads();
+  uint32_t bin;
+  find_bin(s, s.bin, [&](uint64_t) { return need; }, bin, need);
+  for (int i = threadIdx.x; i < n; i += kThreads)
+    if (keys[i] >= low && span.first_bin(logit_of(keys[i])) == bin) s.list[atomicAdd(&s.count, 1u)] = keys[i];
+  __syncthreads();
+  return border_of<MASS>(s, (int)s.count, row, need);
+}
+
+__device__ __forceinline__ uint64_t block_sum(Shared &s, uint64_t v) {
+  uint64_t total;
+  block_scan(v, s.warp_sum, total);
+  return total;
+}
+
+// The token of a list of keys, from `border` on and of masses of `least` and up: the first id at which the
+// running sum passes u times the whole.
+__device__ __noinline__ void draw_from(Shared &s, const Args &a, int64_t r, const uint64_t *keys, int n, const Row row, uint64_t border,
+                                       uint64_t least, double u) {
+  const int tid = threadIdx.x;
+  auto mass = [&](uint64_t key) -> uint64_t {
+    const uint64_t w = key >= border ? mass_of(s.table, row, logit_of(key)) : 0;
+    return w >= least ? w : 0;
+  };
+  auto bin_of = [&](uint64_t key) { return (uint32_t)~key * (uint32_t)kBins / (uint32_t)a.vocab; };  // (ids below 2^19)
+  for (int i = tid; i < kBins * 3; i += kThreads) (&s.limb[0][0])[i] = 0;
+  if (tid == 0) s.count = 0;
+  __syncthreads();
+  uint64_t mine = 0;
+  for (int i = tid; i < n; i += kThreads) {
+    const uint64_t w = mass(keys[i]);
+    if (w) add_mass(s.limb, bin_of(keys[i]), w);
+    mine += w;
+  }
+  const uint64_t total = block_sum(s, mine);
+  join_limbs<true>(s);
+  __syncthreads();
+  uint32_t bin;
+  uint64_t need;
+  find_bin(s, s.bin, [&](uint64_t) { return min((uint64_t)(u * (double)total), total - 1) + 1; }, bin, need);
+  for (int i = tid; i < n; i += kThreads)
+    if (mass(keys[i]) && bin_of(keys[i]) == bin) s.list[atomicAdd(&s.count, 1u)] = keys[i];
+  __syncthreads();
+  const int few = (int)s.count;
+  for (int i = tid; i < few; i += kThreads) {
+    const uint32_t id = ~(uint32_t)s.list[i];
+    const uint64_t w = mass(s.list[i]);
+    uint64_t run = 0;
+    for (int j = 0; j < few; ++j)
+      if (~(uint32_t)s.list[j] < id) run += mass(s.list[j]);
+    if (need > run && need <= run + w) {
+      a.tokens[r] = (int32_t)id;
+      if (a.probs) a.probs[r] = (float)((double)w / (double)total);
+    }
+  }
+}
+
+// Rows whose options leave few tokens: each CTA gives the first one its largest, those from its q-th largest
+// lane's largest on, and the first one finds the border among them and draws. False where that is not known to
+// be right (too many; a border below what all CTAs have given). `all`: this CTA's sum of masses (top-p alone).
+__device__ __noinline__ bool from_few(Shared &s, const Args &a, const Columns columns, const Row row, int64_t r, int k, float p, uint64_t least,
+                                      double u, float lane_top, float my_top, float my_bottom, uint64_t all) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ctas = (int)cluster.num_blocks();
+  const int most = min(kGiven / ctas, kThreads / 2), q = k > 0 ? min(k, most) : most;
+  const bool sure = k > 0 && k <= most;  // the row's k largest are among each CTA's k largest
+  for (int i = tid; i < kBins; i += kThreads) s.limb[0][i] = 0;
+  if (tid == 0) s.count = 0;
+  __syncthreads();
+  Span span;
+  span.top = my_top;
+  span.per_logit = (float)(kBins - 1) / (my_top - my_bottom);
+  const bool some = lane_top > -INFINITY;
+  if (some) atomicAdd(&s.limb[0][span.first_bin(lane_top)], 1u);
+  join_limbs<false>(s);
+  __syncthreads();
+  uint32_t bin;
+  uint64_t need, lanes = 0;
+  find_bin(s, s.bin, [&](uint64_t n) -> uint64_t { return lanes = n, min((uint64_t)q, n); }, bin, need);
+  float from = some && span.first_bin(lane_top) <= bin ? lane_top : INFINITY;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) from = fminf(from, __shfl_xor_sync(0xffffffffu, from, o));
+  if (lane == 0) s.warp_bottom[warp] = from;
+  __syncthreads();
+  for (int i = 0; i < kWarps; ++i) from = fminf(from, s.warp_bottom[i]);
+  if (lanes < (uint64_t)q) from = -INFINITY;  // (all that there are)
+  // its keys, in the bins' place
+  for (int i = 0; i < columns.n; ++i) {
+    const float4 x = columns.v[i * 32];
+    const float v[4] = {x.x, x.y, x.z, x.w};
+    if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) < from) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (v[j] >= from && v[j] > -INFINITY) {
+        const uint32_t at = atomicAdd(&s.count, 1u);
+        if (at < (uint32_t)kList) s.list[at] = rank_key(v[j], columns.id + i * 128 + j);
+      }
+  }
+  __syncthreads();
+  const uint32_t n_mine = s.count;
+  if (tid == 0) {
+    s.bin_at = atomicAdd(cluster.map_shared_rank(&s.given, 0), n_mine);
+    cluster.map_shared_rank(s.cta_sum, 0)[cluster.block_rank()] = all;
+    cluster.map_shared_rank(s.from, 0)[cluster.block_rank()] = from;
+  }
+  __syncthreads();
+  uint64_t *keys = s.whole;
+  for (uint32_t i = tid; i < n_mine && s.bin_at + i < (uint32_t)kList; i += kThreads) cluster.map_shared_rank(keys, 0)[s.bin_at + i] = s.list[i];
+  cluster.sync();
+  const uint32_t n = *cluster.map_shared_rank(&s.given, 0);
+  cluster.sync();  // (nobody leaves, or goes on with the bins, before the number is read)
+  if (n > (uint32_t)kList) return false;
+  const bool first = cluster.block_rank() == 0;
+  bool known = true;
+  uint64_t border = 0;
+  if (first) {
+    float complete = -INFINITY, least_v = INFINITY;  // from `complete` on the list has all
+    for (int i = 0; i < ctas; ++i) {
+      complete = fmaxf(complete, s.from[i]);
+      least_v = fminf(least_v, s.from[i]);
+    }
+    const float span_v = row.top - (least_v > -INFINITY ? least_v : my_bottom);
+    const uint64_t end = (uint64_t)key_of(complete) << 32;
+    if (k > 0) {
+      uint64_t have = 0;
+      for (int i = tid; i < (int)n; i += kThreads) have += sure || keys[i] >= end;
+      have = block_sum(s, have);
+      if (have < (uint64_t)k && !sure) known = false;
+      else border = list_border<false>(s, keys, (int)n, row, (float)(kBins - 1) / span_v, 0, min((uint64_t)k, have));
+    }
+    if (known && p < 1.0f) {
+      uint64_t mass = 0;
+      for (int i = tid; i < (int)n; i += kThreads)
+        if (keys[i] >= (k > 0 ? border : end)) mass += mass_of(s.table, row, logit_of(keys[i]));
+      mass = block_sum(s, mass);
+      uint64_t whole = mass;
+      if (k <= 0) {
+        whole = 0;
+        for (int i = 0; i < ctas; ++i) whole += s.cta_sum[i];
+      }
+      const double x = ceil(fmax((double)p, 0.0) * (double)whole);
+      const uint64_t want = min(x >= 1.0 ? (uint64_t)x : (uint64_t)1, whole);
+      if (mass < want) known = false;
+      else border = list_border<true>(s, keys, (int)n, row, (float)(kBins - 1) / span_v, border, want);
+    }
+  }
+  if (!sure) {
+    if (first && tid < ctas) *cluster.map_shared_rank(&s.known, tid) = known;
+    cluster.sync();
+    known = s.known;
+  }
+  if (first && known) {
+    __syncthreads();
+    draw_from(s, a, r, keys, (int)n, row, border, least, u);
+  }
+  return known;
 }
 
 __device__ __forceinline__ double next_f64(uint64_t z) {  // of the advanced state
@@ -352,6 +742,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
   const int64_t r = blockIdx.x / ctas;
   if (tid < kTable) s.table[tid] = exp2((double)tid / kTable);
+  if (tid < 2) s.listed[tid] = 0;
+  if (tid == 2) s.given = 0;
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
   const float t = a.temperature ? a.temperature[r] : 1.0f;
@@ -362,15 +754,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args
   const double given = a.uniforms ? a.uniforms[r] : 0.0;
   const uint32_t id0 = (uint32_t)rank * a.share;
   const int n = min(max(a.vocab - (int)id0, 0), a.share);
-  float top = -INFINITY, bottom = INFINITY;  // of the numbers
+  float top = -INFINITY, bottom = INFINITY;  // of the numbers (the smallest of one in four: it only scales bins)
   {
     const float *from = a.logits + r * a.ld + id0;
-    auto take = [&](float v) {
-      v = v != v ? -INFINITY : v + 0.0f;  // (a NaN is never drawn; -0 counts as 0)
-      top = fmaxf(top, v);
-      if (v > -INFINITY) bottom = fminf(bottom, v);
-      return v;
-    };
+    auto take = [](float v) { return fmaxf(v, -INFINITY) + 0.0f; };  // (a NaN is never drawn: -inf; -0 counts as 0)
+#pragma unroll 4
     for (int c = warp * a.run + lane * 4; c < (warp + 1) * a.run; c += 128) {
       float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
       if (a.wide && c + 3 < n) {
@@ -381,9 +769,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args
         if (c + 2 < n) v.z = from[c + 2];
         if (c + 3 < n) v.w = from[c + 3];
       }
-      *reinterpret_cast<float4 *>(vals + c) = make_float4(take(v.x), take(v.y), take(v.z), take(v.w));
+      v = make_float4(take(v.x), take(v.y), take(v.z), take(v.w));
+      top = fmaxf(top, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+      if (v.x > -INFINITY) bottom = fminf(bottom, v.x);
+      *reinterpret_cast<float4 *>(vals + c) = v;
     }
   }
+  float lane_top = top;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -394,92 +786,107 @@ __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args
     s.warp_bottom[warp] = bottom;
   }
   __syncthreads();
+  for (int i = 0; i < kWarps; ++i) {
+    top = fmaxf(top, s.warp_top[i]);
+    bottom = fminf(bottom, s.warp_bottom[i]);
+  }
+  float my_top = top;
+  const float my_bottom = fminf(bottom, top);
   if (tid < ctas) {
-    for (int i = 0; i < kWarps; ++i) {
-      top = fmaxf(top, s.warp_top[i]);
-      bottom = fminf(bottom, s.warp_bottom[i]);
-    }
     cluster.map_shared_rank(s.top, tid)[rank] = top;
-    cluster.map_shared_rank(s.bottom, tid)[rank] = bottom;
+    cluster.map_shared_rank(s.bottom, tid)[rank] = my_bottom;
   }
   cluster.sync();
   for (int i = 0; i < ctas; ++i) {
     top = fmaxf(top, s.top[i]);
-    bottom = fminf(bottom, s.bottom[i]);
+    if (s.top[i] > -INFINITY) bottom = fminf(bottom, s.bottom[i]);
   }
+  if (top == INFINITY) {  // only infinities are drawn: they become 0, the others -inf
+    for (int c = tid; c < kWarps * a.run; c += kThreads) vals[c] = vals[c] == INFINITY ? 0.0f : -INFINITY;
+    my_top = my_top == INFINITY ? 0.0f : -INFINITY;
+    lane_top = lane_top == INFINITY ? 0.0f : -INFINITY;
+    top = bottom = 0.0f;
+    __syncthreads();
+  }
+  const Columns columns{reinterpret_cast<const float4 *>(vals) + warp * (a.run / 4) + lane, a.run / 128, id0 + warp * a.run + lane * 4};
   const bool greedy = !(t > 0.0f);
-  Row row;
-  row.top = top;
-  row.scale = greedy ? 0.0 : kTable * 1.4426950408889634074 / (double)t;
-  uint64_t above = 0, least = 1;
-  double u = 0.0;
-  if (greedy) {
-    above = (uint64_t)key_of(top) << 32;  // all that are as large as the largest: the first is drawn, with u = 0
-  } else {
+  // (greedy: the limit of small temperatures, in which all that are as large as the largest are left; the
+  // first is drawn, with u = 0)
+  const Row row = row_of(top, greedy ? 0.0f : t);
+  uint64_t above = 0;
+  double u = 0.0, least = kWhole + 1.0;
+  if (!greedy) {
     if (a.rng) {
       state += kStep;
       u = next_f64(state);
+      if (rank == 0 && tid == 0) a.rng[r] = state;  // (every CTA has read it: it has met the others)
     } else {
       u = given;
     }
     u = u >= 0.0 ? fmin(u, 1.0 - 0x1p-53) : 0.0;
+    if (low_p > 0.0f) least = fmax(least, kWhole + ceil(fmin((double)low_p, 1.0) * (double)(1ull << kOne)));
     if (top > -INFINITY) {
+      int round = 0;
+      const bool some = k > 0 && k < a.vocab;
+      if (some || p < 1.0f) {
+        const uint64_t all = some ? 0 : block_sum(s, sum_kept<false, false>(columns, Kept{}, row, s.table));
+        if (from_few(s, a, columns, row, r, some ? k : 0, p, (uint64_t)(least - kWhole), u, lane_top, my_top, my_bottom, all)) return;
+      }
       // bins over the row's numbers, for masses over those that have any
       const float span = top - bottom, heavy = 32.0f * t;
-      row.bins_per_logit = (float)(kBins - 1) / span;
-      if (k > 0 && k < a.vocab) above = find_border<false>(cluster, s, a, row, vals, id0, 0, 0.0, (uint64_t)k);
-      row.bins_per_logit = (float)(kBins - 1) / fminf(span, heavy);
-      if (p < 1.0f) above = find_border<true>(cluster, s, a, row, vals, id0, above, fmax((double)p, 0.0), 0);
+      if (some) above = find_border<false>(s, columns, row, (float)(kBins - 1) / span, 0, 0.0, (uint64_t)k, round);
+      if (p < 1.0f)
+        above = find_border<true>(s, columns, row, (float)(kBins - 1) / fminf(span, heavy), above, fmax((double)p, 0.0), 0, round);
     }
-    if (low_p > 0.0f) least = max(least, (uint64_t)ceil(fmin((double)low_p, 1.0) * (double)(1ull << kOne)));
   }
-  auto kept = [&](float v, uint32_t id) -> uint64_t {
-    if (v == -INFINITY || rank_key(v, id) < above) return 0;
-    const uint64_t w = mass_of(s, row, v);
-    return w >= least ? w : 0;
-  };
+  const Kept kept{logit_of(above), ~(uint32_t)above, least};
   uint64_t sum = 0;
-  each(a, vals, id0, [&](float v, uint32_t id) { sum += kept(v, id); });
+  if (top > -INFINITY) {
+    if (above) sum = sum_kept<true, true>(columns, kept, row, s.table);
+    else if (low_p > 0.0f) sum = sum_kept<false, true>(columns, kept, row, s.table);
+    else sum = sum_kept<false, false>(columns, kept, row, s.table);
+  }
   sum = warp_sum(sum);
   if (lane == 0) s.warp_sum[warp] = sum;
   __syncthreads();
   if (tid < ctas) {
     uint64_t whole = 0;
     for (int i = 0; i < kWarps; ++i) whole += s.warp_sum[i];
-    cluster.map_shared_rank(s.cta_sum[1], tid)[rank] = whole;
+    cluster.map_shared_rank(s.cta_sum, tid)[rank] = whole;
   }
   cluster.sync();
   uint64_t total = 0, before = 0;
   for (int i = 0; i < ctas; ++i) {
-    total += s.cta_sum[1][i];
-    if (i < rank) before += s.cta_sum[1][i];
+    total += s.cta_sum[i];
+    if (i < rank) before += s.cta_sum[i];
   }
-  if (rank == 0 && tid == 0) {
-    if (a.rng && !greedy) a.rng[r] = state;
-    if (total == 0) {  // nothing that can be drawn
-      a.tokens[r] = -1;
-      if (a.probs) a.probs[r] = 0.0f;
-    }
+  if (rank == 0 && tid == 0 && total == 0) {  // nothing that can be drawn
+    a.tokens[r] = -1;
+    if (a.probs) a.probs[r] = 0.0f;
   }
   uint64_t at = (uint64_t)(u * (double)total);
   if (total > 0) at = min(at, total - 1);
   for (int i = 0; i < warp; ++i) before += s.warp_sum[i];
   if (at < before || at >= before + s.warp_sum[warp]) return;
   // the warp in whose run the sum passes `at`
-  for (int c = warp * a.run + lane * 4; c < (warp + 1) * a.run; c += 128) {
-    const float4 v = *reinterpret_cast<const float4 *>(vals + c);
-    const uint64_t w[4] = {kept(v.x, id0 + c), kept(v.y, id0 + c + 1), kept(v.z, id0 + c + 2), kept(v.w, id0 + c + 3)};
-    const uint64_t four = w[0] + w[1] + w[2] + w[3];
+  for (int i = 0; i < columns.n; ++i) {
+    double m[4];
+    uint64_t w[4] = {0, 0, 0, 0};
+    const uint32_t at_id = columns.id + i * 128;
+    if (above ? !kept.masses<true, true>(columns.v[i * 32], at_id, row, s.table, m) : !kept.masses<false, true>(columns.v[i * 32], at_id, row, s.table, m))
+      continue;
+    for (int k = 0; k < 4; ++k) w[k] = (uint64_t)(m[k] - kWhole);
+    const uint64_t four = (w[0] + w[1]) + (w[2] + w[3]);
     const uint64_t incl = warp_scan(four) + before;
     const uint32_t past = __ballot_sync(0xffffffffu, incl > at);
     if (past) {
       if (lane == __ffs(past) - 1) {
         uint64_t run = incl - four;
-        for (int i = 0; i < 4; ++i) {
-          run += w[i];
+        for (int k = 0; k < 4; ++k) {
+          run += w[k];
           if (run > at) {
-            a.tokens[r] = (int32_t)(id0 + c + i);
-            if (a.probs) a.probs[r] = greedy ? 1.0f : (float)((double)w[i] / (double)total);
+            a.tokens[r] = (int32_t)(columns.id + i * 128 + k);
+            if (a.probs) a.probs[r] = greedy ? 1.0f : (float)((double)w[k] / (double)total);
             break;
           }
         }
