@@ -189,6 +189,7 @@ int gq_ctx_destroy(gq_ctx *ctx) {
     if (ctx->scratch[i]) cudaFree(ctx->scratch[i]);
   if (ctx->ws) cudaFree(ctx->ws);
   if (ctx->paged_ws) cudaFree(ctx->paged_ws);
+  if (ctx->sample_ws) cudaFree(ctx->sample_ws);
   if (ctx->counters) cudaFree(ctx->counters);
   if (ctx->dev_err) cudaFree(ctx->dev_err);
   if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);

@@ -55,6 +55,7 @@ struct gq_ctx {
   // zero between launches, the last CTA to arrive at one puts it back to zero
   uint32_t *counters = nullptr;
   void *paged_ws = nullptr;  // parts of gq_paged_attention: made by its first call, never moved
+  void *sample_ws = nullptr; // what the launches of gq_sample_requests tell one another: likewise
   // set by gq_linear_softcap_peers(_signal) for the duration of one call
   PeerDst peers = {};
   PeerDst peer_signal = {};

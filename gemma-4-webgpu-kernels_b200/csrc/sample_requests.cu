@@ -39,9 +39,13 @@ constexpr int kMaxShare = 32768;  // columns of a CTA
 constexpr int kTwoPerSm = 16384;  // columns of a CTA that leave room for two on an SM
 constexpr int kList = 2048;       // keys that are sorted
 constexpr int kFew = 128;         // keys that are compared with one another in place of that
-constexpr int kGiven = 1024;      // keys that a cluster's CTAs give together where few may be enough
+constexpr int kGiven = 1024;      // keys that a row's pieces give together, or up to twice as many
+constexpr int kSurvey = 256;      // threads that survey a piece
+constexpr int kMaxPiece = 8192;
+constexpr int kRows = 512;        // rows of a launch
 constexpr int kTable = 16;
 constexpr int64_t kMaxVocab = (int64_t)kMaxShare * kMaxCluster;
+constexpr int kMaxPieces = 256;
 
 struct Args {
   const float *logits;
@@ -55,9 +59,16 @@ struct Args {
   uint64_t *rng;
   int32_t *tokens;
   float *probs;
+  // what the first launch finds in each piece of a row, and whether the last one has to do the row
+  int pieces, piece, give;  // of a row; columns of a piece; the most keys of one
+  float *piece_top, *piece_from;
+  uint64_t *piece_mass, *piece_keys;
+  int32_t *piece_given, *todo;
+  double *drawn;  // the row's random number
 };
 
-struct Shared {
+// What a CTA works with by itself.
+struct Scratch {
   union {
     uint32_t limb[3][kBins];  // sums of a mass's bits 0-14, 15-29 and 30-44 (counts: the first)
     uint64_t bin[kBins];      // the same as one number
@@ -66,16 +77,19 @@ struct Shared {
       uint64_t mass[kFew];
     };
   };
+  double table[kTable];  // 2^(j / 16): 128 bytes, a lane's entry is on banks of its own
+  uint64_t warp_sum[kWarps];
+  uint64_t border, need;
+  uint32_t bin_at, count;
+};
+
+// With what the CTAs of a cluster exchange.
+struct Shared : Scratch {
   uint64_t whole[kBins];  // the bins of the whole row, written by every CTA of the cluster
   uint64_t part[kThreads];
-  double table[kTable];   // 2^(j / 16): 128 bytes, a lane's entry is on banks of its own
-  uint64_t warp_sum[kWarps];
   uint64_t cta_sum[kMaxCluster];  // written by every CTA, as these:
   float top[kMaxCluster], bottom[kMaxCluster];
   uint32_t listed[2];  // of the first CTA: keys in the lists, in this round and the next
-  float from[kMaxCluster];
-  uint64_t border, need;
-  uint32_t bin_at, count, given, known;
   float warp_top[kWarps], warp_bottom[kWarps];
   uint64_t low[kWarps], high[kWarps];
 };
@@ -304,7 +318,7 @@ __device__ __noinline__ void collect(const Columns c, const Span p, uint32_t bin
 
 // The key of the list at which the sum of masses (or the number), from the largest key on, reaches `need`.
 template <bool MASS>
-__device__ __noinline__ uint64_t border_of(Shared &s, int n, const Row row, uint64_t need) {
+__device__ __noinline__ uint64_t border_of(Scratch &s, int n, const Row row, uint64_t need) {
   const int tid = threadIdx.x;
   if (n <= kFew) {
     // few: thread t adds up what is at or ahead of its key
@@ -346,7 +360,7 @@ __device__ __noinline__ uint64_t border_of(Shared &s, int n, const Row row, uint
 
 // One number for each of this CTA's bins.
 template <bool MASS>
-__device__ __forceinline__ void join_limbs(Shared &s) {
+__device__ __forceinline__ void join_limbs(Scratch &s) {
   uint64_t w[kBins / kThreads];
   __syncthreads();
 #pragma unroll
@@ -362,7 +376,7 @@ __device__ __forceinline__ void join_limbs(Shared &s) {
 // The bin in which the sum of bins, from the first on, reaches what is needed, and what is needed of it.
 // `wanted(total)` is asked once.
 template <typename F>
-__device__ __forceinline__ void find_bin(Shared &s, const uint64_t *bins, F wanted, uint32_t &bin, uint64_t &need) {
+__device__ __forceinline__ void find_bin(Scratch &s, const uint64_t *bins, F wanted, uint32_t &bin, uint64_t &need) {
   constexpr int kEach = kBins / kThreads;
   uint64_t w[kEach], mine = 0, total;
 #pragma unroll
@@ -553,7 +567,7 @@ __device__ __noinline__ uint64_t sum_kept(const Columns c, const Kept kept, cons
 
 // find_border over a list of keys in this CTA alone: `need` of their masses or number, from `low` on.
 template <bool MASS>
-__device__ __noinline__ uint64_t list_border(Shared &s, const uint64_t *keys, int n, const Row row, float per_logit, uint64_t low, uint64_t need) {
+__device__ __noinline__ uint64_t list_border(Scratch &s, const uint64_t *keys, int n, const Row row, float per_logit, uint64_t low, uint64_t need) {
   Span span;
   span.top = row.top;
   span.per_logit = per_logit;
@@ -577,7 +591,7 @@ __device__ __noinline__ uint64_t list_border(Shared &s, const uint64_t *keys, in
   return border_of<MASS>(s, (int)s.count, row, need);
 }
 
-__device__ __forceinline__ uint64_t block_sum(Shared &s, uint64_t v) {
+__device__ __forceinline__ uint64_t block_sum(Scratch &s, uint64_t v) {
   uint64_t total;
   block_scan(v, s.warp_sum, total);
   return total;
@@ -585,7 +599,7 @@ __device__ __forceinline__ uint64_t block_sum(Shared &s, uint64_t v) {
 
 // The token of a list of keys, from `border` on and of masses of `least` and up: the first id at which the
 // running sum passes u times the whole.
-__device__ __noinline__ void draw_from(Shared &s, const Args &a, int64_t r, const uint64_t *keys, int n, const Row row, uint64_t border,
+__device__ __noinline__ void draw_from(Scratch &s, const Args &a, int64_t r, const uint64_t *keys, int n, const Row row, uint64_t border,
                                        uint64_t least, double u) {
   const int tid = threadIdx.x;
   auto mass = [&](uint64_t key) -> uint64_t {
@@ -625,107 +639,6 @@ __device__ __noinline__ void draw_from(Shared &s, const Args &a, int64_t r, cons
   }
 }
 
-// Rows whose options leave few tokens: each CTA gives the first one its largest, those from its q-th largest
-// lane's largest on, and the first one finds the border among them and draws. False where that is not known to
-// be right (too many; a border below what all CTAs have given). `all`: this CTA's sum of masses (top-p alone).
-__device__ __noinline__ bool from_few(Shared &s, const Args &a, const Columns columns, const Row row, int64_t r, int k, float p, uint64_t least,
-                                      double u, float lane_top, float my_top, float my_bottom, uint64_t all) {
-  cg::cluster_group cluster = cg::this_cluster();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ctas = (int)cluster.num_blocks();
-  const int most = min(kGiven / ctas, kThreads / 2), q = k > 0 ? min(k, most) : most;
-  const bool sure = k > 0 && k <= most;  // the row's k largest are among each CTA's k largest
-  for (int i = tid; i < kBins; i += kThreads) s.limb[0][i] = 0;
-  if (tid == 0) s.count = 0;
-  __syncthreads();
-  Span span;
-  span.top = my_top;
-  span.per_logit = (float)(kBins - 1) / (my_top - my_bottom);
-  const bool some = lane_top > -INFINITY;
-  if (some) atomicAdd(&s.limb[0][span.first_bin(lane_top)], 1u);
-  join_limbs<false>(s);
-  __syncthreads();
-  uint32_t bin;
-  uint64_t need, lanes = 0;
-  find_bin(s, s.bin, [&](uint64_t n) -> uint64_t { return lanes = n, min((uint64_t)q, n); }, bin, need);
-  float from = some && span.first_bin(lane_top) <= bin ? lane_top : INFINITY;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) from = fminf(from, __shfl_xor_sync(0xffffffffu, from, o));
-  if (lane == 0) s.warp_bottom[warp] = from;
-  __syncthreads();
-  for (int i = 0; i < kWarps; ++i) from = fminf(from, s.warp_bottom[i]);
-  if (lanes < (uint64_t)q) from = -INFINITY;  // (all that there are)
-  // its keys, in the bins' place
-  for (int i = 0; i < columns.n; ++i) {
-    const float4 x = columns.v[i * 32];
-    const float v[4] = {x.x, x.y, x.z, x.w};
-    if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) < from) continue;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (v[j] >= from && v[j] > -INFINITY) {
-        const uint32_t at = atomicAdd(&s.count, 1u);
-        if (at < (uint32_t)kList) s.list[at] = rank_key(v[j], columns.id + i * 128 + j);
-      }
-  }
-  __syncthreads();
-  const uint32_t n_mine = s.count;
-  if (tid == 0) {
-    s.bin_at = atomicAdd(cluster.map_shared_rank(&s.given, 0), n_mine);
-    cluster.map_shared_rank(s.cta_sum, 0)[cluster.block_rank()] = all;
-    cluster.map_shared_rank(s.from, 0)[cluster.block_rank()] = from;
-  }
-  __syncthreads();
-  uint64_t *keys = s.whole;
-  for (uint32_t i = tid; i < n_mine && s.bin_at + i < (uint32_t)kList; i += kThreads) cluster.map_shared_rank(keys, 0)[s.bin_at + i] = s.list[i];
-  cluster.sync();
-  const uint32_t n = *cluster.map_shared_rank(&s.given, 0);
-  cluster.sync();  // (nobody leaves, or goes on with the bins, before the number is read)
-  if (n > (uint32_t)kList) return false;
-  const bool first = cluster.block_rank() == 0;
-  bool known = true;
-  uint64_t border = 0;
-  if (first) {
-    float complete = -INFINITY, least_v = INFINITY;  // from `complete` on the list has all
-    for (int i = 0; i < ctas; ++i) {
-      complete = fmaxf(complete, s.from[i]);
-      least_v = fminf(least_v, s.from[i]);
-    }
-    const float span_v = row.top - (least_v > -INFINITY ? least_v : my_bottom);
-    const uint64_t end = (uint64_t)key_of(complete) << 32;
-    if (k > 0) {
-      uint64_t have = 0;
-      for (int i = tid; i < (int)n; i += kThreads) have += sure || keys[i] >= end;
-      have = block_sum(s, have);
-      if (have < (uint64_t)k && !sure) known = false;
-      else border = list_border<false>(s, keys, (int)n, row, (float)(kBins - 1) / span_v, 0, min((uint64_t)k, have));
-    }
-    if (known && p < 1.0f) {
-      uint64_t mass = 0;
-      for (int i = tid; i < (int)n; i += kThreads)
-        if (keys[i] >= (k > 0 ? border : end)) mass += mass_of(s.table, row, logit_of(keys[i]));
-      mass = block_sum(s, mass);
-      uint64_t whole = mass;
-      if (k <= 0) {
-        whole = 0;
-        for (int i = 0; i < ctas; ++i) whole += s.cta_sum[i];
-      }
-      const double x = ceil(fmax((double)p, 0.0) * (double)whole);
-      const uint64_t want = min(x >= 1.0 ? (uint64_t)x : (uint64_t)1, whole);
-      if (mass < want) known = false;
-      else border = list_border<true>(s, keys, (int)n, row, (float)(kBins - 1) / span_v, border, want);
-    }
-  }
-  if (!sure) {
-    if (first && tid < ctas) *cluster.map_shared_rank(&s.known, tid) = known;
-    cluster.sync();
-    known = s.known;
-  }
-  if (first && known) {
-    __syncthreads();
-    draw_from(s, a, r, keys, (int)n, row, border, least, u);
-  }
-  return known;
-}
-
 __device__ __forceinline__ double next_f64(uint64_t z) {  // of the advanced state
   z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
   z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
@@ -734,6 +647,324 @@ __device__ __forceinline__ double next_f64(uint64_t z) {  // of the advanced sta
 }
 constexpr uint64_t kStep = 0x9e3779b97f4a7c15ull;
 
+__device__ __forceinline__ bool is_greedy(const Args &a, int64_t r) { return a.temperature && !(a.temperature[r] > 0.0f); }
+__device__ __forceinline__ int top_k_of(const Args &a, int64_t r) {  // 0: all
+  const int k = a.top_k ? a.top_k[r] : 0;
+  return k > 0 && k < a.vocab ? k : 0;
+}
+__device__ __forceinline__ float top_p_of(const Args &a, int64_t r) { return a.top_p ? a.top_p[r] : 1.0f; }
+
+// ---- first launch: a CTA a piece of a row. Its largest logit; where all of the row counts, its sum of
+// masses, relative to its own largest; and its largest keys, those from the q-th largest thread's largest on.
+__global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
+  extern __shared__ __align__(16) float4 vals4[];  // [piece / 4], thread t's at t, t + kSurvey, ...
+  __shared__ double table[kTable];
+  __shared__ uint32_t bins[kSurvey];
+  __shared__ float tops[kSurvey / 32], bottoms[kSurvey / 32];
+  __shared__ uint32_t counts[kSurvey / 32], border, given;
+  __shared__ uint64_t sums[kSurvey / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t r = blockIdx.x / a.pieces;
+  const int piece = blockIdx.x - (int)r * a.pieces;
+  if (tid < kTable) table[tid] = exp2((double)tid / kTable);
+  bins[tid] = 0;
+  if (tid == 0) given = 0;
+  gqd::griddep_wait();
+  gqd::griddep_launch_dependents();
+  const int id0 = piece * a.piece, n = min(a.vocab - id0, a.piece);
+  const float *from = a.logits + r * a.ld + id0;
+  const bool greedy = is_greedy(a, r);
+  const int k = top_k_of(a, r);
+  const float p = top_p_of(a, r), t = greedy ? 0.0f : a.temperature ? a.temperature[r] : 1.0f;
+  const bool sum_all = !greedy && k == 0 && (p < 1.0f || !(a.min_p && a.min_p[r] > 0.0f));
+  const int steps = a.piece / (4 * kSurvey);
+  float top = -INFINITY;
+  auto take = [](float v) { return fmaxf(v, -INFINITY) + 0.0f; };  // (a NaN is never drawn: -inf; -0 counts as 0)
+#pragma unroll 4
+  for (int i = 0; i < steps; ++i) {
+    const int c = 4 * (tid + i * kSurvey);
+    float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    if (a.wide && c + 3 < n) {
+      v = *reinterpret_cast<const float4 *>(from + c);
+    } else {
+      if (c < n) v.x = from[c];
+      if (c + 1 < n) v.y = from[c + 1];
+      if (c + 2 < n) v.z = from[c + 2];
+      if (c + 3 < n) v.w = from[c + 3];
+    }
+    v = make_float4(take(v.x), take(v.y), take(v.z), take(v.w));
+    top = fmaxf(top, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+    vals4[tid + i * kSurvey] = v;
+  }
+  const float mine = top;
+  float bottom = mine > -INFINITY ? mine : INFINITY;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    bottom = fminf(bottom, __shfl_xor_sync(0xffffffffu, bottom, o));
+  }
+  if (lane == 0) {
+    tops[warp] = top;
+    bottoms[warp] = bottom;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kSurvey / 32; ++i) {
+    top = fmaxf(top, tops[i]);
+    bottom = fminf(bottom, bottoms[i]);
+  }
+  // the q-th largest of the threads' largest, by its bin
+  const int q = min(max(kGiven / a.pieces, 1), kSurvey / 2);
+  const float per = (float)(kSurvey - 1) / (top - bottom);
+  const uint32_t b = __float_as_uint(fminf((top - mine) * per, (float)(kSurvey - 1)) + 8388608.0f) & (kSurvey - 1);
+  if (mine > -INFINITY) atomicAdd(&bins[b], 1u);
+  __syncthreads();
+  uint32_t run = bins[tid];
+  const uint32_t own = run;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t up = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += up;
+  }
+  if (lane == 31) counts[warp] = run;
+  __syncthreads();
+  uint32_t lanes = 0;
+#pragma unroll
+  for (int i = 0; i < kSurvey / 32; ++i) {
+    if (i < warp) run += counts[i];
+    lanes += counts[i];
+  }
+  if (run >= (uint32_t)q && run - own < (uint32_t)q) border = tid;
+  __syncthreads();
+  float least = mine > -INFINITY && lanes >= (uint32_t)q && b <= border ? mine : INFINITY;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) least = fminf(least, __shfl_xor_sync(0xffffffffu, least, o));
+  if (lane == 0) bottoms[warp] = least;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kSurvey / 32; ++i) least = fminf(least, bottoms[i]);
+  if (lanes < (uint32_t)q) least = -INFINITY;  // (all that there are)
+  uint64_t *keys = a.piece_keys + ((int64_t)r * a.pieces + piece) * a.give;
+  if (mine >= least && mine > -INFINITY)
+    for (int i = 0; i < steps; ++i) {
+      const float4 x = vals4[tid + i * kSurvey];
+      const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (v[j] >= least && v[j] > -INFINITY) {
+          const uint32_t at = atomicAdd(&given, 1u);
+          if (at < (uint32_t)a.give) keys[at] = rank_key(v[j], id0 + 4 * (tid + i * kSurvey) + j);
+        }
+    }
+  uint64_t all = 0;
+  if (sum_all && top > -INFINITY && top < INFINITY) {  // (infinities: the last launch)
+    const Row row = row_of(top, t);
+    double sum = 0.0;  // (32 multiples of 1 up to 2^44: exact)
+#pragma unroll 1
+    for (int i = 0; i < steps; ++i) {
+      const float4 x = vals4[tid + i * kSurvey];
+      const float v[4] = {x.x, x.y, x.z, x.w};
+      double m[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) m[j] = rounded_mass(table, row, v[j]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum += row.far && v[j] == -INFINITY ? 0.0 : m[j] - kWhole;
+    }
+    all = warp_sum((uint64_t)sum);
+  }
+  if (lane == 0) sums[warp] = all;
+  __syncthreads();
+  if (tid == 0) {
+    all = 0;
+    for (int i = 0; i < kSurvey / 32; ++i) all += sums[i];
+    const int64_t at = (int64_t)r * a.pieces + piece;
+    a.piece_top[at] = top;
+    a.piece_from[at] = given > (uint32_t)a.give ? INFINITY : least;  // (from there on all are given: not more than there is room for)
+    a.piece_given[at] = (int)min(given, (uint32_t)a.give);
+    a.piece_mass[at] = all;
+  }
+}
+
+// ---- second launch: a CTA a row, from what was found in its pieces. Rows that it cannot be sure of are left to
+// the last launch: a border below what all pieces have given, infinities.
+__global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
+  __shared__ Scratch s;
+  __shared__ uint64_t keys[2 * kGiven];
+  __shared__ double piece_sum[kMaxPieces], warp_d[kWarps];
+  __shared__ float tops[kWarps], froms[kWarps];
+  __shared__ int n_keys, chosen;
+  __shared__ double rest;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t r = blockIdx.x;
+  if (tid < kTable) s.table[tid] = exp2((double)tid / kTable);
+  if (tid == 0) {
+    n_keys = 0;
+    chosen = -1;
+  }
+  gqd::griddep_wait();
+  gqd::griddep_launch_dependents();
+  const bool greedy = is_greedy(a, r);
+  const int k = greedy ? 0 : top_k_of(a, r);
+  const float p = greedy ? 1.0f : top_p_of(a, r), t = greedy ? 0.0f : a.temperature ? a.temperature[r] : 1.0f;
+  const float low_p = greedy || !a.min_p ? 0.0f : a.min_p[r];
+  double u = 0.0;
+  if (!greedy) {
+    if (a.rng) u = next_f64(a.rng[r] + kStep);
+    else u = a.uniforms[r];
+    u = u >= 0.0 ? fmin(u, 1.0 - 0x1p-53) : 0.0;
+  }
+  const int64_t at0 = r * a.pieces;
+  // (kMaxPieces <= kThreads: a thread a piece)
+  const bool has = tid < a.pieces;
+  const float my_top = has ? a.piece_top[at0 + tid] : -INFINITY;
+  const int my_n = has ? a.piece_given[at0 + tid] : 0;
+  float top = my_top, from = has ? a.piece_from[at0 + tid] : -INFINITY;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    from = fmaxf(from, __shfl_xor_sync(0xffffffffu, from, o));
+  }
+  if (lane == 0) {
+    tops[warp] = top;
+    froms[warp] = from;
+  }
+  __syncthreads();
+  for (int i = 0; i < kWarps; ++i) {
+    top = fmaxf(top, tops[i]);
+    from = fmaxf(from, froms[i]);  // from there on the pieces have given all
+  }
+  if (tid == 0) {
+    a.drawn[r] = u;
+    if (a.rng && !greedy) a.rng[r] += kStep;
+    a.todo[r] = top == INFINITY;
+    if (top == -INFINITY) {  // nothing that can be drawn
+      a.tokens[r] = -1;
+      if (a.probs) a.probs[r] = 0.0f;
+    }
+  }
+  if (top == INFINITY || top == -INFINITY) return;
+  const Row row = row_of(top, t);
+  uint64_t least = 1;
+  if (low_p > 0.0f) least = max(least, (uint64_t)ceil(fmin((double)low_p, 1.0) * (double)(1ull << kOne)));
+
+  if (!greedy && k == 0 && !(p < 1.0f) && !(low_p > 0.0f)) {
+    // all tokens: the piece in which the sum passes u times the whole, and the token in it
+    double mass = 0.0;
+    if (my_top > -INFINITY) mass = (double)a.piece_mass[at0 + tid] * exp(((double)my_top - (double)top) / (double)t);
+    double run = mass;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double up = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += up;
+    }
+    if (lane == 31) warp_d[warp] = run;
+    __syncthreads();
+    double total = 0.0, before = 0.0;
+    for (int i = 0; i < kWarps; ++i) {
+      if (i == warp) before = total;
+      total += warp_d[i];
+    }
+    run += before;
+    const double want = u * total;
+    if (has) piece_sum[tid] = run;
+    // (roundings may leave the end of the last piece short of the whole: the last piece that has any takes it)
+    if (mass > 0.0 && run > want) atomicMin(reinterpret_cast<unsigned int *>(&chosen), (unsigned int)tid);
+    __syncthreads();
+    if (chosen < 0 && mass > 0.0) atomicMax(&n_keys, tid);
+    __syncthreads();
+    const int piece = chosen >= 0 ? chosen : n_keys;
+    if (tid == piece) rest = fmax(want - (piece > 0 ? piece_sum[piece - 1] : 0.0), 0.0) / exp(((double)my_top - (double)top) / (double)t);
+    __syncthreads();
+    const float piece_top = a.piece_top[at0 + piece];
+    const uint64_t whole = a.piece_mass[at0 + piece];
+    const uint64_t aim = min((uint64_t)rest, whole - 1);
+    const Row prow = row_of(piece_top, t);
+    const int id0 = piece * a.piece, n = min(a.vocab - id0, a.piece);
+    const float *vals = a.logits + r * a.ld + id0;
+    // a warp a run of columns
+    const int each = a.piece / kWarps;
+    auto mass_at = [&](int c) -> uint64_t {
+      if (c >= n) return 0;
+      const float v = fmaxf(vals[c], -INFINITY) + 0.0f;
+      return mass_of(s.table, prow, v);
+    };
+    uint64_t sum = 0;
+#pragma unroll 4
+    for (int c = warp * each + lane; c < (warp + 1) * each; c += 32) sum += mass_at(c);
+    sum = warp_sum(sum);
+    if (lane == 0) s.warp_sum[warp] = sum;
+    __syncthreads();
+    uint64_t ahead = 0;
+    for (int i = 0; i < warp; ++i) ahead += s.warp_sum[i];
+    if (aim < ahead || aim >= ahead + sum) return;
+    for (int c = warp * each + lane; c < (warp + 1) * each; c += 32) {
+      const uint64_t w = mass_at(c), incl = warp_scan(w) + ahead;
+      const uint32_t past = __ballot_sync(0xffffffffu, incl > aim);
+      if (past) {
+        if (lane == __ffs(past) - 1) {
+          a.tokens[r] = id0 + c;
+          if (a.probs) a.probs[r] = (float)((double)w * exp(((double)piece_top - (double)top) / (double)t) / total);
+        }
+        return;
+      }
+      ahead = __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return;
+  }
+
+  // the keys that were given, together
+  {
+    uint64_t total;
+    const uint64_t ends = block_scan((uint64_t)my_n, s.warp_sum, total);
+    if (has) s.list[tid] = ends - my_n;
+    if (tid == 0) n_keys = (int)total;
+    __syncthreads();
+    for (int i = tid; i < a.pieces * a.give; i += kThreads) {
+      const int piece = i / a.give, j = i - piece * a.give;
+      if (j < a.piece_given[at0 + piece]) keys[s.list[piece] + j] = a.piece_keys[at0 * a.give + i];
+    }
+    __syncthreads();
+  }
+  const int n = n_keys;
+  const uint64_t end = (uint64_t)key_of(from) << 32;  // from there on the list has all
+  const float per_logit = (float)(kBins - 1) / fminf(from > -INFINITY && from < top ? top - from : 64.0f, 64.0f);
+  bool known = from <= top;
+  uint64_t border = end;
+  if (greedy) {
+    border = (uint64_t)key_of(top) << 32;
+  } else if (known) {
+    if (k > 0) {
+      uint64_t have = 0;
+      for (int i = tid; i < n; i += kThreads) have += keys[i] >= end;
+      have = block_sum(s, have);
+      if (have < (uint64_t)k && from > -INFINITY) known = false;
+      else border = list_border<false>(s, keys, n, row, per_logit, end, min((uint64_t)k, have));
+    }
+    if (known && p < 1.0f) {
+      uint64_t mass = 0;
+      for (int i = tid; i < n; i += kThreads)
+        if (keys[i] >= border) mass += mass_of(s.table, row, logit_of(keys[i]));
+      mass = block_sum(s, mass);
+      uint64_t whole = mass;
+      if (k == 0) {
+        const double f = my_top > -INFINITY ? exp(((double)my_top - (double)top) / (double)t) : 0.0;
+        whole = block_sum(s, has ? (uint64_t)((double)a.piece_mass[at0 + tid] * f) : 0);
+      }
+      const double x = ceil(fmax((double)p, 0.0) * (double)whole);
+      const uint64_t want = min(x >= 1.0 ? (uint64_t)x : (uint64_t)1, whole);
+      if (mass < want) known = false;
+      else border = list_border<true>(s, keys, n, row, per_logit, border, want);
+    }
+    // min_p alone: what is not in the list must be below it
+    if (known && k == 0 && !(p < 1.0f) && from > -INFINITY && mass_of(s.table, row, from) >= least) known = false;
+  }
+  __syncthreads();
+  if (known) draw_from(s, a, r, keys, n, row, border, least, u);
+  else if (tid == 0) a.todo[r] = 1;
+  if (known && greedy && tid == 0 && a.probs) a.probs[r] = 1.0f;
+}
+
+// ---- last launch: a cluster a row, whatever the options leave.
 __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args a) {
   extern __shared__ __align__(16) float vals[];  // [kWarps * run]: this CTA's columns, -inf past them
   __shared__ Shared s;
@@ -743,15 +974,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args
   const int64_t r = blockIdx.x / ctas;
   if (tid < kTable) s.table[tid] = exp2((double)tid / kTable);
   if (tid < 2) s.listed[tid] = 0;
-  if (tid == 2) s.given = 0;
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
-  const float t = a.temperature ? a.temperature[r] : 1.0f;
-  const int k = a.top_k ? a.top_k[r] : 0;
-  const float p = a.top_p ? a.top_p[r] : 1.0f;
-  const float low_p = a.min_p ? a.min_p[r] : 0.0f;
-  uint64_t state = a.rng ? a.rng[r] : 0;
-  const double given = a.uniforms ? a.uniforms[r] : 0.0;
+  if (!a.todo[r]) return;
+  const bool greedy = is_greedy(a, r);
+  const int k = top_k_of(a, r);
+  const float p = top_p_of(a, r), t = greedy ? 0.0f : a.temperature ? a.temperature[r] : 1.0f;
+  const float low_p = greedy || !a.min_p ? 0.0f : a.min_p[r];
+  const double u = a.drawn[r];
   const uint32_t id0 = (uint32_t)rank * a.share;
   const int n = min(max(a.vocab - (int)id0, 0), a.share);
   float top = -INFINITY, bottom = INFINITY;  // of the numbers (the smallest of one in four: it only scales bins)
@@ -775,7 +1005,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args
       *reinterpret_cast<float4 *>(vals + c) = v;
     }
   }
-  float lane_top = top;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -790,11 +1019,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args
     top = fmaxf(top, s.warp_top[i]);
     bottom = fminf(bottom, s.warp_bottom[i]);
   }
-  float my_top = top;
-  const float my_bottom = fminf(bottom, top);
   if (tid < ctas) {
     cluster.map_shared_rank(s.top, tid)[rank] = top;
-    cluster.map_shared_rank(s.bottom, tid)[rank] = my_bottom;
+    cluster.map_shared_rank(s.bottom, tid)[rank] = fminf(bottom, top);
   }
   cluster.sync();
   for (int i = 0; i < ctas; ++i) {
@@ -803,38 +1030,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args
   }
   if (top == INFINITY) {  // only infinities are drawn: they become 0, the others -inf
     for (int c = tid; c < kWarps * a.run; c += kThreads) vals[c] = vals[c] == INFINITY ? 0.0f : -INFINITY;
-    my_top = my_top == INFINITY ? 0.0f : -INFINITY;
-    lane_top = lane_top == INFINITY ? 0.0f : -INFINITY;
     top = bottom = 0.0f;
     __syncthreads();
   }
   const Columns columns{reinterpret_cast<const float4 *>(vals) + warp * (a.run / 4) + lane, a.run / 128, id0 + warp * a.run + lane * 4};
-  const bool greedy = !(t > 0.0f);
   // (greedy: the limit of small temperatures, in which all that are as large as the largest are left; the
   // first is drawn, with u = 0)
-  const Row row = row_of(top, greedy ? 0.0f : t);
+  const Row row = row_of(top, t);
   uint64_t above = 0;
-  double u = 0.0, least = kWhole + 1.0;
+  double least = kWhole + 1.0;
   if (!greedy) {
-    if (a.rng) {
-      state += kStep;
-      u = next_f64(state);
-      if (rank == 0 && tid == 0) a.rng[r] = state;  // (every CTA has read it: it has met the others)
-    } else {
-      u = given;
-    }
-    u = u >= 0.0 ? fmin(u, 1.0 - 0x1p-53) : 0.0;
     if (low_p > 0.0f) least = fmax(least, kWhole + ceil(fmin((double)low_p, 1.0) * (double)(1ull << kOne)));
     if (top > -INFINITY) {
       int round = 0;
-      const bool some = k > 0 && k < a.vocab;
-      if (some || p < 1.0f) {
-        const uint64_t all = some ? 0 : block_sum(s, sum_kept<false, false>(columns, Kept{}, row, s.table));
-        if (from_few(s, a, columns, row, r, some ? k : 0, p, (uint64_t)(least - kWhole), u, lane_top, my_top, my_bottom, all)) return;
-      }
       // bins over the row's numbers, for masses over those that have any
       const float span = top - bottom, heavy = 32.0f * t;
-      if (some) above = find_border<false>(s, columns, row, (float)(kBins - 1) / span, 0, 0.0, (uint64_t)k, round);
+      if (k > 0) above = find_border<false>(s, columns, row, (float)(kBins - 1) / span, 0, 0.0, (uint64_t)k, round);
       if (p < 1.0f)
         above = find_border<true>(s, columns, row, (float)(kBins - 1) / fminf(span, heavy), above, fmax((double)p, 0.0), 0, round);
     }
@@ -859,10 +1070,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args
   for (int i = 0; i < ctas; ++i) {
     total += s.cta_sum[i];
     if (i < rank) before += s.cta_sum[i];
-  }
-  if (rank == 0 && tid == 0 && total == 0) {  // nothing that can be drawn
-    a.tokens[r] = -1;
-    if (a.probs) a.probs[r] = 0.0f;
   }
   uint64_t at = (uint64_t)(u * (double)total);
   if (total > 0) at = min(at, total - 1);
@@ -926,32 +1133,72 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
   a.tokens = tokens;
   a.probs = probs;
   a.wide = (uintptr_t)logits % 16 == 0 && ld % 4 == 0;
-  // CTAs of a row: as few as hold it at two CTAs per SM, more while a share is large and the GPU not full
+  // pieces of a row: as large as leaves two for every SM
+  a.piece = kMaxPiece;
+  const int64_t together = std::min<int64_t>(m, kRows);
+  while (a.piece > 2048 && together * ((vocab + a.piece - 1) / a.piece) < 2 * (int64_t)ctx->num_sms) a.piece /= 2;
+  a.pieces = (int)((vocab + a.piece - 1) / a.piece);
+  a.give = 2 * kGiven / a.pieces;
+  // the last launch: CTAs of a row, as few as hold it at two CTAs per SM
   int cluster = 1;
-  while (cluster < kMaxCluster && (vocab > (int64_t)cluster * kTwoPerSm || (vocab > cluster * 2048 && m * cluster * 2 <= 2 * ctx->num_sms)))
-    cluster *= 2;
+  while (vocab > (int64_t)cluster * kTwoPerSm && cluster < kMaxCluster) cluster *= 2;
   a.share = (int)((vocab + cluster - 1) / cluster + 3) / 4 * 4;
   a.run = (a.share + kWarps * 128 - 1) / (kWarps * 128) * 128;
+  // what the launches tell one another: made by the context's first call and kept, so that a recorded
+  // graph's addresses stay good
+  constexpr size_t kBytes = (size_t)kRows * (kMaxPieces * 20 + 2 * kGiven * 8 + 16);
+  if (!ctx->sample_ws) {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // (also while a stream is being recorded)
+    GQ_CUDA_TRY(ctx, cudaThreadExchangeStreamCaptureMode(&mode));
+    const cudaError_t e = cudaMalloc(&ctx->sample_ws, kBytes);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) {
+      ctx->sample_ws = nullptr;
+      return gq_cuda_fail(ctx, e, "sample_requests: cudaMalloc");
+    }
+  }
+  a.piece_keys = static_cast<uint64_t *>(ctx->sample_ws);
+  a.piece_mass = a.piece_keys + (size_t)kRows * 2 * kGiven;
+  a.drawn = reinterpret_cast<double *>(a.piece_mass + (size_t)kRows * kMaxPieces);
+  a.piece_top = reinterpret_cast<float *>(a.drawn + kRows);
+  a.piece_from = a.piece_top + (size_t)kRows * kMaxPieces;
+  a.piece_given = reinterpret_cast<int32_t *>(a.piece_from + (size_t)kRows * kMaxPieces);
+  a.todo = a.piece_given + (size_t)kRows * kMaxPieces;
   static bool attr_set[64] = {};
   if (!attr_set[ctx->device & 63]) {
     GQ_CUDA_TRY(ctx, cudaFuncSetAttribute(sample_requests_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMaxShare + 4 * kWarps * 128) * 4));
     GQ_CUDA_TRY(ctx, cudaFuncSetAttribute(sample_requests_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr_set[ctx->device & 63] = true;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(m * cluster));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)a.run * kWarps * 4;
-  cfg.stream = ctx->stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)cluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = ctx->pdl ? 2 : 1;
-  GQ_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, sample_requests_kernel, (const Args)a));
+  for (int64_t r0 = 0; r0 < m; r0 += kRows) {
+    const int64_t rows = std::min<int64_t>(m - r0, kRows);
+    Args b = a;
+    b.logits += r0 * ld;
+    if (b.temperature) b.temperature += r0;
+    if (b.top_k) b.top_k += r0;
+    if (b.top_p) b.top_p += r0;
+    if (b.min_p) b.min_p += r0;
+    if (b.uniforms) b.uniforms += r0;
+    if (b.rng) b.rng += r0;
+    b.tokens += r0;
+    if (b.probs) b.probs += r0;
+    GQ_CUDA_TRY(ctx, gq_launch(ctx, survey_kernel, dim3((unsigned)(rows * a.pieces)), dim3(kSurvey), (size_t)a.piece * 4, b));
+    GQ_CUDA_TRY(ctx, gq_launch(ctx, finish_kernel, dim3((unsigned)rows), dim3(kThreads), 0, b));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * cluster));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)a.run * kWarps * 4;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ctx->pdl ? 2 : 1;
+    GQ_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, sample_requests_kernel, (const Args)b));
+  }
   return GQ_OK;
 }
