@@ -744,18 +744,6 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
 #pragma unroll
   for (int i = 0; i < kSurvey / 32; ++i) least = fminf(least, bottoms[i]);
   if (lanes < (uint32_t)q) least = -INFINITY;  // (all that there are)
-  uint64_t *keys = a.piece_keys + ((int64_t)r * a.pieces + piece) * a.give;
-  if (mine >= least && mine > -INFINITY)
-    for (int i = 0; i < steps; ++i) {
-      const float4 x = vals4[tid + i * kSurvey];
-      const float v[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (v[j] >= least && v[j] > -INFINITY) {
-          const uint32_t at = atomicAdd(&given, 1u);
-          if (at < (uint32_t)a.give) keys[at] = rank_key(v[j], id0 + 4 * (tid + i * kSurvey) + j);
-        }
-    }
   uint64_t all = 0;
   if (sum_all && top > -INFINITY && top < INFINITY) {  // (infinities: the last launch)
     const Row row = row_of(top, t);
@@ -766,12 +754,28 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
       const float v[4] = {x.x, x.y, x.z, x.w};
       double m[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) m[j] = rounded_mass(table, row, v[j]);
+      for (int j = 0; j < 4; ++j) m[j] = rounded_mass(table, row, v[j]) - kWhole;
+      if (row.far)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum += row.far && v[j] == -INFINITY ? 0.0 : m[j] - kWhole;
+        for (int j = 0; j < 4; ++j) m[j] = v[j] == -INFINITY ? 0.0 : m[j];
+      sum += (m[0] + m[1]) + (m[2] + m[3]);
     }
     all = warp_sum((uint64_t)sum);
   }
+  __syncwarp();
+  uint64_t *keys = a.piece_keys + ((int64_t)r * a.pieces + piece) * a.give;
+  if (mine >= least && mine > -INFINITY)
+    for (int i = 0; i < steps; ++i) {
+      const float4 x = vals4[tid + i * kSurvey];
+      const float v[4] = {x.x, x.y, x.z, x.w};
+      if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) < least) continue;
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j)
+        if (v[j] >= least && v[j] > -INFINITY) {
+          const uint32_t at = atomicAdd(&given, 1u);
+          if (at < (uint32_t)a.give) keys[at] = rank_key(v[j], id0 + 4 * (tid + i * kSurvey) + j);
+        }
+    }
   if (lane == 0) sums[warp] = all;
   __syncthreads();
   if (tid == 0) {
