@@ -8,14 +8,15 @@
 * writes each KV layer's new rows into their pages (``gq_paged_append``),
 * attends every request over its own pages (``gq_paged_attention``),
 * applies each request's penalties, biases and grammar mask to its logits
-  (``gq_process_logits``) and samples (``gq_sample_rows``),
+  (``gq_process_logits``) and samples, with one set of options (``gq_sample_rows``) or with
+  each request's own (``gq_sample_requests``),
 * takes back the pages of requests that have ended (``gq_paged_release``).
 
 Lengths, tables, free pages, histories and controls live on the device, so one recorded
 graph serves every step. No counterpart in the reference (one sequence, contiguous
 caches).
 
-    python -m gq.paged [--requests 64] [--steps 32] [--type bf16]
+    python -m gq.paged [--requests 64] [--steps 32] [--type bf16] [--own-options]
 
 decodes with synthetic E2B-shaped weights and prints the time of a step.
 """
@@ -40,11 +41,11 @@ class PagedDecoder(e2b.Decoder):
     """One decode step of ``batch`` requests through the C ABI, over pages.
 
     max_len: the most tokens of a request (its block table row); page_size, kv_type
-    ("f32", "f16", "bf16", "e4m3" with k_scale / v_scale) and n_pages (default: enough
-    for every request at max_len) describe the pool that each source layer has. ``lens``
-    are the requests' lengths, filled by ``extend``. A place whose request has ended idles,
-    and a request of max_len tokens stands still: a step takes no page for them, leaves
-    their token as it is, and their rows of the logits mean nothing.
+    ("f32", "f16", "bf16", "e4m3" or the 4-bit "e2m1" with k_scale / v_scale) and n_pages
+    (default: enough for every request at max_len) describe the pool that each source layer
+    has. ``lens`` are the requests' lengths, filled by ``extend``. A place whose request has
+    ended idles, and a request of max_len tokens stands still: a step takes no page for
+    them, leaves their token as it is, and their rows of the logits mean nothing.
 
     Controls, all device tensors that may be changed between steps on torch's current
     stream (whatever stream the backend has, a step comes after what that stream was given
@@ -53,7 +54,10 @@ class PagedDecoder(e2b.Decoder):
     max_len] (tokens by position, -1 where they are not known), and, given at construction
     because their sizes belong to the recorded step, ``bias`` (ids, values, offsets) and
     ``masks`` (words, rows); see gq_process_logits in include/gq.h. ``sample``: temperature,
-    top_k, top_p of gq_sample_rows."""
+    top_k, top_p of gq_sample_rows for all requests, or None: every request has its own, the
+    controls ``temperature`` (1 at first), ``top_p`` (1), ``min_p`` (0) [batch] f32 and ``top_k`` (0)
+    [batch] int32 of gq_sample_requests, and ``probs`` [batch] are the probabilities that the
+    last step's tokens were drawn with."""
 
     def __init__(self, g, cfg: e2b.Config, weights: Optional[e2b.Weights], batch: int, max_len: int, page_size: int = 16,
                  kv_type: str = "bf16", n_pages: Optional[int] = None, k_scale: float = 1.0, v_scale: float = 1.0,
@@ -62,7 +66,7 @@ class PagedDecoder(e2b.Decoder):
         self.n_pages = n_pages if n_pages is not None else batch * self.width
         self.k_scale, self.v_scale = k_scale, v_scale
         self.bias, self.masks = bias, masks
-        self.opts = _abi.SampleOpts(float(sample[0]), int(sample[1]), float(sample[2]), 1.0)
+        self.opts = None if sample is None else _abi.SampleOpts(float(sample[0]), int(sample[1]), float(sample[2]), 1.0)
         self.seed = seed
         super().__init__(g, cfg, weights, batch, cache_len=0, capacity=max_len, device_init_seed=device_init_seed,
                          fuse_norms=False)
@@ -73,13 +77,17 @@ class PagedDecoder(e2b.Decoder):
     def _make_kv(self, weights, kv_gen, kv_device_seed) -> None:
         torch, c, g, B = self.torch, self.cfg, self.g, self.batch
         dev, i32 = g.torch_device, torch.int32
-        dtypes = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "e4m3": torch.float8_e4m3fn}
+        dtypes = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "e4m3": torch.float8_e4m3fn,
+                  "e2m1": torch.uint8}
         if self.kv_type not in dtypes:
             raise GqError(_abi.GQ_ERR_UNSUPPORTED, f"PagedDecoder: kv_type {self.kv_type}")
         self.kcache, self.vcache, self.pages = {}, {}, {}
         for i in range(c.layers):
             if c.kv_source(i) == i:
-                shape = (self.n_pages, c.heads_kv, self.page_size, c.dh(i))
+                if self.kv_type == "e2m1" and c.dh(i) % 16:
+                    raise GqError(_abi.GQ_ERR_UNSUPPORTED, f"PagedDecoder: e2m1 pages of head_dim {c.dh(i)}")
+                row = c.dh(i) // 16 * 9 if self.kv_type == "e2m1" else c.dh(i)
+                shape = (self.n_pages, c.heads_kv, self.page_size, row)
                 k, v = (torch.empty(shape, dtype=dtypes[self.kv_type], device=dev) for _ in range(2))
                 self.pages[i] = g.kv_pages(k, v, self.k_scale, self.v_scale)
         self.table = torch.full((B, max(self.width, 1)), -1, dtype=i32, device=dev)
@@ -113,6 +121,10 @@ class PagedDecoder(e2b.Decoder):
         self.tokens = torch.zeros(B, dtype=i32, device=dev)
         self.rng = torch.arange(self.seed, self.seed + B, dtype=torch.int64, device=dev)
         self.drawn, self.rng_after = torch.zeros_like(self.tokens), torch.zeros_like(self.rng)  # of the step
+        if self.opts is None:
+            self.temperature, self.top_p = (torch.ones(B, device=dev) for _ in range(2))
+            self.min_p, self.probs = (torch.zeros(B, device=dev) for _ in range(2))
+            self.top_k = torch.zeros(B, dtype=i32, device=dev)
         torch.cuda.synchronize(dev)
 
     def _stream(self):
@@ -186,6 +198,27 @@ class PagedDecoder(e2b.Decoder):
         self.ending -= {b for b, n in enumerate(new_lens) if n > 0}
         torch.cuda.synchronize(dev)
 
+    def rows_of(self, place: int):
+        """What the request at this place has in the cache: a function of a source layer that
+        gives its keys and values, f32 [tokens, heads_kv * head_dim], as ``extend`` takes them
+        (of this decoder or another, whose pages may be of another type). Read when it is
+        called, at the lengths of this call."""
+        torch, c, g = self.torch, self.cfg, self.g
+        if not 0 <= int(place) < self.batch:
+            raise GqError(_abi.GQ_ERR_INVALID_ARGUMENT, f"rows_of: places are 0 to {self.batch - 1}")
+        g.flush()
+        n = int(self.lens[place])
+        at = torch.arange(n, device=g.torch_device)
+        slots = self.table[place].long()[at // self.page_size] * self.page_size + at % self.page_size
+
+        def rows(layer):
+            torch.cuda.synchronize(g.torch_device)
+            kv = [torch.empty(n, c.heads_kv, c.dh(layer), device=g.torch_device) for _ in range(2)]
+            g.paged_read(self.pages[layer], slots, *kv)
+            g.flush()
+            return [x.view(n, c.heads_kv * c.dh(layer)) for x in kv]
+        return rows
+
     def end(self, places: Sequence[int]) -> None:
         """The requests at these places end: the next step is their last, and gives their pages
         back. The places idle from then on, until ``extend`` gives them a request."""
@@ -249,13 +282,20 @@ class PagedDecoder(e2b.Decoder):
         add("process_logits", lib.gq_process_logits_bounded, ctx, V(self.logits), B, vocab, vocab, V(self.ids_at),
             self.capacity + 1, V(self.prompt_lens), V(self.now), V(self.penalties), ids, values, offsets, n_bias, words,
             n_masks, mask_words, rows, V(self.controlled), vocab)
-        if self.opts.temperature > 0:
+        if self._draws():
             add("rng", self._torch_call, lambda: self.rng_after.copy_(self.rng))
-        add("sample", lib.gq_sample_rows, ctx, V(self.controlled), B, vocab, vocab, ctypes.byref(self.opts), None, 0, 0,
-            V(self.rng_after), V(self.drawn))
+        if self.opts is None:
+            add("sample", lib.gq_sample_requests, ctx, V(self.controlled), B, vocab, vocab, V(self.temperature), V(self.top_k),
+                V(self.top_p), V(self.min_p), None, V(self.rng_after), V(self.drawn), V(self.probs))
+        else:
+            add("sample", lib.gq_sample_rows, ctx, V(self.controlled), B, vocab, vocab, ctypes.byref(self.opts), None, 0, 0,
+                V(self.rng_after), V(self.drawn))
         add("keep", self._torch_call, self._take_tokens)
         add("release", lib.gq_paged_release, ctx, B, self.page_size, V(self.now), V(self.keep), V(self.table),
             self.table.shape[1], V(self.free), self.n_pages, V(self.count), V(self.count), V(self.lens))
+
+    def _draws(self) -> bool:
+        return self.opts is None or self.opts.temperature > 0
 
     def _torch_call(self, fn) -> int:
         """One of the step's calls that is torch's: on the backend's stream, into tensors that
@@ -269,7 +309,7 @@ class PagedDecoder(e2b.Decoder):
         torch = self.torch
         torch.ne(self.now, self.lens, out=self.took)
         torch.where(self.took, self.drawn, self.tokens, out=self.tokens)
-        if self.opts.temperature > 0:  # (a greedy step draws no numbers)
+        if self._draws():  # (a greedy step draws no numbers)
             torch.where(self.took, self.rng_after, self.rng, out=self.rng)
 
     def step(self, ids=None):
@@ -321,13 +361,13 @@ class PagedDecoder(e2b.Decoder):
 
     def kv_bytes(self) -> int:
         """K and V bytes that a step's attention reads at the present lengths."""
-        c, size = self.cfg, {"f32": 4, "e4m3": 1}.get(self.kv_type, 2)
+        c, size = self.cfg, {"f32": 4, "e4m3": 1, "e2m1": 9 / 16}.get(self.kv_type, 2)
         self._stream().synchronize()
         lens, tot = self.lens.tolist(), 0
         for i in range(c.layers):
             w = c.window_of(i)
             tot += 2 * sum(min(n, w) if w else n for n in lens) * c.heads_kv * c.dh(i) * size
-        return tot
+        return int(tot)
 
 
 def main(argv=None) -> int:
@@ -335,7 +375,8 @@ def main(argv=None) -> int:
     ap.add_argument("--requests", type=int, default=64)
     ap.add_argument("--max-len", type=int, default=2048)
     ap.add_argument("--steps", type=int, default=32)
-    ap.add_argument("--type", choices=["f32", "f16", "bf16", "e4m3"], default="bf16")
+    ap.add_argument("--type", choices=["f32", "f16", "bf16", "e4m3", "e2m1"], default="bf16")
+    ap.add_argument("--own-options", action="store_true", help="sampling options of each request's own")
     args = ap.parse_args(argv)
 
     import torch
@@ -344,8 +385,12 @@ def main(argv=None) -> int:
 
     g = CudaBackend(0, own_stream=True)
     cfg, B = e2b.e2b_config(), args.requests
-    scales = dict(k_scale=1 / 32, v_scale=1 / 32) if args.type == "e4m3" else {}
-    dec = PagedDecoder(g, cfg, None, B, args.max_len, kv_type=args.type, sample=(1.0, 64, 0.95), device_init_seed=5, **scales)
+    scales = dict(k_scale=1 / 32, v_scale=1 / 32) if args.type in ("e4m3", "e2m1") else {}
+    dec = PagedDecoder(g, cfg, None, B, args.max_len, kv_type=args.type, sample=None if args.own_options else (1.0, 64, 0.95),
+                       device_init_seed=5, **scales)
+    if args.own_options:
+        dec.top_k.fill_(64)
+        dec.top_p.fill_(0.95)
     gen = torch.Generator(device=g.torch_device)
     gen.manual_seed(6)
     room = max(1, args.max_len - args.steps - 4)

@@ -18,7 +18,7 @@ def encode(v, scale):
     """Rows [..., head_dim] f32 -> [..., head_dim / 16 * 9] uint8. (A quotient of two numbers of 24 and
     of 4 bits is a tie or at least 2^-28 of itself away from one: 64 bits tell them apart.)"""
     x = (np.asarray(v, np.float32) * np.float32(1.0 / np.float32(scale))).astype(np.float64)
-    x = x.reshape(*x.shape[:-1], -1, 16)
+    x = x.reshape(*x.shape[:-1], x.shape[-1] // 16, 16)
     a = np.abs(x)
     top = a.max(-1)
     with np.errstate(invalid="ignore"):
@@ -28,7 +28,7 @@ def encode(v, scale):
     with np.errstate(invalid="ignore"):
         y = np.where(np.isinf(a), np.where(np.isinf(div), 0.0, 6.0), a / div)
     c = nearest(np.minimum(np.nan_to_num(y, nan=0.0), 6.0), CODES) + 8 * np.signbit(x)
-    c = c.reshape(*c.shape[:-2], -1, 2).astype(np.uint8)
+    c = c.reshape(*c.shape[:-2], c.shape[-2] * 8, 2).astype(np.uint8)
     return np.concatenate([c[..., 0] | (c[..., 1] << 4), s.astype(np.uint8)], -1)
 
 
