@@ -36,13 +36,13 @@ constexpr int kBins = 2048;
 constexpr int kOne = 44;          // w = 1 is 2^44
 constexpr int kLimb = 15;         // bits of a mass that one 32-bit sum takes: a CTA has at most 2^15 columns
 constexpr int kMaxShare = 32768;  // columns of a CTA
-constexpr int kTwoPerSm = 16384;  // columns of a CTA that leave room for two on an SM
 constexpr int kList = 2048;       // keys that are sorted
 constexpr int kFew = 128;         // keys that are compared with one another in place of that
-constexpr int kGiven = 1024;      // keys that a row's pieces give together, or up to twice as many
+constexpr int kGiven = 1024;      // keys that a row's pieces give together, about; a larger top_k has twice as many
+constexpr int kMostGiven = 4096;  // and no more
 constexpr int kSurvey = 256;      // threads that survey a piece
 constexpr int kMaxPiece = 8192;
-constexpr int kRows = 512;        // rows of a launch
+constexpr int kRows = 256;        // rows of a launch
 constexpr int kTable = 16;
 constexpr int64_t kMaxVocab = (int64_t)kMaxShare * kMaxCluster;
 constexpr int kMaxPieces = 256;
@@ -88,9 +88,8 @@ struct Shared : Scratch {
   uint64_t whole[kBins];  // the bins of the whole row, written by every CTA of the cluster
   uint64_t part[kThreads];
   uint64_t cta_sum[kMaxCluster];  // written by every CTA, as these:
-  float top[kMaxCluster], bottom[kMaxCluster];
   uint32_t listed[2];  // of the first CTA: keys in the lists, in this round and the next
-  float warp_top[kWarps], warp_bottom[kWarps];
+  float warp_top[kWarps], warp_from[kWarps];
   uint64_t low[kWarps], high[kWarps];
 };
 
@@ -202,12 +201,38 @@ __device__ void sort_down(uint64_t *k, int n) {
 // Of two logits and ids: whether the first is at or ahead of the second in the order.
 __device__ __forceinline__ bool from_on(float v, uint32_t id, float v0, uint32_t id0) { return v > v0 || (v == v0 && id <= id0); }
 
-// A lane's columns: four from v[0] on, whose first id is `id`, four from v[32] on, ... (n times). The passes
-// over them are functions of their own, so that each has the registers that it needs.
+// A NaN is never drawn: -inf. -0 counts as 0.
+__device__ __forceinline__ float4 clean(float4 v) {
+  return make_float4(fmaxf(v.x, -INFINITY) + 0.0f, fmaxf(v.y, -INFINITY) + 0.0f, fmaxf(v.z, -INFINITY) + 0.0f, fmaxf(v.w, -INFINITY) + 0.0f);
+}
+// Four logits of a row from column c on, -inf past its n columns.
+__device__ __forceinline__ float4 four_logits(const float *row, int c, int n, bool wide) {
+  float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+  if (wide && c + 3 < n) {
+    v = *reinterpret_cast<const float4 *>(row + c);
+  } else {
+    if (c < n) v.x = row[c];
+    if (c + 1 < n) v.y = row[c + 1];
+    if (c + 2 < n) v.z = row[c + 2];
+    if (c + 3 < n) v.w = row[c + 3];
+  }
+  return clean(v);
+}
+
+// A lane's columns of a row: four from `id` on, four 128 on, ... (n times). The passes over them are functions
+// of their own, so that each has the registers that it needs.
 struct Columns {
-  const float4 *v;
-  int n;
+  const float *row;
+  int n, end;     // end: of this CTA's columns
   uint32_t id;
+  bool wide, infinite;  // infinite: the row's largest is +inf; such logits become 0, the others -inf
+  __device__ __forceinline__ float4 at(int i) const {
+    float4 v = four_logits(row, (int)id + i * 128, end, wide);
+    if (infinite)
+      v = make_float4(v.x == INFINITY ? 0.0f : -INFINITY, v.y == INFINITY ? 0.0f : -INFINITY, v.z == INFINITY ? 0.0f : -INFINITY,
+                      v.w == INFINITY ? 0.0f : -INFINITY);
+    return v;
+  }
 };
 
 // Where the border may be, and the bin of a logit there.
@@ -227,28 +252,32 @@ struct Span {
   __device__ __forceinline__ uint32_t key_bin(float v, uint32_t id) const { return (uint32_t)((high - rank_key(v, id)) >> shift); }
 };
 
+// Adds to shared memory what is not 0 (a predicate, no branch).
+__device__ __forceinline__ void add_some(uint32_t *to, uint32_t v) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p red.shared.add.u32 [%0], %1;\n\t}" ::"r"(gqd::smem_u32(to)), "r"(v) : "memory");
+}
 __device__ __forceinline__ void add_mass(uint32_t (*limb)[kBins], uint32_t b, uint64_t w) {
   const uint32_t rest = (uint32_t)(w >> kLimb);
-  if (w) atomicAdd(&limb[0][b], (uint32_t)w & ((1u << kLimb) - 1));
-  if (rest & ((1u << kLimb) - 1)) atomicAdd(&limb[1][b], rest & ((1u << kLimb) - 1));
-  if (rest >> kLimb) atomicAdd(&limb[2][b], rest >> kLimb);
+  add_some(&limb[0][b], (uint32_t)w & ((1u << kLimb) - 1));
+  add_some(&limb[1][b], rest & ((1u << kLimb) - 1));
+  add_some(&limb[2][b], rest >> kLimb);
 }
 
 // The first round's bins: all numbers (counts), or those from a border on (masses).
 __device__ __noinline__ void count_bins(const Columns c, const Span p, uint32_t *count) {
 #pragma unroll 2
   for (int i = 0; i < c.n; ++i) {
-    const float4 x = c.v[i * 32];
+    const float4 x = c.at(i);
     const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (v[k] > -INFINITY) atomicAdd(&count[p.first_bin(v[k])], 1u);
+      add_some(&count[p.first_bin(v[k])], v[k] > -INFINITY);
   }
 }
 __device__ __noinline__ void mass_bins(const Columns c, const Span p, const Row row, const double *table, uint32_t (*limb)[kBins]) {
 #pragma unroll 1
   for (int i = 0; i < c.n; ++i) {
-    const float4 x = c.v[i * 32];
+    const float4 x = c.at(i);
     float v[4] = {x.x, x.y, x.z, x.w};
     const uint32_t id = c.id + i * 128;
     bool any = false;
@@ -263,7 +292,8 @@ __device__ __noinline__ void mass_bins(const Columns c, const Span p, const Row 
     for (int k = 0; k < 4; ++k) m[k] = rounded_mass(table, row, v[k]);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (v[k] > row.least) add_mass(limb, p.first_bin(v[k]), ((uint64_t)(__double2hiint(m[k]) & 0xfffff) << 32) | (uint32_t)__double2loint(m[k]));
+      add_mass(limb, p.first_bin(v[k]),
+               v[k] > row.least ? ((uint64_t)(__double2hiint(m[k]) & 0xfffff) << 32) | (uint32_t)__double2loint(m[k]) : 0);
   }
 }
 // A later round's.
@@ -271,7 +301,7 @@ template <bool MASS>
 __device__ __noinline__ void key_bins(const Columns c, const Span p, const Row row, const double *table, uint32_t (*limb)[kBins]) {
 #pragma unroll 1
   for (int i = 0; i < c.n; ++i) {
-    const float4 x = c.v[i * 32];
+    const float4 x = c.at(i);
     const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll 1
     for (int k = 0; k < 4; ++k) {
@@ -291,7 +321,7 @@ __device__ __noinline__ void collect(const Columns c, const Span p, uint32_t bin
   uint32_t *listed = cluster.map_shared_rank(my_listed, 0);
 #pragma unroll 1
   for (int i = 0; i < c.n; ++i) {
-    const float4 x = c.v[i * 32];
+    const float4 x = c.at(i);
     const float v[4] = {x.x, x.y, x.z, x.w};
     const uint32_t id = c.id + i * 128;
     uint32_t in = 0;
@@ -470,7 +500,7 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
       // the smallest and the largest key whose bin it is
       uint64_t lo = ~0ull, hi = 0;
       for (int i = 0; i < columns.n; ++i) {
-        const float4 x = columns.v[i * 32];
+        const float4 x = columns.at(i);
         const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -558,14 +588,15 @@ __device__ __noinline__ uint64_t sum_kept(const Columns c, const Kept kept, cons
 #pragma unroll 1
   for (int i = 0; i < c.n; ++i) {
     double m[4];
-    if (kept.masses<BORDER, LIMIT>(c.v[i * 32], c.id + i * 128, row, table, m))
+    if (kept.masses<BORDER, LIMIT>(c.at(i), c.id + i * 128, row, table, m))
 #pragma unroll
       for (int k = 0; k < 4; ++k) sum += m[k] - kWhole;
   }
   return (uint64_t)sum;
 }
 
-// find_border over a list of keys in this CTA alone: `need` of their masses or number, from `low` on.
+// find_border over a list of keys in this CTA alone: `need` of their masses or number, from `low` on. 0 where
+// more of them are alike than a list holds.
 template <bool MASS>
 __device__ __noinline__ uint64_t list_border(Scratch &s, const uint64_t *keys, int n, const Row row, float per_logit, uint64_t low, uint64_t need) {
   Span span;
@@ -586,8 +617,12 @@ __device__ __noinline__ uint64_t list_border(Scratch &s, const uint64_t *keys, i
   uint32_t bin;
   find_bin(s, s.bin, [&](uint64_t) { return need; }, bin, need);
   for (int i = threadIdx.x; i < n; i += kThreads)
-    if (keys[i] >= low && span.first_bin(logit_of(keys[i])) == bin) s.list[atomicAdd(&s.count, 1u)] = keys[i];
+    if (keys[i] >= low && span.first_bin(logit_of(keys[i])) == bin) {
+      const uint32_t at = atomicAdd(&s.count, 1u);
+      if (at < (uint32_t)kList) s.list[at] = keys[i];
+    }
   __syncthreads();
+  if (s.count > (uint32_t)kList) return 0;
   return border_of<MASS>(s, (int)s.count, row, need);
 }
 
@@ -679,20 +714,9 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
   const bool sum_all = !greedy && k == 0 && (p < 1.0f || !(a.min_p && a.min_p[r] > 0.0f));
   const int steps = a.piece / (4 * kSurvey);
   float top = -INFINITY;
-  auto take = [](float v) { return fmaxf(v, -INFINITY) + 0.0f; };  // (a NaN is never drawn: -inf; -0 counts as 0)
 #pragma unroll 4
   for (int i = 0; i < steps; ++i) {
-    const int c = 4 * (tid + i * kSurvey);
-    float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-    if (a.wide && c + 3 < n) {
-      v = *reinterpret_cast<const float4 *>(from + c);
-    } else {
-      if (c < n) v.x = from[c];
-      if (c + 1 < n) v.y = from[c + 1];
-      if (c + 2 < n) v.z = from[c + 2];
-      if (c + 3 < n) v.w = from[c + 3];
-    }
-    v = make_float4(take(v.x), take(v.y), take(v.z), take(v.w));
+    const float4 v = four_logits(from, 4 * (tid + i * kSurvey), n, a.wide);
     top = fmaxf(top, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
     vals4[tid + i * kSurvey] = v;
   }
@@ -714,7 +738,9 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
     bottom = fminf(bottom, bottoms[i]);
   }
   // the q-th largest of the threads' largest, by its bin
-  const int q = min(max(kGiven / a.pieces, 1), kSurvey / 2);
+  // (a piece has k / pieces of the row's k largest, give or take: twice that and 12 leave one row in a million
+  // of independent logits to the last launch)
+  const int q = min((k > 0 ? 2 * min(k, kGiven) : kGiven) / a.pieces + 12, kSurvey / 2);
   const float per = (float)(kSurvey - 1) / (top - bottom);
   const uint32_t b = __float_as_uint(fminf((top - mine) * per, (float)(kSurvey - 1)) + 8388608.0f) & (kSurvey - 1);
   if (mine > -INFINITY) atomicAdd(&bins[b], 1u);
@@ -793,7 +819,7 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
 // the last launch: a border below what all pieces have given, infinities.
 __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
   __shared__ Scratch s;
-  __shared__ uint64_t keys[2 * kGiven];
+  extern __shared__ __align__(16) uint64_t keys[];  // [kMostGiven]
   __shared__ double piece_sum[kMaxPieces], warp_d[kWarps];
   __shared__ float tops[kWarps], froms[kWarps];
   __shared__ int n_keys, chosen;
@@ -942,7 +968,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
       for (int i = tid; i < n; i += kThreads) have += keys[i] >= end;
       have = block_sum(s, have);
       if (have < (uint64_t)k && from > -INFINITY) known = false;
-      else border = list_border<false>(s, keys, n, row, per_logit, end, min((uint64_t)k, have));
+      else known = (border = list_border<false>(s, keys, n, row, per_logit, end, min((uint64_t)k, have))) != 0;
     }
     if (known && p < 1.0f) {
       uint64_t mass = 0;
@@ -957,7 +983,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
       const double x = ceil(fmax((double)p, 0.0) * (double)whole);
       const uint64_t want = min(x >= 1.0 ? (uint64_t)x : (uint64_t)1, whole);
       if (mass < want) known = false;
-      else border = list_border<true>(s, keys, n, row, per_logit, border, want);
+      else known = (border = list_border<true>(s, keys, n, row, per_logit, border, want)) != 0;
     }
     // min_p alone: what is not in the list must be below it
     if (known && k == 0 && !(p < 1.0f) && from > -INFINITY && mass_of(s.table, row, from) >= least) known = false;
@@ -970,7 +996,6 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
 
 // ---- last launch: a cluster a row, whatever the options leave.
 __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args a) {
-  extern __shared__ __align__(16) float vals[];  // [kWarps * run]: this CTA's columns, -inf past them
   __shared__ Shared s;
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -982,64 +1007,36 @@ __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args
   gqd::griddep_launch_dependents();
   if (!a.todo[r]) return;
   const bool greedy = is_greedy(a, r);
-  const int k = top_k_of(a, r);
-  const float p = top_p_of(a, r), t = greedy ? 0.0f : a.temperature ? a.temperature[r] : 1.0f;
+  const int k = greedy ? 0 : top_k_of(a, r);
+  const float p = greedy ? 1.0f : top_p_of(a, r), t = greedy ? 0.0f : a.temperature ? a.temperature[r] : 1.0f;
   const float low_p = greedy || !a.min_p ? 0.0f : a.min_p[r];
   const double u = a.drawn[r];
-  const uint32_t id0 = (uint32_t)rank * a.share;
-  const int n = min(max(a.vocab - (int)id0, 0), a.share);
-  float top = -INFINITY, bottom = INFINITY;  // of the numbers (the smallest of one in four: it only scales bins)
-  {
-    const float *from = a.logits + r * a.ld + id0;
-    auto take = [](float v) { return fmaxf(v, -INFINITY) + 0.0f; };  // (a NaN is never drawn: -inf; -0 counts as 0)
-#pragma unroll 4
-    for (int c = warp * a.run + lane * 4; c < (warp + 1) * a.run; c += 128) {
-      float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-      if (a.wide && c + 3 < n) {
-        v = __ldcs(reinterpret_cast<const float4 *>(from + c));
-      } else {
-        if (c < n) v.x = from[c];
-        if (c + 1 < n) v.y = from[c + 1];
-        if (c + 2 < n) v.z = from[c + 2];
-        if (c + 3 < n) v.w = from[c + 3];
-      }
-      v = make_float4(take(v.x), take(v.y), take(v.z), take(v.w));
-      top = fmaxf(top, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
-      if (v.x > -INFINITY) bottom = fminf(bottom, v.x);
-      *reinterpret_cast<float4 *>(vals + c) = v;
-    }
-  }
+  // the row's largest, and the smallest from which on a piece has given its keys
+  float top = tid < a.pieces ? a.piece_top[r * a.pieces + tid] : -INFINITY;
+  float from = tid < a.pieces ? a.piece_from[r * a.pieces + tid] : INFINITY;
+  if (from == -INFINITY) from = INFINITY;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    bottom = fminf(bottom, __shfl_xor_sync(0xffffffffu, bottom, o));
+    from = fminf(from, __shfl_xor_sync(0xffffffffu, from, o));
   }
   if (lane == 0) {
     s.warp_top[warp] = top;
-    s.warp_bottom[warp] = bottom;
+    s.warp_from[warp] = from;
   }
   __syncthreads();
   for (int i = 0; i < kWarps; ++i) {
     top = fmaxf(top, s.warp_top[i]);
-    bottom = fminf(bottom, s.warp_bottom[i]);
+    from = fminf(from, s.warp_from[i]);
   }
-  if (tid < ctas) {
-    cluster.map_shared_rank(s.top, tid)[rank] = top;
-    cluster.map_shared_rank(s.bottom, tid)[rank] = fminf(bottom, top);
-  }
-  cluster.sync();
-  for (int i = 0; i < ctas; ++i) {
-    top = fmaxf(top, s.top[i]);
-    if (s.top[i] > -INFINITY) bottom = fminf(bottom, s.bottom[i]);
-  }
-  if (top == INFINITY) {  // only infinities are drawn: they become 0, the others -inf
-    for (int c = tid; c < kWarps * a.run; c += kThreads) vals[c] = vals[c] == INFINITY ? 0.0f : -INFINITY;
-    top = bottom = 0.0f;
-    __syncthreads();
-  }
-  const Columns columns{reinterpret_cast<const float4 *>(vals) + warp * (a.run / 4) + lane, a.run / 128, id0 + warp * a.run + lane * 4};
-  // (greedy: the limit of small temperatures, in which all that are as large as the largest are left; the
-  // first is drawn, with u = 0)
+  cluster.sync();  // (the counters above are 0 everywhere)
+  const bool infinite = top == INFINITY;
+  if (infinite) top = 0.0f;
+  const int id0 = rank * a.share;
+  const Columns columns{a.logits + r * a.ld, a.run / 128, min(id0 + a.share, a.vocab), (uint32_t)(id0 + warp * a.run + lane * 4), a.wide != 0, infinite};
+  // bins over some times the span of the keys that were given, for masses over those that have any: what lies
+  // below is one bin, which another round can cut
+  const float span = from < top && !infinite ? 4.0f * (top - from) : 64.0f, heavy = 32.0f * t;
   const Row row = row_of(top, t);
   uint64_t above = 0;
   double least = kWhole + 1.0;
@@ -1047,8 +1044,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args
     if (low_p > 0.0f) least = fmax(least, kWhole + ceil(fmin((double)low_p, 1.0) * (double)(1ull << kOne)));
     if (top > -INFINITY) {
       int round = 0;
-      // bins over the row's numbers, for masses over those that have any
-      const float span = top - bottom, heavy = 32.0f * t;
       if (k > 0) above = find_border<false>(s, columns, row, (float)(kBins - 1) / span, 0, 0.0, (uint64_t)k, round);
       if (p < 1.0f)
         above = find_border<true>(s, columns, row, (float)(kBins - 1) / fminf(span, heavy), above, fmax((double)p, 0.0), 0, round);
@@ -1084,7 +1079,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args
     double m[4];
     uint64_t w[4] = {0, 0, 0, 0};
     const uint32_t at_id = columns.id + i * 128;
-    if (above ? !kept.masses<true, true>(columns.v[i * 32], at_id, row, s.table, m) : !kept.masses<false, true>(columns.v[i * 32], at_id, row, s.table, m))
+    if (above ? !kept.masses<true, true>(columns.at(i), at_id, row, s.table, m) : !kept.masses<false, true>(columns.at(i), at_id, row, s.table, m))
       continue;
     for (int k = 0; k < 4; ++k) w[k] = (uint64_t)(m[k] - kWhole);
     const uint64_t four = (w[0] + w[1]) + (w[2] + w[3]);
@@ -1142,15 +1137,15 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
   const int64_t together = std::min<int64_t>(m, kRows);
   while (a.piece > 2048 && together * ((vocab + a.piece - 1) / a.piece) < 2 * (int64_t)ctx->num_sms) a.piece /= 2;
   a.pieces = (int)((vocab + a.piece - 1) / a.piece);
-  a.give = 2 * kGiven / a.pieces;
-  // the last launch: CTAs of a row, as few as hold it at two CTAs per SM
+  a.give = kMostGiven / a.pieces;
+  // the last launch: CTAs of a row, sixteen where that gives each two thousand columns
   int cluster = 1;
-  while (vocab > (int64_t)cluster * kTwoPerSm && cluster < kMaxCluster) cluster *= 2;
+  while (vocab > (int64_t)cluster * kMaxShare || (cluster < kMaxCluster && vocab > cluster * 2048)) cluster *= 2;
   a.share = (int)((vocab + cluster - 1) / cluster + 3) / 4 * 4;
   a.run = (a.share + kWarps * 128 - 1) / (kWarps * 128) * 128;
   // what the launches tell one another: made by the context's first call and kept, so that a recorded
   // graph's addresses stay good
-  constexpr size_t kBytes = (size_t)kRows * (kMaxPieces * 20 + 2 * kGiven * 8 + 16);
+  constexpr size_t kBytes = (size_t)kRows * (kMaxPieces * 20 + kMostGiven * 8 + 16);
   if (!ctx->sample_ws) {
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // (also while a stream is being recorded)
     GQ_CUDA_TRY(ctx, cudaThreadExchangeStreamCaptureMode(&mode));
@@ -1162,7 +1157,7 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
     }
   }
   a.piece_keys = static_cast<uint64_t *>(ctx->sample_ws);
-  a.piece_mass = a.piece_keys + (size_t)kRows * 2 * kGiven;
+  a.piece_mass = a.piece_keys + (size_t)kRows * kMostGiven;
   a.drawn = reinterpret_cast<double *>(a.piece_mass + (size_t)kRows * kMaxPieces);
   a.piece_top = reinterpret_cast<float *>(a.drawn + kRows);
   a.piece_from = a.piece_top + (size_t)kRows * kMaxPieces;
@@ -1170,7 +1165,7 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
   a.todo = a.piece_given + (size_t)kRows * kMaxPieces;
   static bool attr_set[64] = {};
   if (!attr_set[ctx->device & 63]) {
-    GQ_CUDA_TRY(ctx, cudaFuncSetAttribute(sample_requests_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMaxShare + 4 * kWarps * 128) * 4));
+    GQ_CUDA_TRY(ctx, cudaFuncSetAttribute(finish_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostGiven * 8));
     GQ_CUDA_TRY(ctx, cudaFuncSetAttribute(sample_requests_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr_set[ctx->device & 63] = true;
   }
@@ -1187,11 +1182,11 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
     b.tokens += r0;
     if (b.probs) b.probs += r0;
     GQ_CUDA_TRY(ctx, gq_launch(ctx, survey_kernel, dim3((unsigned)(rows * a.pieces)), dim3(kSurvey), (size_t)a.piece * 4, b));
-    GQ_CUDA_TRY(ctx, gq_launch(ctx, finish_kernel, dim3((unsigned)rows), dim3(kThreads), 0, b));
+    GQ_CUDA_TRY(ctx, gq_launch(ctx, finish_kernel, dim3((unsigned)rows), dim3(kThreads), (size_t)kMostGiven * 8, b));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * cluster));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = (size_t)a.run * kWarps * 4;
+    cfg.dynamicSmemBytes = 0;
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
