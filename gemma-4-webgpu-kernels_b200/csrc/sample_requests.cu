@@ -37,7 +37,7 @@ constexpr int kOne = 44;          // w = 1 is 2^44
 constexpr int kLimb = 15;         // bits of a mass that one 32-bit sum takes: a CTA has at most 2^15 columns
 constexpr int kMaxShare = 32768;  // columns of a CTA
 constexpr int kList = 2048;       // keys that are sorted
-constexpr int kFew = 128;         // keys that are compared with one another in place of that
+constexpr int kFew = 256;         // keys that are compared with one another in place of that
 constexpr int kGiven = 1024;      // keys that a row's pieces give together, about; a larger top_k has twice as many
 constexpr int kMostGiven = 4096;  // and no more
 constexpr int kSurvey = 256;      // threads that survey a piece
@@ -72,26 +72,28 @@ struct Scratch {
   union {
     uint32_t limb[3][kBins];  // sums of a mass's bits 0-14, 15-29 and 30-44 (counts: the first)
     uint64_t bin[kBins];      // the same as one number
-    struct {                  // the keys of the border's bin, and the masses of few
-      uint64_t list[kList];
-      uint64_t mass[kFew];
+    uint64_t list[kList];     // keys of some bins
+    struct {
+      uint64_t few[kFew], few_mass[kFew];
     };
   };
   double table[kTable];  // 2^(j / 16): 128 bytes, a lane's entry is on banks of its own
   uint64_t warp_sum[kWarps];
-  uint64_t border, need;
-  uint32_t bin_at, count;
+  uint64_t border, border_mass, total, need, range[2][kWarps];
+  uint32_t bin_at, bin_to, count;
 };
 
 // With what the CTAs of a cluster exchange.
 struct Shared : Scratch {
-  uint64_t whole[kBins];  // the bins of the whole row, written by every CTA of the cluster
+  uint64_t whole[kBins];  // the bins of the whole row, then the keys of all CTAs' lists: written by every CTA
+  uint64_t masses[kList]; // of those keys
   uint64_t part[kThreads];
-  uint64_t cta_sum[kMaxCluster];  // written by every CTA, as these:
-  uint32_t listed[2];  // of the first CTA: keys in the lists, in this round and the next
+  uint64_t cta_sum[kMaxCluster];  // written by every CTA, as is this:
+  uint32_t cta_count[kMaxCluster];
+  unsigned long long kept[kWarps];  // masses of the warps' columns that are kept
   float warp_top[kWarps], warp_from[kWarps];
-  uint64_t low[kWarps], high[kWarps];
 };
+static_assert(kBins >= kList && kBins >= 2 * kMaxCluster);
 
 // Order of the logits as an order of numbers (no logit is NaN here, and no zero negative).
 __device__ __forceinline__ uint32_t key_of(float v) {
@@ -152,6 +154,11 @@ __device__ __forceinline__ uint64_t mass_of(const double *table, const Row &row,
   return row.far && v == -INFINITY ? 0 : w;
 }
 
+// (called, where a key's mass is made by itself: code that runs once is bound by being fetched)
+__device__ __noinline__ uint64_t mass_of_key(const double *table, const Row row, uint64_t key) { return mass_of(table, row, logit_of(key)); }
+__device__ __forceinline__ uint64_t bits_of(double m) { return (uint64_t)__double_as_longlong(m); }
+constexpr uint64_t kWholeBits = 0x4330000000000000ull;  // of kWhole: the bits of kWhole + m are these plus m
+
 __device__ __forceinline__ uint64_t warp_sum(uint64_t v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -181,23 +188,6 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *sums, uint6
   return v;
 }
 
-// Descending sort of n (a power of two) keys by all threads.
-__device__ void sort_down(uint64_t *k, int n) {
-  for (int size = 2; size <= n; size <<= 1)
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < n / 2; i += kThreads) {
-        const int lo = 2 * i - (i & (stride - 1)), hi = lo + stride;
-        const uint64_t x = k[lo], y = k[hi];
-        if ((x < y) == ((lo & size) == 0)) {
-          k[lo] = y;
-          k[hi] = x;
-        }
-      }
-    }
-  __syncthreads();
-}
-
 // Of two logits and ids: whether the first is at or ahead of the second in the order.
 __device__ __forceinline__ bool from_on(float v, uint32_t id, float v0, uint32_t id0) { return v > v0 || (v == v0 && id <= id0); }
 
@@ -223,7 +213,7 @@ __device__ __forceinline__ float4 four_logits(const float *row, int c, int n, bo
 // of their own, so that each has the registers that it needs.
 struct Columns {
   const float *row;
-  int n, end;     // end: of this CTA's columns
+  int n, end, share;  // end: of this CTA's columns, share of them
   uint32_t id;
   bool wide, infinite;  // infinite: the row's largest is +inf; such logits become 0, the others -inf
   __device__ __forceinline__ float4 at(int i) const {
@@ -232,6 +222,22 @@ struct Columns {
       v = make_float4(v.x == INFINITY ? 0.0f : -INFINITY, v.y == INFINITY ? 0.0f : -INFINITY, v.z == INFINITY ? 0.0f : -INFINITY,
                       v.w == INFINITY ? 0.0f : -INFINITY);
     return v;
+  }
+};
+
+// A lane's columns one after another, the next two on their way.
+struct Stream {
+  const Columns &c;
+  float4 ahead[2];
+  __device__ __forceinline__ explicit Stream(const Columns &columns) : c(columns) {
+    ahead[0] = c.at(0);
+    ahead[1] = c.at(1);
+  }
+  __device__ __forceinline__ float4 take(int i) {  // i = 0, 1, ..., c.n - 1 (what is read past those is not used)
+    const float4 x = ahead[0];
+    ahead[0] = ahead[1];
+    ahead[1] = c.at(i + 2);
+    return x;
   }
 };
 
@@ -265,43 +271,41 @@ __device__ __forceinline__ void add_mass(uint32_t (*limb)[kBins], uint32_t b, ui
 
 // The first round's bins: all numbers (counts), or those from a border on (masses).
 __device__ __noinline__ void count_bins(const Columns c, const Span p, uint32_t *count) {
+  Stream next(c);
 #pragma unroll 2
   for (int i = 0; i < c.n; ++i) {
-    const float4 x = c.at(i);
+    const float4 x = next.take(i);
     const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
     for (int k = 0; k < 4; ++k)
       add_some(&count[p.first_bin(v[k])], v[k] > -INFINITY);
   }
 }
-__device__ __noinline__ void mass_bins(const Columns c, const Span p, const Row row, const double *table, uint32_t (*limb)[kBins]) {
+// Masses to some 2^-17, as shares of 2^31 of the whole: which bins the border can be in.
+__device__ __noinline__ void share_bins(const Columns c, const Span p, float rate, float unit, uint32_t *sum) {
+  Stream next(c);
 #pragma unroll 1
   for (int i = 0; i < c.n; ++i) {
-    const float4 x = c.at(i);
-    float v[4] = {x.x, x.y, x.z, x.w};
+    const float4 x = next.take(i);
+    const float v[4] = {x.x, x.y, x.z, x.w};
     const uint32_t id = c.id + i * 128;
-    bool any = false;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (p.low_v > -INFINITY && !from_on(v[k], id + k, p.low_v, p.low_id)) v[k] = -INFINITY;
-      any |= v[k] > row.least;
+      float w;  // (halves: a difference of two numbers may be infinite)
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"((0.5f * v[k] - 0.5f * p.top) * rate));
+      if (v[k] == p.top) w = 1.0f;
+      const bool in = v[k] > -INFINITY && from_on(v[k], id + k, p.low_v, p.low_id);
+      add_some(&sum[p.first_bin(v[k])], in ? __float2uint_rn(w * unit) : 0u);
     }
-    if (!__any_sync(0xffffffffu, any)) continue;
-    double m[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) m[k] = rounded_mass(table, row, v[k]);
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      add_mass(limb, p.first_bin(v[k]),
-               v[k] > row.least ? ((uint64_t)(__double2hiint(m[k]) & 0xfffff) << 32) | (uint32_t)__double2loint(m[k]) : 0);
   }
 }
 // A later round's.
 template <bool MASS>
 __device__ __noinline__ void key_bins(const Columns c, const Span p, const Row row, const double *table, uint32_t (*limb)[kBins]) {
+  Stream next(c);
 #pragma unroll 1
   for (int i = 0; i < c.n; ++i) {
-    const float4 x = c.at(i);
+    const float4 x = next.take(i);
     const float v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll 1
     for (int k = 0; k < 4; ++k) {
@@ -313,22 +317,36 @@ __device__ __noinline__ void key_bins(const Columns c, const Span p, const Row r
     }
   }
 }
-// A bin's keys to the lists of all CTAs (kList at most; the first CTA counts them).
-template <bool FIRST>
-__device__ __noinline__ void collect(const Columns c, const Span p, uint32_t bin, uint64_t *my_list, uint32_t *my_listed) {
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = (int)cluster.num_blocks(), lane = threadIdx.x & 31;
-  uint32_t *listed = cluster.map_shared_rank(my_listed, 0);
+// The keys of some bins to this CTA's list (kList at most). The masses of the bins ahead of those (SUM) are
+// added up.
+template <bool FIRST, bool SUM>
+__device__ __noinline__ uint64_t collect(const Columns c, const Span p, const Row row, const double *table, uint32_t bin, uint32_t last,
+                                         uint64_t *list, uint32_t *listed) {
+  const int lane = threadIdx.x & 31;
+  uint64_t sum = 0;
+  Stream next(c);
 #pragma unroll 1
   for (int i = 0; i < c.n; ++i) {
-    const float4 x = c.at(i);
+    const float4 x = next.take(i);
     const float v[4] = {x.x, x.y, x.z, x.w};
     const uint32_t id = c.id + i * 128;
-    uint32_t in = 0;
+    uint32_t in = 0, ahead = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (FIRST) in |= (uint32_t)(p.first_bin(v[k]) == bin) << k;
-      else in |= (uint32_t)(p.has(v[k], id + k) && p.key_bin(v[k], id + k) == bin) << k;
+      if (FIRST) {
+        const uint32_t b = p.first_bin(v[k]);
+        in |= (uint32_t)(b >= bin && b <= last) << k;
+        if (SUM) ahead |= (uint32_t)(b < bin && v[k] > row.least && from_on(v[k], id + k, p.low_v, p.low_id)) << k;
+      } else {
+        in |= (uint32_t)(p.has(v[k], id + k) && p.key_bin(v[k], id + k) == bin) << k;
+      }
+    }
+    if (SUM && __any_sync(0xffffffffu, ahead)) {
+      double m[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m[k] = rounded_mass(table, row, v[k]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum += ahead >> k & 1 ? bits_of(m[k]) - kWholeBits : 0;
     }
     if (!__any_sync(0xffffffffu, in)) continue;
 #pragma unroll 1
@@ -340,52 +358,10 @@ __device__ __noinline__ void collect(const Columns c, const Span p, uint32_t bin
       uint32_t at = 0;
       if (lane == __ffs(who) - 1) at = atomicAdd(listed, (uint32_t)__popc(who));
       at = __shfl_sync(0xffffffffu, at, __ffs(who) - 1) + __popc(who & ((1u << lane) - 1));
-      if (mine && at < (uint32_t)kList)
-        for (int r = 0; r < ctas; ++r) cluster.map_shared_rank(my_list, r)[at] = rank_key(l, id + k);
+      if (mine && at < (uint32_t)kList) list[at] = rank_key(l, id + k);
     }
   }
-}
-
-// The key of the list at which the sum of masses (or the number), from the largest key on, reaches `need`.
-template <bool MASS>
-__device__ __noinline__ uint64_t border_of(Scratch &s, int n, const Row row, uint64_t need) {
-  const int tid = threadIdx.x;
-  if (n <= kFew) {
-    // few: thread t adds up what is at or ahead of its key
-    const uint64_t key = tid < n ? s.list[tid] : 0, w = MASS ? mass_of(s.table, row, logit_of(key)) : 1ull;
-    if (tid < n) s.mass[tid] = w;
-    __syncthreads();
-    if (tid < n) {
-      uint64_t run = 0;
-      for (int i = 0; i < n; ++i) run += s.list[i] >= key ? s.mass[i] : 0;
-      if (run >= need && run - w < need) s.border = key;
-    }
-  } else {
-    int n2 = 1;
-    while (n2 < n) n2 <<= 1;
-    for (int i = n + tid; i < n2; i += kThreads) s.list[i] = 0;
-    sort_down(s.list, n2);
-    // thread t has neighbouring keys; the one whose sum reaches what is needed says so
-    const int e = (n2 + kThreads - 1) / kThreads;
-    uint64_t sum = 0;
-    for (int i = 0; i < e; ++i) {
-      const int p = tid * e + i;
-      if (p < n) sum += MASS ? mass_of(s.table, row, logit_of(s.list[p])) : 1ull;
-    }
-    uint64_t whole;
-    uint64_t run = block_scan(sum, s.warp_sum, whole) - sum;
-    if (need > run && need <= run + sum)
-      for (int i = 0; i < e; ++i) {
-        const int p = tid * e + i;
-        run += MASS ? mass_of(s.table, row, logit_of(s.list[p])) : 1ull;
-        if (run >= need) {
-          s.border = s.list[p];
-          break;
-        }
-      }
-  }
-  __syncthreads();
-  return s.border;
+  return sum;
 }
 
 // One number for each of this CTA's bins.
@@ -403,56 +379,205 @@ __device__ __forceinline__ void join_limbs(Scratch &s) {
   for (int i = 0; i < kBins / kThreads; ++i) s.bin[threadIdx.x + i * kThreads] = w[i];
 }
 
-// The bin in which the sum of bins, from the first on, reaches what is needed, and what is needed of it.
-// `wanted(total)` is asked once.
-template <typename F>
-__device__ __forceinline__ void find_bin(Scratch &s, const uint64_t *bins, F wanted, uint32_t &bin, uint64_t &need) {
+// The bin in which the sum of bins, from the first on, reaches what is needed, and what is needed of it; and the
+// bin in which it reaches more (`to`).
+__device__ __forceinline__ void find_bin(Scratch &s, const uint64_t *bins, uint64_t &need, uint64_t to, uint32_t &bin, uint32_t &last) {
   constexpr int kEach = kBins / kThreads;
   uint64_t w[kEach], mine = 0, total;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) mine += w[i] = bins[threadIdx.x * kEach + i];
   uint64_t at = block_scan(mine, s.warp_sum, total) - mine;
-  need = wanted(total);
-  if (need > at && need <= at + mine)
+  need = min(need, total);
+  if (threadIdx.x == 0 && to > total) s.bin_to = kBins - 1;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      if (need > at && need <= at + w[i]) {
-        s.bin_at = threadIdx.x * kEach + i;
-        s.need = need - at;
-      }
-      at += w[i];
+  for (int i = 0; i < kEach; ++i) {
+    if (need > at && need <= at + w[i]) {
+      s.bin_at = threadIdx.x * kEach + i;
+      s.need = need - at;
     }
+    if (to > at && to <= at + w[i]) s.bin_to = threadIdx.x * kEach + i;
+    at += w[i];
+  }
   __syncthreads();
   bin = s.bin_at;
+  last = s.bin_to;
   need = s.need;
 }
 
-// The border of the shortest beginning of the order (of the keys from `above` on) whose mass reaches `share`
-// of the whole, or whose number reaches `count`: the key of its last member.
-template <bool MASS>
-__device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, const Row row, float per_logit, uint64_t above, double share,
-                                             uint64_t count, int &round) {
+// What is looked for in a list of keys: the key at which the sum of masses, from the largest key on, reaches
+//   count: `whole`      share: x of `whole` (0: of the list's mass)      draw: more than x of the list's
+// Where the list's sum does not reach it, and `all` does not say that there is nothing else: none.
+enum class Mode { count, share, draw };
+struct Want {
+  Mode mode;
+  double x;
+  uint64_t whole;
+  bool all;
+  __device__ __forceinline__ uint64_t of(uint64_t total) const {
+    if (total == 0) return 0;
+    if (mode == Mode::draw) return min((uint64_t)(x * (double)total), total - 1) + 1;
+    uint64_t n = whole;
+    if (mode == Mode::share) {
+      const double need = ceil(fmax(x, 0.0) * (double)(whole ? whole : total));
+      n = need >= 1.0 ? (uint64_t)need : 1;
+    }
+    return n <= total ? n : all ? total : 0;
+  }
+};
+
+// That key, among the keys from `low` on with masses of `least` and up (masses null: of 1 each), and its mass in
+// s.border_mass; 0 if there is none. Drawn is in the order of the ids: a key's halves are exchanged for that, and
+// so are those of the result. The keys are cut into bins by their distance from `high` (the range is looked up
+// where high is below `end`), the one with the border again, until it has few, which are compared.
+// (One function for all three, which a row calls in turn: it is bound by its code's way to the SM.)
+__device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const uint64_t *masses, int n, uint64_t low, uint64_t least, uint64_t high,
+                                      uint64_t end, const Want want) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool turned = want.mode == Mode::draw;
+  if (high < end) {
+    uint64_t from = ~0ull, to = 0;
+    for (int i = tid; i < n; i += kThreads) {
+      from = min(from, keys[i]);
+      to = max(to, keys[i]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      from = min(from, __shfl_xor_sync(0xffffffffu, from, o));
+      to = max(to, __shfl_xor_sync(0xffffffffu, to, o));
+    }
+    if (lane == 0) {
+      s.range[0][warp] = from;
+      s.range[1][warp] = to;
+    }
+    __syncthreads();
+    for (int i = 0; i < kWarps; ++i) {
+      from = min(from, s.range[0][i]);
+      to = max(to, s.range[1][i]);
+    }
+    high = to;
+    end = from;
+  }
+  uint64_t need = 0;
+  for (bool first = true;; first = false) {
+    const int shift = max(0, 64 - __clzll((long long)((high - end) | 1)) - 11);
+    __syncthreads();  // (what was in the bins' place is read)
+#pragma unroll 4
+    for (int i = tid; i < kBins * 3; i += kThreads) (&s.limb[0][0])[i] = 0;
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    auto at = [&](int i, uint64_t &pos, uint64_t &w) -> bool {
+      const uint64_t key = keys[i];
+      w = masses ? masses[i] : 1;
+      pos = turned ? (key << 32) | (key >> 32) : key;
+      return key >= low && w >= least && pos <= high && pos >= end;
+    };
+    uint64_t pos, w;
+#pragma unroll 1
+    for (int i = tid; i < n; i += kThreads)
+      if (at(i, pos, w)) add_mass(s.limb, (uint32_t)((high - pos) >> shift), w);
+    join_limbs<true>(s);
+    __syncthreads();
+    constexpr int kEach = kBins / kThreads;
+    uint64_t mine[kEach], sum = 0, total;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) sum += mine[i] = s.bin[tid * kEach + i];
+    uint64_t run = block_scan(sum, s.warp_sum, total) - sum;
+    if (first) {
+      need = want.of(total);
+      if (tid == 0) s.total = total;
+    }
+    if (need == 0) return 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (need > run && need <= run + mine[i]) {
+        s.bin_at = tid * kEach + i;
+        s.need = need - run;
+      }
+      run += mine[i];
+    }
+    __syncthreads();
+    const uint32_t bin = s.bin_at;
+    need = s.need;
+#pragma unroll 1
+    for (int i = tid; i < n; i += kThreads)
+      if (at(i, pos, w) && (uint32_t)((high - pos) >> shift) == bin) {
+        const uint32_t to = atomicAdd(&s.count, 1u);
+        if (to < (uint32_t)kFew) {
+          s.few[to] = pos;
+          s.few_mass[to] = w;
+        }
+      }
+    __syncthreads();
+    if (s.count <= (uint32_t)kFew) break;
+    high -= (uint64_t)bin << shift;
+    end = max(end, high - (((uint64_t)1 << shift) - 1));
+  }
+  // few: what is at or ahead of a key is added up, by some neighbouring threads a key
+  const int few = (int)s.count;
+  int parts = 1;
+  while (parts < 32 && 2 * parts * few <= kThreads) parts *= 2;
+  const int at = tid / parts;
+  const uint64_t key = at < few ? s.few[at] : ~0ull;
+  uint64_t run = 0;
+  for (int i = tid & (parts - 1); i < few; i += parts) run += s.few[i] >= key ? s.few_mass[i] : 0;
+  for (int o = parts >> 1; o > 0; o >>= 1) run += __shfl_xor_sync(0xffffffffu, run, o);
+  if (at < few && run >= need && run - s.few_mass[at] < need) {
+    s.border = key;
+    s.border_mass = s.few_mass[at];
+  }
+  __syncthreads();
+  return s.border;
+}
+
+// The masses of all CTAs' warps (s.kept) together, and what is ahead of this warp's.
+__device__ __forceinline__ uint64_t cluster_sum(Shared &s, uint64_t &before) {
   cg::cluster_group cluster = cg::this_cluster();
-  const int tid = threadIdx.x;
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  uint64_t need = count;
+  __syncthreads();
+  if (threadIdx.x < ctas) {
+    uint64_t whole = 0;
+    for (int i = 0; i < kWarps; ++i) whole += s.kept[i];
+    cluster.map_shared_rank(s.cta_sum, threadIdx.x)[rank] = whole;
+  }
+  cluster.sync();
+  uint64_t total = 0;
+  before = 0;
+  for (int i = 0; i < ctas; ++i) {
+    total += s.cta_sum[i];
+    if (i < rank) before += s.cta_sum[i];
+  }
+  for (int i = 0; i < (int)threadIdx.x >> 5; ++i) before += s.kept[i];
+  return total;
+}
+
+// The border of the shortest beginning of the order (of the keys from `above` on) whose mass, or whose number,
+// reaches `need`: the key of its last member. MASS: they have the mass `whole` together; s.kept becomes the
+// warps' masses from the border on, or `summed` false.
+template <bool MASS>
+__device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, const Row row, float t, float per_logit,
+                                             uint64_t above, uint64_t whole, uint64_t need, bool &summed) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, warp = tid >> 5;
+  const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   Span span;
   span.low_v = above ? logit_of(above) : -INFINITY;
-  span.low_id = ~(uint32_t)above;
+  span.low_id = above ? ~(uint32_t)above : ~0u;
   span.high_v = INFINITY;
   span.high_id = 0;
   span.high = ~0ull;
   span.shift = -1;
   span.top = row.top;
   span.per_logit = per_logit;
-  for (;; ++round) {
+  for (;;) {
+    const bool first = span.shift < 0;
     __syncthreads();  // (what was in the bins' place is read)
-    for (int i = tid; i < kBins * (MASS ? 3 : 1); i += kThreads) (&s.limb[0][0])[i] = 0;
+    for (int i = tid; i < kBins * (MASS && !first ? 3 : 1); i += kThreads) (&s.limb[0][0])[i] = 0;
     __syncthreads();
-    if (span.shift >= 0) key_bins<MASS>(columns, span, row, s.table, s.limb);
-    else if (MASS) mass_bins(columns, span, row, s.table, s.limb);
+    if (!first) key_bins<MASS>(columns, span, row, s.table, s.limb);
+    else if (MASS) share_bins(columns, span, 2.0f * 1.44269504f / t, 0x1p75f / (float)whole, s.limb[0]);
     else count_bins(columns, span, s.limb[0]);
-    join_limbs<MASS>(s);
+    if (MASS && !first) join_limbs<true>(s);
+    else join_limbs<false>(s);
     cluster.sync();
     // every CTA adds up a share of the bins and gives it to all: `parts` threads a bin, some CTAs each
     {
@@ -476,23 +601,62 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
       }
     }
     cluster.sync();
-    uint32_t bin;
-    const bool first = span.shift < 0;
-    find_bin(s, s.whole, [&](uint64_t all) -> uint64_t {
-      if (MASS && first) {
-        const double x = ceil(share * (double)all);
-        return min(x >= 1.0 ? (uint64_t)x : (uint64_t)1, all);
-      }
-      return min(need, all);
-    }, bin, need);
-    if (rank == 0 && tid == 0) s.listed[(round + 1) & 1] = 0;
-    if (first) collect<true>(columns, span, bin, s.list, &s.listed[round & 1]);
-    else collect<false>(columns, span, bin, s.list, &s.listed[round & 1]);
+    uint32_t bin, last;
+    if (MASS && first) {
+      // shares are off by 1/2 each, and by 2^-17 where e^x is made in f32: 46 powers of 2 at most with three
+      // roundings of 2^-24, and the instruction's 2^-22. The border lies in the bins between.
+      const double aim = (double)need * (0x1p31 / (double)whole), off = 0.5 * columns.share * ctas + 0x1p15;
+      uint64_t from = aim - off > 1.0 ? (uint64_t)(aim - off) : 1;
+      find_bin(s, s.whole, from, (uint64_t)(aim + off) + 2, bin, last);
+      if (t < 1e-30f || t > 1e30f) bin = 0, last = kBins - 1;  // (e^x in f32 may be anything)
+    } else {
+      find_bin(s, s.whole, need, 0, bin, last);
+      last = bin;
+    }
+    // the bins' keys: of each CTA, then of all in every one
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    uint64_t ahead = 0;
+    if (first) ahead = collect<true, MASS>(columns, span, row, s.table, bin, last, s.list, &s.count);
+    else collect<false, false>(columns, span, row, s.table, bin, bin, s.list, &s.count);
+    if (MASS && first) {
+      ahead = warp_sum(ahead);
+      if ((tid & 31) == 0) s.kept[warp] = ahead;
+    }
+    __syncthreads();
+    if (tid < ctas) {
+      uint64_t sum = 0;
+      if (MASS && first)
+        for (int i = 0; i < kWarps; ++i) sum += s.kept[i];
+      cluster.map_shared_rank(s.cta_sum, tid)[rank] = sum;
+      cluster.map_shared_rank(s.cta_count, tid)[rank] = s.count;
+    }
     cluster.sync();
-    const uint32_t n = *cluster.map_shared_rank(&s.listed[round & 1], 0);
+    uint32_t n = 0, at = 0;
+    uint64_t sum = 0;
+    for (int i = 0; i < ctas; ++i) {
+      if (i == rank) at = n;
+      n += s.cta_count[i];
+      sum += s.cta_sum[i];
+    }
+    if (MASS && first) need = need > sum ? need - sum : 1;
+    if (n <= (uint32_t)kList)
+      for (int i = tid; i < (int)s.count * ctas; i += kThreads)
+        cluster.map_shared_rank(s.whole, i & (ctas - 1))[at + i / ctas] = s.list[i / ctas];
+    cluster.sync();
     if (n <= (uint32_t)kList) {
-      const uint64_t border = border_of<MASS>(s, (int)n, row, need);
-      ++round;
+      if (MASS)
+        for (int i = tid; i < (int)n; i += kThreads) s.masses[i] = mass_of_key(s.table, row, s.whole[i]);
+      __syncthreads();
+      const uint64_t border = pick(s, s.whole, MASS ? s.masses : nullptr, (int)n, 0, 0, 0, 1, Want{Mode::count, 0.0, need, true});
+      if (MASS && first) {
+        summed = true;
+        for (int i = tid; i < (int)n; i += kThreads) {
+          const uint32_t id = ~(uint32_t)s.whole[i] - (uint32_t)(rank * columns.share);
+          if (s.whole[i] >= border && id < (uint32_t)columns.share)
+            atomicAdd(&s.kept[id / (uint32_t)(columns.n * 128)], (unsigned long long)s.masses[i]);
+        }
+      }
       return border;
     }
     // too many: their range, from the few that are listed and the bin's own
@@ -505,7 +669,7 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const uint32_t id = columns.id + i * 128 + k;
-          if (span.first_bin(v[k]) != bin || !span.has(v[k], id)) continue;
+          if (span.first_bin(v[k]) < bin || span.first_bin(v[k]) > last || !span.has(v[k], id)) continue;
           lo = min(lo, rank_key(v[k], id));
           hi = max(hi, rank_key(v[k], id));
         }
@@ -516,13 +680,13 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
         hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
       }
       if ((tid & 31) == 0) {
-        s.low[tid >> 5] = lo;
-        s.high[tid >> 5] = hi;
+        s.range[0][warp] = lo;
+        s.range[1][warp] = hi;
       }
       __syncthreads();
       for (int i = 0; i < kWarps; ++i) {
-        lo = min(lo, s.low[i]);
-        hi = max(hi, s.high[i]);
+        lo = min(lo, s.range[0][i]);
+        hi = max(hi, s.range[1][i]);
       }
       if (tid < ctas) {
         cluster.map_shared_rank(s.whole, tid)[2 * rank] = lo;
@@ -553,13 +717,13 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
   }
 }
 
-// What the options leave: logits from a border on (LIMIT: of a mass of `least` and up). A lane's four
+// What the options leave: logits from a border on (BORDER: there is one), of a mass of `least` and up. A lane's four
 // masses, as 2^52 plus each; false where the whole warp has none.
 struct Kept {
   float v;
   uint32_t id;
   double least;
-  template <bool BORDER, bool LIMIT>
+  template <bool BORDER>
   __device__ __forceinline__ bool masses(const float4 x, uint32_t at, const Row &row, const double *table, double (&m)[4]) const {
     float l[4] = {x.x, x.y, x.z, x.w};
     if (BORDER) {
@@ -573,105 +737,32 @@ struct Kept {
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) m[k] = rounded_mass(table, row, l[k]);
-    if (LIMIT)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) m[k] = m[k] >= least ? m[k] : kWhole;
+    for (int k = 0; k < 4; ++k) m[k] = m[k] >= least ? m[k] : kWhole;
     if (row.far)
 #pragma unroll
       for (int k = 0; k < 4; ++k) m[k] = l[k] > -INFINITY ? m[k] : kWhole;
     return true;
   }
 };
-template <bool BORDER, bool LIMIT>
+template <bool BORDER>
 __device__ __noinline__ uint64_t sum_kept(const Columns c, const Kept kept, const Row row, const double *table) {
-  double sum = 0.0;  // (64 multiples of 1 up to 2^44 at most: exact)
+  uint64_t sum = 0;
+  Stream next(c);
 #pragma unroll 1
   for (int i = 0; i < c.n; ++i) {
     double m[4];
-    if (kept.masses<BORDER, LIMIT>(c.at(i), c.id + i * 128, row, table, m))
+    if (kept.masses<BORDER>(next.take(i), c.id + i * 128, row, table, m))
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum += m[k] - kWhole;
+      for (int k = 0; k < 4; ++k) sum += bits_of(m[k]) - kWholeBits;
   }
-  return (uint64_t)sum;
-}
-
-// find_border over a list of keys in this CTA alone: `need` of their masses or number, from `low` on. 0 where
-// more of them are alike than a list holds.
-template <bool MASS>
-__device__ __noinline__ uint64_t list_border(Scratch &s, const uint64_t *keys, int n, const Row row, float per_logit, uint64_t low, uint64_t need) {
-  Span span;
-  span.top = row.top;
-  span.per_logit = per_logit;
-  __syncthreads();
-  for (int i = threadIdx.x; i < kBins * (MASS ? 3 : 1); i += kThreads) (&s.limb[0][0])[i] = 0;
-  if (threadIdx.x == 0) s.count = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    if (keys[i] < low) continue;
-    const float v = logit_of(keys[i]);
-    if (MASS) add_mass(s.limb, span.first_bin(v), mass_of(s.table, row, v));
-    else atomicAdd(&s.limb[0][span.first_bin(v)], 1u);
-  }
-  join_limbs<MASS>(s);
-  __syncthreads();
-  uint32_t bin;
-  find_bin(s, s.bin, [&](uint64_t) { return need; }, bin, need);
-  for (int i = threadIdx.x; i < n; i += kThreads)
-    if (keys[i] >= low && span.first_bin(logit_of(keys[i])) == bin) {
-      const uint32_t at = atomicAdd(&s.count, 1u);
-      if (at < (uint32_t)kList) s.list[at] = keys[i];
-    }
-  __syncthreads();
-  if (s.count > (uint32_t)kList) return 0;
-  return border_of<MASS>(s, (int)s.count, row, need);
+  return sum;
 }
 
 __device__ __forceinline__ uint64_t block_sum(Scratch &s, uint64_t v) {
   uint64_t total;
   block_scan(v, s.warp_sum, total);
   return total;
-}
-
-// The token of a list of keys, from `border` on and of masses of `least` and up: the first id at which the
-// running sum passes u times the whole.
-__device__ __noinline__ void draw_from(Scratch &s, const Args &a, int64_t r, const uint64_t *keys, int n, const Row row, uint64_t border,
-                                       uint64_t least, double u) {
-  const int tid = threadIdx.x;
-  auto mass = [&](uint64_t key) -> uint64_t {
-    const uint64_t w = key >= border ? mass_of(s.table, row, logit_of(key)) : 0;
-    return w >= least ? w : 0;
-  };
-  auto bin_of = [&](uint64_t key) { return (uint32_t)~key * (uint32_t)kBins / (uint32_t)a.vocab; };  // (ids below 2^19)
-  for (int i = tid; i < kBins * 3; i += kThreads) (&s.limb[0][0])[i] = 0;
-  if (tid == 0) s.count = 0;
-  __syncthreads();
-  uint64_t mine = 0;
-  for (int i = tid; i < n; i += kThreads) {
-    const uint64_t w = mass(keys[i]);
-    if (w) add_mass(s.limb, bin_of(keys[i]), w);
-    mine += w;
-  }
-  const uint64_t total = block_sum(s, mine);
-  join_limbs<true>(s);
-  __syncthreads();
-  uint32_t bin;
-  uint64_t need;
-  find_bin(s, s.bin, [&](uint64_t) { return min((uint64_t)(u * (double)total), total - 1) + 1; }, bin, need);
-  for (int i = tid; i < n; i += kThreads)
-    if (mass(keys[i]) && bin_of(keys[i]) == bin) s.list[atomicAdd(&s.count, 1u)] = keys[i];
-  __syncthreads();
-  const int few = (int)s.count;
-  for (int i = tid; i < few; i += kThreads) {
-    const uint32_t id = ~(uint32_t)s.list[i];
-    const uint64_t w = mass(s.list[i]);
-    uint64_t run = 0;
-    for (int j = 0; j < few; ++j)
-      if (~(uint32_t)s.list[j] < id) run += mass(s.list[j]);
-    if (need > run && need <= run + w) {
-      a.tokens[r] = (int32_t)id;
-      if (a.probs) a.probs[r] = (float)((double)w / (double)total);
-    }
-  }
 }
 
 __device__ __forceinline__ double next_f64(uint64_t z) {  // of the advanced state
@@ -682,12 +773,27 @@ __device__ __forceinline__ double next_f64(uint64_t z) {  // of the advanced sta
 }
 constexpr uint64_t kStep = 0x9e3779b97f4a7c15ull;
 
-__device__ __forceinline__ bool is_greedy(const Args &a, int64_t r) { return a.temperature && !(a.temperature[r] > 0.0f); }
-__device__ __forceinline__ int top_k_of(const Args &a, int64_t r) {  // 0: all
-  const int k = a.top_k ? a.top_k[r] : 0;
-  return k > 0 && k < a.vocab ? k : 0;
+// A row's options. (All are loaded whatever the others are: their latencies overlap.)
+struct Options {
+  bool greedy;
+  int k;  // 0: all
+  float p, t, low_p;
+};
+__device__ __forceinline__ Options options_of(const Args &a, int64_t r) {
+  Options o;
+  o.t = a.temperature ? a.temperature[r] : 1.0f;
+  o.k = a.top_k ? a.top_k[r] : 0;
+  o.p = a.top_p ? a.top_p[r] : 1.0f;
+  o.low_p = a.min_p ? a.min_p[r] : 0.0f;
+  o.greedy = !(o.t > 0.0f);
+  if (o.k < 0 || o.k >= a.vocab) o.k = 0;
+  if (o.greedy) {
+    o.k = 0;
+    o.p = 1.0f;
+    o.t = o.low_p = 0.0f;
+  }
+  return o;
 }
-__device__ __forceinline__ float top_p_of(const Args &a, int64_t r) { return a.top_p ? a.top_p[r] : 1.0f; }
 
 // ---- first launch: a CTA a piece of a row. Its largest logit; where all of the row counts, its sum of
 // masses, relative to its own largest; and its largest keys, those from the q-th largest thread's largest on.
@@ -708,10 +814,11 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
   gqd::griddep_launch_dependents();
   const int id0 = piece * a.piece, n = min(a.vocab - id0, a.piece);
   const float *from = a.logits + r * a.ld + id0;
-  const bool greedy = is_greedy(a, r);
-  const int k = top_k_of(a, r);
-  const float p = top_p_of(a, r), t = greedy ? 0.0f : a.temperature ? a.temperature[r] : 1.0f;
-  const bool sum_all = !greedy && k == 0 && (p < 1.0f || !(a.min_p && a.min_p[r] > 0.0f));
+  const Options o = options_of(a, r);
+  const bool greedy = o.greedy;
+  const int k = o.k;
+  const float p = o.p, t = o.t;
+  const bool sum_all = !greedy && k == 0 && (p < 1.0f || !(o.low_p > 0.0f));
   const int steps = a.piece / (4 * kSurvey);
   float top = -INFINITY;
 #pragma unroll 4
@@ -773,20 +880,20 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
   uint64_t all = 0;
   if (sum_all && top > -INFINITY && top < INFINITY) {  // (infinities: the last launch)
     const Row row = row_of(top, t);
-    double sum = 0.0;  // (32 multiples of 1 up to 2^44: exact)
 #pragma unroll 1
     for (int i = 0; i < steps; ++i) {
       const float4 x = vals4[tid + i * kSurvey];
       const float v[4] = {x.x, x.y, x.z, x.w};
       double m[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) m[j] = rounded_mass(table, row, v[j]) - kWhole;
+      for (int j = 0; j < 4; ++j) m[j] = rounded_mass(table, row, v[j]);
       if (row.far)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m[j] = v[j] == -INFINITY ? 0.0 : m[j];
-      sum += (m[0] + m[1]) + (m[2] + m[3]);
+        for (int j = 0; j < 4; ++j) m[j] = v[j] == -INFINITY ? kWhole : m[j];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) all += bits_of(m[j]) - kWholeBits;
     }
-    all = warp_sum((uint64_t)sum);
+    all = warp_sum(all);
   }
   __syncwarp();
   uint64_t *keys = a.piece_keys + ((int64_t)r * a.pieces + piece) * a.give;
@@ -819,7 +926,9 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
 // the last launch: a border below what all pieces have given, infinities.
 __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
   __shared__ Scratch s;
-  extern __shared__ __align__(16) uint64_t keys[];  // [kMostGiven]
+  extern __shared__ __align__(16) uint64_t keys[];  // [kMostGiven], and their masses
+  uint64_t *masses = keys + kMostGiven;
+  __shared__ int starts[kMaxPieces + 1];
   __shared__ double piece_sum[kMaxPieces], warp_d[kWarps];
   __shared__ float tops[kWarps], froms[kWarps];
   __shared__ int n_keys, chosen;
@@ -833,22 +942,29 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
   }
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
-  const bool greedy = is_greedy(a, r);
-  const int k = greedy ? 0 : top_k_of(a, r);
-  const float p = greedy ? 1.0f : top_p_of(a, r), t = greedy ? 0.0f : a.temperature ? a.temperature[r] : 1.0f;
-  const float low_p = greedy || !a.min_p ? 0.0f : a.min_p[r];
-  double u = 0.0;
-  if (!greedy) {
-    if (a.rng) u = next_f64(a.rng[r] + kStep);
-    else u = a.uniforms[r];
-    u = u >= 0.0 ? fmin(u, 1.0 - 0x1p-53) : 0.0;
-  }
+  // all that may be needed is loaded at once
+  const Options o = options_of(a, r);
+  const uint64_t state = a.rng ? a.rng[r] : 0;
+  const double given_u = a.rng ? 0.0 : a.uniforms[r];
   const int64_t at0 = r * a.pieces;
   // (kMaxPieces <= kThreads: a thread a piece)
   const bool has = tid < a.pieces;
   const float my_top = has ? a.piece_top[at0 + tid] : -INFINITY;
   const int my_n = has ? a.piece_given[at0 + tid] : 0;
+  const uint64_t my_mass = has ? a.piece_mass[at0 + tid] : 0;
   float top = my_top, from = has ? a.piece_from[at0 + tid] : -INFINITY;
+  uint64_t some[kMostGiven / kThreads];
+#pragma unroll
+  for (int i = 0; i < kMostGiven / kThreads; ++i)
+    some[i] = tid + i * kThreads < a.pieces * a.give ? a.piece_keys[at0 * a.give + tid + i * kThreads] : 0;
+  const bool greedy = o.greedy;
+  const int k = o.k;
+  const float p = o.p, t = o.t, low_p = o.low_p;
+  double u = 0.0;
+  if (!greedy) {
+    u = a.rng ? next_f64(state + kStep) : given_u;
+    u = u >= 0.0 ? fmin(u, 1.0 - 0x1p-53) : 0.0;
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -865,7 +981,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
   }
   if (tid == 0) {
     a.drawn[r] = u;
-    if (a.rng && !greedy) a.rng[r] += kStep;
+    if (a.rng && !greedy) a.rng[r] = state + kStep;
     a.todo[r] = top == INFINITY;
     if (top == -INFINITY) {  // nothing that can be drawn
       a.tokens[r] = -1;
@@ -880,7 +996,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
   if (!greedy && k == 0 && !(p < 1.0f) && !(low_p > 0.0f)) {
     // all tokens: the piece in which the sum passes u times the whole, and the token in it
     double mass = 0.0;
-    if (my_top > -INFINITY) mass = (double)a.piece_mass[at0 + tid] * exp(((double)my_top - (double)top) / (double)t);
+    if (my_top > -INFINITY) mass = (double)my_mass * exp(((double)my_top - (double)top) / (double)t);
     double run = mass;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -946,70 +1062,66 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
   {
     uint64_t total;
     const uint64_t ends = block_scan((uint64_t)my_n, s.warp_sum, total);
-    if (has) s.list[tid] = ends - my_n;
-    if (tid == 0) n_keys = (int)total;
+    if (has) starts[tid + 1] = (int)ends;
+    if (tid == 0) starts[0] = 0;
     __syncthreads();
-    for (int i = tid; i < a.pieces * a.give; i += kThreads) {
-      const int piece = i / a.give, j = i - piece * a.give;
-      if (j < a.piece_given[at0 + piece]) keys[s.list[piece] + j] = a.piece_keys[at0 * a.give + i];
+#pragma unroll
+    for (int i = 0; i < kMostGiven / kThreads; ++i) {
+      const int at = tid + i * kThreads, piece = at / a.give, j = at - piece * a.give;
+      if (piece < a.pieces && j < starts[piece + 1] - starts[piece]) keys[starts[piece] + j] = some[i];
     }
     __syncthreads();
   }
-  const int n = n_keys;
-  const uint64_t end = (uint64_t)key_of(from) << 32;  // from there on the list has all
-  const float per_logit = (float)(kBins - 1) / fminf(from > -INFINITY && from < top ? top - from : 64.0f, 64.0f);
+  const int n = starts[a.pieces];
+#pragma unroll 1
+  for (int i = tid; i < n; i += kThreads) masses[i] = mass_of_key(s.table, row, keys[i]);
+  __syncthreads();
+  const uint64_t end = (uint64_t)key_of(from) << 32, high = rank_key(top, 0);  // from `end` on the list has all
+  const bool all = from == -INFINITY;
   bool known = from <= top;
   uint64_t border = end;
   if (greedy) {
     border = (uint64_t)key_of(top) << 32;
   } else if (known) {
-    if (k > 0) {
-      uint64_t have = 0;
-      for (int i = tid; i < n; i += kThreads) have += keys[i] >= end;
-      have = block_sum(s, have);
-      if (have < (uint64_t)k && from > -INFINITY) known = false;
-      else known = (border = list_border<false>(s, keys, n, row, per_logit, end, min((uint64_t)k, have))) != 0;
-    }
+    if (k > 0) known = (border = pick(s, keys, nullptr, n, end, 0, high, end, Want{Mode::count, 0.0, (uint64_t)k, all})) != 0;
     if (known && p < 1.0f) {
-      uint64_t mass = 0;
-      for (int i = tid; i < n; i += kThreads)
-        if (keys[i] >= border) mass += mass_of(s.table, row, logit_of(keys[i]));
-      mass = block_sum(s, mass);
-      uint64_t whole = mass;
+      uint64_t whole = 0;
       if (k == 0) {
         const double f = my_top > -INFINITY ? exp(((double)my_top - (double)top) / (double)t) : 0.0;
-        whole = block_sum(s, has ? (uint64_t)((double)a.piece_mass[at0 + tid] * f) : 0);
+        whole = block_sum(s, has ? (uint64_t)((double)my_mass * f) : 0);
       }
-      const double x = ceil(fmax((double)p, 0.0) * (double)whole);
-      const uint64_t want = min(x >= 1.0 ? (uint64_t)x : (uint64_t)1, whole);
-      if (mass < want) known = false;
-      else known = (border = list_border<true>(s, keys, n, row, per_logit, border, want)) != 0;
+      known = (border = pick(s, keys, masses, n, border, 0, high, border, Want{Mode::share, (double)p, whole, false})) != 0;
     }
     // min_p alone: what is not in the list must be below it
-    if (known && k == 0 && !(p < 1.0f) && from > -INFINITY && mass_of(s.table, row, from) >= least) known = false;
+    if (known && k == 0 && !(p < 1.0f) && !all && mass_of_key(s.table, row, end) >= least) known = false;
   }
-  __syncthreads();
-  if (known) draw_from(s, a, r, keys, n, row, border, least, u);
-  else if (tid == 0) a.todo[r] = 1;
-  if (known && greedy && tid == 0 && a.probs) a.probs[r] = 1.0f;
+  if (!known) {
+    if (tid == 0) a.todo[r] = 1;
+    return;
+  }
+  const uint64_t drawn = pick(s, keys, masses, n, border, least, ~0ull << 32 | ~0u, (uint64_t)~(uint32_t)a.vocab << 32, Want{Mode::draw, u, 0, true});
+  if (tid == 0) {
+    a.tokens[r] = (int32_t)~(uint32_t)(drawn >> 32);
+    if (a.probs) a.probs[r] = greedy ? 1.0f : (float)((double)s.border_mass / (double)s.total);
+  }
 }
 
 // ---- last launch: a cluster a row, whatever the options leave.
 __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args a) {
-  __shared__ Shared s;
+  extern __shared__ __align__(16) uint8_t of_cta[];
+  Shared &s = *reinterpret_cast<Shared *>(of_cta);
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
   const int64_t r = blockIdx.x / ctas;
   if (tid < kTable) s.table[tid] = exp2((double)tid / kTable);
-  if (tid < 2) s.listed[tid] = 0;
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
   if (!a.todo[r]) return;
-  const bool greedy = is_greedy(a, r);
-  const int k = greedy ? 0 : top_k_of(a, r);
-  const float p = greedy ? 1.0f : top_p_of(a, r), t = greedy ? 0.0f : a.temperature ? a.temperature[r] : 1.0f;
-  const float low_p = greedy || !a.min_p ? 0.0f : a.min_p[r];
+  const Options o = options_of(a, r);
+  const bool greedy = o.greedy;
+  const int k = o.k;
+  const float p = o.p, t = o.t, low_p = o.low_p;
   const double u = a.drawn[r];
   // the row's largest, and the smallest from which on a piece has given its keys
   float top = tid < a.pieces ? a.piece_top[r * a.pieces + tid] : -INFINITY;
@@ -1029,58 +1141,62 @@ __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args
     top = fmaxf(top, s.warp_top[i]);
     from = fminf(from, s.warp_from[i]);
   }
-  cluster.sync();  // (the counters above are 0 everywhere)
+  cluster.sync();  // (all have begun)
   const bool infinite = top == INFINITY;
   if (infinite) top = 0.0f;
   const int id0 = rank * a.share;
-  const Columns columns{a.logits + r * a.ld, a.run / 128, min(id0 + a.share, a.vocab), (uint32_t)(id0 + warp * a.run + lane * 4), a.wide != 0, infinite};
+  const Columns columns{a.logits + r * a.ld, a.run / 128, min(id0 + a.share, a.vocab), a.share, (uint32_t)(id0 + warp * a.run + lane * 4), a.wide != 0, infinite};
   // bins over some times the span of the keys that were given, for masses over those that have any: what lies
   // below is one bin, which another round can cut
   const float span = from < top && !infinite ? 4.0f * (top - from) : 64.0f, heavy = 32.0f * t;
   const Row row = row_of(top, t);
-  uint64_t above = 0;
+  uint64_t above = 0, before;
   double least = kWhole + 1.0;
-  if (!greedy) {
-    if (low_p > 0.0f) least = fmax(least, kWhole + ceil(fmin((double)low_p, 1.0) * (double)(1ull << kOne)));
-    if (top > -INFINITY) {
-      int round = 0;
-      if (k > 0) above = find_border<false>(s, columns, row, (float)(kBins - 1) / span, 0, 0.0, (uint64_t)k, round);
-      if (p < 1.0f)
-        above = find_border<true>(s, columns, row, (float)(kBins - 1) / fminf(span, heavy), above, fmax((double)p, 0.0), 0, round);
+  bool summed = false;  // s.kept is the warps' masses that are kept
+  auto sum_of = [&](uint64_t border) {
+    const Kept kept{logit_of(border), ~(uint32_t)border, least};
+    uint64_t sum = 0;
+    if (top > -INFINITY) sum = border ? sum_kept<true>(columns, kept, row, s.table) : sum_kept<false>(columns, kept, row, s.table);
+    sum = warp_sum(sum);
+    if (lane == 0) s.kept[warp] = sum;
+  };
+  if (!greedy && top > -INFINITY) {
+    if (k > 0)
+      above = find_border<false>(s, columns, row, t, (float)(kBins - 1) / span, 0, 0, (uint64_t)k, summed);
+    if (p < 1.0f) {
+      uint64_t whole;
+      if (k == 0 && !infinite) {  // the pieces' masses
+        const int64_t piece = r * a.pieces + tid;
+        uint64_t part = 0;
+        if (tid < a.pieces && a.piece_top[piece] > -INFINITY)
+          part = (uint64_t)((double)a.piece_mass[piece] * exp(((double)a.piece_top[piece] - (double)top) / (double)t));
+        whole = block_sum(s, part);
+      } else {
+        sum_of(above);
+        whole = cluster_sum(s, before);
+        cluster.sync();  // (before the sums are written again)
+      }
+      const double want = ceil(fmax((double)p, 0.0) * (double)whole);
+      above = find_border<true>(s, columns, row, t, (float)(kBins - 1) / fminf(span, heavy), above, whole,
+                                min(want >= 1.0 ? (uint64_t)want : (uint64_t)1, whole), summed);
+    }
+    if (low_p > 0.0f) {
+      least = fmax(least, kWhole + ceil(fmin((double)low_p, 1.0) * (double)(1ull << kOne)));
+      summed = false;
     }
   }
-  const Kept kept{logit_of(above), ~(uint32_t)above, least};
-  uint64_t sum = 0;
-  if (top > -INFINITY) {
-    if (above) sum = sum_kept<true, true>(columns, kept, row, s.table);
-    else if (low_p > 0.0f) sum = sum_kept<false, true>(columns, kept, row, s.table);
-    else sum = sum_kept<false, false>(columns, kept, row, s.table);
-  }
-  sum = warp_sum(sum);
-  if (lane == 0) s.warp_sum[warp] = sum;
-  __syncthreads();
-  if (tid < ctas) {
-    uint64_t whole = 0;
-    for (int i = 0; i < kWarps; ++i) whole += s.warp_sum[i];
-    cluster.map_shared_rank(s.cta_sum, tid)[rank] = whole;
-  }
-  cluster.sync();
-  uint64_t total = 0, before = 0;
-  for (int i = 0; i < ctas; ++i) {
-    total += s.cta_sum[i];
-    if (i < rank) before += s.cta_sum[i];
-  }
+  if (!summed) sum_of(above);
+  const Kept kept{above ? logit_of(above) : -INFINITY, above ? ~(uint32_t)above : ~0u, least};
+  const uint64_t total = cluster_sum(s, before);
   uint64_t at = (uint64_t)(u * (double)total);
   if (total > 0) at = min(at, total - 1);
-  for (int i = 0; i < warp; ++i) before += s.warp_sum[i];
-  if (at < before || at >= before + s.warp_sum[warp]) return;
+  if (at < before || at >= before + s.kept[warp]) return;
   // the warp in whose run the sum passes `at`
   for (int i = 0; i < columns.n; ++i) {
     double m[4];
     uint64_t w[4] = {0, 0, 0, 0};
     const uint32_t at_id = columns.id + i * 128;
-    if (above ? !kept.masses<true, true>(columns.at(i), at_id, row, s.table, m) : !kept.masses<false, true>(columns.at(i), at_id, row, s.table, m))
-      continue;
+    if (!kept.masses<true>(columns.at(i), at_id, row, s.table, m)) continue;
     for (int k = 0; k < 4; ++k) w[k] = (uint64_t)(m[k] - kWhole);
     const uint64_t four = (w[0] + w[1]) + (w[2] + w[3]);
     const uint64_t incl = warp_scan(four) + before;
@@ -1165,7 +1281,8 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
   a.todo = a.piece_given + (size_t)kRows * kMaxPieces;
   static bool attr_set[64] = {};
   if (!attr_set[ctx->device & 63]) {
-    GQ_CUDA_TRY(ctx, cudaFuncSetAttribute(finish_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostGiven * 8));
+    GQ_CUDA_TRY(ctx, cudaFuncSetAttribute(finish_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostGiven * 16));
+    GQ_CUDA_TRY(ctx, cudaFuncSetAttribute(sample_requests_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared)));
     GQ_CUDA_TRY(ctx, cudaFuncSetAttribute(sample_requests_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr_set[ctx->device & 63] = true;
   }
@@ -1182,11 +1299,11 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
     b.tokens += r0;
     if (b.probs) b.probs += r0;
     GQ_CUDA_TRY(ctx, gq_launch(ctx, survey_kernel, dim3((unsigned)(rows * a.pieces)), dim3(kSurvey), (size_t)a.piece * 4, b));
-    GQ_CUDA_TRY(ctx, gq_launch(ctx, finish_kernel, dim3((unsigned)rows), dim3(kThreads), (size_t)kMostGiven * 8, b));
+    GQ_CUDA_TRY(ctx, gq_launch(ctx, finish_kernel, dim3((unsigned)rows), dim3(kThreads), (size_t)kMostGiven * 16, b));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * cluster));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = 0;
+    cfg.dynamicSmemBytes = sizeof(Shared);
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
