@@ -30,7 +30,9 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 512;     // of the second launch, a CTA a row
+constexpr int kLast = 512;        // of the last one
+constexpr int kMaxWarps = 32;
 constexpr int kMaxCluster = 16;
 constexpr int kBins = 2048;
 constexpr int kOne = 44;          // w = 1 is 2^44
@@ -41,7 +43,8 @@ constexpr int kFew = 256;         // keys that are compared with one another in 
 constexpr int kGiven = 1024;      // keys that a row's pieces give together, about; a larger top_k has twice as many
 constexpr int kMostGiven = 4096;  // and no more
 constexpr int kSurvey = 256;      // threads that survey a piece
-constexpr int kMaxPiece = 8192;
+constexpr int kMaxPiece = 8192;   // (a thread's 32 columns: a bit each)
+static_assert(kMaxPiece <= 32 * kSurvey);
 constexpr int kRows = 256;        // rows of a launch
 constexpr int kTable = 16;
 constexpr int64_t kMaxVocab = (int64_t)kMaxShare * kMaxCluster;
@@ -51,7 +54,7 @@ struct Args {
   const float *logits;
   int64_t ld;
   int vocab, share;  // share: columns of a CTA
-  int run;           // columns of a warp, a multiple of 128; kWarps * run >= share
+  int run;           // columns of a warp, a multiple of 128; kLast / 32 * run >= share
   int wide;          // rows are read 16 bytes at a time
   const float *temperature, *top_p, *min_p;
   const int32_t *top_k;
@@ -64,7 +67,8 @@ struct Args {
   float *piece_top, *piece_from;
   uint64_t *piece_mass, *piece_keys;
   int32_t *piece_given, *todo;
-  double *drawn;  // the row's random number
+  double *drawn;       // the row's random number
+  uint64_t *row_mass;  // all of a row's, where top_p asks for it
 };
 
 // What a CTA works with by itself.
@@ -78,8 +82,8 @@ struct Scratch {
     };
   };
   double table[kTable];  // 2^(j / 16): 128 bytes, a lane's entry is on banks of its own
-  uint64_t warp_sum[kWarps];
-  uint64_t border, border_mass, total, need, range[2][kWarps];
+  uint64_t warp_sum[kMaxWarps];
+  uint64_t border, border_mass, total, need, range[2][kMaxWarps];
   uint32_t bin_at, bin_to, count;
 };
 
@@ -87,11 +91,11 @@ struct Scratch {
 struct Shared : Scratch {
   uint64_t whole[kBins];  // the bins of the whole row, then the keys of all CTAs' lists: written by every CTA
   uint64_t masses[kList]; // of those keys
-  uint64_t part[kThreads];
+  uint64_t part[kLast];
   uint64_t cta_sum[kMaxCluster];  // written by every CTA, as is this:
   uint32_t cta_count[kMaxCluster];
-  unsigned long long kept[kWarps];  // masses of the warps' columns that are kept
-  float warp_top[kWarps], warp_from[kWarps];
+  unsigned long long kept[kMaxWarps];  // masses of the warps' columns that are kept
+  float warp_top[kMaxWarps], warp_from[kMaxWarps];
 };
 static_assert(kBins >= kList && kBins >= 2 * kMaxCluster);
 
@@ -173,6 +177,7 @@ __device__ __forceinline__ uint64_t warp_scan(uint64_t v) {  // inclusive
   return v;
 }
 // Inclusive scan over the block; sums[] of scratch. The total too.
+template <int NT>
 __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *sums, uint64_t &total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   v = warp_scan(v);
@@ -180,7 +185,7 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *sums, uint6
   __syncthreads();
   total = 0;
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
+  for (int i = 0; i < NT / 32; ++i) {
     if (i < warp) v += sums[i];
     total += sums[i];
   }
@@ -365,28 +370,28 @@ __device__ __noinline__ uint64_t collect(const Columns c, const Span p, const Ro
 }
 
 // One number for each of this CTA's bins.
-template <bool MASS>
+template <int NT, bool MASS>
 __device__ __forceinline__ void join_limbs(Scratch &s) {
-  uint64_t w[kBins / kThreads];
+  uint64_t w[kBins / NT];
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kBins / kThreads; ++i) {
-    const int b = threadIdx.x + i * kThreads;
+  for (int i = 0; i < kBins / NT; ++i) {
+    const int b = threadIdx.x + i * NT;
     w[i] = MASS ? s.limb[0][b] + ((uint64_t)s.limb[1][b] << kLimb) + ((uint64_t)s.limb[2][b] << (2 * kLimb)) : s.limb[0][b];
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kBins / kThreads; ++i) s.bin[threadIdx.x + i * kThreads] = w[i];
+  for (int i = 0; i < kBins / NT; ++i) s.bin[threadIdx.x + i * NT] = w[i];
 }
 
 // The bin in which the sum of bins, from the first on, reaches what is needed, and what is needed of it; and the
 // bin in which it reaches more (`to`).
 __device__ __forceinline__ void find_bin(Scratch &s, const uint64_t *bins, uint64_t &need, uint64_t to, uint32_t &bin, uint32_t &last) {
-  constexpr int kEach = kBins / kThreads;
+  constexpr int kEach = kBins / kLast;
   uint64_t w[kEach], mine = 0, total;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) mine += w[i] = bins[threadIdx.x * kEach + i];
-  uint64_t at = block_scan(mine, s.warp_sum, total) - mine;
+  uint64_t at = block_scan<kLast>(mine, s.warp_sum, total) - mine;
   need = min(need, total);
   if (threadIdx.x == 0 && to > total) s.bin_to = kBins - 1;
 #pragma unroll
@@ -430,13 +435,14 @@ struct Want {
 // so are those of the result. The keys are cut into bins by their distance from `high` (the range is looked up
 // where high is below `end`), the one with the border again, until it has few, which are compared.
 // (One function for all three, which a row calls in turn: it is bound by its code's way to the SM.)
+template <int NT>
 __device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const uint64_t *masses, int n, uint64_t low, uint64_t least, uint64_t high,
                                       uint64_t end, const Want want) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool turned = want.mode == Mode::draw;
   if (high < end) {
     uint64_t from = ~0ull, to = 0;
-    for (int i = tid; i < n; i += kThreads) {
+    for (int i = tid; i < n; i += NT) {
       from = min(from, keys[i]);
       to = max(to, keys[i]);
     }
@@ -450,7 +456,7 @@ __device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const ui
       s.range[1][warp] = to;
     }
     __syncthreads();
-    for (int i = 0; i < kWarps; ++i) {
+    for (int i = 0; i < NT / 32; ++i) {
       from = min(from, s.range[0][i]);
       to = max(to, s.range[1][i]);
     }
@@ -462,7 +468,7 @@ __device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const ui
     const int shift = max(0, 64 - __clzll((long long)((high - end) | 1)) - 11);
     __syncthreads();  // (what was in the bins' place is read)
 #pragma unroll 4
-    for (int i = tid; i < kBins * 3; i += kThreads) (&s.limb[0][0])[i] = 0;
+    for (int i = tid; i < kBins * 3; i += NT) (&s.limb[0][0])[i] = 0;
     if (tid == 0) s.count = 0;
     __syncthreads();
     auto at = [&](int i, uint64_t &pos, uint64_t &w) -> bool {
@@ -473,15 +479,15 @@ __device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const ui
     };
     uint64_t pos, w;
 #pragma unroll 1
-    for (int i = tid; i < n; i += kThreads)
+    for (int i = tid; i < n; i += NT)
       if (at(i, pos, w)) add_mass(s.limb, (uint32_t)((high - pos) >> shift), w);
-    join_limbs<true>(s);
+    join_limbs<NT, true>(s);
     __syncthreads();
-    constexpr int kEach = kBins / kThreads;
+    constexpr int kEach = kBins / NT;
     uint64_t mine[kEach], sum = 0, total;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) sum += mine[i] = s.bin[tid * kEach + i];
-    uint64_t run = block_scan(sum, s.warp_sum, total) - sum;
+    uint64_t run = block_scan<NT>(sum, s.warp_sum, total) - sum;
     if (first) {
       need = want.of(total);
       if (tid == 0) s.total = total;
@@ -499,7 +505,7 @@ __device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const ui
     const uint32_t bin = s.bin_at;
     need = s.need;
 #pragma unroll 1
-    for (int i = tid; i < n; i += kThreads)
+    for (int i = tid; i < n; i += NT)
       if (at(i, pos, w) && (uint32_t)((high - pos) >> shift) == bin) {
         const uint32_t to = atomicAdd(&s.count, 1u);
         if (to < (uint32_t)kFew) {
@@ -515,7 +521,7 @@ __device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const ui
   // few: what is at or ahead of a key is added up, by some neighbouring threads a key
   const int few = (int)s.count;
   int parts = 1;
-  while (parts < 32 && 2 * parts * few <= kThreads) parts *= 2;
+  while (parts < 32 && 2 * parts * few <= NT) parts *= 2;
   const int at = tid / parts;
   const uint64_t key = at < few ? s.few[at] : ~0ull;
   uint64_t run = 0;
@@ -536,7 +542,7 @@ __device__ __forceinline__ uint64_t cluster_sum(Shared &s, uint64_t &before) {
   __syncthreads();
   if (threadIdx.x < ctas) {
     uint64_t whole = 0;
-    for (int i = 0; i < kWarps; ++i) whole += s.kept[i];
+    for (int i = 0; i < kLast / 32; ++i) whole += s.kept[i];
     cluster.map_shared_rank(s.cta_sum, threadIdx.x)[rank] = whole;
   }
   cluster.sync();
@@ -571,19 +577,19 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
   for (;;) {
     const bool first = span.shift < 0;
     __syncthreads();  // (what was in the bins' place is read)
-    for (int i = tid; i < kBins * (MASS && !first ? 3 : 1); i += kThreads) (&s.limb[0][0])[i] = 0;
+    for (int i = tid; i < kBins * (MASS && !first ? 3 : 1); i += kLast) (&s.limb[0][0])[i] = 0;
     __syncthreads();
     if (!first) key_bins<MASS>(columns, span, row, s.table, s.limb);
     else if (MASS) share_bins(columns, span, 2.0f * 1.44269504f / t, 0x1p75f / (float)whole, s.limb[0]);
     else count_bins(columns, span, s.limb[0]);
-    if (MASS && !first) join_limbs<true>(s);
-    else join_limbs<false>(s);
+    if (MASS && !first) join_limbs<kLast, true>(s);
+    else join_limbs<kLast, false>(s);
     cluster.sync();
     // every CTA adds up a share of the bins and gives it to all: `parts` threads a bin, some CTAs each
     {
-      const int per = kBins / ctas, parts = max(1, kThreads / per), each = ctas / min(parts, ctas);
-      const int b0 = tid % min(per, kThreads), part = tid / min(per, kThreads);
-      for (int b = b0; b < per; b += kThreads) {
+      const int per = kBins / ctas, parts = max(1, kLast / per), each = ctas / min(parts, ctas);
+      const int b0 = tid % min(per, kLast), part = tid / min(per, kLast);
+      for (int b = b0; b < per; b += kLast) {
         uint64_t x[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -627,7 +633,7 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
     if (tid < ctas) {
       uint64_t sum = 0;
       if (MASS && first)
-        for (int i = 0; i < kWarps; ++i) sum += s.kept[i];
+        for (int i = 0; i < kLast / 32; ++i) sum += s.kept[i];
       cluster.map_shared_rank(s.cta_sum, tid)[rank] = sum;
       cluster.map_shared_rank(s.cta_count, tid)[rank] = s.count;
     }
@@ -641,17 +647,17 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
     }
     if (MASS && first) need = need > sum ? need - sum : 1;
     if (n <= (uint32_t)kList)
-      for (int i = tid; i < (int)s.count * ctas; i += kThreads)
+      for (int i = tid; i < (int)s.count * ctas; i += kLast)
         cluster.map_shared_rank(s.whole, i & (ctas - 1))[at + i / ctas] = s.list[i / ctas];
     cluster.sync();
     if (n <= (uint32_t)kList) {
       if (MASS)
-        for (int i = tid; i < (int)n; i += kThreads) s.masses[i] = mass_of_key(s.table, row, s.whole[i]);
+        for (int i = tid; i < (int)n; i += kLast) s.masses[i] = mass_of_key(s.table, row, s.whole[i]);
       __syncthreads();
-      const uint64_t border = pick(s, s.whole, MASS ? s.masses : nullptr, (int)n, 0, 0, 0, 1, Want{Mode::count, 0.0, need, true});
+      const uint64_t border = pick<kLast>(s, s.whole, MASS ? s.masses : nullptr, (int)n, 0, 0, 0, 1, Want{Mode::count, 0.0, need, true});
       if (MASS && first) {
         summed = true;
-        for (int i = tid; i < (int)n; i += kThreads) {
+        for (int i = tid; i < (int)n; i += kLast) {
           const uint32_t id = ~(uint32_t)s.whole[i] - (uint32_t)(rank * columns.share);
           if (s.whole[i] >= border && id < (uint32_t)columns.share)
             atomicAdd(&s.kept[id / (uint32_t)(columns.n * 128)], (unsigned long long)s.masses[i]);
@@ -684,7 +690,7 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
         s.range[1][warp] = hi;
       }
       __syncthreads();
-      for (int i = 0; i < kWarps; ++i) {
+      for (int i = 0; i < kLast / 32; ++i) {
         lo = min(lo, s.range[0][i]);
         hi = max(hi, s.range[1][i]);
       }
@@ -759,9 +765,10 @@ __device__ __noinline__ uint64_t sum_kept(const Columns c, const Kept kept, cons
   return sum;
 }
 
+template <int NT>
 __device__ __forceinline__ uint64_t block_sum(Scratch &s, uint64_t v) {
   uint64_t total;
-  block_scan(v, s.warp_sum, total);
+  block_scan<NT>(v, s.warp_sum, total);
   return total;
 }
 
@@ -896,19 +903,29 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
     all = warp_sum(all);
   }
   __syncwarp();
-  uint64_t *keys = a.piece_keys + ((int64_t)r * a.pieces + piece) * a.give;
-  if (mine >= least && mine > -INFINITY)
+  // the keys: a lane marks its own, a warp takes places for all of them
+  if (__any_sync(0xffffffffu, mine >= least && mine > -INFINITY)) {
+    uint32_t mark = 0;
     for (int i = 0; i < steps; ++i) {
       const float4 x = vals4[tid + i * kSurvey];
-      const float v[4] = {x.x, x.y, x.z, x.w};
-      if (fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) < least) continue;
-#pragma unroll 1
-      for (int j = 0; j < 4; ++j)
-        if (v[j] >= least && v[j] > -INFINITY) {
-          const uint32_t at = atomicAdd(&given, 1u);
-          if (at < (uint32_t)a.give) keys[at] = rank_key(v[j], id0 + 4 * (tid + i * kSurvey) + j);
-        }
+      mark |= (uint32_t)((x.x >= least && x.x > -INFINITY) | (x.y >= least && x.y > -INFINITY) << 1 | (x.z >= least && x.z > -INFINITY) << 2 |
+                         (x.w >= least && x.w > -INFINITY) << 3) << (4 * i);
     }
+    uint32_t to = __popc(mark);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t up = __shfl_up_sync(0xffffffffu, to, o);
+      if (lane >= o) to += up;
+    }
+    uint32_t from0 = 0;
+    if (lane == 31) from0 = atomicAdd(&given, to);
+    to += __shfl_sync(0xffffffffu, from0, 31) - __popc(mark);
+    uint64_t *keys = a.piece_keys + ((int64_t)r * a.pieces + piece) * a.give;
+    for (; mark && to < (uint32_t)a.give; mark &= mark - 1, ++to) {
+      const int i = __ffs(mark) - 1, c = 4 * (tid + (i >> 2) * kSurvey) + (i & 3);
+      keys[to] = rank_key(reinterpret_cast<const float *>(vals4)[c], id0 + c);
+    }
+  }
   if (lane == 0) sums[warp] = all;
   __syncthreads();
   if (tid == 0) {
@@ -929,8 +946,8 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
   extern __shared__ __align__(16) uint64_t keys[];  // [kMostGiven], and their masses
   uint64_t *masses = keys + kMostGiven;
   __shared__ int starts[kMaxPieces + 1];
-  __shared__ double piece_sum[kMaxPieces], warp_d[kWarps];
-  __shared__ float tops[kWarps], froms[kWarps];
+  __shared__ double piece_sum[kMaxPieces], warp_d[kThreads / 32];
+  __shared__ float tops[kThreads / 32], froms[kThreads / 32];
   __shared__ int n_keys, chosen;
   __shared__ double rest;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -975,7 +992,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
     froms[warp] = from;
   }
   __syncthreads();
-  for (int i = 0; i < kWarps; ++i) {
+  for (int i = 0; i < kThreads / 32; ++i) {
     top = fmaxf(top, tops[i]);
     from = fmaxf(from, froms[i]);  // from there on the pieces have given all
   }
@@ -1006,7 +1023,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
     if (lane == 31) warp_d[warp] = run;
     __syncthreads();
     double total = 0.0, before = 0.0;
-    for (int i = 0; i < kWarps; ++i) {
+    for (int i = 0; i < kThreads / 32; ++i) {
       if (i == warp) before = total;
       total += warp_d[i];
     }
@@ -1028,7 +1045,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
     const int id0 = piece * a.piece, n = min(a.vocab - id0, a.piece);
     const float *vals = a.logits + r * a.ld + id0;
     // a warp a run of columns
-    const int each = a.piece / kWarps;
+    const int each = a.piece / (kThreads / 32);
     auto mass_at = [&](int c) -> uint64_t {
       if (c >= n) return 0;
       const float v = fmaxf(vals[c], -INFINITY) + 0.0f;
@@ -1061,7 +1078,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
   // the keys that were given, together
   {
     uint64_t total;
-    const uint64_t ends = block_scan((uint64_t)my_n, s.warp_sum, total);
+    const uint64_t ends = block_scan<kThreads>((uint64_t)my_n, s.warp_sum, total);
     if (has) starts[tid + 1] = (int)ends;
     if (tid == 0) starts[0] = 0;
     __syncthreads();
@@ -1078,20 +1095,20 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
   __syncthreads();
   const uint64_t end = (uint64_t)key_of(from) << 32, high = rank_key(top, 0);  // from `end` on the list has all
   const bool all = from == -INFINITY;
+  uint64_t whole = 0;  // (0: of the list)
+  if (k == 0 && p < 1.0f) {
+    const double f = my_top > -INFINITY ? exp(((double)my_top - (double)top) / (double)t) : 0.0;
+    whole = block_sum<kThreads>(s, has ? (uint64_t)((double)my_mass * f) : 0);
+    if (tid == 0) a.row_mass[r] = whole;
+  }
   bool known = from <= top;
   uint64_t border = end;
   if (greedy) {
     border = (uint64_t)key_of(top) << 32;
   } else if (known) {
-    if (k > 0) known = (border = pick(s, keys, nullptr, n, end, 0, high, end, Want{Mode::count, 0.0, (uint64_t)k, all})) != 0;
-    if (known && p < 1.0f) {
-      uint64_t whole = 0;
-      if (k == 0) {
-        const double f = my_top > -INFINITY ? exp(((double)my_top - (double)top) / (double)t) : 0.0;
-        whole = block_sum(s, has ? (uint64_t)((double)my_mass * f) : 0);
-      }
-      known = (border = pick(s, keys, masses, n, border, 0, high, border, Want{Mode::share, (double)p, whole, false})) != 0;
-    }
+    if (k > 0) known = (border = pick<kThreads>(s, keys, nullptr, n, end, 0, high, end, Want{Mode::count, 0.0, (uint64_t)k, all})) != 0;
+    if (known && p < 1.0f)
+      known = (border = pick<kThreads>(s, keys, masses, n, border, 0, high, border, Want{Mode::share, (double)p, whole, false})) != 0;
     // min_p alone: what is not in the list must be below it
     if (known && k == 0 && !(p < 1.0f) && !all && mass_of_key(s.table, row, end) >= least) known = false;
   }
@@ -1099,7 +1116,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
     if (tid == 0) a.todo[r] = 1;
     return;
   }
-  const uint64_t drawn = pick(s, keys, masses, n, border, least, ~0ull << 32 | ~0u, (uint64_t)~(uint32_t)a.vocab << 32, Want{Mode::draw, u, 0, true});
+  const uint64_t drawn = pick<kThreads>(s, keys, masses, n, border, least, ~0ull << 32 | ~0u, (uint64_t)~(uint32_t)a.vocab << 32, Want{Mode::draw, u, 0, true});
   if (tid == 0) {
     a.tokens[r] = (int32_t)~(uint32_t)(drawn >> 32);
     if (a.probs) a.probs[r] = greedy ? 1.0f : (float)((double)s.border_mass / (double)s.total);
@@ -1107,7 +1124,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
 }
 
 // ---- last launch: a cluster a row, whatever the options leave.
-__global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args a) {
+__global__ void __launch_bounds__(kLast, 2) sample_requests_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t of_cta[];
   Shared &s = *reinterpret_cast<Shared *>(of_cta);
   cg::cluster_group cluster = cg::this_cluster();
@@ -1137,7 +1154,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args
     s.warp_from[warp] = from;
   }
   __syncthreads();
-  for (int i = 0; i < kWarps; ++i) {
+  for (int i = 0; i < kLast / 32; ++i) {
     top = fmaxf(top, s.warp_top[i]);
     from = fminf(from, s.warp_from[i]);
   }
@@ -1165,12 +1182,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_requests_kernel(const Args
       above = find_border<false>(s, columns, row, t, (float)(kBins - 1) / span, 0, 0, (uint64_t)k, summed);
     if (p < 1.0f) {
       uint64_t whole;
-      if (k == 0 && !infinite) {  // the pieces' masses
-        const int64_t piece = r * a.pieces + tid;
-        uint64_t part = 0;
-        if (tid < a.pieces && a.piece_top[piece] > -INFINITY)
-          part = (uint64_t)((double)a.piece_mass[piece] * exp(((double)a.piece_top[piece] - (double)top) / (double)t));
-        whole = block_sum(s, part);
+      if (k == 0 && !infinite) {
+        whole = a.row_mass[r];
       } else {
         sum_of(above);
         whole = cluster_sum(s, before);
@@ -1258,10 +1271,10 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
   int cluster = 1;
   while (vocab > (int64_t)cluster * kMaxShare || (cluster < kMaxCluster && vocab > cluster * 2048)) cluster *= 2;
   a.share = (int)((vocab + cluster - 1) / cluster + 3) / 4 * 4;
-  a.run = (a.share + kWarps * 128 - 1) / (kWarps * 128) * 128;
+  a.run = (a.share + 4 * kLast - 1) / (4 * kLast) * 128;
   // what the launches tell one another: made by the context's first call and kept, so that a recorded
   // graph's addresses stay good
-  constexpr size_t kBytes = (size_t)kRows * (kMaxPieces * 20 + kMostGiven * 8 + 16);
+  constexpr size_t kBytes = (size_t)kRows * (kMaxPieces * 20 + kMostGiven * 8 + 24);
   if (!ctx->sample_ws) {
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // (also while a stream is being recorded)
     GQ_CUDA_TRY(ctx, cudaThreadExchangeStreamCaptureMode(&mode));
@@ -1275,7 +1288,8 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
   a.piece_keys = static_cast<uint64_t *>(ctx->sample_ws);
   a.piece_mass = a.piece_keys + (size_t)kRows * kMostGiven;
   a.drawn = reinterpret_cast<double *>(a.piece_mass + (size_t)kRows * kMaxPieces);
-  a.piece_top = reinterpret_cast<float *>(a.drawn + kRows);
+  a.row_mass = reinterpret_cast<uint64_t *>(a.drawn + kRows);
+  a.piece_top = reinterpret_cast<float *>(a.row_mass + kRows);
   a.piece_from = a.piece_top + (size_t)kRows * kMaxPieces;
   a.piece_given = reinterpret_cast<int32_t *>(a.piece_from + (size_t)kRows * kMaxPieces);
   a.todo = a.piece_given + (size_t)kRows * kMaxPieces;
@@ -1302,7 +1316,7 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
     GQ_CUDA_TRY(ctx, gq_launch(ctx, finish_kernel, dim3((unsigned)rows), dim3(kThreads), (size_t)kMostGiven * 16, b));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * cluster));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kLast);
     cfg.dynamicSmemBytes = sizeof(Shared);
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[2];
