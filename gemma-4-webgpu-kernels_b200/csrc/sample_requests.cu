@@ -7,18 +7,25 @@
 //   token: in the order of the ids, the first kept one at which the running sum of w passes u * (their sum)
 //
 // All three options keep a beginning of the order, so what is left is one border: a logit and an id,
-// together a key of 64 bits. It is found without sorting the row: a histogram of counts (top-k) or masses
-// (top-p) says in which of 2048 bins the border lies, and the keys of that bin alone are sorted; where
-// they are too many (equal logits, far outliers) the bin's keys are cut into 2048 bins again. Where
-// few tokens may be enough (a small top_k, a top_p that they reach) each CTA gives its own largest to the
-// first one, which does all of this with some hundreds of keys.
+// together a key of 64 bits. It is found without sorting: a histogram of counts (top-k) or masses (top-p) over
+// 2048 bins says in which bin the border lies, and that bin is cut again until few keys are left to be
+// compared. Nor are all of a row's keys needed, mostly: three launches.
+//   survey  a CTA per piece of a row, for all SMs to read the logits: its largest, its largest keys (as many as
+//           make some 1024 of a row), and its sum of masses where the whole row's counts
+//   finish  a CTA per row, among the keys that the pieces have given; without top-k, top-p and min-p there are
+//           no keys: the piece in which the sum passes u of the whole, and the token in it
+//   last    a cluster of CTAs per row, for the rows whose border is below what the pieces have given (a top_p
+//           of a flat distribution, more equal logits than there is room for) or whose largest is infinite
 // Masses are whole numbers, w * 2^44 rounded: their sums (vocab <= 2^19) fit 64 bits and do not depend on
 // the order of additions, so atomics may add them up. The weights are made in f64: with f32's 2^-24 a
 // draw over 262144 tokens would land on a neighbour of the right token every few hundred rows; 2^-45
 // leaves less than one in 10^6.
 //
-// A row is kept in the shared memory of a cluster of CTAs, each with a share of its columns: the logits
-// are read once, and every pass over them is on chip.
+// 64 rows of 262144 logits, 67 MB, 10 us of memory traffic: 32 us with a top_k of 64, 36 with a top_p of
+// 0.95 of those or a top_k of 1000, 57 over all tokens, 102 of mixed options (survey 35, finish 19, last 50 for
+// three of the rows); 22 us for one row. The survey is bound by its instructions (issue 58%, f64 among them; the
+// logits at 1.9 TB/s), the finish by the latencies of its steps (a search 3 us, three of them), the last launch
+// by those of some passes and six cluster barriers (1.3 us each), 40 us a row: 280 us where all 64 come to it.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -31,24 +38,24 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512;     // of the second launch, a CTA a row
-constexpr int kLast = 512;        // of the last one
+constexpr int kLast = 512;        // of the last one, two on an SM (with 1024 and one, 450 us for 280 where all of 64 rows come to it)
 constexpr int kMaxWarps = 32;
-constexpr int kMaxCluster = 16;
+constexpr int kMaxCluster = 16;  // (of the last launch's CTAs: see there)
 constexpr int kBins = 2048;
 constexpr int kOne = 44;          // w = 1 is 2^44
 constexpr int kLimb = 15;         // bits of a mass that one 32-bit sum takes: a CTA has at most 2^15 columns
 constexpr int kMaxShare = 32768;  // columns of a CTA
-constexpr int kList = 2048;       // keys that are sorted
-constexpr int kFew = 256;         // keys that are compared with one another in place of that
+constexpr int kList = 2048;       // keys of a row that the last launch lists
+constexpr int kFew = 256;         // keys that are compared with one another
 constexpr int kGiven = 1024;      // keys that a row's pieces give together, about; a larger top_k has twice as many
 constexpr int kMostGiven = 4096;  // and no more
 constexpr int kSurvey = 256;      // threads that survey a piece
-constexpr int kMaxPiece = 8192;   // (a thread's 32 columns: a bit each)
+constexpr int kMaxPiece = 8192;   // (a thread's 32 columns: a bit each; with 4096 as the most, mixed options took 109 us in place of 102)
 static_assert(kMaxPiece <= 32 * kSurvey);
 constexpr int kRows = 256;        // rows of a launch
 constexpr int kTable = 16;
 constexpr int64_t kMaxVocab = (int64_t)kMaxShare * kMaxCluster;
-constexpr int kMaxPieces = 256;
+constexpr int kMaxPieces = 128;
 
 struct Args {
   const float *logits;
@@ -200,8 +207,8 @@ __device__ __forceinline__ bool from_on(float v, uint32_t id, float v0, uint32_t
 __device__ __forceinline__ float4 clean(float4 v) {
   return make_float4(fmaxf(v.x, -INFINITY) + 0.0f, fmaxf(v.y, -INFINITY) + 0.0f, fmaxf(v.z, -INFINITY) + 0.0f, fmaxf(v.w, -INFINITY) + 0.0f);
 }
-// Four logits of a row from column c on, -inf past its n columns.
-__device__ __forceinline__ float4 four_logits(const float *row, int c, int n, bool wide) {
+// Four logits of a row from column c on, -inf past its n columns, as they are.
+__device__ __forceinline__ float4 raw_logits(const float *row, int c, int n, bool wide) {
   float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
   if (wide && c + 3 < n) {
     v = *reinterpret_cast<const float4 *>(row + c);
@@ -211,7 +218,7 @@ __device__ __forceinline__ float4 four_logits(const float *row, int c, int n, bo
     if (c + 2 < n) v.z = row[c + 2];
     if (c + 3 < n) v.w = row[c + 3];
   }
-  return clean(v);
+  return v;
 }
 
 // A lane's columns of a row: four from `id` on, four 128 on, ... (n times). The passes over them are functions
@@ -222,7 +229,7 @@ struct Columns {
   uint32_t id;
   bool wide, infinite;  // infinite: the row's largest is +inf; such logits become 0, the others -inf
   __device__ __forceinline__ float4 at(int i) const {
-    float4 v = four_logits(row, (int)id + i * 128, end, wide);
+    float4 v = clean(raw_logits(row, (int)id + i * 128, end, wide));
     if (infinite)
       v = make_float4(v.x == INFINITY ? 0.0f : -INFINITY, v.y == INFINITY ? 0.0f : -INFINITY, v.z == INFINITY ? 0.0f : -INFINITY,
                       v.w == INFINITY ? 0.0f : -INFINITY);
@@ -830,10 +837,11 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
   float top = -INFINITY;
 #pragma unroll 4
   for (int i = 0; i < steps; ++i) {
-    const float4 v = four_logits(from, 4 * (tid + i * kSurvey), n, a.wide);
+    const float4 v = raw_logits(from, 4 * (tid + i * kSurvey), n, a.wide);
     top = fmaxf(top, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
     vals4[tid + i * kSurvey] = v;
   }
+  top += 0.0f;  // (0 for -0; a NaN is no maximum)
   const float mine = top;
   float bottom = mine > -INFINITY ? mine : INFINITY;
 #pragma unroll
@@ -853,8 +861,8 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
   }
   // the q-th largest of the threads' largest, by its bin
   // (a piece has k / pieces of the row's k largest, give or take: twice that and 12 leave one row in a million
-  // of independent logits to the last launch)
-  const int q = min((k > 0 ? 2 * min(k, kGiven) : kGiven) / a.pieces + 12, kSurvey / 2);
+  // of independent logits to the last launch; and a thread's largest stands for others of its own, which need room)
+  const int q = min((k > 0 ? 2 * min(k, kGiven) : kGiven) / a.pieces + 12, min(kSurvey / 2, a.give * 3 / 4));
   const float per = (float)(kSurvey - 1) / (top - bottom);
   const uint32_t b = __float_as_uint(fminf((top - mine) * per, (float)(kSurvey - 1)) + 8388608.0f) & (kSurvey - 1);
   if (mine > -INFINITY) atomicAdd(&bins[b], 1u);
@@ -896,7 +904,7 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
       for (int j = 0; j < 4; ++j) m[j] = rounded_mass(table, row, v[j]);
       if (row.far)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m[j] = v[j] == -INFINITY ? kWhole : m[j];
+        for (int j = 0; j < 4; ++j) m[j] = v[j] > -INFINITY ? m[j] : kWhole;
 #pragma unroll
       for (int j = 0; j < 4; ++j) all += bits_of(m[j]) - kWholeBits;
     }
@@ -904,12 +912,12 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
   }
   __syncwarp();
   // the keys: a lane marks its own, a warp takes places for all of them
-  if (__any_sync(0xffffffffu, mine >= least && mine > -INFINITY)) {
+  const float from_there = fmaxf(least, -3.402823466e+38f);  // (-inf is not given)
+  if (__any_sync(0xffffffffu, mine >= from_there)) {
     uint32_t mark = 0;
     for (int i = 0; i < steps; ++i) {
       const float4 x = vals4[tid + i * kSurvey];
-      mark |= (uint32_t)((x.x >= least && x.x > -INFINITY) | (x.y >= least && x.y > -INFINITY) << 1 | (x.z >= least && x.z > -INFINITY) << 2 |
-                         (x.w >= least && x.w > -INFINITY) << 3) << (4 * i);
+      mark |= (uint32_t)((x.x >= from_there) | (x.y >= from_there) << 1 | (x.z >= from_there) << 2 | (x.w >= from_there) << 3) << (4 * i);
     }
     uint32_t to = __popc(mark);
 #pragma unroll
@@ -923,7 +931,7 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
     uint64_t *keys = a.piece_keys + ((int64_t)r * a.pieces + piece) * a.give;
     for (; mark && to < (uint32_t)a.give; mark &= mark - 1, ++to) {
       const int i = __ffs(mark) - 1, c = 4 * (tid + (i >> 2) * kSurvey) + (i & 3);
-      keys[to] = rank_key(reinterpret_cast<const float *>(vals4)[c], id0 + c);
+      keys[to] = rank_key(reinterpret_cast<const float *>(vals4)[c] + 0.0f, id0 + c);
     }
   }
   if (lane == 0) sums[warp] = all;
@@ -1264,10 +1272,13 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
   // pieces of a row: as large as leaves two for every SM
   a.piece = kMaxPiece;
   const int64_t together = std::min<int64_t>(m, kRows);
-  while (a.piece > 2048 && together * ((vocab + a.piece - 1) / a.piece) < 2 * (int64_t)ctx->num_sms) a.piece /= 2;
-  a.pieces = (int)((vocab + a.piece - 1) / a.piece);
+  auto pieces = [&](int piece) { return (vocab + piece - 1) / piece; };
+  while (a.piece > 2048 && together * pieces(a.piece) < 2 * (int64_t)ctx->num_sms && pieces(a.piece / 2) <= kMaxPieces) a.piece /= 2;
+  a.pieces = (int)pieces(a.piece);
   a.give = kMostGiven / a.pieces;
-  // the last launch: CTAs of a row, sixteen where that gives each two thousand columns
+  // the last launch: CTAs of a row, sixteen where that gives each two thousand columns. (Few rows come to it
+  // as a rule, and their time is the call's: 102 us with 16, 120 with 8 for three of 64 rows. Where all of them
+  // do, 8 leave less waiting: 280 and 190 us.)
   int cluster = 1;
   while (vocab > (int64_t)cluster * kMaxShare || (cluster < kMaxCluster && vocab > cluster * 2048)) cluster *= 2;
   a.share = (int)((vocab + cluster - 1) / cluster + 3) / 4 * 4;
