@@ -669,6 +669,7 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
           if (s.whole[i] >= border && id < (uint32_t)columns.share)
             atomicAdd(&s.kept[id / (uint32_t)(columns.n * 128)], (unsigned long long)s.masses[i]);
         }
+        __syncthreads();  // (a caller may write the sums anew)
       }
       return border;
     }

@@ -206,6 +206,9 @@ def test_recorded_and_on_two_contexts():
             s["u"].copy_(torch.rand(m, dtype=torch.float64))
             s["x"].mul_(1.05)
         torch.cuda.synchronize()
+        if i == 3:  # (a larger call of the same contexts meanwhile)
+            for g, s in work:
+                g.sample_requests(torch.zeros(300, v, device=g.torch_device), uniforms=torch.zeros(300, dtype=torch.float64, device=g.torch_device))
         for g, s in work:
             g.replay(s["graph"])
         for g, s in work:
@@ -216,6 +219,36 @@ def test_recorded_and_on_two_contexts():
     for g, s in work:
         g.destroy_graph(s["graph"])
         g.close()
+
+
+@pytest.mark.parametrize("v", [20011, 262144])
+def test_borders_that_lie_far_down(g, v):
+    """Options that leave more tokens than the pieces of a row give by themselves."""
+    rng = np.random.default_rng(v + 1)
+    m = 20
+    x = rng.standard_normal((m, v)).astype(np.float32)
+    x[4:8] = np.sort(x[4:8], axis=1)[:, ::-1]  # all that counts in the first columns
+    x[8:12] *= 1e-3
+    x[10:12, :3000] = 0.5  # many of one kind at the border, and outliers above them
+    x[10:12, 5] = [9.0, 300.0]
+    x[12, [3, v // 2, v - 1]] = np.inf
+    x[13, rng.random(v) < 0.7] = np.inf
+    x[14, ::3] = np.nan
+    x[15] = np.where(rng.random(v) < 0.5, -np.inf, x[15])
+    x[16:18] = rng.standard_cauchy((2, v)).astype(np.float32)
+    x[18:] = rng.random((2, v)).astype(np.float32) * np.float32(1e38)
+    t = np.ones(m, np.float32)
+    t[18:] = 1e37
+    f = lambda a, dt=np.float32: np.full(m, a, dt)  # noqa: E731
+    for p in (0.3, 0.95, 0.9999999):
+        check(g, x, t, p=f(p), u=rng.random(m))
+    _, left = check(g, x, t, f(v // 3, np.int32), u=rng.random(m))
+    assert left[0] == v // 3
+    check(g, x, t, f(v // 3, np.int32), f(0.9), u=rng.random(m))
+    check(g, x, t, f(5000, np.int32), f(0.99), f(1e-3), u=rng.random(m))
+    check(g, x, t, p=f(0.9), low=f(0.05), u=rng.random(m))
+    check(g, x, t, low=f(0.02), u=rng.random(m))
+    check(g, x[:18], 30 * t[:18], p=f(0.5)[:18], u=rng.random(18))
 
 
 def test_refusals(g):
