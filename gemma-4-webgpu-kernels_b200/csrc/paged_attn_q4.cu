@@ -13,8 +13,16 @@
 //     instruction's rows stand for is free, so a lane reads 16 bytes of one key and uses all of them.
 //     For V the codes of two keys are put side by side (one byte, two keys) before they become f16.
 //   * A key that is not visible gets the scale 0 (a code is never NaN): nothing is cleared.
-// Copies are untiled bulk copies, one per page (or part of a page) of 32 keys, into a ring of each
-// warp's own. Rows of 512 are shared by two warps, which add up their halves of the scores.
+// Copies are untiled bulk copies, one per page (or part of a page) of 32 keys, into a ring of each team's
+// own: a team is one warp, or D / 128 of 128 columns each, which add up their parts of the scores (256
+// columns a warp leave registers for three warps to a scheduler: 50.0 us in place of 47.8 for 64 requests
+// of up to 4096 keys of 512).
+//
+// 64 requests of up to 4096 keys of 512 (80 MB): 47 us; 23 of up to 10007, 4 key-value heads of 128, capped
+// scores (72 MB): 39 us; 4 of up to 131072 of 512 (205 MB): 77 us, 2.7 TB/s. Bound by the instructions: issue
+// slots 60% taken at 16 warps per SM, the matrix pipe 31%, conversions 35%. A warp has 830 for 32 keys of 128
+// columns, 320 of them conversions, products with scales and matrix products. Some 12 us of a call are not
+// keys: the cut 2, code that is run once, parts brought together 2, the join's launch 5.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -228,6 +236,7 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
   bool more = true;        // the cursor is on a tile
   bool has = false;        // this lane has a copy of it
   int page = 0, row = 0;   // of this lane's copy
+  int lhead = (lu / a.sub) << a.page_shift;  // the first row of the unit's key-value head in a page
   auto step = [&](int n) {  // n tiles on
     if (lt < 0) {
       lt = 0;
@@ -242,6 +251,7 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
         lu = 0;
         lr = range_of<kKeys>(a, visible(a, ++lb));
       }
+      lhead = (lu / a.sub) << a.page_shift;
     }
     lt += n;
     lw += n;
@@ -250,7 +260,7 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
     if (!more) return;
     const int j = (lr.tile0 + lt) * kKeys + (lane << rows_shift);
     if (lane < boxes && j < lr.hi && j + rows > lr.lo) {
-      row = ((lu / a.sub) << a.page_shift) + (j & (a.page_size - 1));
+      row = lhead + (j & (a.page_size - 1));
       page = a.table[lb * a.table_stride + (j >> a.page_shift)];  // (not looked at before its copy is due)
       has = true;
     }
@@ -636,7 +646,10 @@ int launch(gq_ctx *ctx, Args &a) {
     GQ_CUDA_TRY(ctx, cudaFuncSetAttribute(paged_q4_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     attr_set[ctx->device & 63] = true;
   }
-  // Units that cannot have many tiles get a cluster of CTAs each (see paged_attn_tc.cu).
+  // Units that cannot have many tiles get a cluster of CTAs each: no cut, no join. (One request of 333 keys 7.5 us,
+  // cut 10.2; 64 of 512 keys in a window 13.4 and 18.6; 225 of up to 62 keys, 8 heads, 20 and 25.) Where units are long
+  // or uneven a cluster waits for its longest: 64 of up to 4096 keys 59 us, cut 47. Hence 8 tiles of a CTA at the
+  // most, and not many more than equal pieces had.
   const int64_t units = (int64_t)a.batch * a.units_per_req, tiles = most_tiles(a, kKeys);
   const int slots = C::kPerSm * ctx->num_sms;
   int cluster = 8;
@@ -671,7 +684,8 @@ int launch(gq_ctx *ctx, Args &a) {
 
 }  // namespace
 
-// Head_dims of the instantiated kernels, power-of-two pages, and copies of whole 16 bytes.
+// Head_dims of the instantiated kernels, power-of-two pages, and copies of whole 16 bytes. (What is left goes
+// to the kernel that takes keys one by one: 4 requests of up to 131072 keys of 512 733 us, here 77.)
 bool gq_paged_attn_q4_supported(const gq_kv_pages *p) {
   const int64_t d = p->head_dim, stride = gq_kv_page_stride(p);
   return p->type == GQ_KV_E2M1 && (d == 64 || d == 128 || d == 256 || d == 512) && p->page_size >= 8 &&

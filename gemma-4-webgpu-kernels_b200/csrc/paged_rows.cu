@@ -8,6 +8,11 @@
 // codes is not moved onto it. Neither quotient is computed exactly for that. An interval that holds it
 // is rounded at both ends, and where the ends differ the number is compared with the middle of the
 // two, multiplied out, which is exact in f32 (few bits times few bits).
+//
+// Both directions are bound by memory traffic and, nearly as much, by instructions: with pieces of four values
+// a lane and 16-byte accesses they took a third more. 16411 tokens' rows of 512 written and read back 33 us (144 MB,
+// 4.3 TB/s; the first kernels, a piece at a time, 54), 32771 tokens' read 28 us (153 MB, 5.4 TB/s; 43). A few rows
+// take the time of their launches: 5 us.
 #include <cuda_bf16.h>
 
 #include <algorithm>
