@@ -57,6 +57,13 @@ constexpr int kTable = 16;
 constexpr int64_t kMaxVocab = (int64_t)kMaxShare * kMaxCluster;
 constexpr int kMaxPieces = 128;
 
+// 2^(j / 16)
+__constant__ double kPowers[kTable] = {
+    1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916,
+    1.189207115002721, 1.241857812073484, 1.2968395546510096, 1.3542555469368927,
+    1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543,
+    1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+
 struct Args {
   const float *logits;
   int64_t ld;
@@ -76,6 +83,7 @@ struct Args {
   int32_t *piece_given, *todo;
   double *drawn;       // the row's random number
   uint64_t *row_mass;  // all of a row's, where top_p asks for it
+  uint32_t *err;
 };
 
 // What a CTA works with by itself.
@@ -819,12 +827,17 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
   __shared__ float tops[kSurvey / 32], bottoms[kSurvey / 32];
   __shared__ uint32_t counts[kSurvey / 32], border, given;
   __shared__ uint64_t sums[kSurvey / 32];
+  __shared__ __align__(8) uint64_t arrived;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t r = blockIdx.x / a.pieces;
   const int piece = blockIdx.x - (int)r * a.pieces;
-  if (tid < kTable) table[tid] = exp2((double)tid / kTable);
+  if (tid < kTable) table[tid] = kPowers[tid];
   bins[tid] = 0;
-  if (tid == 0) given = 0;
+  if (tid == 0) {
+    given = 0;
+    gqd::mbar_init(&arrived, 1);
+    gqd::fence_mbar_init();
+  }
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
   const int id0 = piece * a.piece, n = min(a.vocab - id0, a.piece);
@@ -835,12 +848,37 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
   const float p = o.p, t = o.t;
   const bool sum_all = !greedy && k == 0 && (p < 1.0f || !(o.low_p > 0.0f));
   const int steps = a.piece / (4 * kSurvey);
+  // the piece as one copy: all of an SM's pieces are on their way at once (loads by the threads: 102 us for the
+  // mixed options, this way 96)
+  if (a.wide && n % 4 == 0) {
+    if (tid == 0) {
+      gqd::mbar_arrive_expect_tx(&arrived, (uint32_t)n * 4);
+      gqd::bulk_g2s(vals4, from, (uint32_t)n * 4, &arrived);
+    }
+    for (int i = n / 4 + tid; i < a.piece / 4; i += kSurvey) vals4[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+    __syncthreads();  // (the barrier is made)
+    if (!__syncthreads_and(gqd::mbar_wait_bounded(&arrived, 0))) {
+      // a copy that does not come: an error, and a piece without a token
+      if (tid == 0) {
+        gqd::report(a.err, GQ_DEVERR_WAIT_TIMEOUT);
+        (void)gqd::mbar_wait_bounded(&arrived, 0, 100000000ull);
+        const int64_t at = r * a.pieces + piece;
+        a.piece_top[at] = -INFINITY;
+        a.piece_from[at] = -INFINITY;
+        a.piece_given[at] = 0;
+        a.piece_mass[at] = 0;
+      }
+      return;
+    }
+  } else {
+#pragma unroll 4
+    for (int i = 0; i < steps; ++i) vals4[tid + i * kSurvey] = raw_logits(from, 4 * (tid + i * kSurvey), n, a.wide);
+  }
   float top = -INFINITY;
 #pragma unroll 4
   for (int i = 0; i < steps; ++i) {
-    const float4 v = raw_logits(from, 4 * (tid + i * kSurvey), n, a.wide);
+    const float4 v = vals4[tid + i * kSurvey];  // (its own, or what has arrived)
     top = fmaxf(top, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
-    vals4[tid + i * kSurvey] = v;
   }
   top += 0.0f;  // (0 for -0; a NaN is no maximum)
   const float mine = top;
@@ -961,7 +999,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
   __shared__ double rest;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t r = blockIdx.x;
-  if (tid < kTable) s.table[tid] = exp2((double)tid / kTable);
+  if (tid < kTable) s.table[tid] = kPowers[tid];
   if (tid == 0) {
     n_keys = 0;
     chosen = -1;
@@ -1140,7 +1178,7 @@ __global__ void __launch_bounds__(kLast, 2) sample_requests_kernel(const Args a)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
   const int64_t r = blockIdx.x / ctas;
-  if (tid < kTable) s.table[tid] = exp2((double)tid / kTable);
+  if (tid < kTable) s.table[tid] = kPowers[tid];
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
   if (!a.todo[r]) return;
@@ -1269,6 +1307,7 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
   a.rng = rng_state;
   a.tokens = tokens;
   a.probs = probs;
+  a.err = ctx->dev_err;
   a.wide = (uintptr_t)logits % 16 == 0 && ld % 4 == 0;
   // pieces of a row: as large as leaves two for every SM
   a.piece = kMaxPiece;
