@@ -21,11 +21,12 @@
 // draw over 262144 tokens would land on a neighbour of the right token every few hundred rows; 2^-45
 // leaves less than one in 10^6.
 //
-// 64 rows of 262144 logits, 67 MB, 10 us of memory traffic: 32 us with a top_k of 64, 36 with a top_p of
-// 0.95 of those or a top_k of 1000, 57 over all tokens, 102 of mixed options (survey 35, finish 19, last 50 for
-// three of the rows); 22 us for one row. The survey is bound by its instructions (issue 58%, f64 among them; the
-// logits at 1.9 TB/s), the finish by the latencies of its steps (a search 3 us, three of them), the last launch
-// by those of some passes and six cluster barriers (1.3 us each), 40 us a row: 280 us where all 64 come to it.
+// 64 rows of 262144 logits, 67 MB, 10 us of memory traffic: 30 us with a top_k of 64, 33 with a top_p of
+// 0.95 of those or a top_k of 1000, 54 over all tokens, 96 of mixed options (survey 30, finish 19, last 50 for
+// three of the rows); 22 us for one row. The survey is bound by its instructions (issue 57%, f64 among them), the
+// finish by the latencies of its steps (a search 3 us, three of them), the last launch by those of some passes
+// (8 us the one that adds up masses) and six cluster barriers (1.3 us each), 40 us a row: 270 us where all 64
+// come to it, 620 where their logits are equal.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -54,6 +55,7 @@ constexpr int kMaxPiece = 8192;   // (a thread's 32 columns: a bit each; with 40
 static_assert(kMaxPiece <= 32 * kSurvey);
 constexpr int kRows = 256;        // rows of a launch
 constexpr int kTable = 16;
+static_assert(kMaxShare <= 64 * kLast);  // (a thread's columns: a bit each)
 constexpr int64_t kMaxVocab = (int64_t)kMaxShare * kMaxCluster;
 constexpr int kMaxPieces = 128;
 
@@ -343,7 +345,7 @@ template <bool FIRST, bool SUM>
 __device__ __noinline__ uint64_t collect(const Columns c, const Span p, const Row row, const double *table, uint32_t bin, uint32_t last,
                                          uint64_t *list, uint32_t *listed) {
   const int lane = threadIdx.x & 31;
-  uint64_t sum = 0;
+  uint64_t sum = 0, mark = 0;  // a bit for each of the lane's columns
   Stream next(c);
 #pragma unroll 1
   for (int i = 0; i < c.n; ++i) {
@@ -355,12 +357,14 @@ __device__ __noinline__ uint64_t collect(const Columns c, const Span p, const Ro
     for (int k = 0; k < 4; ++k) {
       if (FIRST) {
         const uint32_t b = p.first_bin(v[k]);
-        in |= (uint32_t)(b >= bin && b <= last) << k;
-        if (SUM) ahead |= (uint32_t)(b < bin && v[k] > row.least && from_on(v[k], id + k, p.low_v, p.low_id)) << k;
+        const bool from = v[k] > -INFINITY && from_on(v[k], id + k, p.low_v, p.low_id);
+        in |= (uint32_t)(b >= bin && b <= last && from) << k;
+        if (SUM) ahead |= (uint32_t)(b < bin && v[k] > row.least && from) << k;
       } else {
         in |= (uint32_t)(p.has(v[k], id + k) && p.key_bin(v[k], id + k) == bin) << k;
       }
     }
+    mark |= (uint64_t)in << (4 * i);
     if (SUM && __any_sync(0xffffffffu, ahead)) {
       double m[4];
 #pragma unroll
@@ -368,18 +372,20 @@ __device__ __noinline__ uint64_t collect(const Columns c, const Span p, const Ro
 #pragma unroll
       for (int k = 0; k < 4; ++k) sum += ahead >> k & 1 ? bits_of(m[k]) - kWholeBits : 0;
     }
-    if (!__any_sync(0xffffffffu, in)) continue;
-#pragma unroll 1
-    for (int k = 0; k < 4; ++k) {
-      const float l = k == 0 ? v[0] : k == 1 ? v[1] : k == 2 ? v[2] : v[3];
-      const bool mine = (in >> k & 1) && (!FIRST || (l > -INFINITY && from_on(l, id + k, p.low_v, p.low_id)));
-      const uint32_t who = __ballot_sync(0xffffffffu, mine);
-      if (who == 0) continue;
-      uint32_t at = 0;
-      if (lane == __ffs(who) - 1) at = atomicAdd(listed, (uint32_t)__popc(who));
-      at = __shfl_sync(0xffffffffu, at, __ffs(who) - 1) + __popc(who & ((1u << lane) - 1));
-      if (mine && at < (uint32_t)kList) list[at] = rank_key(l, id + k);
-    }
+  }
+  const uint32_t own = __popcll(mark);
+  uint32_t to = own, from = 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t up = __shfl_up_sync(0xffffffffu, to, o);
+    if (lane >= o) to += up;
+  }
+  if (lane == 31 && to > 0) from = atomicAdd(listed, to);
+  to += __shfl_sync(0xffffffffu, from, 31) - own;
+  for (; mark && to < (uint32_t)kList; mark &= mark - 1, ++to) {
+    const int at = __ffsll((long long)mark) - 1;
+    const uint32_t id = c.id + (at >> 2) * 128 + (at & 3);
+    list[to] = rank_key(c.infinite ? 0.0f : c.row[id] + 0.0f, id);
   }
   return sum;
 }
@@ -1317,7 +1323,7 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
   a.pieces = (int)pieces(a.piece);
   a.give = kMostGiven / a.pieces;
   // the last launch: CTAs of a row, sixteen where that gives each two thousand columns. (Few rows come to it
-  // as a rule, and their time is the call's: 102 us with 16, 120 with 8 for three of 64 rows. Where all of them
+  // as a rule, and their time is the call's: 102 us with 16, 120 with 8 for three of 64 rows, before the copies. Where all of them
   // do, 8 leave less waiting: 280 and 190 us.)
   int cluster = 1;
   while (vocab > (int64_t)cluster * kMaxShare || (cluster < kMaxCluster && vocab > cluster * 2048)) cluster *= 2;
