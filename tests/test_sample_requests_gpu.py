@@ -249,6 +249,9 @@ def test_borders_that_lie_far_down(g, v):
     check(g, x, t, p=f(0.9), low=f(0.05), u=rng.random(m))
     check(g, x, t, low=f(0.02), u=rng.random(m))
     check(g, x[:18], 30 * t[:18], p=f(0.5)[:18], u=rng.random(18))
+    for far in (np.inf, 1e33, 1e-35):
+        check(g, x, f(far), p=f(0.7), u=rng.random(m))
+        check(g, x, f(far), f(6000, np.int32), f(0.7), u=rng.random(m))
 
 
 def test_refusals(g):
