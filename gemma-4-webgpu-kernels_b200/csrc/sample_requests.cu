@@ -78,11 +78,11 @@ struct Args {
   uint64_t *rng;
   int32_t *tokens;
   float *probs;
-  // what the first launch finds in each piece of a row, and whether the last one has to do the row
+  // what the first launch finds in each piece of a row
   int pieces, piece, give;  // of a row; columns of a piece; the most keys of one
   float *piece_top, *piece_from;
   uint64_t *piece_mass, *piece_keys;
-  int32_t *piece_given, *todo;
+  int32_t *piece_given, *todo, *n_todo;  // todo: rows that are left to the last launch; how many, and how many it has begun
   double *drawn;       // the row's random number
   uint64_t *row_mass;  // all of a row's, where top_p asks for it
   uint32_t *err;
@@ -111,6 +111,7 @@ struct Shared : Scratch {
   uint64_t part[kLast];
   uint64_t cta_sum[kMaxCluster];  // written by every CTA, as is this:
   uint32_t cta_count[kMaxCluster];
+  int turn;
   unsigned long long kept[kMaxWarps];  // masses of the warps' columns that are kept
   float warp_top[kMaxWarps], warp_from[kMaxWarps];
 };
@@ -846,6 +847,7 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
   }
   gqd::griddep_wait();
   gqd::griddep_launch_dependents();
+  if (blockIdx.x == 0 && tid < 2) a.n_todo[tid] = 0;
   const int id0 = piece * a.piece, n = min(a.vocab - id0, a.piece);
   const float *from = a.logits + r * a.ld + id0;
   const Options o = options_of(a, r);
@@ -1052,7 +1054,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
   if (tid == 0) {
     a.drawn[r] = u;
     if (a.rng && !greedy) a.rng[r] = state + kStep;
-    a.todo[r] = top == INFINITY;
+    if (top == INFINITY) a.todo[atomicAdd(a.n_todo, 1)] = (int)r;
     if (top == -INFINITY) {  // nothing that can be drawn
       a.tokens[r] = -1;
       if (a.probs) a.probs[r] = 0.0f;
@@ -1166,7 +1168,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
     if (known && k == 0 && !(p < 1.0f) && !all && mass_of_key(s.table, row, end) >= least) known = false;
   }
   if (!known) {
-    if (tid == 0) a.todo[r] = 1;
+    if (tid == 0) a.todo[atomicAdd(a.n_todo, 1)] = (int)r;
     return;
   }
   const uint64_t drawn = pick<kThreads>(s, keys, masses, n, border, least, ~0ull << 32 | ~0u, (uint64_t)~(uint32_t)a.vocab << 32, Want{Mode::draw, u, 0, true});
@@ -1177,17 +1179,10 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
 }
 
 // ---- last launch: a cluster a row, whatever the options leave.
-__global__ void __launch_bounds__(kLast, 2) sample_requests_kernel(const Args a) {
-  extern __shared__ __align__(16) uint8_t of_cta[];
-  Shared &s = *reinterpret_cast<Shared *>(of_cta);
+__device__ __forceinline__ void sample_row(const Args &a, Shared &s, int64_t r) {
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rank = (int)cluster.block_rank(), ctas = (int)cluster.num_blocks();
-  const int64_t r = blockIdx.x / ctas;
-  if (tid < kTable) s.table[tid] = kPowers[tid];
-  gqd::griddep_wait();
-  gqd::griddep_launch_dependents();
-  if (!a.todo[r]) return;
+  const int rank = (int)cluster.block_rank();
   const Options o = options_of(a, r);
   const bool greedy = o.greedy;
   const int k = o.k;
@@ -1211,7 +1206,6 @@ __global__ void __launch_bounds__(kLast, 2) sample_requests_kernel(const Args a)
     top = fmaxf(top, s.warp_top[i]);
     from = fminf(from, s.warp_from[i]);
   }
-  cluster.sync();  // (all have begun)
   const bool infinite = top == INFINITY;
   if (infinite) top = 0.0f;
   const int id0 = rank * a.share;
@@ -1285,6 +1279,29 @@ __global__ void __launch_bounds__(kLast, 2) sample_requests_kernel(const Args a)
   }
 }
 
+__global__ void __launch_bounds__(kLast, 1) sample_requests_kernel(const Args a) {
+  extern __shared__ __align__(16) uint8_t of_cta[];
+  Shared &s = *reinterpret_cast<Shared *>(of_cta);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = (int)cluster.num_blocks();
+  if (threadIdx.x < kTable) s.table[threadIdx.x] = kPowers[threadIdx.x];
+  gqd::griddep_wait();
+  gqd::griddep_launch_dependents();
+  const int n = *a.n_todo;
+  if (n == 0) return;
+  // a cluster takes the next row that is left, until there is none
+  for (;;) {
+    cluster.sync();  // (all have begun, and are done with the row before)
+    if (threadIdx.x == 0 && cluster.block_rank() == 0) {
+      const int i = atomicAdd(a.n_todo + 1, 1);
+      for (int c = 0; c < ctas; ++c) *cluster.map_shared_rank(&s.turn, c) = i;
+    }
+    cluster.sync();
+    if (s.turn >= n) return;
+    sample_row(a, s, a.todo[s.turn]);
+  }
+}
+
 }  // namespace
 
 extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, int64_t vocab, int64_t ld, const float *temperature,
@@ -1331,7 +1348,7 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
   a.run = (a.share + 4 * kLast - 1) / (4 * kLast) * 128;
   // what the launches tell one another: made by the context's first call and kept, so that a recorded
   // graph's addresses stay good
-  constexpr size_t kBytes = (size_t)kRows * (kMaxPieces * 20 + kMostGiven * 8 + 24);
+  constexpr size_t kBytes = (size_t)kRows * (kMaxPieces * 20 + kMostGiven * 8 + 24) + 16;
   if (!ctx->sample_ws) {
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // (also while a stream is being recorded)
     GQ_CUDA_TRY(ctx, cudaThreadExchangeStreamCaptureMode(&mode));
@@ -1350,6 +1367,7 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
   a.piece_from = a.piece_top + (size_t)kRows * kMaxPieces;
   a.piece_given = reinterpret_cast<int32_t *>(a.piece_from + (size_t)kRows * kMaxPieces);
   a.todo = a.piece_given + (size_t)kRows * kMaxPieces;
+  a.n_todo = a.todo + kRows;
   static bool attr_set[64] = {};
   if (!attr_set[ctx->device & 63]) {
     GQ_CUDA_TRY(ctx, cudaFuncSetAttribute(finish_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostGiven * 16));
@@ -1372,7 +1390,7 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
     GQ_CUDA_TRY(ctx, gq_launch(ctx, survey_kernel, dim3((unsigned)(rows * a.pieces)), dim3(kSurvey), (size_t)a.piece * 4, b));
     GQ_CUDA_TRY(ctx, gq_launch(ctx, finish_kernel, dim3((unsigned)rows), dim3(kThreads), (size_t)kMostGiven * 16, b));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * cluster));
+    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(rows, std::max(1, ctx->num_sms / cluster)) * cluster));
     cfg.blockDim = dim3(kLast);
     cfg.dynamicSmemBytes = sizeof(Shared);
     cfg.stream = ctx->stream;
