@@ -43,6 +43,7 @@ constexpr int kLast = 512;        // of the last one, two on an SM (with 1024 an
 constexpr int kMaxWarps = 32;
 constexpr int kMaxCluster = 16;  // (of the last launch's CTAs: see there)
 constexpr int kBins = 2048;
+constexpr int kFirst = 2 * kBins; // of a row's first round: sums of 32 bits
 constexpr int kOne = 44;          // w = 1 is 2^44
 constexpr int kLimb = 15;         // bits of a mass that one 32-bit sum takes: a CTA has at most 2^15 columns
 constexpr int kMaxShare = 32768;  // columns of a CTA
@@ -93,6 +94,7 @@ struct Scratch {
   union {
     uint32_t limb[3][kBins];  // sums of a mass's bits 0-14, 15-29 and 30-44 (counts: the first)
     uint64_t bin[kBins];      // the same as one number
+    uint32_t first[kFirst];   // two to a word of those
     uint64_t list[kList];     // keys of some bins
     struct {
       uint64_t few[kFew], few_mass[kFew];
@@ -273,7 +275,7 @@ struct Span {
   float top, per_logit;
   // (rounded by the addition; only the order matters, and that equal logits have equal bins)
   __device__ __forceinline__ uint32_t first_bin(float v) const {
-    return __float_as_uint(fminf((top - v) * per_logit, (float)(kBins - 1)) + 8388608.0f) & (kBins - 1);
+    return __float_as_uint(fminf((top - v) * per_logit, (float)(kFirst - 1)) + 8388608.0f) & (kFirst - 1);
   }
   __device__ __forceinline__ bool has(float v, uint32_t id) const {
     return from_on(v, id, low_v, low_id) && v > -INFINITY && from_on(high_v, high_id, v, id);
@@ -305,6 +307,7 @@ __device__ __noinline__ void count_bins(const Columns c, const Span p, uint32_t 
   }
 }
 // Masses to some 2^-17, as shares of 2^31 of the whole: which bins the border can be in.
+template <bool LOW>
 __device__ __noinline__ void share_bins(const Columns c, const Span p, float rate, float unit, uint32_t *sum) {
   Stream next(c);
 #pragma unroll 1
@@ -317,7 +320,7 @@ __device__ __noinline__ void share_bins(const Columns c, const Span p, float rat
       float w;  // (halves: a difference of two numbers may be infinite)
       asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"((0.5f * v[k] - 0.5f * p.top) * rate));
       if (v[k] == p.top) w = 1.0f;
-      const bool in = v[k] > -INFINITY && from_on(v[k], id + k, p.low_v, p.low_id);
+      const bool in = v[k] > -INFINITY && (!LOW || from_on(v[k], id + k, p.low_v, p.low_id));
       add_some(&sum[p.first_bin(v[k])], in ? __float2uint_rn(w * unit) : 0u);
     }
   }
@@ -341,8 +344,8 @@ __device__ __noinline__ void key_bins(const Columns c, const Span p, const Row r
   }
 }
 // The keys of some bins to this CTA's list (kList at most). The masses of the bins ahead of those (SUM) are
-// added up.
-template <bool FIRST, bool SUM>
+// added up. (LOW: the span has an end.)
+template <bool FIRST, bool SUM, bool LOW>
 __device__ __noinline__ uint64_t collect(const Columns c, const Span p, const Row row, const double *table, uint32_t bin, uint32_t last,
                                          uint64_t *list, uint32_t *listed) {
   const int lane = threadIdx.x & 31;
@@ -358,7 +361,7 @@ __device__ __noinline__ uint64_t collect(const Columns c, const Span p, const Ro
     for (int k = 0; k < 4; ++k) {
       if (FIRST) {
         const uint32_t b = p.first_bin(v[k]);
-        const bool from = v[k] > -INFINITY && from_on(v[k], id + k, p.low_v, p.low_id);
+        const bool from = v[k] > -INFINITY && (!LOW || from_on(v[k], id + k, p.low_v, p.low_id));
         in |= (uint32_t)(b >= bin && b <= last && from) << k;
         if (SUM) ahead |= (uint32_t)(b < bin && v[k] > row.least && from) << k;
       } else {
@@ -407,15 +410,17 @@ __device__ __forceinline__ void join_limbs(Scratch &s) {
 }
 
 // The bin in which the sum of bins, from the first on, reaches what is needed, and what is needed of it; and the
-// bin in which it reaches more (`to`).
+// bin in which it reaches more (`to`). PAIRS: of the first round's.
+template <bool PAIRS>
 __device__ __forceinline__ void find_bin(Scratch &s, const uint64_t *bins, uint64_t &need, uint64_t to, uint32_t &bin, uint32_t &last) {
-  constexpr int kEach = kBins / kLast;
+  constexpr int kEach = (PAIRS ? kFirst : kBins) / kLast;
   uint64_t w[kEach], mine = 0, total;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) mine += w[i] = bins[threadIdx.x * kEach + i];
+  for (int i = 0; i < kEach; ++i)
+    mine += w[i] = PAIRS ? reinterpret_cast<const uint32_t *>(bins)[threadIdx.x * kEach + i] : bins[threadIdx.x * kEach + i];
   uint64_t at = block_scan<kLast>(mine, s.warp_sum, total) - mine;
   need = min(need, total);
-  if (threadIdx.x == 0 && to > total) s.bin_to = kBins - 1;
+  if (threadIdx.x == 0 && to > total) s.bin_to = kEach * kLast - 1;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     if (need > at && need <= at + w[i]) {
@@ -462,7 +467,7 @@ __device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const ui
                                       uint64_t end, const Want want) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool turned = want.mode == Mode::draw;
-  if (high < end) {
+  if (high < end && n > kFew) {
     uint64_t from = ~0ull, to = 0;
     for (int i = tid; i < n; i += NT) {
       from = min(from, keys[i]);
@@ -486,7 +491,25 @@ __device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const ui
     end = from;
   }
   uint64_t need = 0;
-  for (bool first = true;; first = false) {
+  if (n <= kFew) {
+    __syncthreads();  // (what was in the keys' place is read)
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    uint64_t w = 0, total;
+    if (tid < n && keys[tid] >= low) {
+      w = masses ? masses[tid] : 1;
+      if (w < least) w = 0;
+      if (w > 0) {
+        const uint32_t to = atomicAdd(&s.count, 1u);
+        s.few[to] = turned ? (keys[tid] << 32) | (keys[tid] >> 32) : keys[tid];
+        s.few_mass[to] = w;
+      }
+    }
+    block_scan<NT>(w, s.warp_sum, total);
+    need = want.of(total);
+    if (tid == 0) s.total = total;
+    if (need == 0) return 0;
+  } else for (bool first = true;; first = false) {
     const int shift = max(0, 64 - __clzll((long long)((high - end) | 1)) - 11);
     __syncthreads();  // (what was in the bins' place is read)
 #pragma unroll 4
@@ -599,13 +622,13 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
   for (;;) {
     const bool first = span.shift < 0;
     __syncthreads();  // (what was in the bins' place is read)
-    for (int i = tid; i < kBins * (MASS && !first ? 3 : 1); i += kLast) (&s.limb[0][0])[i] = 0;
+    for (int i = tid; i < (first ? kFirst : kBins * (MASS ? 3 : 1)); i += kLast) (&s.limb[0][0])[i] = 0;
     __syncthreads();
     if (!first) key_bins<MASS>(columns, span, row, s.table, s.limb);
-    else if (MASS) share_bins(columns, span, 2.0f * 1.44269504f / t, 0x1p75f / (float)whole, s.limb[0]);
-    else count_bins(columns, span, s.limb[0]);
-    if (MASS && !first) join_limbs<kLast, true>(s);
-    else join_limbs<kLast, false>(s);
+    else if (MASS && above) share_bins<true>(columns, span, 2.0f * 1.44269504f / t, 0x1p75f / (float)whole, s.first);
+    else if (MASS) share_bins<false>(columns, span, 2.0f * 1.44269504f / t, 0x1p75f / (float)whole, s.first);
+    else count_bins(columns, span, s.first);
+    if (!first) join_limbs<kLast, MASS>(s);
     cluster.sync();
     // every CTA adds up a share of the bins and gives it to all: `parts` threads a bin, some CTAs each
     {
@@ -635,18 +658,20 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
       // roundings of 2^-24, and the instruction's 2^-22. The border lies in the bins between.
       const double aim = (double)need * (0x1p31 / (double)whole), off = 0.5 * columns.share * ctas + 0x1p15;
       uint64_t from = aim - off > 1.0 ? (uint64_t)(aim - off) : 1;
-      find_bin(s, s.whole, from, (uint64_t)(aim + off) + 2, bin, last);
-      if (t < 1e-30f || t > 1e30f) bin = 0, last = kBins - 1;  // (e^x in f32 may be anything)
+      find_bin<true>(s, s.whole, from, (uint64_t)(aim + off) + 2, bin, last);
+      if (t < 1e-30f || t > 1e30f) bin = 0, last = kFirst - 1;  // (e^x in f32 may be anything)
     } else {
-      find_bin(s, s.whole, need, 0, bin, last);
+      if (first) find_bin<true>(s, s.whole, need, 0, bin, last);
+      else find_bin<false>(s, s.whole, need, 0, bin, last);
       last = bin;
     }
     // the bins' keys: of each CTA, then of all in every one
     if (tid == 0) s.count = 0;
     __syncthreads();
     uint64_t ahead = 0;
-    if (first) ahead = collect<true, MASS>(columns, span, row, s.table, bin, last, s.list, &s.count);
-    else collect<false, false>(columns, span, row, s.table, bin, bin, s.list, &s.count);
+    if (first && MASS && above) ahead = collect<true, MASS, MASS>(columns, span, row, s.table, bin, last, s.list, &s.count);
+    else if (first) ahead = collect<true, MASS, false>(columns, span, row, s.table, bin, last, s.list, &s.count);
+    else collect<false, false, true>(columns, span, row, s.table, bin, bin, s.list, &s.count);
     if (MASS && first) {
       ahead = warp_sum(ahead);
       if ((tid & 31) == 0) s.kept[warp] = ahead;
@@ -1226,7 +1251,7 @@ __device__ __forceinline__ void sample_row(const Args &a, Shared &s, int64_t r) 
   };
   if (!greedy && top > -INFINITY) {
     if (k > 0)
-      above = find_border<false>(s, columns, row, t, (float)(kBins - 1) / span, 0, 0, (uint64_t)k, summed);
+      above = find_border<false>(s, columns, row, t, (float)(kFirst - 1) / span, 0, 0, (uint64_t)k, summed);
     if (p < 1.0f) {
       uint64_t whole;
       if (k == 0 && !infinite) {
@@ -1237,7 +1262,7 @@ __device__ __forceinline__ void sample_row(const Args &a, Shared &s, int64_t r) 
         cluster.sync();  // (before the sums are written again)
       }
       const double want = ceil(fmax((double)p, 0.0) * (double)whole);
-      above = find_border<true>(s, columns, row, t, (float)(kBins - 1) / fminf(span, heavy), above, whole,
+      above = find_border<true>(s, columns, row, t, (float)(kFirst - 1) / fminf(span, heavy), above, whole,
                                 min(want >= 1.0 ? (uint64_t)want : (uint64_t)1, whole), summed);
     }
     if (low_p > 0.0f) {
