@@ -21,12 +21,11 @@
 // draw over 262144 tokens would land on a neighbour of the right token every few hundred rows; 2^-45
 // leaves less than one in 10^6.
 //
-// 64 rows of 262144 logits, 67 MB, 10 us of memory traffic: 30 us with a top_k of 64, 33 with a top_p of
-// 0.95 of those or a top_k of 1000, 54 over all tokens, 96 of mixed options (survey 30, finish 19, last 50 for
+// 64 rows of 262144 logits, 67 MB, 10 us of memory traffic: 27 us with a top_k of 64, 30 with a top_p of
+// 0.95 of those or a top_k of 1000, 51 over all tokens, 84 of mixed options (survey 28, finish 19, last 37 for
 // three of the rows); 22 us for one row. The survey is bound by its instructions (issue 57%, f64 among them), the
-// finish by the latencies of its steps (a search 3 us, three of them), the last launch by those of some passes
-// (8 us the one that adds up masses) and six cluster barriers (1.3 us each), 40 us a row: 270 us where all 64
-// come to it, 620 where their logits are equal.
+// finish by the latencies of its steps (a search 2.5 us, three of them), the last launch by those of some passes
+// (8 us the one that adds up masses) and six cluster barriers (1.2 us each), 33 us a row.
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -38,9 +37,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;     // of the second launch, a CTA a row
-constexpr int kLast = 512;        // of the last one, two on an SM (with 1024 and one, 450 us for 280 where all of 64 rows come to it)
-constexpr int kMaxWarps = 32;
+constexpr int kThreads = 512;     // of the second and the last launch
+constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 16;  // (of the last launch's CTAs: see there)
 constexpr int kBins = 2048;
 constexpr int kFirst = 2 * kBins; // of a row's first round: sums of 32 bits
@@ -56,7 +54,7 @@ constexpr int kMaxPiece = 8192;   // (a thread's 32 columns: a bit each; with 40
 static_assert(kMaxPiece <= 32 * kSurvey);
 constexpr int kRows = 256;        // rows of a launch
 constexpr int kTable = 16;
-static_assert(kMaxShare <= 64 * kLast);  // (a thread's columns: a bit each)
+static_assert(kMaxShare <= 64 * kThreads);  // (a thread's columns: a bit each)
 constexpr int64_t kMaxVocab = (int64_t)kMaxShare * kMaxCluster;
 constexpr int kMaxPieces = 128;
 
@@ -71,7 +69,7 @@ struct Args {
   const float *logits;
   int64_t ld;
   int vocab, share;  // share: columns of a CTA
-  int run;           // columns of a warp, a multiple of 128; kLast / 32 * run >= share
+  int run;           // columns of a warp, a multiple of 128; kWarps * run >= share
   int wide;          // rows are read 16 bytes at a time
   const float *temperature, *top_p, *min_p;
   const int32_t *top_k;
@@ -101,8 +99,8 @@ struct Scratch {
     };
   };
   double table[kTable];  // 2^(j / 16): 128 bytes, a lane's entry is on banks of its own
-  uint64_t warp_sum[kMaxWarps];
-  uint64_t border, border_mass, total, need, range[2][kMaxWarps];
+  uint64_t warp_sum[kWarps];
+  uint64_t border, border_mass, total, need, range[2][kWarps];
   uint32_t bin_at, bin_to, count;
 };
 
@@ -110,12 +108,12 @@ struct Scratch {
 struct Shared : Scratch {
   uint64_t whole[kBins];  // the bins of the whole row, then the keys of all CTAs' lists: written by every CTA
   uint64_t masses[kList]; // of those keys
-  uint64_t part[kLast];
+  uint64_t part[kThreads];
   uint64_t cta_sum[kMaxCluster];  // written by every CTA, as is this:
   uint32_t cta_count[kMaxCluster];
   int turn;
-  unsigned long long kept[kMaxWarps];  // masses of the warps' columns that are kept
-  float warp_top[kMaxWarps], warp_from[kMaxWarps];
+  unsigned long long kept[kWarps];  // masses of the warps' columns that are kept
+  float warp_top[kWarps], warp_from[kWarps];
 };
 static_assert(kBins >= kList && kBins >= 2 * kMaxCluster);
 
@@ -197,7 +195,6 @@ __device__ __forceinline__ uint64_t warp_scan(uint64_t v) {  // inclusive
   return v;
 }
 // Inclusive scan over the block; sums[] of scratch. The total too.
-template <int NT>
 __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *sums, uint64_t &total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   v = warp_scan(v);
@@ -205,7 +202,7 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *sums, uint6
   __syncthreads();
   total = 0;
 #pragma unroll
-  for (int i = 0; i < NT / 32; ++i) {
+  for (int i = 0; i < kWarps; ++i) {
     if (i < warp) v += sums[i];
     total += sums[i];
   }
@@ -395,32 +392,32 @@ __device__ __noinline__ uint64_t collect(const Columns c, const Span p, const Ro
 }
 
 // One number for each of this CTA's bins.
-template <int NT, bool MASS>
+template <bool MASS>
 __device__ __forceinline__ void join_limbs(Scratch &s) {
-  uint64_t w[kBins / NT];
+  uint64_t w[kBins / kThreads];
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kBins / NT; ++i) {
-    const int b = threadIdx.x + i * NT;
+  for (int i = 0; i < kBins / kThreads; ++i) {
+    const int b = threadIdx.x + i * kThreads;
     w[i] = MASS ? s.limb[0][b] + ((uint64_t)s.limb[1][b] << kLimb) + ((uint64_t)s.limb[2][b] << (2 * kLimb)) : s.limb[0][b];
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kBins / NT; ++i) s.bin[threadIdx.x + i * NT] = w[i];
+  for (int i = 0; i < kBins / kThreads; ++i) s.bin[threadIdx.x + i * kThreads] = w[i];
 }
 
 // The bin in which the sum of bins, from the first on, reaches what is needed, and what is needed of it; and the
 // bin in which it reaches more (`to`). PAIRS: of the first round's.
 template <bool PAIRS>
 __device__ __forceinline__ void find_bin(Scratch &s, const uint64_t *bins, uint64_t &need, uint64_t to, uint32_t &bin, uint32_t &last) {
-  constexpr int kEach = (PAIRS ? kFirst : kBins) / kLast;
+  constexpr int kEach = (PAIRS ? kFirst : kBins) / kThreads;
   uint64_t w[kEach], mine = 0, total;
 #pragma unroll
   for (int i = 0; i < kEach; ++i)
     mine += w[i] = PAIRS ? reinterpret_cast<const uint32_t *>(bins)[threadIdx.x * kEach + i] : bins[threadIdx.x * kEach + i];
-  uint64_t at = block_scan<kLast>(mine, s.warp_sum, total) - mine;
+  uint64_t at = block_scan(mine, s.warp_sum, total) - mine;
   need = min(need, total);
-  if (threadIdx.x == 0 && to > total) s.bin_to = kEach * kLast - 1;
+  if (threadIdx.x == 0 && to > total) s.bin_to = kEach * kThreads - 1;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     if (need > at && need <= at + w[i]) {
@@ -462,14 +459,13 @@ struct Want {
 // so are those of the result. The keys are cut into bins by their distance from `high` (the range is looked up
 // where high is below `end`), the one with the border again, until it has few, which are compared.
 // (One function for all three, which a row calls in turn: it is bound by its code's way to the SM.)
-template <int NT>
 __device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const uint64_t *masses, int n, uint64_t low, uint64_t least, uint64_t high,
                                       uint64_t end, const Want want) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const bool turned = want.mode == Mode::draw;
   if (high < end && n > kFew) {
     uint64_t from = ~0ull, to = 0;
-    for (int i = tid; i < n; i += NT) {
+    for (int i = tid; i < n; i += kThreads) {
       from = min(from, keys[i]);
       to = max(to, keys[i]);
     }
@@ -483,7 +479,7 @@ __device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const ui
       s.range[1][warp] = to;
     }
     __syncthreads();
-    for (int i = 0; i < NT / 32; ++i) {
+    for (int i = 0; i < kWarps; ++i) {
       from = min(from, s.range[0][i]);
       to = max(to, s.range[1][i]);
     }
@@ -505,7 +501,7 @@ __device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const ui
         s.few_mass[to] = w;
       }
     }
-    block_scan<NT>(w, s.warp_sum, total);
+    block_scan(w, s.warp_sum, total);
     need = want.of(total);
     if (tid == 0) s.total = total;
     if (need == 0) return 0;
@@ -513,7 +509,7 @@ __device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const ui
     const int shift = max(0, 64 - __clzll((long long)((high - end) | 1)) - 11);
     __syncthreads();  // (what was in the bins' place is read)
 #pragma unroll 4
-    for (int i = tid; i < kBins * 3; i += NT) (&s.limb[0][0])[i] = 0;
+    for (int i = tid; i < kBins * 3; i += kThreads) (&s.limb[0][0])[i] = 0;
     if (tid == 0) s.count = 0;
     __syncthreads();
     auto at = [&](int i, uint64_t &pos, uint64_t &w) -> bool {
@@ -524,15 +520,17 @@ __device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const ui
     };
     uint64_t pos, w;
 #pragma unroll 1
-    for (int i = tid; i < n; i += NT)
+    for (int i = tid; i < n; i += kThreads)
       if (at(i, pos, w)) add_mass(s.limb, (uint32_t)((high - pos) >> shift), w);
-    join_limbs<NT, true>(s);
     __syncthreads();
-    constexpr int kEach = kBins / NT;
+    constexpr int kEach = kBins / kThreads;
     uint64_t mine[kEach], sum = 0, total;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) sum += mine[i] = s.bin[tid * kEach + i];
-    uint64_t run = block_scan<NT>(sum, s.warp_sum, total) - sum;
+    for (int i = 0; i < kEach; ++i) {
+      const int b = tid * kEach + i;
+      sum += mine[i] = s.limb[0][b] + ((uint64_t)s.limb[1][b] << kLimb) + ((uint64_t)s.limb[2][b] << (2 * kLimb));
+    }
+    uint64_t run = block_scan(sum, s.warp_sum, total) - sum;
     if (first) {
       need = want.of(total);
       if (tid == 0) s.total = total;
@@ -550,7 +548,7 @@ __device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const ui
     const uint32_t bin = s.bin_at;
     need = s.need;
 #pragma unroll 1
-    for (int i = tid; i < n; i += NT)
+    for (int i = tid; i < n; i += kThreads)
       if (at(i, pos, w) && (uint32_t)((high - pos) >> shift) == bin) {
         const uint32_t to = atomicAdd(&s.count, 1u);
         if (to < (uint32_t)kFew) {
@@ -566,7 +564,7 @@ __device__ __noinline__ uint64_t pick(Scratch &s, const uint64_t *keys, const ui
   // few: what is at or ahead of a key is added up, by some neighbouring threads a key
   const int few = (int)s.count;
   int parts = 1;
-  while (parts < 32 && 2 * parts * few <= NT) parts *= 2;
+  while (parts < 32 && 2 * parts * few <= kThreads) parts *= 2;
   const int at = tid / parts;
   const uint64_t key = at < few ? s.few[at] : ~0ull;
   uint64_t run = 0;
@@ -587,7 +585,7 @@ __device__ __forceinline__ uint64_t cluster_sum(Shared &s, uint64_t &before) {
   __syncthreads();
   if (threadIdx.x < ctas) {
     uint64_t whole = 0;
-    for (int i = 0; i < kLast / 32; ++i) whole += s.kept[i];
+    for (int i = 0; i < kWarps; ++i) whole += s.kept[i];
     cluster.map_shared_rank(s.cta_sum, threadIdx.x)[rank] = whole;
   }
   cluster.sync();
@@ -622,19 +620,19 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
   for (;;) {
     const bool first = span.shift < 0;
     __syncthreads();  // (what was in the bins' place is read)
-    for (int i = tid; i < (first ? kFirst : kBins * (MASS ? 3 : 1)); i += kLast) (&s.limb[0][0])[i] = 0;
+    for (int i = tid; i < (first ? kFirst : kBins * (MASS ? 3 : 1)); i += kThreads) (&s.limb[0][0])[i] = 0;
     __syncthreads();
     if (!first) key_bins<MASS>(columns, span, row, s.table, s.limb);
     else if (MASS && above) share_bins<true>(columns, span, 2.0f * 1.44269504f / t, 0x1p75f / (float)whole, s.first);
     else if (MASS) share_bins<false>(columns, span, 2.0f * 1.44269504f / t, 0x1p75f / (float)whole, s.first);
     else count_bins(columns, span, s.first);
-    if (!first) join_limbs<kLast, MASS>(s);
+    if (!first) join_limbs<MASS>(s);
     cluster.sync();
     // every CTA adds up a share of the bins and gives it to all: `parts` threads a bin, some CTAs each
     {
-      const int per = kBins / ctas, parts = max(1, kLast / per), each = ctas / min(parts, ctas);
-      const int b0 = tid % min(per, kLast), part = tid / min(per, kLast);
-      for (int b = b0; b < per; b += kLast) {
+      const int per = kBins / ctas, parts = max(1, kThreads / per), each = ctas / min(parts, ctas);
+      const int b0 = tid % min(per, kThreads), part = tid / min(per, kThreads);
+      for (int b = b0; b < per; b += kThreads) {
         uint64_t x[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -680,7 +678,7 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
     if (tid < ctas) {
       uint64_t sum = 0;
       if (MASS && first)
-        for (int i = 0; i < kLast / 32; ++i) sum += s.kept[i];
+        for (int i = 0; i < kWarps; ++i) sum += s.kept[i];
       cluster.map_shared_rank(s.cta_sum, tid)[rank] = sum;
       cluster.map_shared_rank(s.cta_count, tid)[rank] = s.count;
     }
@@ -694,17 +692,17 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
     }
     if (MASS && first) need = need > sum ? need - sum : 1;
     if (n <= (uint32_t)kList)
-      for (int i = tid; i < (int)s.count * ctas; i += kLast)
+      for (int i = tid; i < (int)s.count * ctas; i += kThreads)
         cluster.map_shared_rank(s.whole, i & (ctas - 1))[at + i / ctas] = s.list[i / ctas];
     cluster.sync();
     if (n <= (uint32_t)kList) {
       if (MASS)
-        for (int i = tid; i < (int)n; i += kLast) s.masses[i] = mass_of_key(s.table, row, s.whole[i]);
+        for (int i = tid; i < (int)n; i += kThreads) s.masses[i] = mass_of_key(s.table, row, s.whole[i]);
       __syncthreads();
-      const uint64_t border = pick<kLast>(s, s.whole, MASS ? s.masses : nullptr, (int)n, 0, 0, 0, 1, Want{Mode::count, 0.0, need, true});
+      const uint64_t border = pick(s, s.whole, MASS ? s.masses : nullptr, (int)n, 0, 0, 0, 1, Want{Mode::count, 0.0, need, true});
       if (MASS && first) {
         summed = true;
-        for (int i = tid; i < (int)n; i += kLast) {
+        for (int i = tid; i < (int)n; i += kThreads) {
           const uint32_t id = ~(uint32_t)s.whole[i] - (uint32_t)(rank * columns.share);
           if (s.whole[i] >= border && id < (uint32_t)columns.share)
             atomicAdd(&s.kept[id / (uint32_t)(columns.n * 128)], (unsigned long long)s.masses[i]);
@@ -738,7 +736,7 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
         s.range[1][warp] = hi;
       }
       __syncthreads();
-      for (int i = 0; i < kLast / 32; ++i) {
+      for (int i = 0; i < kWarps; ++i) {
         lo = min(lo, s.range[0][i]);
         hi = max(hi, s.range[1][i]);
       }
@@ -813,10 +811,9 @@ __device__ __noinline__ uint64_t sum_kept(const Columns c, const Kept kept, cons
   return sum;
 }
 
-template <int NT>
 __device__ __forceinline__ uint64_t block_sum(Scratch &s, uint64_t v) {
   uint64_t total;
-  block_scan<NT>(v, s.warp_sum, total);
+  block_scan(v, s.warp_sum, total);
   return total;
 }
 
@@ -1026,8 +1023,8 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
   extern __shared__ __align__(16) uint64_t keys[];  // [kMostGiven], and their masses
   uint64_t *masses = keys + kMostGiven;
   __shared__ int starts[kMaxPieces + 1];
-  __shared__ double piece_sum[kMaxPieces], warp_d[kThreads / 32];
-  __shared__ float tops[kThreads / 32], froms[kThreads / 32];
+  __shared__ double piece_sum[kMaxPieces], warp_d[kWarps];
+  __shared__ float tops[kWarps], froms[kWarps];
   __shared__ int n_keys, chosen;
   __shared__ double rest;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -1072,7 +1069,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
     froms[warp] = from;
   }
   __syncthreads();
-  for (int i = 0; i < kThreads / 32; ++i) {
+  for (int i = 0; i < kWarps; ++i) {
     top = fmaxf(top, tops[i]);
     from = fmaxf(from, froms[i]);  // from there on the pieces have given all
   }
@@ -1103,7 +1100,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
     if (lane == 31) warp_d[warp] = run;
     __syncthreads();
     double total = 0.0, before = 0.0;
-    for (int i = 0; i < kThreads / 32; ++i) {
+    for (int i = 0; i < kWarps; ++i) {
       if (i == warp) before = total;
       total += warp_d[i];
     }
@@ -1125,7 +1122,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
     const int id0 = piece * a.piece, n = min(a.vocab - id0, a.piece);
     const float *vals = a.logits + r * a.ld + id0;
     // a warp a run of columns
-    const int each = a.piece / (kThreads / 32);
+    const int each = a.piece / kWarps;
     auto mass_at = [&](int c) -> uint64_t {
       if (c >= n) return 0;
       const float v = fmaxf(vals[c], -INFINITY) + 0.0f;
@@ -1158,7 +1155,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
   // the keys that were given, together
   {
     uint64_t total;
-    const uint64_t ends = block_scan<kThreads>((uint64_t)my_n, s.warp_sum, total);
+    const uint64_t ends = block_scan((uint64_t)my_n, s.warp_sum, total);
     if (has) starts[tid + 1] = (int)ends;
     if (tid == 0) starts[0] = 0;
     __syncthreads();
@@ -1178,7 +1175,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
   uint64_t whole = 0;  // (0: of the list)
   if (k == 0 && p < 1.0f) {
     const double f = my_top > -INFINITY ? exp(((double)my_top - (double)top) / (double)t) : 0.0;
-    whole = block_sum<kThreads>(s, has ? (uint64_t)((double)my_mass * f) : 0);
+    whole = block_sum(s, has ? (uint64_t)((double)my_mass * f) : 0);
     if (tid == 0) a.row_mass[r] = whole;
   }
   bool known = from <= top;
@@ -1186,9 +1183,9 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
   if (greedy) {
     border = (uint64_t)key_of(top) << 32;
   } else if (known) {
-    if (k > 0) known = (border = pick<kThreads>(s, keys, nullptr, n, end, 0, high, end, Want{Mode::count, 0.0, (uint64_t)k, all})) != 0;
+    if (k > 0) known = (border = pick(s, keys, nullptr, n, end, 0, high, end, Want{Mode::count, 0.0, (uint64_t)k, all})) != 0;
     if (known && p < 1.0f)
-      known = (border = pick<kThreads>(s, keys, masses, n, border, 0, high, border, Want{Mode::share, (double)p, whole, false})) != 0;
+      known = (border = pick(s, keys, masses, n, border, 0, high, border, Want{Mode::share, (double)p, whole, false})) != 0;
     // min_p alone: what is not in the list must be below it
     if (known && k == 0 && !(p < 1.0f) && !all && mass_of_key(s.table, row, end) >= least) known = false;
   }
@@ -1196,7 +1193,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const Args a) {
     if (tid == 0) a.todo[atomicAdd(a.n_todo, 1)] = (int)r;
     return;
   }
-  const uint64_t drawn = pick<kThreads>(s, keys, masses, n, border, least, ~0ull << 32 | ~0u, (uint64_t)~(uint32_t)a.vocab << 32, Want{Mode::draw, u, 0, true});
+  const uint64_t drawn = pick(s, keys, masses, n, border, least, ~0ull << 32 | ~0u, (uint64_t)~(uint32_t)a.vocab << 32, Want{Mode::draw, u, 0, true});
   if (tid == 0) {
     a.tokens[r] = (int32_t)~(uint32_t)(drawn >> 32);
     if (a.probs) a.probs[r] = greedy ? 1.0f : (float)((double)s.border_mass / (double)s.total);
@@ -1227,7 +1224,7 @@ __device__ __forceinline__ void sample_row(const Args &a, Shared &s, int64_t r) 
     s.warp_from[warp] = from;
   }
   __syncthreads();
-  for (int i = 0; i < kLast / 32; ++i) {
+  for (int i = 0; i < kWarps; ++i) {
     top = fmaxf(top, s.warp_top[i]);
     from = fminf(from, s.warp_from[i]);
   }
@@ -1304,7 +1301,7 @@ __device__ __forceinline__ void sample_row(const Args &a, Shared &s, int64_t r) 
   }
 }
 
-__global__ void __launch_bounds__(kLast, 1) sample_requests_kernel(const Args a) {
+__global__ void __launch_bounds__(kThreads, 1) sample_requests_kernel(const Args a) {
   extern __shared__ __align__(16) uint8_t of_cta[];
   Shared &s = *reinterpret_cast<Shared *>(of_cta);
   cg::cluster_group cluster = cg::this_cluster();
@@ -1364,13 +1361,13 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
   while (a.piece > 2048 && together * pieces(a.piece) < 2 * (int64_t)ctx->num_sms && pieces(a.piece / 2) <= kMaxPieces) a.piece /= 2;
   a.pieces = (int)pieces(a.piece);
   a.give = kMostGiven / a.pieces;
-  // the last launch: CTAs of a row, sixteen where that gives each two thousand columns. (Few rows come to it
-  // as a rule, and their time is the call's: 102 us with 16, 120 with 8 for three of 64 rows, before the copies. Where all of them
-  // do, 8 leave less waiting: 280 and 190 us.)
+  // The last launch: CTAs of a row, sixteen where that gives each two thousand columns, and one on an SM. Few rows come
+  // to it as a rule, and their time is the call's: 88 us for 64 rows of which three do; 103 with clusters of 8, and
+  // with two CTAs on an SM 101. Where all 64 do, those leave less waiting: 360, 269 and 294 us.
   int cluster = 1;
   while (vocab > (int64_t)cluster * kMaxShare || (cluster < kMaxCluster && vocab > cluster * 2048)) cluster *= 2;
   a.share = (int)((vocab + cluster - 1) / cluster + 3) / 4 * 4;
-  a.run = (a.share + 4 * kLast - 1) / (4 * kLast) * 128;
+  a.run = (a.share + 4 * kThreads - 1) / (4 * kThreads) * 128;
   // what the launches tell one another: made by the context's first call and kept, so that a recorded
   // graph's addresses stay good
   constexpr size_t kBytes = (size_t)kRows * (kMaxPieces * 20 + kMostGiven * 8 + 24) + 16;
@@ -1416,7 +1413,7 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
     GQ_CUDA_TRY(ctx, gq_launch(ctx, finish_kernel, dim3((unsigned)rows), dim3(kThreads), (size_t)kMostGiven * 16, b));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(std::min<int64_t>(rows, std::max(1, ctx->num_sms / cluster)) * cluster));
-    cfg.blockDim = dim3(kLast);
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = sizeof(Shared);
     cfg.stream = ctx->stream;
     cudaLaunchAttribute attr[2];
