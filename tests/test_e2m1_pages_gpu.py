@@ -104,6 +104,33 @@ def test_every_scale_and_code_stands_for_its_value(g):
     assert np.array_equal(v.cpu().numpy()[:, 0], (want * 2.0).astype(np.float32), equal_nan=True)
 
 
+@pytest.mark.parametrize("heads,dim", [(1, 512), (2, 48), (1, 16), (3, 256)])
+@pytest.mark.parametrize("pad,skip", [(0, 0), (8, 0), (4, 0), (0, 4), (16, 8)])
+def test_rows_of_every_alignment(g, heads, dim, pad, skip):
+    """Rows of f32 that begin on 16 or on 32 bytes and lie any multiple of 4 values apart."""
+    torch = g._torch
+    rng = np.random.default_rng(dim + pad)
+    n, ps, row = 70, 8, heads * dim
+    x = [hard_rows(rng, n, row) for _ in range(2)]
+    slots = dev(g, rng.permutation(12 * ps)[:n])
+    pool = [torch.zeros(12, heads, ps, dim // 16 * 9, dtype=torch.uint8, device=g.torch_device) for _ in range(2)]
+    stores = [torch.full((n * (row + pad) + skip,), 7.0, device=g.torch_device) for _ in range(4)]
+    rows = [t[skip:].view(n, row + pad)[:, :row] for t in stores]
+    for i in range(2):
+        rows[i].copy_(dev(g, x[i]))
+    pages = g.kv_pages(*pool)
+    g.paged_append(pages, rows[0], rows[1], slots)
+    g.paged_read(pages, slots, k_out=rows[2], v_out=rows[3])
+    g.flush()
+    with np.errstate(over="ignore"):
+        for i in range(2):
+            want = ref.decode(ref.encode(x[i].reshape(n, heads, dim), 1.0)).astype(np.float32).reshape(n, row)
+            assert np.array_equal(rows[2 + i].cpu().numpy(), want, equal_nan=True)
+            kept = stores[2 + i].clone()
+            kept[skip:].view(n, row + pad)[:, :row] = 7.0
+            assert bool((kept == 7.0).all())
+
+
 @pytest.mark.parametrize("typ", ["f32", "f16", "bf16", "e4m3", "e2m1"])
 @pytest.mark.parametrize("heads,dim,ps", [(1, 256, 16), (1, 512, 64), (4, 128, 32), (3, 16, 1), (2, 48, 7), (1, 64, 16), (7, 112, 3)])
 def test_read_gives_the_rows(g, typ, heads, dim, ps):
