@@ -263,11 +263,10 @@ struct Stream {
   }
 };
 
-// Where the border may be, and the bin of a logit there.
+// Where the border may be, and the bin of a logit there. (Ends are keys and compared as such: a bin's end need not be
+// a logit's key, and there is one among them that stands for -0, which as a logit were equal to 0.)
 struct Span {
-  float low_v, high_v;  // the last and the first key, as logit and id
-  uint32_t low_id, high_id;
-  uint64_t high;
+  uint64_t low, high;   // the last and the first key
   int shift;            // -1: bins by the distance from the largest logit; else by (high - key) >> shift
   float top, per_logit;
   // (rounded by the addition; only the order matters, and that equal logits have equal bins)
@@ -275,7 +274,8 @@ struct Span {
     return __float_as_uint(fminf((top - v) * per_logit, (float)(kFirst - 1)) + 8388608.0f) & (kFirst - 1);
   }
   __device__ __forceinline__ bool has(float v, uint32_t id) const {
-    return from_on(v, id, low_v, low_id) && v > -INFINITY && from_on(high_v, high_id, v, id);
+    const uint64_t key = rank_key(v, id);
+    return v > -INFINITY && key >= low && key <= high;
   }
   __device__ __forceinline__ uint32_t key_bin(float v, uint32_t id) const { return (uint32_t)((high - rank_key(v, id)) >> shift); }
 };
@@ -306,6 +306,8 @@ __device__ __noinline__ void count_bins(const Columns c, const Span p, uint32_t 
 // Masses to some 2^-17, as shares of 2^31 of the whole: which bins the border can be in.
 template <bool LOW>
 __device__ __noinline__ void share_bins(const Columns c, const Span p, float rate, float unit, uint32_t *sum) {
+  const float low_v = logit_of(p.low);
+  const uint32_t low_id = ~(uint32_t)p.low;
   Stream next(c);
 #pragma unroll 1
   for (int i = 0; i < c.n; ++i) {
@@ -317,7 +319,7 @@ __device__ __noinline__ void share_bins(const Columns c, const Span p, float rat
       float w;  // (halves: a difference of two numbers may be infinite)
       asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"((0.5f * v[k] - 0.5f * p.top) * rate));
       if (v[k] == p.top) w = 1.0f;
-      const bool in = v[k] > -INFINITY && (!LOW || from_on(v[k], id + k, p.low_v, p.low_id));
+      const bool in = v[k] > -INFINITY && (!LOW || from_on(v[k], id + k, low_v, low_id));
       add_some(&sum[p.first_bin(v[k])], in ? __float2uint_rn(w * unit) : 0u);
     }
   }
@@ -347,6 +349,8 @@ __device__ __noinline__ uint64_t collect(const Columns c, const Span p, const Ro
                                          uint64_t *list, uint32_t *listed) {
   const int lane = threadIdx.x & 31;
   uint64_t sum = 0, mark = 0;  // a bit for each of the lane's columns
+  const float low_v = logit_of(p.low);  // (FIRST and LOW: a logit's key)
+  const uint32_t low_id = ~(uint32_t)p.low;
   Stream next(c);
 #pragma unroll 1
   for (int i = 0; i < c.n; ++i) {
@@ -358,7 +362,7 @@ __device__ __noinline__ uint64_t collect(const Columns c, const Span p, const Ro
     for (int k = 0; k < 4; ++k) {
       if (FIRST) {
         const uint32_t b = p.first_bin(v[k]);
-        const bool from = v[k] > -INFINITY && (!LOW || from_on(v[k], id + k, p.low_v, p.low_id));
+        const bool from = v[k] > -INFINITY && (!LOW || from_on(v[k], id + k, low_v, low_id));
         in |= (uint32_t)(b >= bin && b <= last && from) << k;
         if (SUM) ahead |= (uint32_t)(b < bin && v[k] > row.least && from) << k;
       } else {
@@ -609,10 +613,7 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
   const int tid = threadIdx.x, warp = tid >> 5;
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   Span span;
-  span.low_v = above ? logit_of(above) : -INFINITY;
-  span.low_id = above ? ~(uint32_t)above : ~0u;
-  span.high_v = INFINITY;
-  span.high_id = 0;
+  span.low = above;
   span.high = ~0ull;
   span.shift = -1;
   span.top = row.top;
@@ -750,22 +751,15 @@ __device__ __noinline__ uint64_t find_border(Shared &s, const Columns columns, c
         hi = max(hi, s.whole[2 * r + 1]);
       }
       span.high = hi;
-      span.low_v = logit_of(lo);
-      span.low_id = ~(uint32_t)lo;
+      span.low = lo;
       span.shift = max(0, 64 - __clzll((long long)(hi - lo)) - 11);
       cluster.sync();  // (before the bins of the next round are written there)
     } else {
       // the bin's own range of keys
       span.high -= (uint64_t)bin << span.shift;
-      const uint64_t lo = span.high - ((1ull << span.shift) - 1);
-      if (lo > rank_key(span.low_v, span.low_id)) {
-        span.low_v = logit_of(lo);
-        span.low_id = ~(uint32_t)lo;
-      }
+      span.low = max(span.low, span.high - (((uint64_t)1 << span.shift) - 1));
       span.shift = max(0, span.shift - 11);
     }
-    span.high_v = logit_of(span.high);
-    span.high_id = ~(uint32_t)span.high;
   }
 }
 
