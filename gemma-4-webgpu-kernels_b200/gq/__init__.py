@@ -217,6 +217,12 @@ class CudaBackend:
     def stream_ptr(self) -> int:
         return int(self.lib.gq_ctx_get_stream(self.ctx) or 0)
 
+    def torch_stream(self):
+        """The backend's stream as one of torch's."""
+        ptr, cuda = self.stream_ptr(), self._torch.cuda
+        # (torch has no external stream of the legacy default stream's handle)
+        return cuda.default_stream(self.torch_device) if ptr == 1 else cuda.ExternalStream(ptr, device=self.torch_device)
+
     # ---- record / replay (include/gq.h gq_graph_*) ------------------------------
     def record(self, fn):
         """Record the ops `fn()` issues into a replayable graph (own_stream only)."""

@@ -128,14 +128,14 @@ class PagedDecoder(e2b.Decoder):
         torch.cuda.synchronize(dev)
 
     def _stream(self):
-        return self.torch.cuda.ExternalStream(self.g.stream_ptr(), device=self.g.torch_device)
+        return self.g.torch_stream()
 
     @contextmanager
     def _ordered(self):
         """Work on the backend's stream that comes after what torch's current stream was given
         so far, and before what it is given next."""
         mine, callers = self._stream(), self.torch.cuda.current_stream(self.g.torch_device)
-        apart = (callers.cuda_stream or 1) != mine.cuda_stream  # (1: the legacy default stream, as the backend has it)
+        apart = callers.cuda_stream != mine.cuda_stream
         if apart:
             mine.wait_stream(callers)
         try:
