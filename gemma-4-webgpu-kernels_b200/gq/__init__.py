@@ -194,6 +194,23 @@ class CudaBackend:
         self._frame.append(g)
         return g
 
+    def _fresh(self, make, *shape, dtype):
+        """make (torch.zeros or torch.empty) a new tensor that a call is about to write. Where
+        the backend's stream is not torch's current one it is made on the backend's: filled
+        ahead of the call, out of memory that only that stream's work is given once the caller
+        lets go of it. What torch's stream still does with such memory is waited for (not
+        while the stream is recorded: keep what a recorded call returns as long as its graph)."""
+        torch = self._torch
+        if self.torch_device.type == "cuda":
+            callers = torch.cuda.current_stream(self.torch_device)
+            if (callers.cuda_stream or 1) != self.stream_ptr():  # (1: the legacy default stream, as the backend has it)
+                mine = self.torch_stream()
+                with torch.cuda.stream(mine):
+                    if not torch.cuda.is_current_stream_capturing():
+                        mine.wait_stream(callers)
+                    return make(*shape, dtype=dtype, device=self.torch_device)
+        return make(*shape, dtype=dtype, device=self.torch_device)
+
     def close(self) -> None:
         if getattr(self, "ctx", None):
             for q in self._qweights:
@@ -635,7 +652,7 @@ class CudaBackend:
         (gq_paged_read): `k_out` and `v_out` (token strides free), whose rows of negative
         slots stay as they are, or new tensors, where such rows are 0."""
         n, heads = slots.numel(), pages.row // pages.head_dim
-        new = lambda: self._torch.zeros(n, heads, pages.head_dim, dtype=self._torch.float32, device=self.torch_device)  # noqa: E731
+        new = lambda: self._fresh(self._torch.zeros, n, heads, pages.head_dim, dtype=self._torch.float32)  # noqa: E731
         k, v = k_out if k_out is not None else new(), v_out if v_out is not None else new()
         if pages.row != pages.head_dim:  # (as in paged_append)
             for x in (k, v):
