@@ -751,7 +751,7 @@ class CudaBackend:
         m, vocab = shape
         lp, ld = self._rows(lt, m, vocab, "sample_requests: logits")
         if tokens is None:
-            tokens = torch.empty(m, dtype=torch.int32, device=self.torch_device)
+            tokens = self._fresh(torch.empty, m, dtype=torch.int32)
         rc = self.lib.gq_sample_requests(
             self.ctx, lp, m, vocab, ld, d(temperature, f32, "temperature", m) if temperature is not None else None,
             d(top_k, torch.int32, "top_k", m) if top_k is not None else None,
