@@ -651,7 +651,7 @@ class CudaBackend:
         """The rows at slots [T] int64 of the pages as f32 k, v [T, heads, head_dim]
         (gq_paged_read): `k_out` and `v_out` (token strides free), whose rows of negative
         slots stay as they are, or new tensors, where such rows are 0."""
-        n, heads = slots.numel(), pages.row // pages.head_dim
+        n, heads = slots.numel(), pages.struct.heads
         new = lambda: self._fresh(self._torch.zeros, n, heads, pages.head_dim, dtype=self._torch.float32)  # noqa: E731
         k, v = k_out if k_out is not None else new(), v_out if v_out is not None else new()
         if pages.row != pages.head_dim:  # (as in paged_append)
