@@ -198,9 +198,10 @@ __device__ __forceinline__ void join_cluster(const Args &a, const float *mine, c
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
-      if (ml[p].x == -INFINITY) continue;  // no CTA, or one without a visible key: its columns are not written
+      if (p >= n) continue;
+      // (a part whose largest is -inf has no visible key, and zeros, or scores that are no numbers: its NaNs are kept)
       const float4 v = reinterpret_cast<const float4 *>(cluster.map_shared_rank(mine, p))[at];
-      const float w = exp_of(ml[p].x - m);
+      const float w = ml[p].x == -INFINITY ? 0.0f : exp_of(ml[p].x - m);
       l = fmaf(w, ml[p].y, l);
       o.x = fmaf(w, v.x, o.x);
       o.y = fmaf(w, v.y, o.y);
