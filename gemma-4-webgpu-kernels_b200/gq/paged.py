@@ -57,7 +57,9 @@ class PagedDecoder(e2b.Decoder):
     top_k, top_p of gq_sample_rows for all requests, or None: every request has its own, the
     controls ``temperature`` (1 at first), ``top_p`` (1), ``min_p`` (0) [batch] f32 and ``top_k`` (0)
     [batch] int32 of gq_sample_requests, and ``probs`` [batch] are the probabilities that the
-    last step's tokens were drawn with."""
+    places' last ``tokens`` were drawn with. A request of which the controls leave no token
+    gets -1, with probability 0: it goes on with another id in ``tokens``, put there before
+    it is ended too (a step that is given -1 raises at the next ``g.flush()``)."""
 
     def __init__(self, g, cfg: e2b.Config, weights: Optional[e2b.Weights], batch: int, max_len: int, page_size: int = 16,
                  kv_type: str = "bf16", n_pages: Optional[int] = None, k_scale: float = 1.0, v_scale: float = 1.0,
@@ -123,7 +125,7 @@ class PagedDecoder(e2b.Decoder):
         self.drawn, self.rng_after = torch.zeros_like(self.tokens), torch.zeros_like(self.rng)  # of the step
         if self.opts is None:
             self.temperature, self.top_p = (torch.ones(B, device=dev) for _ in range(2))
-            self.min_p, self.probs = (torch.zeros(B, device=dev) for _ in range(2))
+            self.min_p, self.probs, self.drawn_probs = (torch.zeros(B, device=dev) for _ in range(3))
             self.top_k = torch.zeros(B, dtype=i32, device=dev)
         torch.cuda.synchronize(dev)
 
@@ -286,7 +288,8 @@ class PagedDecoder(e2b.Decoder):
             add("rng", self._torch_call, lambda: self.rng_after.copy_(self.rng))
         if self.opts is None:
             add("sample", lib.gq_sample_requests, ctx, V(self.controlled), B, vocab, vocab, V(self.temperature), V(self.top_k),
-                V(self.top_p), V(self.min_p), None, V(self.rng_after), V(self.drawn), V(self.probs))
+                V(self.top_p), V(self.min_p), None, V(self.rng_after), V(self.drawn),
+                V(self.drawn_probs))
         else:
             add("sample", lib.gq_sample_rows, ctx, V(self.controlled), B, vocab, vocab, ctypes.byref(self.opts), None, 0, 0,
                 V(self.rng_after), V(self.drawn))
@@ -309,6 +312,8 @@ class PagedDecoder(e2b.Decoder):
         torch = self.torch
         torch.ne(self.now, self.lens, out=self.took)
         torch.where(self.took, self.drawn, self.tokens, out=self.tokens)
+        if self.opts is None:
+            torch.where(self.took, self.drawn_probs, self.probs, out=self.probs)
         if self._draws():  # (a greedy step draws no numbers)
             torch.where(self.took, self.rng_after, self.rng, out=self.rng)
 
@@ -338,10 +343,11 @@ class PagedDecoder(e2b.Decoder):
     def record_steps(self) -> None:
         """Record the step into a graph that ``step`` replays from now on (the backend must
         own its stream). Runs one step first, which sizes the workspaces, and takes its
-        token back: lengths, pages and random states are as before."""
+        token back: lengths, pages, random states and probabilities are as before."""
         torch = self.torch
         self.g.flush()
-        saved = [(t, t.clone()) for t in (self.lens, self.table, self.free, self.count, self.rng, self.tokens, self.took)]
+        keep = [self.lens, self.table, self.free, self.count, self.rng, self.tokens, self.took]
+        saved = [(t, t.clone()) for t in keep + ([self.probs] if self.opts is None else [])]
         torch.cuda.synchronize(self.g.torch_device)
         try:
             self.run()
