@@ -10,7 +10,8 @@
 //     the m16n8k16 instruction: no row is idle. Its result is laid out as the second operand of
 //     O^T = V^T P^T wants the weights, so they stay where they are.
 //   * Codes go from shared memory to fragments without a transposing load: which keys and columns an
-//     instruction's rows stand for is free, so a lane reads 16 bytes of one key and uses all of them.
+//     instruction's rows stand for is free, so a lane reads 8 bytes of one key (4 of 64 columns) and
+//     uses all of them.
 //     For V the codes of two keys are put side by side (one byte, two keys) before they become f16.
 //   * A key that is not visible gets the scale 0 (a code is never NaN): nothing is cleared.
 // Copies are untiled bulk copies, one per page (or part of a page) of 32 keys, into a ring of each team's
@@ -45,7 +46,7 @@ struct Conf {
   static constexpr int kRow = D / 16 * 9;        // bytes of a key's row
   static constexpr int CB = DW / 16;             // bytes of codes that a lane takes at once
   static constexpr int NC = DW / (8 * CB);       // times it does for K
-  static constexpr int W = CB / 4;               // words of it
+  static constexpr int W = CB / 4;               // words of it: 2, or 1 of 64 columns
   static constexpr int kWarps = D > 128 ? 8 : 4;
   static constexpr int kTeams = kWarps / PS;
   static constexpr int kThreads = kWarps * 32;
@@ -56,6 +57,7 @@ struct Conf {
   static constexpr int kSwap = PS > 1 ? kTeams * 2 * PS * 32 * 8 * 4 : 0;
   static constexpr int kSmem = kTeams * kStages * kSlot + kQBytes + kSwap;
   static_assert(kSlot >= 8 * D * 4, "a team's part of the output fits a slot");
+  static_assert(W <= 2, "a lane's codes have one scale");
 };
 
 // The key that stands at place n of the r-th 8 keys: rows of the 8 lanes that load together (K: keys of
@@ -108,10 +110,7 @@ __device__ __forceinline__ uint32_t select(uint32_t mask, uint32_t x, uint32_t y
 }
 template <int W>
 __device__ __forceinline__ void lds(const uint8_t *p, uint32_t (&w)[W]) {
-  if constexpr (W == 4) {
-    const uint4 v = *reinterpret_cast<const uint4 *>(p);
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-  } else if constexpr (W == 2) {
+  if constexpr (W == 2) {
     const uint2 v = *reinterpret_cast<const uint2 *>(p);
     w[0] = v.x, w[1] = v.y;
   } else {
@@ -382,20 +381,14 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
         }
 #pragma unroll
         for (int cc = 0; cc < NC; ++cc) {
-          uint32_t kw[4][W], sc[4][W == 4 ? 2 : 1];
+          uint32_t kw[4][W], sc[4];
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
             const uint8_t *kr = kt + key_at<D>(y, g) * ROW;
             lds<W>(kr + half * (DW / 2) + cc * (4 * CB) + q4 * CB, kw[y]);
             const uint8_t *ks = kr + D / 2 + half * (DW / 16);
-            if constexpr (W == 4) {
-              const uint32_t two = e4m3_pair(*reinterpret_cast<const uint16_t *>(ks + cc * 8 + q4 * 2));
-              sc[y][0] = __byte_perm(two, two, 0x1010);
-              sc[y][W == 4 ? 1 : 0] = __byte_perm(two, two, 0x3232);
-            } else {
-              const uint32_t one = e4m3_pair(ks[(cc * 4 + q4) * CB / 8]);
-              sc[y][0] = __byte_perm(one, one, 0x1010);
-            }
+            const uint32_t one = e4m3_pair(ks[(cc * 4 + q4) * CB / 8]);
+            sc[y] = __byte_perm(one, one, 0x1010);
           }
 #pragma unroll
           for (int wd = 0; wd < W; ++wd) {
@@ -405,7 +398,7 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
             for (int y = 0; y < 4; ++y) {
               uint32_t h[4];
               e2m1_word(kw[y][wd], h);
-              const uint32_t f = sc[y][W == 4 ? wd / 2 : 0];
+              const uint32_t f = sc[y];
               mma_f16(c[y], q0.x, q0.y, q0.z, q0.w, mul2(h[0], f), mul2(h[1], f));
               mma_f16(c[y], q1.x, q1.y, q1.z, q1.w, mul2(h[2], f), mul2(h[3], f));
               // (the instruction truncates its sums: four are added up in it, the rest here)
@@ -492,14 +485,13 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
 
       // ---- output: 16 columns by 8 heads per instruction, over 16 keys
       const uint8_t *vt = kt + kKeys * ROW;
-      uint32_t vw[8][W], sb[8], sp[4][W == 4 ? 2 : 1];
+      uint32_t vw[8][W], sb[8], sp[4];
 #pragma unroll
       for (int y = 0; y < 8; ++y) {
         const uint8_t *vr = vt + key_at<D>(y >> 1, 2 * q4 + (y & 1)) * ROW;
         lds<W>(vr + half * (DW / 2) + g * CB, vw[y]);
         const uint8_t *vs = vr + D / 2 + half * (DW / 16);
-        if constexpr (W == 4) sb[y] = *reinterpret_cast<const uint16_t *>(vs + g * 2);
-        else sb[y] = vs[g * CB / 8];
+        sb[y] = vs[g * CB / 8];
       }
       if (ragged) {
         asm volatile("");
@@ -510,11 +502,7 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
         }
       }
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const uint32_t pairs = __byte_perm(sb[2 * y], sb[2 * y + 1], 0x5140);
-        sp[y][0] = e4m3_pair(pairs);
-        if constexpr (W == 4) sp[y][W == 4 ? 1 : 0] = e4m3_pair(pairs >> 16);
-      }
+      for (int y = 0; y < 4; ++y) sp[y] = e4m3_pair(__byte_perm(sb[2 * y], sb[2 * y + 1], 0x5140));
 #pragma unroll
       for (int wd = 0; wd < W; ++wd) {
         float c[4][4];
@@ -528,7 +516,7 @@ __global__ void __launch_bounds__(Conf<D>::kThreads, Conf<D>::kPerSm) paged_q4_k
             const uint32_t v0 = vw[4 * ks + 2 * y][wd], v1 = vw[4 * ks + 2 * y + 1][wd];
             e2m1_word(select(0x0f0f0f0fu, v0, v1 << 4), ev[y]);
             e2m1_word(select(0x0f0f0f0fu, v0 >> 4, v1), od[y]);
-            const uint32_t s = sp[2 * ks + y][W == 4 ? wd / 2 : 0];
+            const uint32_t s = sp[2 * ks + y];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               ev[y][k] = mul2(ev[y][k], s);
