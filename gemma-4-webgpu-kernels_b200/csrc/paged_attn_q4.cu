@@ -150,23 +150,23 @@ __device__ __forceinline__ void join_cluster(const Args &a, const float *mine, c
     const int h = at / (D / 4);
     float m = -INFINITY, l = 0.0f;
     float2 ml[8];
+    float4 v[8];
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
+      v[p] = p < n ? reinterpret_cast<const float4 *>(cluster.map_shared_rank(mine, p))[at] : make_float4(0.f, 0.f, 0.f, 0.f);
       ml[p] = p < n ? cluster.map_shared_rank(mine_ml, p)[h] : make_float2(-INFINITY, 0.0f);
       m = fmaxf(m, ml[p].x);
     }
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int p = 0; p < 8; ++p) {
-      if (p >= n) continue;
       // (a part whose largest is -inf has no visible key, and zeros, or scores that are no numbers: its NaNs are kept)
-      const float4 v = reinterpret_cast<const float4 *>(cluster.map_shared_rank(mine, p))[at];
       const float w = ml[p].x == -INFINITY ? 0.0f : exp_of(ml[p].x - m);
       l = fmaf(w, ml[p].y, l);
-      o.x = fmaf(w, v.x, o.x);
-      o.y = fmaf(w, v.y, o.y);
-      o.z = fmaf(w, v.z, o.z);
-      o.w = fmaf(w, v.w, o.w);
+      o.x = fmaf(w, v[p].x, o.x);
+      o.y = fmaf(w, v[p].y, o.y);
+      o.z = fmaf(w, v[p].z, o.z);
+      o.w = fmaf(w, v[p].w, o.w);
     }
     const float s = inv_or_zero(l) * a.v_scale;
     reinterpret_cast<float4 *>(a.out + ((int64_t)b * a.hq + head0) * D)[at] = make_float4(o.x * s, o.y * s, o.z * s, o.w * s);
