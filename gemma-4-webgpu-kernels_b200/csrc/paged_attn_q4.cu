@@ -11,8 +11,7 @@
 //     O^T = V^T P^T wants the weights, so they stay where they are.
 //   * Codes go from shared memory to fragments without a transposing load: which keys and columns an
 //     instruction's rows stand for is free, so a lane reads 8 bytes of one key (4 of 64 columns) and
-//     uses all of them.
-//     For V the codes of two keys are put side by side (one byte, two keys) before they become f16.
+//     uses all of them. For V the codes of two keys are put side by side (one byte, two keys) before they become f16.
 //   * A key that is not visible gets the scale 0 (a code is never NaN): nothing is cleared.
 // Copies are untiled bulk copies, one per page (or part of a page) of 32 keys, into a ring of each team's
 // own: a team is one warp, or D / 128 of 128 columns each, which add up their parts of the scores (256
@@ -20,10 +19,11 @@
 // of up to 4096 keys of 512).
 //
 // 64 requests of up to 4096 keys of 512 (80 MB): 47 us; 23 of up to 10007, 4 key-value heads of 128, capped
-// scores (72 MB): 39 us; 4 of up to 131072 of 512 (205 MB): 77 us, 2.7 TB/s. Bound by the instructions: issue
-// slots 60% taken at 16 warps per SM, the matrix pipe 31%, conversions 35%. A warp has 830 for 32 keys of 128
-// columns, 320 of them conversions, products with scales and matrix products. Some 12 us of a call are not
-// keys: the cut 2, code that is run once, parts brought together 2, the join's launch 5.
+// scores (72 MB): 39 us; 4 of up to 131072 of 512 (205 MB): 76 us, 2.7 TB/s. No unit is full: issue slots are 52-60%
+// taken, conversions 36-39%, the matrix pipe 25-32%. 128 registers a thread (and 8 to 100 bytes of each instance
+// spilled) leave 16 warps per SM, too few to hide a tile's dependent steps, of which it has many: a warp executes 830
+// instructions for 32 keys of 128 columns, 320 of them conversions, products with scales and matrix products. Some
+// 12 us of a call are not keys: the cut 2, code that is run once, parts brought together 2, the join's launch 5.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -635,7 +635,7 @@ int launch(gq_ctx *ctx, Args &a) {
     GQ_CUDA_TRY(ctx, cudaFuncSetAttribute(paged_q4_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     attr_set[ctx->device & 63] = true;
   }
-  // Units that cannot have many tiles get a cluster of CTAs each: no cut, no join. (One request of 333 keys 7.5 us,
+  // Units that cannot have many tiles get a cluster of CTAs each: no cut, no join. (One request of 333 keys 6.9 us,
   // cut 10.2; 64 of 512 keys in a window 13.4 and 18.6; 225 of up to 62 keys, 8 heads, 20 and 25.) Where units are long
   // or uneven a cluster waits for its longest: 64 of up to 4096 keys 59 us, cut 47. Hence 8 tiles of a CTA at the
   // most, and not many more than equal pieces had.
@@ -673,8 +673,10 @@ int launch(gq_ctx *ctx, Args &a) {
 
 }  // namespace
 
-// Head_dims of the instantiated kernels, power-of-two pages, and copies of whole 16 bytes. (What is left goes
-// to the kernel that takes keys one by one: 4 requests of up to 131072 keys of 512 733 us, here 77.)
+// Head_dims of the instantiated kernels, and pages of which a tile has a whole number or the other way round, in copies
+// that begin and end on 16 bytes: a power of two of rows, 8 at least (a row may be 36 bytes), and pages a multiple of 16
+// bytes apart. What is left goes to the kernel that takes keys one by one: 4 requests of up to 131072 keys of 512 733 us,
+// here 76.
 bool gq_paged_attn_q4_supported(const gq_kv_pages *p) {
   const int64_t d = p->head_dim, stride = gq_kv_page_stride(p);
   return p->type == GQ_KV_E2M1 && (d == 64 || d == 128 || d == 256 || d == 512) && p->page_size >= 8 &&

@@ -9,10 +9,13 @@
 // is rounded at both ends, and where the ends differ the number is compared with the middle of the
 // two, multiplied out, which is exact in f32 (few bits times few bits).
 //
-// Both directions are bound by memory traffic and, nearly as much, by instructions: with pieces of four values
-// a lane and 16-byte accesses they took a third more. 16411 tokens' rows of 512 written and read back 33 us (144 MB,
-// 4.3 TB/s; the first kernels, a piece at a time, 54), 32771 tokens' read 28 us (153 MB, 5.4 TB/s; 43). A few rows
-// take the time of their launches: 5 us.
+// Both directions wait for memory (issue slots 50-58% taken; 2.9 stalls on loads per issue when writing, 6.6 when
+// reading). With pieces of four 4-bit values a lane and 16-byte accesses they took a third more. 16411 tokens' rows of 512
+// written and read back 33 us (144 MB, 4.4 TB/s; the first kernels, a piece at a time, 54), 32771 tokens' read 28 us
+// (153 MB, 5.4 TB/s; 43). Rows of whole bytes are read in pieces of four values, four of them in flight, which is near the
+// bytes' time as it is: 16411 rows of 512 in f32 24.4 us (135 MB, 5.5 TB/s; 20.5 at the copy rate), f16 and bf16 18.7
+// (15.4), e4m3 15.9 (12.8), 4-bit 15.6 (11.7); 4 heads of 128 take 7 to 12% more. A few rows take the time of their
+// launches: 5 us.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -62,7 +65,7 @@ __device__ __forceinline__ uint32_t quantise(const float (&x)[8], uint32_t &scal
   const bool up = a > middle || (a == middle && (lo & 1u));
   scale = up ? hi : lo;
   const float s = up ? above : below;
-  if (top > 0x7f800000u) scale = 0x7fu;  // a NaN among them: the block is NaN, its codes are 0
+  if (top > 0x7f800000u) scale = 0x7fu;  // a NaN among them: the block is NaN, its codes are 0 or -0
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
   r = s > 0.0f ? r : 0.0f;

@@ -8,8 +8,8 @@
 //
 // All three options keep a beginning of the order, so what is left is one border: a logit and an id,
 // together a key of 64 bits. It is found without sorting: a histogram of counts (top-k) or masses (top-p) over
-// 2048 bins says in which bin the border lies, and that bin is cut again until few keys are left to be
-// compared. Nor are all of a row's keys needed, mostly: three launches.
+// 2048 bins (4096 of a whole row's first) says in which bin the border lies, and that bin is cut again until few keys
+// are left to be compared. Nor are all of a row's keys needed, mostly: three launches.
 //   survey  a CTA per piece of a row, for all SMs to read the logits: its largest, its largest keys (as many as
 //           make some 1024 of a row), and its sum of masses where the whole row's counts
 //   finish  a CTA per row, among the keys that the pieces have given; without top-k, top-p and min-p there are
@@ -21,11 +21,12 @@
 // draw over 262144 tokens would land on a neighbour of the right token every few hundred rows; 2^-45
 // leaves less than one in 10^6.
 //
-// 64 rows of 262144 logits, 67 MB, 10 us of memory traffic: 27 us with a top_k of 64, 30 with a top_p of
-// 0.95 of those or a top_k of 1000, 51 over all tokens, 84 of mixed options (survey 28, finish 19, last 37 for
-// three of the rows); 22 us for one row. The survey is bound by its instructions (issue 57%, f64 among them), the
-// finish by the latencies of its steps (a search 2.5 us, three of them), the last launch by those of some passes
-// (8 us the one that adds up masses) and six cluster barriers (1.2 us each), 33 us a row.
+// 64 rows of 262144 logits, 67 MB, 10 us of memory traffic: 29 us with a top_k of 64, 32 with a top_p of
+// 0.95 of those or a top_k of 1000, 55 over all tokens, 85 of mixed options (survey 28, finish 20, last 37 for
+// three of the rows); one row 13 to 19 us, 45 where its border lies far down. The survey has its issue slots 68%
+// taken (53% of the time with its ends, f64 18%), and its pieces take turns; the finish is dependent steps of one CTA a
+// row (up to three searches in turn, issue 41%), and so is the last launch: passes over a CTA's columns with six cluster
+// barriers between, 33 us a row (issue 22%; code that is not at the SM yet, barriers and loads are waited for most).
 #include <cooperative_groups.h>
 #include <math.h>
 
@@ -50,7 +51,7 @@ constexpr int kFew = 256;         // keys that are compared with one another
 constexpr int kGiven = 1024;      // keys that a row's pieces give together, about; a larger top_k has twice as many
 constexpr int kMostGiven = 4096;  // and no more
 constexpr int kSurvey = 256;      // threads that survey a piece
-constexpr int kMaxPiece = 8192;   // (a thread's 32 columns: a bit each; with 4096 as the most, mixed options took 109 us in place of 102)
+constexpr int kMaxPiece = 8192;   // (a thread's 32 columns: a bit each; with 4096 as the most, mixed options take 90 us in place of 85)
 static_assert(kMaxPiece <= 32 * kSurvey);
 constexpr int kRows = 256;        // rows of a launch
 constexpr int kTable = 16;
@@ -872,8 +873,8 @@ __global__ void __launch_bounds__(kSurvey) survey_kernel(const Args a) {
   const float p = o.p, t = o.t;
   const bool sum_all = !greedy && k == 0 && (p < 1.0f || !(o.low_p > 0.0f));
   const int steps = a.piece / (4 * kSurvey);
-  // the piece as one copy: all of an SM's pieces are on their way at once (loads by the threads: 102 us for the
-  // mixed options, this way 96)
+  // the piece as one copy: all of an SM's pieces are on their way at once (loads by the threads: 91 us for the
+  // mixed options, this way 85; a top_k of 64 37 and 29)
   if (a.wide && n % 4 == 0) {
     if (tid == 0) {
       gqd::mbar_arrive_expect_tx(&arrived, (uint32_t)n * 4);
@@ -1356,8 +1357,9 @@ extern "C" int gq_sample_requests(gq_ctx *ctx, const float *logits, int64_t m, i
   a.pieces = (int)pieces(a.piece);
   a.give = kMostGiven / a.pieces;
   // The last launch: CTAs of a row, sixteen where that gives each two thousand columns, and one on an SM. Few rows come
-  // to it as a rule, and their time is the call's: 88 us for 64 rows of which three do; 103 with clusters of 8, and
-  // with two CTAs on an SM 101. Where all 64 do, those leave less waiting: 360, 269 and 294 us.
+  // to it as a rule, and their time is the call's: 85 us for 64 rows of which three do; 96 with clusters of 8, and
+  // with two CTAs on an SM 97; one row that does 45, 55 and 49. Where all do, those leave less waiting: 16 rows 113,
+  // 100 and 102 us, 64 rows 344, 248 and 280.
   int cluster = 1;
   while (vocab > (int64_t)cluster * kMaxShare || (cluster < kMaxCluster && vocab > cluster * 2048)) cluster *= 2;
   a.share = (int)((vocab + cluster - 1) / cluster + 3) / 4 * 4;

@@ -664,8 +664,9 @@ int gq_process_logits_bounded(gq_ctx *ctx, const float *logits, int64_t m, int64
  * greedy). probs[r] (f32, may be NULL) is the probability the token was drawn with, its w
  * over the sum (greedy: 1). A NaN is never drawn, nor is -inf; where there is nothing else
  * the token is -1 and its probability 0. +inf: only such tokens are drawn. Weights are
- * f64 and added up as multiples of 2^-44 of the largest: a weight below half of that
- * counts as 0. The logits are not modified. vocab <= 524288 (GQ_ERR_UNSUPPORTED beyond).
+ * f64 and added up as multiples of 2^-44 of the largest (where only a temperature is set,
+ * of the largest of some 2048 to 8192 neighbours): a weight below half of that counts as
+ * 0. The logits are not modified. vocab <= 524288 (GQ_ERR_UNSUPPORTED beyond).
  * The context's first call allocates 9 MB that its calls share (also while the stream is
  * recorded), so calls that may overlap on two streams need a context each; tokens, and the
  * logits of a call, must not change while it runs. */
